@@ -49,6 +49,14 @@ class LrnDesc(C.Structure):
     _fields_ = [("n", C.c_int32), ("k", C.c_double), ("alpha", C.c_double), ("beta", C.c_double)]
 
 
+NORMALIZATIONS = {"rms": 0, "layer": 1}
+
+
+class BlockDesc(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("epsilon", C.c_double), ("residual_scale", C.c_double), ("rows", C.c_int64),
+                ("cols", C.c_int64), ("gate_rows", C.c_int64)]
+
+
 class B200Error(RuntimeError):
     def __init__(self, code, message):
         super().__init__("cortex_b200 error %d: %s" % (code, message))
@@ -120,6 +128,13 @@ SIGNATURES = {
     "cb200_gemm_bias_act": [_vp, _i, _vp, _i64, _i, _i, _d, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _d, _vp, _i],
     "cb200_gemm_bias_act_peers": [_vp, _i, _vp, _i64, _i, _i, _d, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _d, _vp, _i,
                                   _i, C.POINTER(_vp)],
+    "cb200_expert_gemm": [_vp, _i, _vp, _i64, _i, _d, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _d, _vp, _vp, _i],
+    "cb200_expert_gemm_weights": [_vp, _i, _vp, _i64, _i64, _d, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _d, _vp, _vp],
+    "cb200_block_normalize": [_vp, _i] + [_vp, _i64] * 4 + [_vp] * 5 + [C.POINTER(BlockDesc)],
+    "cb200_block_normalize_gradients": [_vp, _i] + [_vp, _i64] * 2 + [_vp] * 5 + [_vp, _i64] * 4 + [_vp] * 4 +
+                                       [C.POINTER(BlockDesc)],
+    "cb200_global_norm": [_vp, _i, _i, _vp, _vp, _vp],
+    "cb200_clip_gradients": [_vp, _i, _i, _vp, _vp, _vp, _d, _vp],
     "cb200_graph_capture_begin": [_vp],
     "cb200_graph_capture_end": [_vp, C.POINTER(_vp)],
     "cb200_graph_launch": [_vp, _vp],

@@ -1,0 +1,253 @@
+// Products grouped by expert: rows of A are grouped by offsets in device memory and every group has a matrix of its own.
+//
+//   expert_gemm           C[r, :]  = act(alpha * A[r, :] . op(B_e) + beta * C[r, :] + bias_e)       r in group e
+//   expert_gemm_weights   C_e      = alpha * sum_{r in group e} A[r, :]^T B[r, :] + beta * C_e
+//                         bias_gradient_e = alpha * sum_{r in group e} A[r, :] + beta * bias_gradient_e
+//
+// Rows outside every group are neither read into a result nor written.
+#include "common.cuh"
+#include "expert_groups.cuh"
+#include <math.h>
+
+namespace {
+
+static __device__ __noinline__ double act_transcendental(double v, int act) {
+  return act == CB200_ACT_TANH ? tanh(v) : 1.0 / (1.0 + exp(-v));
+}
+template <typename T> __device__ __forceinline__ T act_apply(T v, int act) {
+  if (act == CB200_ACT_NONE) return v;
+  if (act == CB200_ACT_RELU) return v > (T)0 ? v : (T)0;
+  return (T)act_transcendental((double)v, act);
+}
+
+template <typename T> struct Product {
+  T* C; long long c_stride, ldc;
+  const T* A; long long lda;
+  const T* B; long long b_stride, ldb;
+  int trans_b, act;
+  int rows, M, N, K, experts;      // expert_gemm: K, N of op(B); expert_gemm_weights: C_e is M x N
+  T alpha, beta;
+  const T* bias;
+  T* bias_g;
+  const int* offsets;
+  int* status;
+};
+
+// 64 x 64 tile, 16 x 16 threads, 4 x 4 values per thread, operands of any pitch and alignment.
+// Element (m, k) of the left operand at a[m * sam + k * sak], (k, n) of the right one at b[k * sbk + n * sbn].
+template <typename T>
+__device__ __forceinline__ void simt_tile(const T* a, long long sam, long long sak, const T* b, long long sbk, long long sbn,
+                                          int m_left, int n_left, int K, T (&acc)[4][4]) {
+  __shared__ T As[16][64 + 1];
+  __shared__ T Bs[16][64 + 1];
+  const int t = threadIdx.x, tx = t % 16, ty = t / 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = (T)0;
+  for (int k0 = 0; k0 < K; k0 += 16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      int k, m;
+      if (sak == 1) { k = t % 16; m = t / 16 + 16 * i; } else { m = t % 64; k = t / 64 + 4 * i; }
+      As[k][m] = (m < m_left && k0 + k < K) ? a[(long long)m * sam + (long long)(k0 + k) * sak] : (T)0;
+      int kb, n;
+      if (sbn == 1) { n = t % 64; kb = t / 64 + 4 * i; } else { kb = t % 16; n = t / 16 + 16 * i; }
+      Bs[kb][n] = (n < n_left && k0 + kb < K) ? b[(long long)(k0 + kb) * sbk + (long long)n * sbn] : (T)0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      T x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = As[k][ty + 16 * i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = Bs[k][tx + 16 * j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += x[i] * y[j];
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void simt_store(T* c, long long ldc, int m_left, int n_left, const T (&acc)[4][4], T alpha, T beta,
+                                           const T* bias, int act) {
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = ty + 16 * i;
+    if (m >= m_left) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = tx + 16 * j;
+      if (n >= n_left) continue;
+      T* to = c + (long long)m * ldc + n;
+      T o = alpha * acc[i][j];
+      if (beta != (T)0) o += beta * (*to);
+      if (bias) o += bias[n];
+      *to = act_apply<T>(o, act);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) expert_rows_simt_kernel(Product<T> p) {
+  __shared__ groups::Tile tile;
+  __shared__ bool found;
+  for (int t = (int)blockIdx.y;; t += (int)gridDim.y) {
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      groups::Tile own;
+      const bool f = groups::find_tile(p.offsets, p.experts, p.rows, 64, t, p.status, own);
+      if (threadIdx.x == 0) { tile = own; found = f; }
+    }
+    __syncthreads();
+    if (!found) return;
+    const int m0 = tile.lo + tile.index * 64, n0 = (int)blockIdx.x * 64;
+    const T* b = p.B + tile.expert * p.b_stride + (p.trans_b ? (long long)n0 * p.ldb : (long long)n0);
+    T acc[4][4];
+    simt_tile<T>(p.A + (long long)m0 * p.lda, p.lda, 1, b, p.trans_b ? 1 : p.ldb, p.trans_b ? p.ldb : 1, tile.hi - m0, p.N - n0,
+                 p.K, acc);
+    simt_store<T>(p.C + (long long)m0 * p.ldc + n0, p.ldc, tile.hi - m0, p.N - n0, acc, p.alpha, p.beta,
+                  p.bias ? p.bias + (long long)tile.expert * p.N + n0 : nullptr, p.act);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) expert_weights_simt_kernel(Product<T> p, int tiles_m) {
+  __shared__ int lo, hi;
+  const int e = (int)blockIdx.z;
+  if (threadIdx.x < 32) {
+    int a, b;
+    groups::group_rows(p.offsets, p.rows, e, p.status, a, b);
+    if (threadIdx.x == 0) { lo = a; hi = b; }
+  }
+  __syncthreads();
+  const int n0 = (int)blockIdx.x * 64;
+  for (int tm = (int)blockIdx.y; tm < tiles_m; tm += (int)gridDim.y) {
+    const int m0 = tm * 64;
+    T acc[4][4];
+    simt_tile<T>(p.A + (long long)lo * p.lda + m0, 1, p.lda, p.B + (long long)lo * p.ldb + n0, p.ldb, 1, p.M - m0, p.N - n0,
+                 hi - lo, acc);
+    simt_store<T>(p.C + e * p.c_stride + (long long)m0 * p.ldc + n0, p.ldc, p.M - m0, p.N - n0, acc, p.alpha, p.beta, nullptr,
+                  CB200_ACT_NONE);
+  }
+}
+
+// bias_gradient[e, m] = alpha * sum of the group's rows + beta * bias_gradient[e, m]; 32 columns and 8 rows at a time
+template <typename T>
+__global__ void __launch_bounds__(256) expert_bias_gradient_kernel(Product<T> p) {
+  __shared__ int lo, hi;
+  __shared__ T part[8][33];
+  const int e = (int)blockIdx.y;
+  if (threadIdx.x < 32) {
+    int a, b;
+    groups::group_rows(p.offsets, p.rows, e, p.status, a, b);
+    if (threadIdx.x == 0) { lo = a; hi = b; }
+  }
+  __syncthreads();
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, m = (int)blockIdx.x * 32 + tx;
+  T s = (T)0;
+  if (m < p.M)
+    for (int r = lo + ty; r < hi; r += 8) s += p.A[(long long)r * p.lda + m];
+  part[ty][tx] = s;
+  __syncthreads();
+  if (ty != 0 || m >= p.M) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += part[w][tx];
+  T* to = p.bias_g + (long long)e * p.M + m;
+  T o = p.alpha * s;
+  if (p.beta != (T)0) o += p.beta * (*to);
+  *to = o;
+}
+
+template <typename T> int run_rows(cb200_stream* s, const Product<T>& p) {
+  DeviceGuard guard(s->device);
+  const long long tiles = (p.rows + 63) / 64 + (p.experts < p.rows ? p.experts : p.rows);
+  expert_rows_simt_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles < 65535 ? tiles : 65535)), 256, 0, s->stream>>>(p);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+template <typename T> int run_weights(cb200_stream* s, const Product<T>& p) {
+  DeviceGuard guard(s->device);
+  const int tiles_m = (p.M + 63) / 64;
+  expert_weights_simt_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles_m < 65535 ? tiles_m : 65535), (unsigned)p.experts),
+                                  256, 0, s->stream>>>(p, tiles_m);
+  CB_LAUNCH_CHECK(s);
+  if (p.bias_g) {
+    expert_bias_gradient_kernel<T><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 256, 0, s->stream>>>(p);
+    CB_LAUNCH_CHECK(s);
+  }
+  return CB200_OK;
+}
+
+int check_common(const char* what, cb200_stream* s, int dtype, const void* C, const void* A, const void* B, int64_t rows,
+                 int64_t experts, const int32_t* offsets) {
+  CB_REQUIRE(s && C && A && B && offsets, "%s: null argument", what);
+  CB_REQUIRE(dtype == CB200_FLOAT || dtype == CB200_DOUBLE, "%s: only defined for float and double tensors", what);
+  CB_REQUIRE(rows >= 0 && rows <= 2147483647LL, "%s: bad row count", what);
+  CB_REQUIRE(experts >= 1 && experts <= groups::MAX_EXPERTS, "%s: %lld experts outside [1, %d]", what, (long long)experts,
+             (int)groups::MAX_EXPERTS);
+  const uintptr_t size = cb200_dtype_size(dtype);
+  CB_REQUIRE((((uintptr_t)C | (uintptr_t)A | (uintptr_t)B) % size) == 0 && ((uintptr_t)offsets & 3) == 0,
+             "%s: an operand is not aligned to its element type", what);
+  return CB200_OK;
+}
+
+template <typename T>
+Product<T> product(cb200_stream* s, void* C, int64_t c_stride, int64_t ldc, int trans_b, double alpha, const void* A,
+                   int64_t rows, int64_t M, int64_t K, int64_t lda, const void* B, int64_t experts, int64_t N, int64_t b_stride,
+                   int64_t ldb, double beta, const int32_t* offsets, const void* bias, void* bias_g, int act) {
+  Product<T> p;
+  p.C = (T*)C; p.c_stride = c_stride; p.ldc = ldc;
+  p.A = (const T*)A; p.lda = lda;
+  p.B = (const T*)B; p.b_stride = b_stride; p.ldb = ldb;
+  p.trans_b = trans_b != 0; p.act = act;
+  p.rows = (int)rows; p.M = (int)M; p.N = (int)N; p.K = (int)K; p.experts = (int)experts;
+  p.alpha = (T)alpha; p.beta = (T)beta;
+  p.bias = (const T*)bias; p.bias_g = (T*)bias_g;
+  p.offsets = offsets; p.status = s->status_dev;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int trans_b, double alpha, const void* A, int64_t rows,
+                      int64_t a_cols, int64_t lda, const void* B, int64_t experts, int64_t b_cols, int64_t b_stride, int64_t ldb,
+                      double beta, const int32_t* offsets, const void* bias, int act) {
+  int rc = check_common("expert_gemm", s, dtype, C, A, B, rows, experts, offsets);
+  if (rc) return rc;
+  CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= 2147483647LL && b_cols <= 2147483647LL, "expert_gemm: bad extents");
+  CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= (trans_b ? a_cols : b_cols), "expert_gemm: pitch smaller than the row");
+  CB_REQUIRE(b_stride >= (trans_b ? b_cols : a_cols) * ldb || experts == 1, "expert_gemm: the experts' matrices overlap");
+  CB_REQUIRE(act >= CB200_ACT_NONE && act <= CB200_ACT_LOGISTIC, "expert_gemm: unknown activation %d", act);
+  if (rows == 0) return CB200_OK;
+  if (dtype == CB200_FLOAT)
+    return run_rows<float>(s, product<float>(s, C, 0, ldc, trans_b, alpha, A, rows, 0, a_cols, lda, B, experts, b_cols, b_stride,
+                                             ldb, beta, offsets, bias, nullptr, act));
+  return run_rows<double>(s, product<double>(s, C, 0, ldc, trans_b, alpha, A, rows, 0, a_cols, lda, B, experts, b_cols, b_stride,
+                                             ldb, beta, offsets, bias, nullptr, act));
+}
+
+int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_stride, int64_t ldc, double alpha, const void* A,
+                              int64_t rows, int64_t a_cols, int64_t lda, const void* B, int64_t b_cols, int64_t ldb,
+                              int64_t experts, double beta, const int32_t* offsets, void* bias_gradient) {
+  int rc = check_common("expert_gemm_weights", s, dtype, C, A, B, rows, experts, offsets);
+  if (rc) return rc;
+  CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= 2147483647LL && b_cols <= 2147483647LL, "expert_gemm_weights: bad extents");
+  CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= b_cols, "expert_gemm_weights: pitch smaller than the row");
+  CB_REQUIRE(c_stride >= a_cols * ldc || experts == 1, "expert_gemm_weights: the experts' matrices overlap");
+  if (dtype == CB200_FLOAT)
+    return run_weights<float>(s, product<float>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb,
+                                                beta, offsets, nullptr, bias_gradient, CB200_ACT_NONE));
+  return run_weights<double>(s, product<double>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb,
+                                                beta, offsets, nullptr, bias_gradient, CB200_ACT_NONE));
+}
+
+}  // extern "C"

@@ -15,6 +15,9 @@ Backward passes of the dense layers (the next ring around the inference path):
   Convolution.backward                                              compute/nn/layers.clj:320-340
   softmax_loss_gradient      calculate-cross-entropy-gradient       src/cortex/loss/softmax.clj:13-20
 
+Layers without a counterpart in the reference: ExpertLinear (a dense layer per expert over ragged groups of rows) and
+ResidualNormalization (the normalisations around a residual block with its gate and the residual add).
+
 ``fused=True`` replaces the reference's three calls per dense layer
 (assign! bias, gemm! NT beta=1, binary-op! max 0) with the backend's single
 gemm_bias_act entry point; results are the same up to fp32 summation order
@@ -281,6 +284,54 @@ class BatchNormalization:
                                      self._view(output), self._view(input), self.batch_means, self.batch_variances,
                                      self.scale, self.bias, self.epsilon)
         return input_gradient
+
+
+class ExpertLinear:
+    """A dense layer per expert: weights [experts, out, in], bias [experts, out] (or None).  The rows of input and output
+    are sorted by expert; `offsets` is the int device tensor [experts + 1] that says where each expert's rows begin.  No
+    counterpart in the reference: Linear with a choice of weights per row."""
+
+    def __init__(self, weights, bias):
+        self.weights, self.bias = weights, bias
+
+    def forward(self, input, output, offsets, act=None):
+        """output[r] = act(input[r] . W_e^T + b_e): one call; rows outside every group keep what output holds."""
+        return ct.expert_gemm(output, True, 1.0, input, self.weights, 0.0, offsets, bias=self.bias, act=act)
+
+    def backward(self, input, input_gradient, output_gradient, weight_gradient, bias_gradient, offsets):
+        """Gradients ACCUMULATE into weight_gradient / bias_gradient, as in Linear.backward.  input_gradient may be None;
+        so may weight_gradient, and bias_gradient (alone, or with weight_gradient)."""
+        ct._require(bias_gradient is None or weight_gradient is not None, "bias_gradient needs weight_gradient")
+        if input_gradient is not None:
+            ct.expert_gemm(input_gradient, False, 1.0, output_gradient, self.weights, 0.0, offsets)
+        if weight_gradient is not None:
+            ct.expert_gemm_weights(weight_gradient, 1.0, output_gradient, input, 1.0, offsets, bias_gradient=bias_gradient)
+        return input_gradient
+
+
+class ResidualNormalization:
+    """The step between two residual blocks: normalise the block's output (`after`), gate it, add it to the residual stream,
+    and normalise the sum for the next block (`before`).  after / before: (scale, bias or None) or None; gate: a tensor
+    [columns] or [g, columns] or None.  No counterpart in the reference: BatchNormalization per row instead of per column."""
+
+    def __init__(self, after=None, before=None, gate=None, residual_scale=1.0, epsilon=1e-5, kind="rms"):
+        self.after, self.before, self.gate = after, before, gate
+        self.residual_scale, self.epsilon, self.kind = residual_scale, epsilon, kind
+
+    def forward(self, block, residual, total, output):
+        """block None (before the first block): output = N(residual).  Returns [total, output]."""
+        there = block is not None
+        return ct.block_normalize(output, total, block, residual, self.gate if there else None, self.residual_scale,
+                                  self.after if there else None, self.before, self.epsilon, self.kind)
+
+    def backward(self, block, total, output_gradient, total_gradient, block_gradient, residual_gradient, gate_gradient=None,
+                 after_gradients=None, before_gradients=None):
+        """total: what forward wrote (the residual where there was no block).  Gradients are overwritten."""
+        there = block is not None
+        return ct.block_normalize_gradients(
+            block_gradient, residual_gradient, gate_gradient, after_gradients, before_gradients, output_gradient, total_gradient,
+            total, block, self.gate if there else None, self.residual_scale, self.after if there else None, self.before,
+            self.epsilon, self.kind)
 
 
 class ConvNet(_Replayable):

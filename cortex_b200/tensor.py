@@ -15,7 +15,7 @@ import numpy as np
 
 from . import dimensions as dims
 from .dimensions import ALL, DimensionError  # noqa: F401  (re-exported)
-from ._lib import NUMPY_NAME
+from ._lib import DTYPE_SIZE, NORMALIZATIONS, NUMPY_NAME, BlockDesc
 
 class _Bindings(threading.local):
     """ct/*stream* and ct/*datatype* are Clojure dynamic vars: bindings are per thread, which is what lets
@@ -589,6 +589,219 @@ def gemv(c, trans_a, alpha, A, x, beta):
     check_stream().gemv(c.buffer, _blas_vector_increment(c), trans_a, alpha, A.buffer, a_rows, a_cols,
                         _column_stride(A.dimensions), x.buffer, _blas_vector_increment(x), beta)
     return c
+
+
+# ------------------------------ products grouped by expert -----------------------
+# (no counterpart in the reference: gemm! over ragged groups of rows, each with a matrix of its own)
+
+def _matrix(t, name):
+    """(rows, columns, row pitch) of a 2-d tensor whose columns are adjacent in memory."""
+    shp, st = t.dimensions["shape"], t.dimensions["strides"]
+    _require(len(shp) == 2 and type(shp[0]) is int and type(shp[1]) is int, "%s must be a matrix with direct dimensions" % name, t)
+    rows, cols = shp
+    _require(cols == 1 or st[1] == 1, "The columns of %s must be adjacent in memory" % name, t)
+    _require(rows <= 1 or st[0] >= cols, "The rows of %s overlap" % name, t)
+    return rows, cols, st[0] if rows > 1 and st[0] >= cols else cols
+
+
+def _matrices(t, name):
+    """(count, rows, columns, distance, row pitch) of a 3-d tensor of matrices."""
+    shp, st = t.dimensions["shape"], t.dimensions["strides"]
+    _require(len(shp) == 3 and dims.direct_shape(shp), "%s must hold one matrix per expert" % name, t)
+    count, rows, cols = shp
+    _require(cols == 1 or st[2] == 1, "The columns of %s must be adjacent in memory" % name, t)
+    pitch = st[1] if rows > 1 else max(st[1], cols)
+    _require(pitch >= cols and (count == 1 or st[0] >= rows * pitch), "The matrices of %s overlap" % name, t)
+    return count, rows, cols, st[0], pitch
+
+
+def _span(t):
+    """First and one-past-last address of what a tensor with direct dimensions covers."""
+    last = 0
+    for n, st in zip(t.dimensions["shape"], t.dimensions["strides"]):
+        if n == 0:
+            return t.buffer.ptr, t.buffer.ptr
+        last += (n - 1) * st
+    return t.buffer.ptr, t.buffer.ptr + (last + 1) * DTYPE_SIZE[t.buffer.dtype]
+
+
+def _ensure_apart(dest, name, *others):
+    lo, hi = _span(dest)
+    for o in others:
+        if o is not None:
+            a, b = _span(o)
+            _require(hi <= a or b <= lo, "%s overlaps another argument" % name, (dest, o))
+
+
+def _packed(t):
+    """Direct dimensions, row-major, no gaps (extents of one may have any stride)."""
+    expect = 1
+    for n, st in zip(reversed(t.dimensions["shape"]), reversed(t.dimensions["strides"])):
+        if type(n) is not int or (n > 1 and st != expect):
+            return False
+        expect *= n
+    return True
+
+
+def _ensure_dense_vector(t, shape, name):
+    _require(t.dimensions["shape"] == shape and _packed(t), "%s must be a dense tensor of shape %r" % (name, shape), t)
+
+
+def _expert_checks(name, offsets, experts, *tensors):
+    first = tensors[0]
+    _ensure_datatypes(first.get_datatype(), *[t for t in tensors if t is not None])
+    _ensure_same_device(offsets, *[t for t in tensors if t is not None])
+    _require(first.get_datatype() in ("float", "double"), "%s is only defined for float and double tensors" % name)
+    _require(offsets.get_datatype() == "int", "offsets must be an integer tensor", offsets)
+    _ensure_dense_vector(offsets, [experts + 1], "offsets")
+
+
+def expert_gemm(C, trans_b, alpha, A, B, beta, offsets, bias=None, act=None):
+    """C[r, :] = act(alpha * A[r, :] . (trans-b? B_e) + beta * C[r, :] + bias_e) for the rows r of every group e.
+
+    A [rows, k] holds the rows sorted by expert, group e = rows offsets[e] .. offsets[e + 1]; B [experts, n, k] (trans_b: the
+    layout of Linear's weights, [out, in] per expert) or [experts, k, n] (the gradient of the input); offsets [experts + 1]:
+    an int tensor on the device; bias [experts, n]; act None, "relu", "tanh" or "logistic".  Groups may be empty; rows outside
+    every group keep what C holds.  Offsets that decrease or leave the rows make the next sync of the stream raise."""
+    experts, b_rows, b_cols, b_stride, ldb = _matrices(B, "B")
+    _expert_checks("expert-gemm", offsets, experts, C, A, B, bias)
+    rows, k, lda = _matrix(A, "A")
+    c_rows, n, ldc = _matrix(C, "C")
+    inner, outer = (b_cols, b_rows) if trans_b else (b_rows, b_cols)
+    _require(k == inner, "A col count doesn't match B row count", ((rows, k), (inner, outer)))
+    _require(c_rows == rows and n == outer, "C shape doesn't match A rows and B columns", ((c_rows, n), (rows, outer)))
+    _require(act in (None, "none", "relu", "tanh", "logistic"), "expert-gemm activation must be relu, tanh or logistic", act)
+    if bias is not None:
+        _ensure_dense_vector(bias, [experts, n], "bias")
+    _ensure_apart(C, "C", A, B, bias, offsets)
+    check_stream().expert_gemm(C.buffer, ldc, trans_b, alpha, A.buffer, rows, k, lda, B.buffer, experts, n, b_stride, ldb, beta,
+                               offsets.buffer, bias.buffer if bias is not None else None, act)
+    return C
+
+
+def expert_gemm_weights(C, alpha, A, B, beta, offsets, bias_gradient=None):
+    """C_e = alpha * A_e^T B_e + beta * C_e, where A_e, B_e are the rows of group e: the gradient of the experts' weights from
+    the gradient of the output (A [rows, n]) and the input (B [rows, k]); C [experts, n, k].  bias_gradient [experts, n], when
+    given, becomes alpha * (column sums of A_e) + beta * bias_gradient.  offsets as in expert_gemm."""
+    experts, c_rows, c_cols, c_stride, ldc = _matrices(C, "C")
+    _expert_checks("expert-gemm-weights", offsets, experts, C, A, B, bias_gradient)
+    rows, n, lda = _matrix(A, "A")
+    b_rows, k, ldb = _matrix(B, "B")
+    _require(b_rows == rows, "A and B must have the same rows", ((rows, n), (b_rows, k)))
+    _require(c_rows == n and c_cols == k, "C shape doesn't match the columns of A and B", ((c_rows, c_cols), (n, k)))
+    _ensure_apart(C, "C", A, B, bias_gradient, offsets)
+    if bias_gradient is not None:
+        _ensure_dense_vector(bias_gradient, [experts, n], "bias_gradient")
+        _ensure_apart(bias_gradient, "bias_gradient", A, B, offsets)
+    check_stream().expert_gemm_weights(C.buffer, c_stride, ldc, alpha, A.buffer, rows, n, lda, B.buffer, k, ldb, experts, beta,
+                                       offsets.buffer, bias_gradient.buffer if bias_gradient is not None else None)
+    return C
+
+
+# ------------------------------ the normalisations around a residual block --------
+# (no counterpart in the reference, next to its batch and local response normalisation)
+
+def _block_setup(name, matrices, vectors, gate, gate_gradient, residual_scale, epsilon, kind):
+    """Shared checks: returns (datatype, flat (address, pitch) list, addresses of the vectors, descriptor).
+    matrices: name -> tensor or None (the first is there); vectors: name -> tensor or None."""
+    first = next(t for t in matrices.values() if t is not None)
+    datatype = first.get_datatype()
+    there = [t for t in list(matrices.values()) + list(vectors.values()) + [gate, gate_gradient] if t is not None]
+    _require(datatype in ("float", "double"), "%s is only defined for float and double tensors" % name, datatype)
+    _ensure_datatypes(datatype, *there)
+    _ensure_same_device(*there)
+    _require(kind in NORMALIZATIONS, "unknown normalisation", kind)
+    _require(epsilon > 0, "Epsilon must be positive", epsilon)
+    rows, cols, _ = _matrix(first, "input")
+    flat = []
+    for label, t in matrices.items():
+        if t is None:
+            flat += [None, 0]
+        else:
+            r, c, pitch = _matrix(t, label)
+            _require(r == rows and c == cols, "Tensor shapes do not match", {label: (r, c), "expected": (rows, cols)})
+            flat += [t.buffer.ptr, pitch]
+    for label, t in vectors.items():
+        if t is not None:
+            _ensure_dense_vector(t, [cols], label)
+    gate_rows = 1
+    if gate is not None:
+        shp = gate.dimensions["shape"]
+        _require(_packed(gate) and shp[-1] == cols and len(shp) <= 2, "gate must be a dense tensor of columns or rows of columns", gate)
+        gate_rows = shp[0] if len(shp) == 2 else 1
+        _require(gate_rows >= 1 and rows % gate_rows == 0, "The rows of the gate must divide the rows of the batch", (gate_rows, rows))
+    if gate_gradient is not None:
+        _require(gate is not None and _packed(gate_gradient) and gate_gradient.dimensions["shape"] == gate.dimensions["shape"],
+                 "gate_gradient must be a dense tensor of the gate's shape", gate_gradient)
+    desc = BlockDesc(NORMALIZATIONS[kind], float(epsilon), float(residual_scale), rows, cols, gate_rows)
+    return datatype, flat, [t.buffer.ptr if t is not None else None for t in vectors.values()], desc
+
+
+def _address(t):
+    return t.buffer.ptr if t is not None else None
+
+
+def block_normalize(output, total, block, residual, gate, residual_scale, after, before, epsilon, kind="rms"):
+    """The step from one residual block to the next, in one pass over the rows:
+
+        u = N(block) * after-scale + after-bias;  total = residual + residual_scale * gate * u;
+        output = N(total) * before-scale + before-bias
+
+    N normalises each row: "rms" by the root of its mean square, "layer" by mean and standard deviation.  after / before:
+    (scale, bias or None), or None for no such normalisation (then u = block; output must be None).  gate: None, [columns], or
+    [g, columns] where g divides the rows (row r uses gate row r * g / rows: one per sample, or one per row).  block None:
+    total is residual (total may be None then).  total and output may be written over residual or block, not over each other.
+    Returns [total, output]."""
+    a_scale, a_bias = after if after is not None else (None, None)
+    b_scale, b_bias = before if before is not None else (None, None)
+    _require(residual is not None, "A residual is needed")
+    _require((output is not None) == (b_scale is not None), "output and the normalisation before the next block go together")
+    _require(output is not None or total is not None, "Neither output nor total is wanted")
+    _require(block is None or total is not None, "A block needs a total to be added into")
+    _require(block is not None or (gate is None and a_scale is None), "gate and after-normalisation belong to a block")
+    datatype, flat, _, desc = _block_setup(
+        "block-normalize", {"residual": residual, "output": output, "total": total, "block": block},
+        {"after scale": a_scale, "after bias": a_bias, "before scale": b_scale, "before bias": b_bias}, gate, None,
+        residual_scale, epsilon, kind)
+    check_stream().block_normalize(datatype, flat[2:] + flat[:2],
+                                   [_address(t) for t in (gate, a_scale, a_bias, b_scale, b_bias)], desc)
+    return [total, output]
+
+
+def block_normalize_gradients(block_gradient, residual_gradient, gate_gradient, after_gradients, before_gradients,
+                              output_gradient, total_gradient, total, block, gate, residual_scale, after, before, epsilon,
+                              kind="rms"):
+    """Gradients of block_normalize, given the total it wrote (the residual itself where there was no block) and its block.
+    output_gradient: of its output (None without `before`); total_gradient: what reaches the sum by the residual path, or
+    None.  after_gradients / before_gradients: (scale gradient, bias gradient), any of them None, or None.  Everything is
+    overwritten; gate, scale and bias gradients are summed over the rows that share them.  residual_gradient may be
+    total_gradient itself.  Returns [block_gradient, residual_gradient]."""
+    a_scale, a_bias = after if after is not None else (None, None)
+    b_scale, _b_bias = before if before is not None else (None, None)
+    ga_scale, ga_bias = after_gradients if after_gradients is not None else (None, None)
+    gb_scale, gb_bias = before_gradients if before_gradients is not None else (None, None)
+    _require(residual_gradient is not None, "A residual_gradient is needed")
+    _require((output_gradient is not None) == (b_scale is not None), "output_gradient and the normalisation before the next block go together")
+    _require(output_gradient is not None or total_gradient is not None, "No gradient arrives")
+    _require(b_scale is None or total is not None, "The normalisation before the next block needs the total")
+    _require((block is None) == (block_gradient is None), "block and block_gradient go together")
+    _require(block is not None or (gate is None and a_scale is None), "gate and after-normalisation belong to a block")
+    _require(a_scale is not None or (ga_scale is None and ga_bias is None), "after_gradients without an after-normalisation")
+    _require(b_scale is not None or (gb_scale is None and gb_bias is None), "before_gradients without a before-normalisation")
+    matrices = {"residual_gradient": residual_gradient, "block_gradient": block_gradient, "output_gradient": output_gradient,
+                "total_gradient": total_gradient, "total": total, "block": block}
+    vectors = {"after scale": a_scale, "after bias": a_bias, "before scale": b_scale, "after scale gradient": ga_scale,
+               "after bias gradient": ga_bias, "before scale gradient": gb_scale, "before bias gradient": gb_bias}
+    datatype, flat, _, desc = _block_setup("block-normalize-gradients", matrices, vectors, gate, gate_gradient, residual_scale,
+                                           epsilon, kind)
+    sums = [t for t in (ga_scale, ga_bias, gb_scale, gb_bias) if t is not None]
+    operands = [output_gradient, total_gradient, total, block, gate, a_scale, a_bias, b_scale]
+    for i, t in enumerate(sums):
+        _ensure_apart(t, "A gradient", block_gradient, residual_gradient, gate_gradient, *sums[i + 1:], *operands)
+    check_stream().block_normalize_gradients(
+        datatype, flat[2:4] + flat[:2], [_address(t) for t in (gate_gradient, ga_scale, ga_bias, gb_scale, gb_bias)], flat[4:],
+        [_address(t) for t in (gate, a_scale, a_bias, b_scale)], desc)
+    return [block_gradient, residual_gradient]
 
 
 def _batch_normalize_setup(io_args, stat_args, epsilon):

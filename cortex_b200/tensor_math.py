@@ -166,6 +166,46 @@ class CTensorMath:
         self._tm("bias_relu_rowstats", DTYPE_CODE[y.dtype], y.ptr, int(ldy), x.ptr, int(ldx), bias.ptr, int(rows),
                  int(cols), rowmax.ptr if rowmax is not None else None, rowsum.ptr if rowsum is not None else None)
 
+    def expert_gemm(self, c, ldc, trans_b, alpha, a, rows, a_cols, lda, b, experts, b_cols, b_stride, ldb, beta, offsets,
+                    bias, act):
+        """C[r] = act(alpha * A[r] . op(B_e) + beta * C[r] + bias_e) for the rows r of every group e."""
+        self._tm("expert_gemm", DTYPE_CODE[c.dtype], c.ptr, ldc, 1 if trans_b else 0, float(alpha), a.ptr, rows, a_cols, lda,
+                 b.ptr, experts, b_cols, b_stride, ldb, float(beta), offsets.ptr, bias.ptr if bias is not None else None,
+                 ACTIVATIONS[act])
+
+    def expert_gemm_weights(self, c, c_stride, ldc, alpha, a, rows, a_cols, lda, b, b_cols, ldb, experts, beta, offsets,
+                            bias_gradient):
+        """C_e = alpha * A_e^T B_e + beta * C_e over the rows of every group e (and the column sums of A_e)."""
+        self._tm("expert_gemm_weights", DTYPE_CODE[c.dtype], c.ptr, c_stride, ldc, float(alpha), a.ptr, rows, a_cols, lda,
+                 b.ptr, b_cols, ldb, experts, float(beta), offsets.ptr,
+                 bias_gradient.ptr if bias_gradient is not None else None)
+
+    def block_normalize(self, dtype, matrices, vectors, desc):
+        """matrices: (address, pitch) of output, total, block, residual; vectors: addresses of gate, after scale / bias,
+        before scale / bias (None = not there); desc: a BlockDesc."""
+        self._tm("block_normalize", DTYPE_CODE[dtype], *matrices, *vectors, C.byref(desc))
+
+    def block_normalize_gradients(self, dtype, gradients, vector_gradients, matrices, vectors, desc):
+        """gradients: (address, pitch) of block and residual gradients; vector_gradients: gate, after scale / bias, before
+        scale / bias; matrices: output_gradient, total_gradient, total, block; vectors: gate, after scale / bias, before
+        scale."""
+        self._tm("block_normalize_gradients", DTYPE_CODE[dtype], *gradients, *vector_gradients, *matrices, *vectors,
+                 C.byref(desc))
+
+    @staticmethod
+    def _pointer_list(buffers):
+        return (C.c_void_p * len(buffers))(*[b.ptr for b in buffers])
+
+    def global_norm(self, dtype, gradients, counts, norm):
+        """norm[0] = sqrt(sum of squares over all buffers)."""
+        n = len(gradients)
+        self._tm("global_norm", DTYPE_CODE[dtype], n, self._pointer_list(gradients), (C.c_int64 * n)(*counts), norm.ptr)
+
+    def clip_gradients(self, dtype, gradients, counts, clipped, max_norm, norm):
+        n = len(gradients)
+        self._tm("clip_gradients", DTYPE_CODE[dtype], n, self._pointer_list(gradients), (C.c_int64 * n)(*counts),
+                 self._pointer_list(clipped), float(max_norm), norm.ptr if norm is not None else None)
+
     def _tm_nostream(self, name, *args):
         from ._lib import call
         return call("cb200_" + name, *args)

@@ -417,6 +417,68 @@ int cb200_graph_capture_end(cb200_stream* s, cb200_graph** out);
 int cb200_graph_launch(cb200_graph* g, cb200_stream* s);
 int cb200_graph_destroy(cb200_graph* g);
 
+/* ---- experts, residual blocks and gradient clipping (no counterpart in the protocol) -----------------------------------
+ * Products grouped by expert.  Group e is rows offsets[e] .. offsets[e + 1] of A (offsets: experts + 1 non-decreasing
+ * int32 values in DEVICE memory, at most `rows`); groups may be empty, and rows outside every group are left as they are.
+ *   expert_gemm:          C[r, :] = act(alpha * A[r, :] . op(B_e) + beta * C[r, :] + bias[e, :])    r in group e
+ *     A [rows, a_cols] pitch lda; C [rows, b_cols] pitch ldc; B_e = B + e * b_stride, [b_cols, a_cols] (trans_b: the :linear
+ *     layout, weights [out, in]) or [a_cols, b_cols], pitch ldb; bias [experts, b_cols] dense or NULL; act: no softmax.
+ *     trans_b = 0 is the gradient of the input.
+ *   expert_gemm_weights:  C_e = alpha * sum_{r in group e} A[r, :]^T B[r, :] + beta * C_e   (C_e [a_cols, b_cols])
+ *     and, where bias_gradient is not NULL, bias_gradient[e, :] = alpha * sum_{r in group e} A[r, :] + beta * bias_gradient[e, :]
+ *     A is the gradient of the layer's output, B its input.  Empty groups: beta * C_e.
+ * float / double, at most 4096 experts; with beta = 0 what C held is not read.  C must not overlap the other operands.
+ * Offsets that decrease or leave [0, rows] are clamped on the device (nothing outside the operands is touched, rows are
+ * never computed twice) and the call is reported as CB200_ERR_CUDA by the next cb200_stream_sync.  fp32 operands are
+ * multiplied on the tensor cores with the split arithmetic of gemm!. */
+int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int trans_b, double alpha, const void* A,
+                      int64_t rows, int64_t a_cols, int64_t lda, const void* B, int64_t experts, int64_t b_cols,
+                      int64_t b_stride, int64_t ldb, double beta, const int32_t* offsets, const void* bias, int act);
+int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_stride, int64_t ldc, double alpha,
+                              const void* A, int64_t rows, int64_t a_cols, int64_t lda, const void* B, int64_t b_cols,
+                              int64_t ldb, int64_t experts, double beta, const int32_t* offsets, void* bias_gradient);
+
+/* The normalisations around a residual block with its gate and the residual add, per row of cols values.
+ * N(x) = x / sqrt(mean(x^2) + epsilon) (kind 0, rms) or (x - mean(x)) / sqrt(mean((x - mean(x))^2) + epsilon) (kind 1, layer):
+ *   u      = N(block) * after_scale + after_bias      (u = block where after_scale is NULL)
+ *   total  = residual + residual_scale * gate * u     (total = residual where block is NULL)
+ *   output = N(total) * before_scale + before_bias    (no output where before_scale is NULL)
+ * Matrices are [rows, cols] with a pitch each; the scales and biases [cols], biases may be NULL; gate [gate_rows, cols]
+ * dense or NULL (1), gate_rows divides rows and gate row g serves rows g * rows / gate_rows and on: 1 = one learned gate per
+ * column, a row per sample, or one value per element.  total may be NULL without a block.  total or output may be written over
+ * residual or block (the same matrix, same pitch), never over each other.
+ * The gradients take the forward call's total and block, output_gradient (with before_scale) and / or total_gradient (what
+ * reaches the sum by the residual path), and overwrite (not accumulate): residual_gradient, block_gradient, gate_gradient
+ * (summed over the rows that share a gate row), and the column sums of the scales and biases; NULL = not wanted, except
+ * residual_gradient, and block_gradient where there is a block.  residual_gradient may be total_gradient itself; otherwise
+ * gradients share no memory with operands.  float / double; statistics and sums in the element type, in a fixed order. */
+typedef struct cb200_block_desc {
+  int32_t kind;
+  double epsilon, residual_scale;
+  int64_t rows, cols, gate_rows;
+} cb200_block_desc;
+int cb200_block_normalize(cb200_stream* s, int dtype, void* output, int64_t ld_output, void* total, int64_t ld_total,
+                          const void* block, int64_t ld_block, const void* residual, int64_t ld_residual,
+                          const void* gate, const void* after_scale, const void* after_bias, const void* before_scale,
+                          const void* before_bias, const cb200_block_desc* desc);
+int cb200_block_normalize_gradients(cb200_stream* s, int dtype, void* block_gradient, int64_t ld_block_gradient,
+                                    void* residual_gradient, int64_t ld_residual_gradient, void* gate_gradient,
+                                    void* after_scale_gradient, void* after_bias_gradient, void* before_scale_gradient,
+                                    void* before_bias_gradient, const void* output_gradient, int64_t ld_output_gradient,
+                                    const void* total_gradient, int64_t ld_total_gradient, const void* total,
+                                    int64_t ld_total, const void* block, int64_t ld_block, const void* gate,
+                                    const void* after_scale, const void* after_bias, const void* before_scale,
+                                    const cb200_block_desc* desc);
+
+/* The global norm over a list of gradient buffers (n host arrays of device addresses and element counts):
+ *   norm = sqrt(sum of all squares), written to the device element `norm` of the buffers' type;
+ *   clip_gradients: clipped[i] = gradients[i] * max_norm / norm where norm > max_norm, otherwise (also when the norm is not
+ *   finite) clipped[i] = gradients[i].  clipped[i] may be gradients[i] itself; norm may be NULL here.
+ * Squares are summed in double and in a fixed order (same bits on every run).  The lists are read before the call returns. */
+int cb200_global_norm(cb200_stream* s, int dtype, int n, const void* const* gradients, const int64_t* counts, void* norm);
+int cb200_clip_gradients(cb200_stream* s, int dtype, int n, const void* const* gradients, const int64_t* counts,
+                         void* const* clipped, double max_norm, void* norm);
+
 /* ---- multi-GPU extras (no counterpart: the reference has no multi-device code, README.md:48) ----
  * The same fused GEMM whose epilogue ALSO stores every finished tile of the C window to the same
  * row-major position (row*ldc + column from the given base) of up to 7 more buffers, typically the

@@ -20,6 +20,7 @@ import subprocess
 
 import numpy as np
 
+from . import plain_operators
 from cortex_b200._lib import DTYPE_CODE, DTYPE_SIZE, NUMPY_NAME, ConvDesc, Dims
 from cortex_b200.driver import Buffer
 from cortex_b200.tensor_math import CTensorMath
@@ -266,6 +267,79 @@ class OracleStream(CTensorMath):
             Cm[...] = dt(alpha) * prod
         else:
             Cm[...] = dt(alpha) * prod + dt(beta) * Cm
+
+    # -- operators without a counterpart in the reference (oracle/plain_operators.py) -------------------------
+    @staticmethod
+    def _view(ptr, dtype, shape, strides):
+        """numpy view (strides in elements) of host memory; None for a null address."""
+        if ptr is None or 0 in shape:
+            return None if ptr is None else np.zeros(shape, NUMPY_NAME[dtype])
+        n = 1 + sum((e - 1) * s for e, s in zip(shape, strides))
+        flat = np.frombuffer((C.c_char * (n * DTYPE_SIZE[dtype])).from_address(ptr), dtype=NUMPY_NAME[dtype])
+        return np.lib.stride_tricks.as_strided(flat, shape=shape, strides=[s * flat.itemsize for s in strides])
+
+    def expert_gemm(self, c, ldc, trans_b, alpha, a, rows, a_cols, lda, b, experts, b_cols, b_stride, ldb, beta, offsets,
+                    bias, act):
+        dt, view = c.dtype, self._view
+        out = view(c.ptr, dt, (rows, b_cols), (ldc, 1))
+        inner = (b_cols, a_cols) if trans_b else (a_cols, b_cols)
+        out[...] = plain_operators.expert_gemm(
+            out, trans_b, alpha, view(a.ptr, dt, (rows, a_cols), (lda, 1)), view(b.ptr, dt, (experts,) + inner, (b_stride, ldb, 1)),
+            beta, view(offsets.ptr, "int", (experts + 1,), (1,)),
+            None if bias is None else view(bias.ptr, dt, (experts, b_cols), (b_cols, 1)), act)[0]
+
+    def expert_gemm_weights(self, c, c_stride, ldc, alpha, a, rows, a_cols, lda, b, b_cols, ldb, experts, beta, offsets,
+                            bias_gradient):
+        dt, view = c.dtype, self._view
+        out = view(c.ptr, dt, (experts, a_cols, b_cols), (c_stride, ldc, 1))
+        bg = None if bias_gradient is None else view(bias_gradient.ptr, dt, (experts, a_cols), (a_cols, 1))
+        w, _, bias, _ = plain_operators.expert_gemm_weights(
+            out, alpha, view(a.ptr, dt, (rows, a_cols), (lda, 1)), view(b.ptr, dt, (rows, b_cols), (ldb, 1)), beta,
+            view(offsets.ptr, "int", (experts + 1,), (1,)), bg)
+        out[...] = w
+        if bg is not None:
+            bg[...] = bias
+
+    def _block_views(self, dtype, desc, matrices, vectors):
+        m = [self._view(p, dtype, (desc.rows, desc.cols), (ld, 1)) for p, ld in zip(matrices[::2], matrices[1::2])]
+        v = [self._view(vectors[0], dtype, (desc.gate_rows, desc.cols), (desc.cols, 1))]
+        return m, v + [self._view(p, dtype, (desc.cols,), (1,)) for p in vectors[1:]]
+
+    def block_normalize(self, dtype, matrices, vectors, desc):
+        (out, total, block, residual), (gate, aw, ab, bw, bb) = self._block_views(dtype, desc, matrices, vectors)
+        t, _, y, _ = plain_operators.block_normalize(
+            block, residual, gate, desc.residual_scale, None if aw is None else (aw, ab), None if bw is None else (bw, bb),
+            desc.epsilon, "layer" if desc.kind else "rms")
+        if total is not None:
+            total[...] = t
+        if out is not None:
+            out[...] = y
+
+    def block_normalize_gradients(self, dtype, gradients, vector_gradients, matrices, vectors, desc):
+        (dy, dt, total, block), (gate, aw, ab, bw) = self._block_views(dtype, desc, matrices, vectors)
+        (bg, rg), (gg, gaw, gab, gbw, gbb) = self._block_views(dtype, desc, gradients, vector_gradients)
+        got = plain_operators.block_normalize_gradients(
+            dy, dt, total, block, gate, desc.residual_scale, None if aw is None else (aw, ab), None if bw is None else (bw, None),
+            desc.epsilon, "layer" if desc.kind else "rms")
+        for name, to in (("block", bg), ("residual", rg), ("gate", gg), ("after", gaw), ("after_b", gab), ("before", gbw),
+                         ("before_b", gbb)):
+            if to is not None:
+                to[...] = got[name][0]
+
+    def _flat(self, buffer, n):
+        return self._view(buffer.ptr, buffer.dtype, (n,), (1,))
+
+    def global_norm(self, dtype, gradients, counts, norm):
+        self._flat(norm, 1)[0] = plain_operators.global_norm([self._flat(g, n) for g, n in zip(gradients, counts)])
+
+    def clip_gradients(self, dtype, gradients, counts, clipped, max_norm, norm):
+        values = [self._flat(g, n) for g, n in zip(gradients, counts)]
+        n = plain_operators.global_norm(values)
+        scale = plain_operators.clip_scale(n, max_norm)
+        for g, c, k in zip(values, clipped, counts):
+            self._flat(c, k)[...] = g.astype(np.float64) * scale
+        if norm is not None:
+            self._flat(norm, 1)[0] = n
 
     def choose_convolution_algorithms(self, conv_descriptor, input_width, input_height, output_width, output_height,
                                       batch_size, max_ideal_workspace_size, use_defaults):
