@@ -9,6 +9,14 @@
 #include "expert_groups.cuh"
 #include <math.h>
 
+bool cb200_expert_tc_ok(const void* A, long long lda, const void* B, long long ldb, long long b_stride);
+int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
+                         long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
+                         const int* offsets, const float* bias, int act);
+int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
+                            int M, long long lda, const float* B, int N, long long ldb, int experts, float beta,
+                            const int* offsets);
+
 namespace {
 
 static __device__ __noinline__ double act_transcendental(double v, int act) {
@@ -185,6 +193,83 @@ template <typename T> int run_weights(cb200_stream* s, const Product<T>& p) {
   return CB200_OK;
 }
 
+// ---- fp32: the tensor-core kernels, behind a copy of operands that TMA cannot address -----------------------------------
+__global__ void __launch_bounds__(256) pack_rows_kernel(float* dst, long long ld_dst, const float* src, long long ld, long long stride,
+                                                        long long rows_per, long long rows, int cols) {
+  const long long total = rows * ld_dst;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long r = i / ld_dst;
+    const int c = (int)(i - r * ld_dst);
+    if (c < cols) dst[i] = src[(r / rows_per) * stride + (r % rows_per) * ld + c];
+  }
+}
+
+// rows x cols (rows_per of them per matrix, matrices `stride` apart) into dense rows of a multiple of 4
+int pack(cb200_stream* s, float* dst, const float* src, long long ld, long long stride, long long rows_per, long long rows, int cols) {
+  const long long ld_dst = (cols + 3) / 4 * 4;
+  long long blocks = (rows * ld_dst + 1023) / 1024;
+  const long long cap = (long long)s->sm_count * 16;
+  if (blocks > cap) blocks = cap;
+  pack_rows_kernel<<<(unsigned)blocks, 256, 0, s->stream>>>(dst, ld_dst, src, ld, stride, rows_per, rows, cols);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+int rows_tc(cb200_stream* s, Product<float> p) {
+  const long long b_rows = p.trans_b ? p.N : p.K;
+  const int b_cols = p.trans_b ? p.K : p.N;
+  if (p.experts == 1) p.b_stride = b_rows * p.ldb;
+  const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, p.b_stride);
+  if (pack_a || pack_b) {
+    DeviceGuard guard(s->device);
+    const long long lda = (p.K + 3) / 4 * 4, ldb = (b_cols + 3) / 4 * 4;
+    const size_t a_n = pack_a ? (size_t)p.rows * lda : 0, b_n = pack_b ? (size_t)p.experts * b_rows * ldb : 0;
+    void* ws = nullptr;
+    int rc = cb200_scratch(s, (a_n + b_n) * sizeof(float), &ws);
+    if (rc) return rc;
+    float* a = (float*)ws;
+    float* b = a + a_n;
+    if (pack_a) {
+      if ((rc = pack(s, a, p.A, p.lda, 0, p.rows, p.rows, p.K))) return rc;
+      p.A = a; p.lda = lda;
+    }
+    if (pack_b) {
+      if ((rc = pack(s, b, p.B, p.ldb, p.b_stride, b_rows, p.experts * b_rows, b_cols))) return rc;
+      p.B = b; p.ldb = ldb; p.b_stride = b_rows * ldb;
+    }
+  }
+  return cb200_expert_rows_tc(s, p.C, p.ldc, p.trans_b, p.alpha, p.A, p.rows, p.K, p.lda, p.B, p.experts, p.N, p.b_stride, p.ldb,
+                              p.beta, p.offsets, p.bias, p.act);
+}
+
+int weights_tc(cb200_stream* s, Product<float> p) {
+  if (p.bias_g) {
+    DeviceGuard guard(s->device);
+    expert_bias_gradient_kernel<float><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 256, 0, s->stream>>>(p);
+    CB_LAUNCH_CHECK(s);
+  }
+  const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
+  if (pack_a || pack_b) {
+    DeviceGuard guard(s->device);
+    const long long lda = (p.M + 3) / 4 * 4, ldb = (p.N + 3) / 4 * 4;
+    const size_t a_n = pack_a ? (size_t)p.rows * lda : 0, b_n = pack_b ? (size_t)p.rows * ldb : 0;
+    void* ws = nullptr;
+    int rc = cb200_scratch(s, (a_n + b_n) * sizeof(float), &ws);
+    if (rc) return rc;
+    float* a = (float*)ws;
+    float* b = a + a_n;
+    if (pack_a) {
+      if ((rc = pack(s, a, p.A, p.lda, 0, p.rows, p.rows, p.M))) return rc;
+      p.A = a; p.lda = lda;
+    }
+    if (pack_b) {
+      if ((rc = pack(s, b, p.B, p.ldb, 0, p.rows, p.rows, p.N))) return rc;
+      p.B = b; p.ldb = ldb;
+    }
+  }
+  return cb200_expert_weights_tc(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta, p.offsets);
+}
+
 int check_common(const char* what, cb200_stream* s, int dtype, const void* C, const void* A, const void* B, int64_t rows,
                  int64_t experts, const int32_t* offsets) {
   CB_REQUIRE(s && C && A && B && offsets, "%s: null argument", what);
@@ -229,8 +314,8 @@ int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int tran
   CB_REQUIRE(act >= CB200_ACT_NONE && act <= CB200_ACT_LOGISTIC, "expert_gemm: unknown activation %d", act);
   if (rows == 0) return CB200_OK;
   if (dtype == CB200_FLOAT)
-    return run_rows<float>(s, product<float>(s, C, 0, ldc, trans_b, alpha, A, rows, 0, a_cols, lda, B, experts, b_cols, b_stride,
-                                             ldb, beta, offsets, bias, nullptr, act));
+    return rows_tc(s, product<float>(s, C, 0, ldc, trans_b, alpha, A, rows, 0, a_cols, lda, B, experts, b_cols, b_stride,
+                                     ldb, beta, offsets, bias, nullptr, act));
   return run_rows<double>(s, product<double>(s, C, 0, ldc, trans_b, alpha, A, rows, 0, a_cols, lda, B, experts, b_cols, b_stride,
                                              ldb, beta, offsets, bias, nullptr, act));
 }
@@ -243,9 +328,11 @@ int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_str
   CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= 2147483647LL && b_cols <= 2147483647LL, "expert_gemm_weights: bad extents");
   CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= b_cols, "expert_gemm_weights: pitch smaller than the row");
   CB_REQUIRE(c_stride >= a_cols * ldc || experts == 1, "expert_gemm_weights: the experts' matrices overlap");
-  if (dtype == CB200_FLOAT)
-    return run_weights<float>(s, product<float>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb,
-                                                beta, offsets, nullptr, bias_gradient, CB200_ACT_NONE));
+  if (dtype == CB200_FLOAT) {
+    const Product<float> p = product<float>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb, beta,
+                                            offsets, nullptr, bias_gradient, CB200_ACT_NONE);
+    return rows > 0 ? weights_tc(s, p) : run_weights<float>(s, p);
+  }
   return run_weights<double>(s, product<double>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb,
                                                 beta, offsets, nullptr, bias_gradient, CB200_ACT_NONE));
 }

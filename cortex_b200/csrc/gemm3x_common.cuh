@@ -97,6 +97,12 @@ __device__ __forceinline__ float4 ld_c4(const float* p, bool partial) {
   return partial ? __ldcg(reinterpret_cast<const float4*>(p)) : *reinterpret_cast<const float4*>(p);
 }
 
+// Four bias values; the bias may be a view that starts anywhere in its buffer.
+__device__ __forceinline__ float4 ld_bias4(const float* p) {
+  if (((uintptr_t)p & 15) == 0) return *reinterpret_cast<const float4*>(p);
+  return make_float4(p[0], p[1], p[2], p[3]);
+}
+
 // Park this CTA's raw accumulators (main + cross terms) for the CTA that combines the K slices of the tile.
 // A parked tile is BN / 4 column groups of [128 rows] float4: the 32 lanes of a warp (32 consecutive rows)
 // write and read 512 contiguous bytes per instruction.
@@ -123,6 +129,32 @@ __device__ __forceinline__ void dump_tile(const GemmParams& p, uint32_t tmem_bas
     for (int j = 0; j < 32; j += 4)
       __stcg(slot + ((col0 + j) >> 2) * 128, make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]),
                                                          __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])));
+  }
+}
+
+// Round this CTA's accumulators to nearest onto a tile that dump_tile parked earlier (the same thread's values).
+template <int BN>
+__device__ __forceinline__ void add_tile(uint32_t tmem_base, float* dst, int warp, int lane) {
+  const int q = warp & 3, half = warp >> 2;
+  constexpr int COLS_PER_HALF = BN / 2;
+  float4* slot = reinterpret_cast<float4*>(dst) + (q * 32 + lane);
+#pragma unroll 1
+  for (int cc = 0; cc < COLS_PER_HALF / 32; ++cc) {
+    const int col0 = half * COLS_PER_HALF + cc * 32;
+    uint32_t r[32], rc[32];
+    tmem_ld_32x32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)col0, r);
+    tmem_ld_32x32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(BN + col0), rc);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      float4* to = slot + ((col0 + j) >> 2) * 128;
+      float4 v = __ldcg(to);
+      v.x += __uint_as_float(r[j]) + __uint_as_float(rc[j]);
+      v.y += __uint_as_float(r[j + 1]) + __uint_as_float(rc[j + 1]);
+      v.z += __uint_as_float(r[j + 2]) + __uint_as_float(rc[j + 2]);
+      v.w += __uint_as_float(r[j + 3]) + __uint_as_float(rc[j + 3]);
+      __stcg(to, v);
+    }
   }
 }
 
@@ -312,7 +344,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tmem
             o.x = __uint_as_float(r[k4 * 4 + 0]); o.y = __uint_as_float(r[k4 * 4 + 1]);
             o.z = __uint_as_float(r[k4 * 4 + 2]); o.w = __uint_as_float(r[k4 * 4 + 3]);
             if (e_bias) {
-              const float4 b = *reinterpret_cast<const float4*>(e_bias + nb + k4 * 4);
+              const float4 b = ld_bias4(e_bias + nb + k4 * 4);
               o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
             }
             if (e_act) { o.x = apply_act(o.x, e_act); o.y = apply_act(o.y, e_act); o.z = apply_act(o.z, e_act); o.w = apply_act(o.w, e_act); }
@@ -415,7 +447,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tmem
                   o.x += beta_now * c.x; o.y += beta_now * c.y; o.z += beta_now * c.z; o.w += beta_now * c.w;
                 }
                 if (e_bias) {
-                  float4 b = *reinterpret_cast<const float4*>(e_bias + nb + j);
+                  const float4 b = ld_bias4(e_bias + nb + j);
                   o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
                 }
                 if (e_act) { o.x = apply_act(o.x, e_act); o.y = apply_act(o.y, e_act); o.z = apply_act(o.z, e_act); o.w = apply_act(o.w, e_act); }

@@ -515,3 +515,41 @@ def test_expert_layers_backward_accumulates(stream):
         want, size, bias, bias_size = plain.expert_gemm_weights(np.zeros_like(w), times, dy, x, 0.0, off, np.zeros_like(b))
         _within(ct.to_array(wg), want, size, _product_tol("float", 18) + 2 * U["float"], "weights")
         _within(ct.to_array(bg), bias, bias_size, 32 * U["float"], "bias")
+
+
+@pytest.mark.parametrize("tile_n", [64, 128, 256])
+@pytest.mark.parametrize("slices", [1, 2, 8])
+def test_expert_gemm_tile_widths_slices_and_long_reductions(stream, tile_n, slices):
+    """Every tile width and slice count (chosen by size otherwise), reductions that are cut into several roundings."""
+    rng = np.random.default_rng(61)
+    stream.set_option("gemm-tile-n", tile_n)
+    stream.set_option("gemm-k-slices", slices)
+    sizes, n, k = [127, 129, 3, 0, 30], 264, 4500
+    rows = sum(sizes) + 2
+    off = ct.to_tensor(_offsets(sizes), "int")
+    X, W, b = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (5, n, k), (5, n)))
+    Xt, Wt, Y = ct.to_tensor(X, "float"), ct.to_tensor(W, "float"), ct.new_tensor([rows, n], "float")
+    ct.expert_gemm(Y, True, 0.5, Xt, Wt, 0.0, off, bias=ct.to_tensor(b, "float"), act="logistic")
+    want, size = plain.expert_gemm(np.zeros((rows, n)), True, 0.5, X, W, 0.0, _offsets(sizes), b, "logistic")
+    _within(ct.to_array(Y), want, size + 8 * U["float"] / _product_tol("float", k), _product_tol("float", k), "forward")
+    sizes, n, k = [4700, 0, 300, 17], 136, 265
+    rows = sum(sizes) + 5
+    off = ct.to_tensor(_offsets(sizes), "int")
+    dY, X, C0 = (rng.standard_normal(s).astype(np.float32) for s in ((rows, n), (rows, k), (4, n, k)))
+    Ct = ct.to_tensor(C0, "float")
+    ct.expert_gemm_weights(Ct, 1.0, ct.to_tensor(dY, "float"), ct.to_tensor(X, "float"), 1.0, off)
+    want, size, _, _ = plain.expert_gemm_weights(C0, 1.0, dY, X, 1.0, _offsets(sizes))
+    _within(ct.to_array(Ct), want, size, _product_tol("float", 4700), "weights")
+
+
+def test_bias_of_a_layer_may_start_anywhere(stream):
+    """A bias that is a view at an odd offset of its buffer, in a layer with an even row pitch."""
+    rng = np.random.default_rng(67)
+    X, W, flat = (rng.standard_normal(s).astype(np.float32) for s in ((40, 64), (36, 64), 64))
+    layer_bias = ct.to_tensor(flat, "float")
+    for at in (1, 2, 3):
+        bias = ct.Tensor(layer_bias.device, {"shape": [36], "strides": [1]}, layer_bias.buffer.sub_buffer(at, 36))
+        Y = ct.new_tensor([40, 36], "float")
+        nn.Linear(ct.to_tensor(W, "float"), bias).forward_fused(ct.to_tensor(X, "float"), Y, "relu")
+        want, size = plain.expert_gemm(np.zeros((40, 36)), True, 1.0, X, W[None], 0.0, [0, 40], flat[None, at:at + 36], "relu")
+        _within(ct.to_array(Y), want, size, _product_tol("float", 64), at)
