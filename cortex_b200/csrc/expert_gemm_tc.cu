@@ -2,12 +2,11 @@
 // which the tensor core reads the top 19 bits, lo = x - trunc(x); main and cross terms in two TMEM accumulators) over
 // ragged groups whose bounds are read from device memory.
 //
-//   WEIGHTS = 0   128 x BN tile of C[rows, N]: rows of one group, that group's matrix as the B operand.  A tile that ends
-//                 behind its group loads rows of the next one (rows of an accumulator are independent) and does not store
-//                 them.  B is a 3-d tensor map, so a tile that ends behind its expert's matrix reads zeros.
-//   WEIGHTS = 1   128 x BN tile of C_e [M, N] = A_e^T B_e: the reduction runs over the group's rows.  Both operands are
-//                 MN-major; rows of the last k-block that belong to the next group are zeroed, hi tile included, by the
-//                 warps that compute the lo tiles (so an infinity or a NaN there does not matter).
+//   expert_rows_kernel      C[r, :] for the rows r of a group, the group's matrix as the other operand (a 3-d tensor map, so
+//                           a tile that ends behind its expert's matrix reads zeros).
+//   expert_weights_kernel   128 x BN tile of C_e [M, N] = A_e^T B_e: the reduction runs over the group's rows.  Both operands
+//                           are MN-major; rows of the last k-block that belong to the next group are zeroed, hi tile
+//                           included, by the warps that compute the lo tiles (an infinity or a NaN there does not matter).
 //
 // Every CTA finds its tile itself (groups::find_tile, ~1 us, while TMEM and barriers are set up); the grid is the most
 // tiles that the sizes allow, and CTAs without a tile leave at once.
@@ -18,7 +17,6 @@
 #include "gemm3x_common.cuh"
 #include "expert_groups.cuh"
 #include <mutex>
-#include <type_traits>
 
 using namespace sm100;
 using namespace gemm3x;
@@ -46,9 +44,318 @@ struct Grouped {
   int tiles_m;             // WEIGHTS: row tiles of one result
 };
 
-template <int BN, int WEIGHTS>
+// ---- C[r, :] for the rows of every group ------------------------------------------------------------------------
+// The expert's matrix is the operand with 128 rows (its N output features, whole tiles but the last) and the ragged
+// rows of the group are the other one, up to BN of them: the tensor core takes any multiple of 16 there, so a group of
+// 30 rows costs 32 columns of accumulator, not 128 lanes.  A tile's columns that belong to the next group are computed
+// (columns of an accumulator are independent) and not stored.  Lane = output feature in TMEM, so the 32 lanes of a warp
+// store 128 consecutive bytes of a row of C whatever its pitch and alignment.
+struct RowsArgs {
+  float* C;
+  long long ldc;
+  const float* bias;           // [experts, N] or null
+  const int* offsets;
+  int* status;
+  int N, K, experts, rows;
+  int w_mn;                    // the matrices are [K, N]: N is their contiguous axis
+  int act;
+  float alpha, beta;
+  int chunk;                   // k-blocks between roundings of the accumulators
+  int slices;                  // CTAs of a cluster that share a tile, each over a slice of K
+};
+
+template <int BN, int BK> struct RowsCfg {
+  static constexpr int A_TILE = BM * BK * 4, B_TILE = BN * BK * 4, RAW = A_TILE + B_TILE, STAGE = 2 * RAW;
+  static constexpr int STAGES = (196608 / STAGE) > 8 ? 8 : (196608 / STAGE);
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int BOX_ROWS = BN < 64 ? BN : 64;          // rows of one TMA box of the ragged operand
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+  static_assert(BM * BN * 4 <= STAGES * STAGE, "a parked tile must fit the pipeline stages");
+};
+
+// 32 accumulator columns (rows first .. first + 31 of C) of one output feature per lane
+__device__ __forceinline__ void store_columns(const RowsArgs& p, const uint32_t (&r)[32], int first, int hi, int n, const float* bias,
+                                              float beta, bool last) {
+  if (n >= p.N) return;
+  float* c = p.C + (long long)first * p.ldc + n;
+  const float b = (bias && last) ? bias[n] : 0.f;
+  const int left = hi - first;
+  if (beta != 0.f) {
+    float old[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) old[j] = j < left ? c[(long long)j * p.ldc] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float v = p.alpha * __uint_as_float(r[j]) + beta * old[j] + b;
+      if (last) v = apply_act(v, p.act);
+      if (j < left) c[(long long)j * p.ldc] = v;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float v = p.alpha * __uint_as_float(r[j]) + b;
+      if (last) v = apply_act(v, p.act);
+      if (j < left) c[(long long)j * p.ldc] = v;
+    }
+  }
+}
+
+template <int BN, int BK>
 __global__ void __launch_bounds__(THREADS, 1)
-expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ RowsArgs p) {
+  typedef RowsCfg<BN, BK> C;
+  constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
+  constexpr int W_BOX = BK * 128;                            // bytes of one 32 x BK box of an MN-major matrix
+  constexpr bool MMA_WHOLE = BN < 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = (uint64_t*)(smem + STAGES * C::STAGE);
+  // bars[0..S) full, [S..2S) conv, [2S..3S) empty, [3S] accumulators ready, [3S+1] accumulators read out
+  uint32_t* tmem_slot = (uint32_t*)(bars + 3 * STAGES + 2);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  int* where = (int*)(tmem_slot + 2);                        // {found, expert, lo, hi, index}
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles_n = (p.N + BM - 1) / BM;
+  const int unit = (int)blockIdx.x / p.slices, slice = (int)blockIdx.x - unit * p.slices;
+  const int n0 = (unit % tiles_n) * BM;
+
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bar_full = smem_u32(bars), bar_conv = smem_u32(bars + STAGES), bar_empty = smem_u32(bars + 2 * STAGES),
+                 bar_acc = smem_u32(bars + 3 * STAGES), bar_read = bar_acc + 8;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_conv + 8 * s, CONV_WARPS);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_acc, 1);
+    mbar_init(bar_read, CONV_WARPS);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == CONV_WARPS + 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == CONV_WARPS && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  if (warp == 1) {
+    groups::Tile t = {0, 0, 0, 0};
+    const bool found = groups::find_tile(p.offsets, p.experts, p.rows, BN, unit / tiles_n, p.status, t);
+    if (lane == 0) { where[0] = found; where[1] = t.expert; where[2] = t.lo; where[3] = t.hi; where[4] = t.index; }
+  }
+  int inject = 0;
+  if (warp == CONV_WARPS) inject = p.status[3];
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  if (!where[0]) {
+    // no such tile: with K slices every CTA of the tile's cluster leaves here
+    if (warp == CONV_WARPS + 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
+    return;
+  }
+  const int expert = where[1], hi = where[3], t0 = where[2] + where[4] * BN;
+  const int cols = min(BN, hi - t0);                         // rows of C in this tile = accumulator columns
+  const int boxes = (cols + C::BOX_ROWS - 1) / C::BOX_ROWS;
+  const int raw_bytes = A_TILE + boxes * C::BOX_ROWS * BK * 4;
+  const int nkb_all = (p.K + BK - 1) / BK;
+  const int kb_begin = (int)((long long)nkb_all * slice / p.slices);
+  const int nkb = (int)((long long)nkb_all * (slice + 1) / p.slices) - kb_begin;
+  const int n_chunks = (nkb + p.chunk - 1) / p.chunk, per = (nkb + n_chunks - 1) / n_chunks;
+  const float* bias = p.bias ? p.bias + (long long)expert * p.N : nullptr;
+
+  if (warp == CONV_WARPS) {
+    // ------------------------------ TMA producer ------------------------------
+    int issued = 0, s = 0;
+    uint32_t ph = 0;
+    const bool withhold = (inject & 1) != 0;                 // host-injected fault: arm nothing, load nothing
+    for (int i = 0; i < nkb; ++i) {
+      if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 100 + s)) break;
+      const uint32_t full = bar_full + 8 * s;
+      const uint32_t w_dst = smem_base + s * C::STAGE, x_dst = w_dst + A_TILE;
+      const int k0 = (kb_begin + i) * BK;
+      if (!withhold && elect_one()) {
+        mbar_arrive_expect_tx(full, (uint32_t)raw_bytes);
+        if (!p.w_mn) {
+          tma_load_3d(w_dst, &tmW, k0, n0, expert, full);
+        } else {
+#pragma unroll
+          for (int j = 0; j < BM / 32; ++j) tma_load_3d(w_dst + j * W_BOX, &tmW, n0 + 32 * j, k0, expert, full);
+        }
+        for (int j = 0; j < boxes; ++j) tma_load_2d(x_dst + j * C::BOX_ROWS * BK * 4, &tmX, k0, t0 + j * C::BOX_ROWS, full);
+      }
+      if (!withhold) issued = i + 1;
+      if (++s == STAGES) { s = 0; ph ^= 1; }
+    }
+    if (*abort_flag) {
+      // copies already issued land before this CTA gives its shared memory back
+      for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+        for (int it = 0; it < (1 << 16); ++it)
+          if (mbar_try_wait(bar_full + 8 * (i % STAGES), (i / STAGES) & 1)) break;
+    }
+  } else if (warp == CONV_WARPS + 1) {
+    // ------------------------------ MMA issuer --------------------------------
+    if (MMA_WHOLE || lane == 0) {
+      const uint32_t idesc = make_idesc_tf32(BM, (cols + 15) / 16 * 16, p.w_mn, 0);
+      constexpr uint32_t K_SWZ = BK == 32 ? SWZ_128B : SWZ_64B, K_SBO = 8 * BK * 4;
+      const uint32_t a_step = (p.w_mn ? 1024u : 32u) >> 4;
+      constexpr uint32_t b_step = 32u >> 4;
+      const uint32_t tmem_main = tmem_base, tmem_cross = tmem_base + BN;
+      const uint64_t d_a = p.w_mn ? make_smem_desc(smem_base, W_BOX, 512, SWZ_128B_BASE32B) : make_smem_desc(smem_base, 16, K_SBO, K_SWZ);
+      const uint64_t d_b = make_smem_desc(smem_base + A_TILE, 16, K_SBO, K_SWZ);
+      const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
+      const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
+      constexpr uint32_t LO_TILE = C::RAW >> 4, STAGE_STEP = C::STAGE >> 4;
+      uint32_t accumulate = 0, ph = 0, stage_off = 0, rph = 0;
+      int s = 0, in_chunk = 0, commits = 0;
+      for (int i = 0; i < nkb; ++i) {
+        if (in_chunk == per) {
+          // the chunk's sums go out before its accumulators are overwritten
+          if (!MMA_WHOLE || elect_one()) mma_commit(bar_acc);
+          if (MMA_WHOLE) __syncwarp();
+          ++commits;
+          if (!mbar_wait(bar_read, rph, abort_flag, p.status, 250)) break;
+          rph ^= 1;
+          tc_fence_after();
+          in_chunk = 0;
+          accumulate = 0;
+        }
+        ++in_chunk;
+        if (!mbar_wait(bar_conv + 8 * s, ph, abort_flag, p.status, 200 + s)) break;
+        tc_fence_after();
+        if (!MMA_WHOLE || elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < BK / 8; ++kk) {
+            const uint32_t al = a_low0 + stage_off + kk * a_step, bl = b_low0 + stage_off + kk * b_step;
+            mma_tf32_ss_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
+            mma_tf32_ss_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
+            mma_tf32_ss_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
+          }
+          mma_commit(bar_empty + 8 * s);
+        }
+        accumulate = 1;
+        if (MMA_WHOLE) __syncwarp();
+        if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
+      }
+      if (!MMA_WHOLE || elect_one()) mma_commit(bar_acc);
+      if (MMA_WHOLE) __syncwarp();
+      if (*abort_flag) {
+        // every MMA issued must have retired before TMEM is freed: the phase of the commit above
+        for (int it = 0; it < (1 << 16); ++it)
+          if (mbar_try_wait(bar_acc, (uint32_t)(commits & 1))) break;
+      }
+    }
+  } else {
+    // ------------------- hi / lo split, then epilogue (warps 0-7) ---------------
+    const int tid = threadIdx.x, q = warp & 3, half = warp >> 2;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16);
+    bool ok = true;
+    int i = 0;
+    for (int c = 0; ok && c < n_chunks; ++c) {
+      const int end = min(nkb, (c + 1) * per);
+      for (; i < end; ++i) {
+        const int s = i % STAGES, ph = (i / STAGES) & 1;
+        if (!mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 300 + s)) { ok = false; break; }
+        uint8_t* raw = smem + s * C::STAGE;
+        uint8_t* low = raw + C::RAW;
+        auto split = [&](int off) {
+          const float4 v = *reinterpret_cast<const float4*>(raw + off);
+          float4 l;
+          l.x = lo_part(v.x); l.y = lo_part(v.y); l.z = lo_part(v.z); l.w = lo_part(v.w);
+          *reinterpret_cast<float4*>(low + off) = l;
+        };
+        constexpr int PASS = CONV_WARPS * 32 * 16;
+        if (raw_bytes == C::RAW) {
+#pragma unroll
+          for (int k = 0; k < C::RAW / PASS; ++k) split(tid * 16 + k * PASS);
+        } else {
+#pragma unroll
+          for (int k = 0; k < A_TILE / PASS; ++k) split(tid * 16 + k * PASS);
+          for (int off = A_TILE + tid * 16; off < raw_bytes; off += PASS) split(off);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_conv + 8 * s);
+      }
+      if (ok) ok = mbar_wait(bar_acc, (uint32_t)(c & 1), abort_flag, p.status, 400);
+      ok = __all_sync(0xffffffffu, ok);                      // tcgen05.ld below is warp-collective
+      if (!ok) break;
+      tc_fence_after();
+      const bool last = c + 1 == n_chunks;
+#pragma unroll 1
+      for (int cc = half; cc * 32 < cols; cc += 2) {
+        uint32_t r[32], rc[32];
+        tmem_ld_32x32(lane_base + (uint32_t)(cc * 32), r);
+        tmem_ld_32x32(lane_base + (uint32_t)(BN + cc * 32), rc);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
+        if (p.slices > 1) {
+          // parked in this CTA's own shared memory ([columns / 4][128 lanes] float4); one chunk only, so the stages are free
+          float4* slot = reinterpret_cast<float4*>(smem) + (q * 32 + lane);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            slot[(cc * 8 + (j >> 2)) * 128] = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
+                                                          __uint_as_float(r[j + 3]));
+        } else {
+          store_columns(p, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, c == 0 ? p.beta : 1.f, last);
+        }
+      }
+      if (!last) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_read);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (p.slices > 1) {
+    // Every thread of every CTA takes both barriers.  Between them the tile's 32 x 32 pieces are dealt round the cluster's
+    // CTAs and warps, each summed in slice order whoever does it.
+    cluster_sync_all();
+    if (warp < CONV_WARPS && !*abort_flag) {
+      const int n = p.slices, items = 4 * ((cols + 31) / 32);
+      for (int it = (int)cluster_ctarank() + n * warp; it < items; it += n * CONV_WARPS) {
+        const int q = it & 3, cc = it >> 2;
+        const uint32_t off = smem_base + (uint32_t)((cc * 8 * 128 + q * 32 + lane) * 16);
+        float4 a[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int sl = 0; sl < n; ++sl) {
+          const uint32_t from = mapa(off, (uint32_t)sl);
+          float4 v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = ld_dsmem_v4(from + j * 2048);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) { a[j].x += v[j].x; a[j].y += v[j].y; a[j].z += v[j].z; a[j].w += v[j].w; }
+        }
+        uint32_t r[32];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          r[4 * j] = __float_as_uint(a[j].x); r[4 * j + 1] = __float_as_uint(a[j].y);
+          r[4 * j + 2] = __float_as_uint(a[j].z); r[4 * j + 3] = __float_as_uint(a[j].w);
+        }
+        store_columns(p, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, p.beta, true);
+      }
+    }
+    cluster_sync_all();
+  }
+  if (warp == CONV_WARPS + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// ---- C_e = A_e^T B_e over the rows of every group ------------------------------------------------------------------
+template <int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+expert_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ Grouped args) {
   typedef Cfg<BN> C;
   constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
@@ -91,16 +398,11 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   }
   if (warp == 1) {
     groups::Tile t = {0, 0, 0, 0};
-    bool found = true;
-    if (WEIGHTS) {
-      const int m_tile = unit / tiles_n;
-      t.expert = m_tile / args.tiles_m;
-      t.index = m_tile - t.expert * args.tiles_m;
-      groups::group_rows(args.offsets, args.rows, t.expert, p.status, t.lo, t.hi);
-    } else {
-      found = groups::find_tile(args.offsets, args.experts, args.rows, BM, unit / tiles_n, p.status, t);
-    }
-    if (lane == 0) { where[0] = found; where[1] = t.expert; where[2] = t.lo; where[3] = t.hi; where[4] = t.index; }
+    const int m_tile = unit / tiles_n;
+    t.expert = m_tile / args.tiles_m;
+    t.index = m_tile - t.expert * args.tiles_m;
+    groups::group_rows(args.offsets, args.rows, t.expert, p.status, t.lo, t.hi);
+    if (lane == 0) { where[0] = t.expert; where[1] = t.lo; where[2] = t.hi; where[3] = t.index; }
   }
   int inject = 0;
   if (warp == CONV_WARPS) inject = p.status[3];
@@ -108,35 +410,19 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int expert = where[1], lo = where[2], hi = where[3];
-  if (!where[0]) {
-    // no such tile: with K slices every CTA of the tile's cluster leaves here
-    if (warp == CONV_WARPS + 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
-    return;
-  }
-  int m0, nkb_all;
-  if (WEIGHTS) {
-    m0 = where[4] * BM;
-    p.C += expert * args.c_stride;
-    nkb_all = (hi - lo + BK - 1) / BK;
-  } else {
-    m0 = lo + where[4] * BM;
-    p.M = hi;
-    if (p.bias) p.bias += (long long)expert * p.N;
-    nkb_all = (p.K + BK - 1) / BK;
-  }
+  const int lo = where[1], hi = where[2], m0 = where[3] * BM;
+  p.C += where[0] * args.c_stride;
+  const int nkb_all = (hi - lo + BK - 1) / BK;
   const int kb_begin = (int)((long long)nkb_all * k_slice / p.ksplit_n);
   int nkb = (int)((long long)nkb_all * (k_slice + 1) / p.ksplit_n) - kb_begin;
   // an empty reduction (a group without rows, a slice without k-blocks): one k-block of zeros
-  const bool empty = WEIGHTS && nkb == 0;
+  const bool empty = nkb == 0;
   if (empty) nkb = 1;
   const int n_chunks = (nkb + args.chunk - 1) / args.chunk, per = (nkb + n_chunks - 1) / n_chunks;
 
   if (warp == CONV_WARPS) {
     // ------------------------------ TMA producer ------------------------------
-    auto producer = [&](auto whole_tag) {
-      constexpr bool PROD_WHOLE = decltype(whole_tag)::value;
-      if (!PROD_WHOLE && lane != 0) return;
+    {
       int issued = 0, s = 0;
       uint32_t ph = 0;
       const bool withhold = (inject & 1) != 0;              // host-injected fault: arm nothing, load nothing
@@ -149,22 +435,12 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           if (++s == STAGES) { s = 0; ph ^= 1; }
           continue;
         }
-        if (!PROD_WHOLE || elect_one()) {
+        if (elect_one()) {
           mbar_arrive_expect_tx(full, C::RAW);
-          if (WEIGHTS) {
 #pragma unroll
-            for (int j = 0; j < BM / 32; ++j) tma_load_2d(a_dst + j * BOX, &tmA, m0 + 32 * j, lo + k0, full);
+          for (int j = 0; j < BM / 32; ++j) tma_load_2d(a_dst + j * BOX, &tmA, m0 + 32 * j, lo + k0, full);
 #pragma unroll
-            for (int j = 0; j < BN / 32; ++j) tma_load_2d(b_dst + j * BOX, &tmB, n0 + 32 * j, lo + k0, full);
-          } else {
-            tma_load_2d(a_dst, &tmA, k0, m0, full);
-            if (!p.b_mn_major) {
-              tma_load_3d(b_dst, &tmB, k0, n0, expert, full);
-            } else {
-#pragma unroll
-              for (int j = 0; j < BN / 32; ++j) tma_load_3d(b_dst + j * BOX, &tmB, n0 + 32 * j, k0, expert, full);
-            }
-          }
+          for (int j = 0; j < BN / 32; ++j) tma_load_2d(b_dst + j * BOX, &tmB, n0 + 32 * j, lo + k0, full);
         }
         issued = i + 1;
         if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -174,22 +450,16 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           for (int it = 0; it < (1 << 16); ++it)
             if (mbar_try_wait(bar_full + 8 * (i % STAGES), (i / STAGES) & 1)) break;
       }
-    };
-    if (BN < 256 || WEIGHTS || p.b_mn_major) producer(std::true_type{});
-    else producer(std::false_type{});
+    }
   } else if (warp == CONV_WARPS + 1) {
     // ------------------------------ MMA issuer --------------------------------
     if (MMA_WHOLE || lane == 0) {
-      const int b_mn = WEIGHTS ? 1 : p.b_mn_major;
-      const uint32_t idesc = make_idesc_tf32(BM, BN, WEIGHTS, b_mn);
-      constexpr uint32_t K_SBO = 8 * BK * 4;
-      const uint32_t a_lbo = WEIGHTS ? (uint32_t)BOX : 16u, b_lbo = b_mn ? (uint32_t)BOX : 16u;
-      const uint32_t a_sbo = WEIGHTS ? 512u : K_SBO, b_sbo = b_mn ? 512u : K_SBO;
-      const uint32_t a_sw = WEIGHTS ? SWZ_128B_BASE32B : SWZ_64B, b_sw = b_mn ? SWZ_128B_BASE32B : SWZ_64B;
-      const uint32_t a_step = (WEIGHTS ? 1024u : 32u) >> 4, b_step = (b_mn ? 1024u : 32u) >> 4;
+      // both operands MN-major: 32-element blocks one TMA box apart, 4-k-row atoms 512 B apart, 1024 B per k-step
+      const uint32_t idesc = make_idesc_tf32(BM, BN, 1, 1);
+      constexpr uint32_t STEP = 1024u >> 4;
       const uint32_t tmem_main = tmem_base, tmem_cross = tmem_base + BN;
-      const uint64_t d_a = make_smem_desc(smem_base, a_lbo, a_sbo, a_sw);
-      const uint64_t d_b = make_smem_desc(smem_base + A_TILE, b_lbo, b_sbo, b_sw);
+      const uint64_t d_a = make_smem_desc(smem_base, BOX, 512, SWZ_128B_BASE32B);
+      const uint64_t d_b = make_smem_desc(smem_base + A_TILE, BOX, 512, SWZ_128B_BASE32B);
       const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
       const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
       constexpr uint32_t LO_TILE = C::RAW >> 4, STAGE_STEP = C::STAGE >> 4;
@@ -214,7 +484,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (!MMA_WHOLE || elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BK / 8; ++kk) {
-            const uint32_t al = a_low0 + stage_off + kk * a_step, bl = b_low0 + stage_off + kk * b_step;
+            const uint32_t al = a_low0 + stage_off + kk * STEP, bl = b_low0 + stage_off + kk * STEP;
             mma_tf32_ss_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
             mma_tf32_ss_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
             mma_tf32_ss_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
@@ -245,8 +515,8 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (!mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 300 + s)) { ok = false; break; }
         uint8_t* raw = smem + s * C::STAGE;
         uint8_t* low = raw + C::RAW;
-        const int valid = empty ? 0 : (WEIGHTS ? hi - lo - (kb_begin + i) * BK : BK);      // rows of this k-block inside the group
-        if (WEIGHTS && valid < BK) {
+        const int valid = empty ? 0 : hi - lo - (kb_begin + i) * BK;      // rows of this k-block inside the group
+        if (valid < BK) {
 #pragma unroll 1
           for (int off = tid * 16; off < C::RAW; off += CONV_WARPS * 32 * 16)
             if (((off & (BOX - 1)) >> 7) >= valid) *reinterpret_cast<float4*>(raw + off) = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -270,13 +540,9 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       tc_fence_after();
       const bool last = c + 1 == n_chunks;
       if (p.ksplit_n > 1) {
-        if (p.ksplit_cluster) {
-          dump_tile_smem<BN>(p, tmem_base, reinterpret_cast<float*>(smem), warp, lane);      // one chunk only
-        } else {
-          float* park = p.ksplit_ws + ((long long)unit * p.ksplit_n + k_slice) * (BM * BN);
-          if (c == 0) dump_tile<BN>(p, tmem_base, park, warp, lane);
-          else add_tile<BN>(tmem_base, park, warp, lane);
-        }
+        float* park = p.ksplit_ws + ((long long)unit * p.ksplit_n + k_slice) * (BM * BN);
+        if (c == 0) dump_tile<BN>(p, tmem_base, park, warp, lane);
+        else add_tile<BN>(tmem_base, park, warp, lane);
       } else {
         // staging lies in the pipeline stages, which are free only behind the last k-block
         epilogue_tile<BN>(p, tmem_base, m0, n0, warp, lane, last ? reinterpret_cast<float*>(smem) : nullptr,
@@ -288,7 +554,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (lane == 0) mbar_arrive(bar_read);
       }
     }
-    if (p.ksplit_n > 1 && !p.ksplit_cluster) {
+    if (p.ksplit_n > 1) {
       // slices parked in L2: the CTA that arrives last sums them in slice order and stores; nobody waits
       if (ok) __threadfence();
       asm volatile("bar.sync 1, %0;" ::"n"(CONV_WARPS * 32) : "memory");
@@ -306,17 +572,6 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
   tc_fence_before();
   __syncthreads();
-  if (p.ksplit_n > 1 && p.ksplit_cluster) {
-    cluster_sync_all();
-    if (warp < CONV_WARPS && !*abort_flag) {
-      const int n = p.ksplit_n, rank = (int)cluster_ctarank();
-      constexpr int ITEMS = 8 * (BN / 64);
-      float* staging = reinterpret_cast<float*>(smem + 128 * BN * 4);       // behind the parked tile
-      for (int it = rank + n * warp; it < ITEMS; it += n * CONV_WARPS)
-        epilogue_tile<BN>(p, tmem_base, m0, n0, warp, lane, staging, p.beta, true, false, nullptr, nullptr, n, smem_u32(smem), it);
-    }
-    cluster_sync_all();
-  }
   if (warp == CONV_WARPS + 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
@@ -368,34 +623,28 @@ int tmap_3d(CUtensorMap* tm, const float* base, long long count, long long rows,
   return tmap(tm, base, 3, dims, strides, box, swizzle);
 }
 
-template <int BN, int WEIGHTS> cudaError_t attributes(int dev) {
+template <typename A, void (*KERNEL)(CUtensorMap, CUtensorMap, A)>
+int launch(cb200_stream* s, int smem, const CUtensorMap& tmA, const CUtensorMap& tmB, const A& a, long long ctas, int cluster) {
   static std::once_flag once[64];
   static cudaError_t result[64];
-  std::call_once(once[dev & 63], [&] {
-    result[dev & 63] = cudaFuncSetAttribute(expert_tf32x3_kernel<BN, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<BN>::SMEM);
-  });
-  return result[dev & 63];
-}
-
-template <int BN, int WEIGHTS>
-int launch(cb200_stream* s, const CUtensorMap& tmA, const CUtensorMap& tmB, const Grouped& a, long long ctas) {
-  cudaError_t e = attributes<BN, WEIGHTS>(s->device);
-  if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaFuncSetAttribute", __FILE__, __LINE__);
+  const int dev = s->device & 63;
+  std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+  if (result[dev] != cudaSuccess) return cb200_cuda_fail(result[dev], "cudaFuncSetAttribute", __FILE__, __LINE__);
   CB_REQUIRE(ctas <= 2147483647LL, "expert_gemm: too many tiles");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas, 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
-  cfg.dynamicSmemBytes = Cfg<BN>::SMEM;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.g.ksplit_cluster ? (unsigned)a.g.ksplit_n : 1;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = a.g.ksplit_cluster ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, expert_tf32x3_kernel<BN, WEIGHTS>, tmA, tmB, a);
-  if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaLaunchKernelEx(expert_tf32x3_kernel)", __FILE__, __LINE__);
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, tmA, tmB, a);
+  if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaLaunchKernelEx(expert kernel)", __FILE__, __LINE__);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
@@ -447,29 +696,35 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
                          long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
                          const int* offsets, const float* bias, int act) {
   DeviceGuard guard(s->device);
-  Grouped a;
-  common(a.g, s, C, ldc, 0, N, K, alpha, beta, bias, act);
-  a.g.b_mn_major = trans_b ? 0 : 1;
-  a.offsets = offsets; a.experts = experts; a.rows = rows; a.chunk = CHUNK; a.c_stride = 0; a.tiles_m = 0;
-  const long long most = (rows + BM - 1) / BM + (experts < rows ? experts : rows) - (experts > 0 ? 1 : 0);
-  const long long tiles_m = most < 1 ? 1 : most;
-  const int nkb = (K + BK - 1) / BK;
-  int BN, slices;
-  // a slice is one chunk: its parked tile is in shared memory, which the next chunk's stages would need
-  choose(s, tiles_m, N, nkb, K <= 8 * 2048 ? 8 : 1, BN, slices);
-  if (slices > 1 && (nkb + slices - 1) / slices > CHUNK) slices = 1;
-  a.g.ksplit_n = slices;
-  a.g.ksplit_cluster = slices > 1;
-  CUtensorMap tmA, tmB;
-  int rc = tmap_2d(&tmA, A, rows, K, lda, BK, BM, CU_TENSOR_MAP_SWIZZLE_64B);
+  // how many rows a tile may take: what an even split of the rows over the experts fills
+  const long long even = (rows + experts - 1) / experts;
+  int BN = s->opt_gemm_tile_n > 0 ? s->opt_gemm_tile_n : (even <= 32 ? 32 : (even <= 64 ? 64 : (even <= 128 ? 128 : 256)));
+  const int bk = BN <= 64 ? 32 : 16;
+  const long long tiles = (rows + BN - 1) / BN + (experts < rows ? experts : rows) - 1, units = tiles * ((N + BM - 1) / BM);
+  const int nkb = (K + bk - 1) / bk, chunk = 2048 / bk;
+  // K slices (the CTAs of a cluster) where the tiles leave SMs free; a slice is one chunk, since its parked tile lies in
+  // shared memory that the next chunk's stages would need
+  int slices = 1;
+  const int forced = s->opt_gemm_k_slices;
+  for (int sl = 2; sl <= 8; sl *= 2)
+    if ((forced > 0 ? sl <= forced : units * sl <= s->sm_count) && nkb / sl >= 4) slices = sl;
+  if ((nkb + slices - 1) / slices > chunk) slices = 1;
+  RowsArgs a;
+  a.C = C; a.ldc = ldc; a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
+  a.N = N; a.K = K; a.experts = experts; a.rows = rows; a.w_mn = trans_b ? 0 : 1; a.act = act;
+  a.alpha = alpha; a.beta = beta; a.chunk = chunk; a.slices = slices;
+  const CUtensorMapSwizzle swz = bk == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  CUtensorMap tmW, tmX;
+  int rc = tmap_2d(&tmX, A, rows, K, lda, bk, BN < 64 ? BN : 64, swz);
   if (rc) return rc;
-  if (trans_b) rc = tmap_3d(&tmB, B, experts, N, K, ldb, b_stride, BK, BN, CU_TENSOR_MAP_SWIZZLE_64B);
-  else rc = tmap_3d(&tmB, B, experts, K, N, ldb, b_stride, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
+  if (trans_b) rc = tmap_3d(&tmW, B, experts, N, K, ldb, b_stride, bk, BM, swz);
+  else rc = tmap_3d(&tmW, B, experts, K, N, ldb, b_stride, 32, bk, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
   if (rc) return rc;
-  const long long ctas = tiles_m * ((N + BN - 1) / BN) * slices;
-  if (BN == 256) return launch<256, 0>(s, tmA, tmB, a, ctas);
-  if (BN == 128) return launch<128, 0>(s, tmA, tmB, a, ctas);
-  return launch<64, 0>(s, tmA, tmB, a, ctas);
+  const long long ctas = units * slices;
+  if (BN == 256) return launch<RowsArgs, expert_rows_kernel<256, 16>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, slices);
+  if (BN == 128) return launch<RowsArgs, expert_rows_kernel<128, 16>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, slices);
+  if (BN == 64) return launch<RowsArgs, expert_rows_kernel<64, 32>>(s, RowsCfg<64, 32>::SMEM, tmW, tmX, a, ctas, slices);
+  return launch<RowsArgs, expert_rows_kernel<32, 32>>(s, RowsCfg<32, 32>::SMEM, tmW, tmX, a, ctas, slices);
 }
 
 int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
@@ -497,7 +752,7 @@ int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long 
   CUtensorMap tmA, tmB;
   if ((rc = tmap_2d(&tmA, A, rows, M, lda, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
   if ((rc = tmap_2d(&tmB, B, rows, N, ldb, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
-  if (BN == 256) return launch<256, 1>(s, tmA, tmB, a, units * slices);
-  if (BN == 128) return launch<128, 1>(s, tmA, tmB, a, units * slices);
-  return launch<64, 1>(s, tmA, tmB, a, units * slices);
+  if (BN == 256) return launch<Grouped, expert_weights_kernel<256>>(s, Cfg<256>::SMEM, tmA, tmB, a, units * slices, 1);
+  if (BN == 128) return launch<Grouped, expert_weights_kernel<128>>(s, Cfg<128>::SMEM, tmA, tmB, a, units * slices, 1);
+  return launch<Grouped, expert_weights_kernel<64>>(s, Cfg<64>::SMEM, tmA, tmB, a, units * slices, 1);
 }
