@@ -12,10 +12,18 @@
 bool cb200_expert_tc_ok(const void* A, long long lda, const void* B, long long ldb, long long b_stride);
 int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
                          long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
-                         const int* offsets, const float* bias, int act);
+                         const int* offsets, const float* bias, int act, const int* only_if);
 int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
                             int M, long long lda, const float* B, int N, long long ldb, int experts, float beta,
-                            const int* offsets);
+                            const int* offsets, const int* only_if);
+bool cb200_expert_f16_ok(cb200_stream* s, int trans_b, long long rows, long long K, long long N, long long experts);
+bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts);
+int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
+                          long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
+                          const int* offsets, const float* bias, int act, const int** guard);
+int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows, int M,
+                             long long lda, const float* B, int N, long long ldb, int experts, float beta, const int* offsets,
+                             const int** guard);
 
 namespace {
 
@@ -38,6 +46,7 @@ template <typename T> struct Product {
   const T* bias;
   T* bias_g;
   const int* offsets;
+  const int* only_if;              // null, or a device word: do nothing while it is zero
   int* status;
 };
 
@@ -105,6 +114,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) expert_rows_simt_kernel(Product<T> p) {
   __shared__ groups::Tile tile;
   __shared__ bool found;
+  if (p.only_if && *p.only_if == 0) return;
   for (int t = (int)blockIdx.y;; t += (int)gridDim.y) {
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -127,6 +137,7 @@ __global__ void __launch_bounds__(256) expert_rows_simt_kernel(Product<T> p) {
 template <typename T>
 __global__ void __launch_bounds__(256) expert_weights_simt_kernel(Product<T> p, int tiles_m) {
   __shared__ int lo, hi;
+  if (p.only_if && *p.only_if == 0) return;
   const int e = (int)blockIdx.z;
   if (threadIdx.x < 32) {
     int a, b;
@@ -145,11 +156,13 @@ __global__ void __launch_bounds__(256) expert_weights_simt_kernel(Product<T> p, 
   }
 }
 
-// bias_gradient[e, m] = alpha * sum of the group's rows + beta * bias_gradient[e, m]; 32 columns and 8 rows at a time
-template <typename T>
+// bias_gradient[e, m] = alpha * sum of the group's rows + beta * bias_gradient[e, m]: a warp reads 32 * V columns of a row,
+// the CTA's eight warps take every eighth row with four rows in flight each; fixed order
+template <typename T, int V>
 __global__ void __launch_bounds__(256) expert_bias_gradient_kernel(Product<T> p) {
+  struct alignas(sizeof(T) * V) Pack { T e[V]; };
   __shared__ int lo, hi;
-  __shared__ T part[8][33];
+  __shared__ T part[8][32 * V + 1];
   const int e = (int)blockIdx.y;
   if (threadIdx.x < 32) {
     int a, b;
@@ -157,19 +170,52 @@ __global__ void __launch_bounds__(256) expert_bias_gradient_kernel(Product<T> p)
     if (threadIdx.x == 0) { lo = a; hi = b; }
   }
   __syncthreads();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, m = (int)blockIdx.x * 32 + tx;
-  T s = (T)0;
-  if (m < p.M)
-    for (int r = lo + ty; r < hi; r += 8) s += p.A[(long long)r * p.lda + m];
-  part[ty][tx] = s;
-  __syncthreads();
-  if (ty != 0 || m >= p.M) return;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, m = ((int)blockIdx.x * 32 + tx) * V;
+  T s[V];
 #pragma unroll
-  for (int w = 1; w < 8; ++w) s += part[w][tx];
-  T* to = p.bias_g + (long long)e * p.M + m;
-  T o = p.alpha * s;
-  if (p.beta != (T)0) o += p.beta * (*to);
-  *to = o;
+  for (int j = 0; j < V; ++j) s[j] = (T)0;
+  if (m < p.M) {
+    const T* a = p.A + m;
+    int r = lo + ty;
+    for (; r + 24 < hi; r += 32) {
+      Pack v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const Pack*>(a + (long long)(r + 8 * i) * p.lda);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] += v[i].e[j];
+    }
+    for (; r < hi; r += 8) {
+      const Pack v = *reinterpret_cast<const Pack*>(a + (long long)r * p.lda);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] += v.e[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) part[ty][tx * V + j] = s[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * V; c += 256) {
+    const int at = (int)blockIdx.x * 32 * V + c;
+    if (at >= p.M) break;
+    T sum = part[0][c];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) sum += part[w][c];
+    T* to = p.bias_g + (long long)e * p.M + at;
+    T o = p.alpha * sum;
+    if (p.beta != (T)0) o += p.beta * (*to);
+    *to = o;
+  }
+}
+
+template <typename T> int run_bias_gradient(cb200_stream* s, const Product<T>& p) {
+  constexpr int V = 16 / sizeof(T);
+  if (((uintptr_t)p.A & 15) == 0 && p.lda % V == 0 && p.M % V == 0)
+    expert_bias_gradient_kernel<T, V><<<dim3((unsigned)((p.M + 32 * V - 1) / (32 * V)), (unsigned)p.experts), 256, 0, s->stream>>>(p);
+  else
+    expert_bias_gradient_kernel<T, 1><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 256, 0, s->stream>>>(p);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
 }
 
 template <typename T> int run_rows(cb200_stream* s, const Product<T>& p) {
@@ -186,11 +232,7 @@ template <typename T> int run_weights(cb200_stream* s, const Product<T>& p) {
   expert_weights_simt_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles_m < 65535 ? tiles_m : 65535), (unsigned)p.experts),
                                   256, 0, s->stream>>>(p, tiles_m);
   CB_LAUNCH_CHECK(s);
-  if (p.bias_g) {
-    expert_bias_gradient_kernel<T><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 256, 0, s->stream>>>(p);
-    CB_LAUNCH_CHECK(s);
-  }
-  return CB200_OK;
+  return p.bias_g ? run_bias_gradient<T>(s, p) : CB200_OK;
 }
 
 // ---- fp32: the tensor-core kernels, behind a copy of operands that TMA cannot address -----------------------------------
@@ -220,7 +262,13 @@ int rows_tc(cb200_stream* s, Product<float> p) {
   const int b_cols = p.trans_b ? p.K : p.N;
   if (p.experts == 1) p.b_stride = b_rows * p.ldb;
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, p.b_stride);
-  if (pack_a || pack_b) {
+  if (cb200_expert_f16_ok(s, p.trans_b, p.rows, p.K, p.N, p.experts)) {
+    // products at twice the rate; what follows runs only where the data do not fit scaled halves
+    int rc = cb200_expert_rows_f16(s, p.C, p.ldc, p.trans_b, p.alpha, p.A, p.rows, p.K, p.lda, p.B, p.experts, p.N, p.b_stride, p.ldb,
+                                   p.beta, p.offsets, p.bias, p.act, &p.only_if);
+    if (rc) return rc;
+    if (pack_a || pack_b) return run_rows<float>(s, p);         // (the workspace holds the halves)
+  } else if (pack_a || pack_b) {
     DeviceGuard guard(s->device);
     const long long lda = (p.K + 3) / 4 * 4, ldb = (b_cols + 3) / 4 * 4;
     const size_t a_n = pack_a ? (size_t)p.rows * lda : 0, b_n = pack_b ? (size_t)p.experts * b_rows * ldb : 0;
@@ -239,17 +287,23 @@ int rows_tc(cb200_stream* s, Product<float> p) {
     }
   }
   return cb200_expert_rows_tc(s, p.C, p.ldc, p.trans_b, p.alpha, p.A, p.rows, p.K, p.lda, p.B, p.experts, p.N, p.b_stride, p.ldb,
-                              p.beta, p.offsets, p.bias, p.act);
+                              p.beta, p.offsets, p.bias, p.act, p.only_if);
 }
 
 int weights_tc(cb200_stream* s, Product<float> p) {
   if (p.bias_g) {
     DeviceGuard guard(s->device);
-    expert_bias_gradient_kernel<float><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 256, 0, s->stream>>>(p);
-    CB_LAUNCH_CHECK(s);
+    int rc = run_bias_gradient<float>(s, p);
+    if (rc) return rc;
   }
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
-  if (pack_a || pack_b) {
+  if (cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts)) {
+    int rc = cb200_expert_weights_f16(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta,
+                                      p.offsets, &p.only_if);
+    if (rc) return rc;
+    p.bias_g = nullptr;                                          // done above
+    if (pack_a || pack_b) return run_weights<float>(s, p);
+  } else if (pack_a || pack_b) {
     DeviceGuard guard(s->device);
     const long long lda = (p.M + 3) / 4 * 4, ldb = (p.N + 3) / 4 * 4;
     const size_t a_n = pack_a ? (size_t)p.rows * lda : 0, b_n = pack_b ? (size_t)p.rows * ldb : 0;
@@ -267,7 +321,7 @@ int weights_tc(cb200_stream* s, Product<float> p) {
       p.B = b; p.ldb = ldb;
     }
   }
-  return cb200_expert_weights_tc(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta, p.offsets);
+  return cb200_expert_weights_tc(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta, p.offsets, p.only_if);
 }
 
 int check_common(const char* what, cb200_stream* s, int dtype, const void* C, const void* A, const void* B, int64_t rows,
@@ -295,7 +349,7 @@ Product<T> product(cb200_stream* s, void* C, int64_t c_stride, int64_t ldc, int 
   p.rows = (int)rows; p.M = (int)M; p.N = (int)N; p.K = (int)K; p.experts = (int)experts;
   p.alpha = (T)alpha; p.beta = (T)beta;
   p.bias = (const T*)bias; p.bias_g = (T*)bias_g;
-  p.offsets = offsets; p.status = s->status_dev;
+  p.offsets = offsets; p.only_if = nullptr; p.status = s->status_dev;
   return p;
 }
 

@@ -1,0 +1,847 @@
+// Large fp32 products grouped by expert at twice the rate of 3xTF32: operands as pairs of scaled halves.
+//
+// The tensor core multiplies fp16 at twice the rate of tf32 with the same 11-bit significands, so the split
+//   x * s = h1 + 2^-11 h2,   h1 = half(x * s),  h2 = half(2^11 (x * s - h1)),   s = a power of two per operand row
+// carries 22 bits like hi + lo of 3xTF32 does, and the three products h1 h1, h1 h2, h2 h1 cost half of what they cost
+// there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-29 of
+// it keep their 22 bits, smaller ones an absolute error of 2^-50 of it.  Rows for which that is not good enough -- more
+// than 1 in 64 values (not counting zeros) below 2^-29 of the row's largest, a largest value outside [2^-48, 2^60], an
+// infinity or a NaN -- raise a flag in device memory; the kernel here then does nothing and the 3xTF32 kernel launched
+// behind it, which otherwise does nothing, does the work.  So results have the accuracy of gemm! whatever the data.
+//
+// Steps of a call: group bounds and the table of tiles (one warp); the operands' halves, K-contiguous, with their scales
+// (HBM-bound; operands whose reduction axis is not contiguous get a pass for the column maxima first); the product; the
+// guarded 3xTF32 kernel.
+//
+// The product runs on CTA pairs (tcgen05.mma.cta_group::2, 256 lanes x up to 256 columns per pair), persistent, six
+// pipeline stages of 32 KB, as the pre-split layer GEMM: every TMA load is a plain one into the issuing CTA, completing on
+// the leader's barrier.  Output features (expert_gemm) or input features (expert_gemm_weights) lie in the lanes, so a warp
+// stores 128 consecutive bytes; the ragged rows (or output features) lie in the columns, in multiples of 32.
+// The tensor core adds with truncation: after every 2048 values of k the epilogue warps add the main accumulator into
+// registers (round to nearest) and it restarts from zero.
+#include "gemm3x_common.cuh"
+#include "expert_groups.cuh"
+#include <cuda_fp16.h>
+#include <math.h>
+#include <mutex>
+#include <type_traits>
+
+using namespace sm100;
+using namespace gemm3x;
+
+namespace {
+
+constexpr int BM = 128, BN = 256, BK = 32;               // per CTA: 128 lanes, 256 columns of the pair, 32 halves of k
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = (EPI_WARPS + 3) * 32;
+constexpr int L_TILE = BM * BK * 2, R_TILE = BN / 2 * BK * 2;       // 8 KiB each
+constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
+constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
+constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES;
+constexpr int TMEM_COLS = 2 * BN;
+constexpr int DRAIN = 2048 / BK;
+
+// what one warp works out at the start of a call, in device memory
+struct Plan {
+  int flag;                    // 1: the operands do not fit scaled halves
+  int tiles;                   // expert_gemm: row tiles in the table
+  int padded;                  // expert_gemm_weights: padded positions in use
+  int unused;
+};
+struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); expert_gemm_weights: rows and first padded position
+
+// bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
+// entry per tile of BN rows.
+__global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, const int* offsets, int experts, int rows, int weights,
+                                                  int* status) {
+  const int lane = threadIdx.x;
+  int carry_max = 0, carry = 0;
+  bool bad = false;
+  for (int base = 0; base < experts; base += 32) {
+    const int e = base + lane;
+    int lo = 0, hi = 0;
+    if (e < experts) {
+      const int raw_lo = offsets[e], raw_hi = offsets[e + 1];
+      lo = min(max(raw_lo, 0), rows);
+      hi = min(max(raw_hi, 0), rows);
+      bad = bad || lo != raw_lo || hi != raw_hi || hi < lo;
+    }
+    hi = max(hi, lo);
+    int run = hi;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, run, d);
+      if (lane >= d) run = max(run, up);
+    }
+    run = max(run, carry_max);
+    int before = __shfl_up_sync(0xffffffffu, run, 1);
+    if (lane == 0) before = carry_max;
+    lo = max(lo, before);
+    hi = max(hi, lo);
+    const int mine = e < experts ? (weights ? (hi - lo + BK - 1) / BK * BK : (hi - lo + BN - 1) / BN) : 0;
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += up;
+    }
+    sum += carry;
+    if (e < experts) {
+      if (weights) table[e] = {e, lo, hi, sum - mine};
+      else for (int i = 0; i < mine; ++i) table[sum - mine + i] = {e, lo + i * BN, hi, 0};
+    }
+    carry_max = __shfl_sync(0xffffffffu, run, 31);
+    carry = __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (__any_sync(0xffffffffu, bad) && lane == 0) groups::report_bad(status);
+  if (lane == 0) {
+    plan->flag = 0;
+    plan->tiles = plan->padded = carry;
+    if (weights) table[experts] = {experts, 0, 0, carry};
+  }
+}
+
+// ---- scaled halves ---------------------------------------------------------------------------------------------
+// Scale of a row (or column) whose largest magnitude has these bits: 2^up; its inverse; false: outside the range.
+__device__ __forceinline__ bool scale_of(uint32_t max_bits, float& up, float& down) {
+  if (max_bits == 0) { up = down = 1.f; return true; }
+  const int ex = (int)(max_bits >> 23) - 127;
+  const bool ok = ex >= -48 && ex <= 60;                   // (two inverse scales multiply to a normal number)
+  const int e = ok ? 14 - ex : 0;
+  up = __uint_as_float((uint32_t)(127 + e) << 23);
+  down = __uint_as_float((uint32_t)(127 - e) << 23);
+  return ok;
+}
+__device__ __forceinline__ void split_half(float y, __half& h1, __half& h2, int& tiny) {
+  h1 = __float2half_rn(y);
+  h2 = __float2half_rn((y - __half2float(h1)) * 2048.f);
+  const float a = fabsf(y);
+  tiny += a < 6.103515625e-5f && a > 0.f;                  // below 2^-14: 2^-29 of the row's largest
+}
+union Half8 { __half h[8]; uint4 v; };
+
+__device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
+  if (vec && left >= 8) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+  }
+}
+
+// Rows along which the product reduces: TPR threads per row, 8 values per thread and step, the first HOLD steps in
+// registers between the maximum and the split (longer rows are read again, from L2).
+// Row r of the operand: x + (r / rows_per) * stride + (r % rows_per) * ld.  hi / lo: pitch kp (a multiple of 8).
+template <int TPR>
+__global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
+                                                         long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan) {
+  constexpr int HOLD = 4;
+  __shared__ uint32_t part_max[8];
+  __shared__ int part_tiny[8];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, warp = threadIdx.x >> 5;
+  const long long r = (long long)blockIdx.x * (256 / TPR) + sub;
+  const bool live = r < rows;
+  const float* src = live ? x + (r / rows_per) * stride + (r % rows_per) * ld : x;
+  const bool vec = ((uintptr_t)src & 15) == 0;
+  const int n = live ? cols : 0;
+  float v[HOLD][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int it = 0; it < HOLD; ++it) {
+    const int c = (it * TPR + t) * 8;
+    if (c < n) load8(src + c, n - c, vec, v[it]);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[it][j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[it][j]) & 0x7fffffffu);
+  }
+  for (int c = (HOLD * TPR + t) * 8; c < n; c += TPR * 8) {
+    float w[8];
+    load8(src + c, n - c, vec, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(w[j]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) part_max[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) m = max(m, part_max[sub * (TPR / 32) + w]);
+  }
+  float up, down;
+  const bool ok = scale_of(m, up, down);
+  int tiny = 0;
+  auto put = [&](int c, const float (&w)[8]) {
+    Half8 a, b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j], tiny);
+    *reinterpret_cast<uint4*>(hi + r * kp + c) = a.v;      // pitch and position are multiples of 8 halves
+    *reinterpret_cast<uint4*>(lo + r * kp + c) = b.v;
+  };
+#pragma unroll
+  for (int it = 0; it < HOLD; ++it) {
+    const int c = (it * TPR + t) * 8;
+    if (c < n) put(c, v[it]);
+  }
+  for (int c = (HOLD * TPR + t) * 8; c < n; c += TPR * 8) {
+    float w[8];
+    load8(src + c, n - c, vec, w);
+    put(c, w);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) tiny += __shfl_xor_sync(0xffffffffu, tiny, d);
+  if (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) part_tiny[warp] = tiny;
+    __syncthreads();
+    tiny = 0;
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) tiny += part_tiny[sub * (TPR / 32) + w];
+  }
+  if (t == 0 && live) {
+    down_out[r] = down;
+    if (!ok || (long long)tiny * 64 > cols) plan->flag = 1;
+  }
+}
+
+// Operands whose reduction runs down their columns, in groups of rows: rows of group g are table[g].lo .. hi (ragged) or
+// g * fixed .. (g + 1) * fixed (the experts' matrices, `stride` apart).
+__device__ __forceinline__ const float* grouped_row(const float* x, long long ld, long long stride, int fixed, int group, int r) {
+  return fixed ? x + group * stride + (long long)r * ld : x + (long long)r * ld;
+}
+
+// maxima[g][c] = bits of the largest magnitude in column c of group g; 64 rows per CTA
+__global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const float* x, long long ld, long long stride, int fixed,
+                                                         const Entry* table, int groups_n, int rows, int cols) {
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= cols) return;
+  if (fixed) {
+    const int chunks = (fixed + 63) / 64;
+    for (long long b = blockIdx.y; b < (long long)groups_n * chunks; b += gridDim.y) {
+      const int g = (int)(b / chunks), r0 = (int)(b - (long long)g * chunks) * 64, r1 = min(fixed, r0 + 64);
+      uint32_t m = 0;
+#pragma unroll 8
+      for (int r = r0; r < r1; ++r) m = max(m, __float_as_uint(grouped_row(x, ld, stride, fixed, g, r)[c]) & 0x7fffffffu);
+      atomicMax(maxima + (long long)g * cols + c, m);
+    }
+    return;
+  }
+  for (long long b = blockIdx.y; b * 64 < rows; b += gridDim.y) {
+    const int r0 = (int)(b * 64), r1 = min(rows, r0 + 64);
+    int g = 0, end = groups_n;                              // the last group that begins at or before r0
+    while (end - g > 1) {
+      const int mid = (g + end) >> 1;
+      if (table[mid].lo <= r0) g = mid; else end = mid;
+    }
+    for (; g < groups_n && table[g].lo < r1; ++g) {
+      const int a = max(r0, table[g].lo), z = min(r1, table[g].hi);
+      uint32_t m = 0;
+#pragma unroll 8
+      for (int r = a; r < z; ++r) m = max(m, __float_as_uint(x[(long long)r * ld + c]) & 0x7fffffffu);
+      if (z > a) atomicMax(maxima + (long long)g * cols + c, m);
+    }
+  }
+}
+
+// hi / lo [cols (x groups where fixed)][positions]: 32 positions x 64 columns per CTA through shared memory.  Ragged groups
+// start at a multiple of 32 positions and are padded with zeros; fixed ones have rows of their own (pitch kp >= fixed).
+__global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* lo, float* down_out, const uint32_t* maxima, const float* x,
+                                                            long long ld, long long stride, int fixed, const Entry* table, int groups_n,
+                                                            int cols, long long kp, Plan* plan) {
+  __shared__ float tile[32][65];
+  __shared__ int tiny_all;
+  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int c0 = blockIdx.x * 64;
+  const int per = fixed ? (fixed + 31) / 32 : 1;
+  const long long blocks = fixed ? (long long)groups_n * per : plan->padded / 32;
+  for (long long b = blockIdx.y; b < blocks; b += gridDim.y) {
+    int g, r0, end;
+    long long pos, row_base;                               // first position written, first row of hi / lo
+    if (fixed) {
+      g = (int)(b / per);
+      r0 = (int)(b - (long long)g * per) * 32;
+      end = fixed;
+      pos = r0;
+      row_base = (long long)g * cols;
+    } else {
+      int a = 0, z = groups_n;                             // the group that owns these positions
+      while (z - a > 1) {
+        const int mid = (a + z) >> 1;
+        if (table[mid].first <= b * 32) a = mid; else z = mid;
+      }
+      g = a;                                               // (of groups without rows that start here, the last one: the owner)
+      pos = b * 32;
+      r0 = table[g].lo + (int)(pos - table[g].first);
+      end = table[g].hi;
+      row_base = 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) tiny_all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + ty + 4 * i, c = c0 + tx;
+      tile[ty + 4 * i][tx] = (r < end && c < cols) ? grouped_row(x, ld, stride, fixed, g, r)[c] : 0.f;
+    }
+    __syncthreads();
+    // a thread: 8 positions of one column
+    const int col = threadIdx.x >> 2, p8 = (threadIdx.x & 3) * 8, c = c0 + col;
+    int tiny = 0;
+    if (c < cols) {
+      float up, down;
+      const bool ok = scale_of(maxima[(long long)g * cols + c], up, down);
+      Half8 a, z;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split_half(tile[p8 + j][col] * up, a.h[j], z.h[j], tiny);
+      if (pos + p8 < kp) {                                 // kp is a multiple of 8
+        *reinterpret_cast<uint4*>(hi + (row_base + c) * kp + pos + p8) = a.v;
+        *reinterpret_cast<uint4*>(lo + (row_base + c) * kp + pos + p8) = z.v;
+      }
+      if (!ok) plan->flag = 1;
+      if (p8 == 0 && pos == (fixed ? 0 : table[g].first)) down_out[(long long)g * cols + c] = down;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) tiny += __shfl_xor_sync(0xffffffffu, tiny, d);
+    if ((threadIdx.x & 31) == 0 && tiny) atomicAdd(&tiny_all, tiny);
+    __syncthreads();
+    if (threadIdx.x == 0 && tiny_all * 64 > 32 * 64) plan->flag = 1;
+  }
+}
+
+// ---- the product -----------------------------------------------------------------------------------------------
+struct PairArgs {
+  float* C;                     // element (column c, lane l) of a tile at C + c * ldc + l
+  long long ldc, c_stride;
+  const float* l_down; const float* r_down;      // inverse scales
+  const float* bias;
+  const Plan* plan;
+  const Entry* table;
+  int* status;
+  int lanes, cols;              // extents: lanes of one expert's matrix; WEIGHTS: columns of one result
+  int K;                        // expert_gemm: reduction length
+  int experts, weights, act;
+  float alpha, beta;
+};
+
+struct Unit { int expert, l0, r0, cols, l_row, kb, nkb; };
+
+__device__ __forceinline__ Unit unit_of(const PairArgs& p, int unit) {
+  const int tiles_l = (p.lanes + 2 * BM - 1) / (2 * BM);
+  Unit u;
+  const int row = unit / tiles_l;
+  u.l0 = (unit - row * tiles_l) * 2 * BM;
+  if (p.weights) {
+    const int tiles_r = (p.cols + BN - 1) / BN;
+    u.expert = row / tiles_r;
+    const Entry e = p.table[u.expert];
+    u.r0 = (row - u.expert * tiles_r) * BN;
+    u.cols = min(BN, p.cols - u.r0);
+    u.l_row = u.l0;
+    u.kb = e.first / BK;
+    u.nkb = (e.hi - e.lo + BK - 1) / BK;
+  } else {
+    const Entry e = p.table[row];
+    u.expert = e.expert;
+    u.r0 = e.lo;
+    u.cols = min(BN, e.hi - e.lo);
+    u.l_row = e.expert * p.lanes + u.l0;
+    u.kb = 0;
+    u.nkb = (p.K + BK - 1) / BK;
+  }
+  return u;
+}
+
+__device__ __forceinline__ void mma_f16_pair_words(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                                   uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// instruction descriptor of kind::f16 with half operands, K-major, fp32 accumulation (the fields of make_idesc_tf32)
+__host__ __device__ __forceinline__ uint32_t make_idesc_f16(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmLlo, const __grid_constant__ CUtensorMap tmR,
+                   const __grid_constant__ CUtensorMap tmRlo, const __grid_constant__ PairArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = (uint64_t*)(smem + STAGES * STAGE);
+  // bars[0..S) full (the leader's copy: its two producers arrive, both CTAs' loads complete bytes), [S..2S) empty,
+  // [2S] accumulators may be read out (each CTA's own), [2S+1] they have been (the leader's: one arrival per epilogue warp
+  // of both CTAs), [2S+2] unwinding only: every MMA issued so far has retired
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 3);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int n_clusters = (int)gridDim.x >> 1, cluster_id = (int)blockIdx.x >> 1;
+
+  if (p.plan->flag) return;               // both CTAs of every pair: nothing has been set up yet
+  const int tiles_l = (p.lanes + 2 * BM - 1) / (2 * BM);
+  const int n_units = (p.weights ? p.experts * ((p.cols + BN - 1) / BN) : p.plan->tiles) * tiles_l;
+
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES), bar_mid = smem_u32(bars + 2 * STAGES),
+                 bar_drained = bar_mid + 8, bar_retired = bar_mid + 16;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 2);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_mid, 1);
+    mbar_init(bar_drained, 2 * EPI_WARPS);
+    mbar_init(bar_retired, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == EPI_WARPS + 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  if (lane == 0 && warp == EPI_WARPS) { tma_prefetch_desc(&tmL); tma_prefetch_desc(&tmLlo); }
+  if (lane == 0 && warp == EPI_WARPS + 2) { tma_prefetch_desc(&tmR); tma_prefetch_desc(&tmRlo); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();     // the peer's barriers exist before anything is signalled across the pair
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == EPI_WARPS || warp == EPI_WARPS + 2) {
+    // ---------------- TMA producers (each CTA, its own tiles) ----------------
+    if (lane == 0) {
+      const bool is_l = warp == EPI_WARPS;
+      const CUtensorMap* hi_map = is_l ? &tmL : &tmR;
+      const CUtensorMap* lo_map = is_l ? &tmLlo : &tmRlo;
+      const uint32_t tile_off = is_l ? 0u : (uint32_t)L_TILE;
+      const uint32_t bytes = 2u * (is_l ? 2u * L_TILE : 2u * R_TILE);         // this CTA's tiles and the peer's
+      const uint32_t leader_full = mapa(bar_full, 0);
+      long long issued = 0;
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      const bool withhold = (p.status[3] & 1) != 0;     // host-injected fault: arm nothing, load nothing
+      for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
+        const Unit u = unit_of(p, unit);
+        const int n_half = (u.cols + 31) / 32 * 16;     // columns of the pair's MMA that this CTA stages
+        const int row0 = is_l ? u.l_row + (int)rank * BM : u.r0 + (int)rank * n_half;
+        for (int i = 0; i < u.nkb; ++i) {
+          if (!mbar_wait_cluster(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 500 + s)) { ok = false; break; }
+          const uint32_t dst = smem_base + s * STAGE + tile_off;
+          const int k0 = (u.kb + i) * BK;
+          if (!withhold) {
+            if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
+            tma_load_2d_pair(dst, hi_map, k0, row0, leader_full + 8 * s);
+            tma_load_2d_pair(dst + RAW, lo_map, k0, row0, leader_full + 8 * s);
+            ++issued;
+          }
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+      }
+      if (leader && *abort_flag) {
+        // loads in flight complete on the leader's full barriers: give them (bounded) time before leaving
+        for (long long i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+          for (int spin = 0; spin < (1 << 16); ++spin)
+            if (mbar_try_wait(bar_full + 8 * (int)(i % STAGES), (uint32_t)((i / STAGES) & 1))) break;
+      }
+    }
+  } else if (warp == EPI_WARPS + 1) {
+    // ---------------- MMA issuer (leader CTA only) ----------------
+    if (leader && lane == 0) {
+      const uint64_t d_a = make_smem_desc(smem_base, 16, 8 * BK * 2, SWZ_64B);
+      const uint64_t d_b = make_smem_desc(smem_base + L_TILE, 16, 8 * BK * 2, SWZ_64B);
+      const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
+      const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
+      constexpr uint32_t LO_TILE = RAW >> 4, STAGE_STEP = STAGE >> 4;
+      const uint32_t tmem_main = tmem_base, tmem_cross = tmem_base + BN;
+      const uint32_t peer_empty = mapa(bar_empty, 1), peer_mid = mapa(bar_mid, 1);
+      int s = 0;
+      uint32_t ph = 0, stage_off = 0, dph = 0;
+      bool ok = true, pending_read_out = false;
+      for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
+        const Unit u = unit_of(p, unit);
+        if (u.nkb == 0) continue;                       // a group without rows: nothing to multiply
+        const uint32_t idesc = make_idesc_f16(2 * BM, (u.cols + 31) / 32 * 32);
+        uint32_t acc_cross = 0, accumulate = 0;
+        int to_drain = DRAIN;
+        for (int i = 0; i < u.nkb; ++i) {
+          if (to_drain == 0) {
+            mma_commit_pair(bar_mid);
+            mma_commit_pair(peer_mid);
+            pending_read_out = true;
+            accumulate = 0;
+            to_drain = DRAIN;
+          }
+          --to_drain;
+          if (!mbar_wait_cluster(bar_full + 8 * s, ph, abort_flag, p.status, 700 + s)) { ok = false; break; }
+          if (pending_read_out) {
+            // the previous read-out must be over before these MMAs overwrite the accumulators
+            if (!mbar_wait_cluster(bar_drained, dph, abort_flag, p.status, 750)) { ok = false; break; }
+            dph ^= 1;
+            pending_read_out = false;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            const uint32_t al = a_low0 + stage_off + kk * 2, bl = b_low0 + stage_off + kk * 2;    // 32 B per k-step
+            mma_f16_pair_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : acc_cross);
+            mma_f16_pair_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
+            mma_f16_pair_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
+          }
+          mma_commit_pair(bar_empty + 8 * s);           // stage free in the leader ...
+          mma_commit_pair(peer_empty + 8 * s);          // ... and in the peer
+          acc_cross = 1;
+          accumulate = 1;
+          if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
+        }
+        if (!ok) break;
+        mma_commit_pair(bar_mid);                       // tile finished: last read-out
+        mma_commit_pair(peer_mid);
+        pending_read_out = true;
+      }
+      if (*abort_flag) {
+        mma_commit_pair(bar_retired);
+        for (int spin = 0; spin < (1 << 20); ++spin)
+          if (mbar_try_wait(bar_retired, 0)) break;
+      }
+    }
+  } else if (warp < EPI_WARPS) {
+    // ---------------- epilogue warps: this CTA's 128 lanes, 128 columns per warp ----------------
+    const int q = warp & 3, half = warp >> 2;
+    const uint32_t leader_drained = mapa(bar_drained, 0);
+    const uint32_t tmem_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
+    float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE + 256) + warp * (BN / 2);
+    float acc[BN / 2];
+    uint32_t mph = 0;
+    bool ok = true;
+    for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
+      const Unit u = unit_of(p, unit);
+      const int ncc = min(BN / 2 / 16, max(0, (u.cols - half * (BN / 2) + 15) / 16));    // 16-column pieces of this thread
+      const int n_mid = u.nkb > 0 ? (u.nkb - 1) / DRAIN : -1;
+      const bool none = n_mid < 0;                        // a group without rows: zeros, and no scales
+      const int l = u.l0 + (int)rank * BM + q * 32 + lane, left = u.cols - half * (BN / 2);
+      // the scales of this thread's lane and (spread over the warp's lanes) of its columns, requested before the wait
+      const float* r_down = (p.weights ? p.r_down + (long long)u.expert * p.cols : p.r_down) + u.r0 + half * (BN / 2);
+      float col_scale[BN / 2 / 32], l_scale = 1.f, b = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < BN / 2 / 32; ++cc) col_scale[cc] = (!none && cc * 32 + lane < left) ? r_down[cc * 32 + lane] : 1.f;
+      if (l < p.lanes) {
+        if (!none) l_scale = p.l_down[(long long)u.expert * p.lanes + l];
+        if (p.bias) b = p.bias[(long long)u.expert * p.lanes + l];
+      }
+#pragma unroll
+      for (int j = 0; j < BN / 2; ++j) acc[j] = 0.f;
+      // (acc starts from zero and every read-out adds: two ways to define it in this loop cost 80 spilled registers)
+#pragma unroll 1
+      for (int ev = 0; ev <= n_mid; ++ev) {
+        ok = mbar_wait_cluster(bar_mid, mph, abort_flag, p.status, 850);
+        mph ^= 1;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int cc = 0; cc < BN / 2 / 16; ++cc) {
+          if (cc < ncc) {
+            uint32_t r[16];
+            tmem_ld_32x16(tmem_lane + cc * 16, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[cc * 16 + j] += __uint_as_float(r[j]);
+            if (ev == n_mid) {
+              tmem_ld_32x16(tmem_lane + BN + cc * 16, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[cc * 16 + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, acc[cc * 16 + j]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(leader_drained);
+      }
+      if (!ok) break;
+      // out of registers, while the tensor cores work on the pair's next tile
+      float* c = p.C + (p.weights ? u.expert * p.c_stride : 0) + (long long)(u.r0 + half * (BN / 2)) * p.ldc + l;
+      const bool live = l < p.lanes, relu = p.act == CB200_ACT_RELU;
+      // whole warps of whole tiles without a beta: about 9 instructions per value (24 with predicates, shuffles and the
+      // three factors apart, which held the epilogue to 9 us per tile where the product takes 3)
+      const bool whole = left >= BN / 2 && __all_sync(0xffffffffu, live) && p.beta == 0.f;
+#pragma unroll
+      for (int cc = 0; cc < BN / 2 / 32; ++cc) scales[cc * 32 + lane] = col_scale[cc];
+      __syncwarp();
+      auto store_whole = [&](auto with_relu) {
+        constexpr bool RELU = decltype(with_relu)::value;
+        float* to = c;
+#pragma unroll
+        for (int j0 = 0; j0 < BN / 2; j0 += 4) {
+          const float4 d = *reinterpret_cast<const float4*>(scales + j0);
+          float v[4] = {acc[j0] * (l_scale * d.x), acc[j0 + 1] * (l_scale * d.y), acc[j0 + 2] * (l_scale * d.z),
+                        acc[j0 + 3] * (l_scale * d.w)};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[j] = fmaf(v[j], p.alpha, b);
+            if (RELU) v[j] = v[j] > 0.f ? v[j] : 0.f;
+            *to = v[j];
+            to += p.ldc;
+          }
+        }
+      };
+      if (whole && relu) {
+        store_whole(std::true_type{});
+      } else if (whole) {
+        store_whole(std::false_type{});
+      } else {
+        float* to = c;
+#pragma unroll
+        for (int j0 = 0; j0 < BN / 2; j0 += 8) {
+          if (j0 < left) {
+            float old[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) old[j] = 0.f;
+            if (p.beta != 0.f) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (live && j0 + j < left) old[j] = to[(long long)j * p.ldc];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float v = fmaf(acc[j0 + j] * (l_scale * scales[j0 + j]), p.alpha, b);
+              if (p.beta != 0.f) v += p.beta * old[j];
+              if (relu) v = v > 0.f ? v : 0.f;
+              if (live && j0 + j < left) *to = v;
+              to += p.ldc;
+            }
+          }
+        }
+      }
+      __syncwarp();                                        // the list is rewritten for the next tile
+      if (p.act > CB200_ACT_RELU && live) {
+        // tanh / logistic over what was just stored: a call among 128 live accumulators would spill them
+        const int n = min(left, BN / 2);
+#pragma unroll 1
+        for (int j0 = 0; j0 < n; j0 += 8) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = j0 + j < n ? c[(long long)j * p.ldc] : 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j0 + j < n) c[(long long)j * p.ldc] = apply_act_transcendental(v[j], p.act);
+          c += 8 * p.ldc;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();     // neither CTA leaves (or frees TMEM) while the pair's MMAs may still touch it
+  if (warp == EPI_WARPS + 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = (EncodeTiledFn)f;
+  });
+  return fn;
+}
+
+int half_map(CUtensorMap* tm, const __half* base, long long rows, long long cols, long long pitch) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) { cb200_set_error("cuTensorMapEncodeTiled is not available from this driver"); return CB200_ERR_CUDA; }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * 2};
+  const cuuint32_t box[2] = {BK, BM}, ones[2] = {1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) { cb200_set_error("cuTensorMapEncodeTiled failed with %d", (int)r); return CB200_ERR_CUDA; }
+  return CB200_OK;
+}
+
+int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
+               long long rows, int cols, int kp, Plan* plan) {
+  if (cols <= 1024)
+    split_rows_kernel<32><<<(unsigned)((rows + 7) / 8), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan);
+  else if (cols <= 4096)
+    split_rows_kernel<128><<<(unsigned)((rows + 1) / 2), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan);
+  else
+    split_rows_kernel<256><<<(unsigned)rows, 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, const float* x, long long ld, long long stride,
+                  int fixed, const Entry* table, int groups_n, int rows, int cols, long long kp, Plan* plan) {
+  CB_CUDA(cudaMemsetAsync(maxima, 0, (size_t)groups_n * cols * sizeof(uint32_t), s->stream));
+  long long chunks = fixed ? (long long)groups_n * ((fixed + 63) / 64) : (rows + 63) / 64;
+  column_max_kernel<<<dim3((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535)), 128, 0, s->stream>>>(
+      maxima, x, ld, stride, fixed, table, groups_n, rows, cols);
+  CB_LAUNCH_CHECK(s);
+  long long blocks = fixed ? (long long)groups_n * ((fixed + 31) / 32) : kp / 32;
+  split_columns_kernel<<<dim3((unsigned)((cols + 63) / 64), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, s->stream>>>(
+      hi, lo, down, maxima, x, ld, stride, fixed, table, groups_n, cols, kp, plan);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long long l_rows, const __half* r_hi, const __half* r_lo,
+                long long r_rows, long long cols, long long l_pitch, long long r_pitch, const PairArgs& a, long long units) {
+  static std::once_flag once[64];
+  static cudaError_t result[64];
+  const int dev = s->device & 63;
+  std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(expert_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+  if (result[dev] != cudaSuccess) return cb200_cuda_fail(result[dev], "cudaFuncSetAttribute", __FILE__, __LINE__);
+  CUtensorMap tmL, tmLlo, tmR, tmRlo;
+  int rc;
+  if ((rc = half_map(&tmL, l_hi, l_rows, cols, l_pitch)) || (rc = half_map(&tmLlo, l_lo, l_rows, cols, l_pitch)) ||
+      (rc = half_map(&tmR, r_hi, r_rows, cols, r_pitch)) || (rc = half_map(&tmRlo, r_lo, r_rows, cols, r_pitch)))
+    return rc;
+  const long long clusters = units < s->sm_count / 2 ? units : s->sm_count / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * clusters), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = s->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, expert_pair_kernel, tmL, tmLlo, tmR, tmRlo, a);
+  if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaLaunchKernelEx(expert_pair_kernel)", __FILE__, __LINE__);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+inline long long up8(long long v) { return (v + 7) / 8 * 8; }
+inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Pieces of the stream's workspace, each on a 256-byte boundary.
+struct Carve {
+  char* base;
+  size_t used;
+  template <typename T> T* take(size_t n) {
+    T* p = (T*)(base + used);
+    used += up256(n * sizeof(T));
+    return p;
+  }
+};
+
+constexpr size_t MOST_WORKSPACE = (size_t)2 << 30;
+
+}  // namespace
+
+// Is this product better off here?  Both sides' times by the sizes, in microseconds: `split` bytes are read and written
+// once at 5.5 TB/s, and again where the reduction axis is not contiguous.
+bool cb200_expert_f16_ok(cb200_stream* s, int trans_b, long long rows, long long K, long long N, long long experts) {
+  if (s->opt_gemm_auto_presplit == 1) return false;
+  const double l = (double)experts * N * K, r = (double)rows * K;
+  if ((l + r) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
+  if (s->opt_gemm_auto_presplit == 2) return true;
+  const double flops = 2.0 * rows * N * K;
+  const double here = 20.0 + (l * (trans_b ? 8 : 12) + r * 8) / 5.5e6 + flops / 330e6, there = flops / 130e6;
+  return rows >= 96 * experts && here < there;
+}
+bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
+  if (s->opt_gemm_auto_presplit == 1) return false;
+  const double operands = (double)(rows + 32 * experts) * (M + N);
+  if (operands * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
+  if (s->opt_gemm_auto_presplit == 2) return true;
+  const double flops = 2.0 * rows * N * M;
+  const double here = 25.0 + operands * 12 / 4.5e6 + flops / 330e6, there = flops / 85e6;
+  return rows >= 64 * experts && here < there;
+}
+
+// The flag that the guarded 3xTF32 launch reads is returned through `guard`.
+int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
+                          long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
+                          const int* offsets, const float* bias, int act, const int** guard_out) {
+  DeviceGuard guard(s->device);
+  const long long kp = up8(K), l_rows = (long long)experts * N;
+  const size_t tiles = (size_t)((rows + BN - 1) / BN + (experts < rows ? experts : rows));
+  const size_t maxima_n = trans_b ? 0 : (size_t)l_rows;
+  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + 2 * up256((size_t)l_rows * kp * 2) +
+                       2 * up256((size_t)rows * kp * 2) + up256((size_t)l_rows * 4) + up256((size_t)rows * 4) + up256(maxima_n * 4);
+  void* ws = nullptr;
+  int rc = cb200_scratch(s, bytes, &ws);
+  if (rc) return rc;
+  Carve w = {(char*)ws, 0};
+  Plan* plan = w.take<Plan>(1);
+  Entry* table = w.take<Entry>(tiles + 1);
+  __half* l_hi = w.take<__half>((size_t)l_rows * kp);
+  __half* l_lo = w.take<__half>((size_t)l_rows * kp);
+  __half* r_hi = w.take<__half>((size_t)rows * kp);
+  __half* r_lo = w.take<__half>((size_t)rows * kp);
+  float* l_down = w.take<float>((size_t)l_rows);
+  float* r_down = w.take<float>((size_t)rows);
+  uint32_t* maxima = w.take<uint32_t>(maxima_n);
+  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, offsets, experts, rows, 0, s->status_dev);
+  CB_LAUNCH_CHECK(s);
+  if ((rc = split_rows(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan))) return rc;
+  if (trans_b) rc = split_rows(s, l_hi, l_lo, l_down, B, ldb, b_stride, N, l_rows, K, (int)kp, plan);
+  else rc = split_columns(s, l_hi, l_lo, l_down, maxima, B, ldb, b_stride, K, table, experts, 0, N, kp, plan);
+  if (rc) return rc;
+  PairArgs a;
+  a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = l_down; a.r_down = r_down; a.bias = bias; a.plan = plan; a.table = table;
+  a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.experts = experts; a.weights = 0; a.act = act;
+  a.alpha = alpha; a.beta = beta;
+  *guard_out = &plan->flag;
+  return launch_pair(s, l_hi, l_lo, l_rows, r_hi, r_lo, rows, K, kp, kp, a, (long long)tiles * ((N + 2 * BM - 1) / (2 * BM)));
+}
+
+int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows, int M,
+                             long long lda, const float* B, int N, long long ldb, int experts, float beta, const int* offsets,
+                             const int** guard_out) {
+  DeviceGuard guard(s->device);
+  // C_e[m, n] = sum A[r, m] B[r, n]: n in the lanes, m in the columns
+  const long long kp = ((long long)rows + 31LL * (experts < rows ? experts : rows) + 31) / 32 * 32;
+  const size_t bytes = up256(sizeof(Plan)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
+                       2 * up256((size_t)M * kp * 2) + 2 * up256((size_t)experts * N * 4) + 2 * up256((size_t)experts * M * 4);
+  void* ws = nullptr;
+  int rc = cb200_scratch(s, bytes, &ws);
+  if (rc) return rc;
+  Carve w = {(char*)ws, 0};
+  Plan* plan = w.take<Plan>(1);
+  Entry* table = w.take<Entry>((size_t)experts + 1);
+  __half* l_hi = w.take<__half>((size_t)N * kp);
+  __half* l_lo = w.take<__half>((size_t)N * kp);
+  __half* r_hi = w.take<__half>((size_t)M * kp);
+  __half* r_lo = w.take<__half>((size_t)M * kp);
+  float* l_down = w.take<float>((size_t)experts * N);
+  float* r_down = w.take<float>((size_t)experts * M);
+  uint32_t* l_max = w.take<uint32_t>((size_t)experts * N);
+  uint32_t* r_max = w.take<uint32_t>((size_t)experts * M);
+  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, offsets, experts, rows, 1, s->status_dev);
+  CB_LAUNCH_CHECK(s);
+  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, B, ldb, 0, 0, table, experts, rows, N, kp, plan))) return rc;
+  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, A, lda, 0, 0, table, experts, rows, M, kp, plan))) return rc;
+  PairArgs a;
+  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.table = table;
+  a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
+  a.alpha = alpha; a.beta = beta;
+  *guard_out = &plan->flag;
+  return launch_pair(s, l_hi, l_lo, N, r_hi, r_lo, M, kp, kp, kp, a,
+                     (long long)experts * ((M + BN - 1) / BN) * ((N + 2 * BM - 1) / (2 * BM)));
+}

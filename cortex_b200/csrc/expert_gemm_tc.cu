@@ -38,7 +38,9 @@ template <int BN> struct Cfg {
 struct Grouped {
   GemmParams g;
   const int* offsets;
+  const int* only_if;      // null, or a device word: do nothing while it is zero
   int experts, rows;
+  int units;               // tiles
   int chunk;               // k-blocks between roundings of the accumulators
   long long c_stride;      // WEIGHTS: distance of the experts' results
   int tiles_m;             // WEIGHTS: row tiles of one result
@@ -57,9 +59,11 @@ struct RowsArgs {
   const int* offsets;
   int* status;
   int N, K, experts, rows;
+  int units;                   // most tiles there can be
   int w_mn;                    // the matrices are [K, N]: N is their contiguous axis
   int act;
   float alpha, beta;
+  const int* only_if;          // null, or a device word: do nothing while it is zero
   int chunk;                   // k-blocks between roundings of the accumulators
   int slices;                  // CTAs of a cluster that share a tile, each over a slice of K
 };
@@ -116,13 +120,26 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   int* where = (int*)(tmem_slot + 2);                        // {found, expert, lo, hi, index}
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.only_if && *p.only_if == 0) return;
   const int tiles_n = (p.N + BM - 1) / BM;
-  const int unit = (int)blockIdx.x / p.slices, slice = (int)blockIdx.x - unit * p.slices;
-  const int n0 = (unit % tiles_n) * BM;
-
+  const int first_unit = (int)blockIdx.x / p.slices, slice = (int)blockIdx.x - first_unit * p.slices;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_full = smem_u32(bars), bar_conv = smem_u32(bars + STAGES), bar_empty = smem_u32(bars + 2 * STAGES),
                  bar_acc = smem_u32(bars + 3 * STAGES), bar_read = bar_acc + 8;
+  if (warp == CONV_WARPS + 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == CONV_WARPS && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  int inject = 0;
+  if (warp == CONV_WARPS) inject = p.status[3];
+  // One tile per CTA; a guarded launch (only_if) has a small grid whose CTAs take tiles in turn.
+#pragma unroll 1
+  for (int unit = first_unit; unit < p.units; unit += (int)gridDim.x / p.slices) {
+  const int n0 = (unit % tiles_n) * BM;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
@@ -134,27 +151,17 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == CONV_WARPS + 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
-    tmem_relinquish();
-  }
-  if (warp == CONV_WARPS && lane == 0) {
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmX);
-  }
   if (warp == 1) {
     groups::Tile t = {0, 0, 0, 0};
     const bool found = groups::find_tile(p.offsets, p.experts, p.rows, BN, unit / tiles_n, p.status, t);
     if (lane == 0) { where[0] = found; where[1] = t.expert; where[2] = t.lo; where[3] = t.hi; where[4] = t.index; }
   }
-  int inject = 0;
-  if (warp == CONV_WARPS) inject = p.status[3];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   if (!where[0]) {
-    // no such tile: with K slices every CTA of the tile's cluster leaves here
+    // no such tile (and none behind it): with K slices every CTA of the tile's cluster leaves here
     if (warp == CONV_WARPS + 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
     return;
   }
@@ -346,9 +353,17 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
     cluster_sync_all();
   }
-  if (warp == CONV_WARPS + 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  const bool more = unit + (int)gridDim.x / p.slices < p.units && !*abort_flag;
+  __syncthreads();
+  if (!more) {
+    if (warp == CONV_WARPS + 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+    return;
+  }
+  if (threadIdx.x == 0)
+    for (int s = 0; s < 3 * STAGES + 2; ++s) mbar_inval(bar_full + 8 * s);
   }
 }
 
@@ -369,14 +384,28 @@ expert_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
   int* where = (int*)(tmem_slot + 3);                      // {found, expert, lo, hi, index}
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  GemmParams p = args.g;
-  const int tiles_n = (p.N + BN - 1) / BN;
-  const int unit = (int)blockIdx.x / p.ksplit_n, k_slice = (int)blockIdx.x - unit * p.ksplit_n;
-  const int n0 = (unit % tiles_n) * BN;
+  if (args.only_if && *args.only_if == 0) return;
+  const int tiles_n = (args.g.N + BN - 1) / BN;
+  const int first_unit = (int)blockIdx.x / args.g.ksplit_n, k_slice = (int)blockIdx.x - first_unit * args.g.ksplit_n;
 
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_full = smem_u32(bars), bar_conv = smem_u32(bars + STAGES), bar_empty = smem_u32(bars + 2 * STAGES),
                  bar_acc = smem_u32(bars + 3 * STAGES), bar_read = bar_acc + 8;
+  if (warp == CONV_WARPS + 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == CONV_WARPS && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  int inject = 0;
+  if (warp == CONV_WARPS) inject = args.g.status[3];
+  // One tile per CTA; a guarded launch (only_if) has a small grid whose CTAs take tiles in turn.
+#pragma unroll 1
+  for (int unit = first_unit; unit < args.units; unit += (int)gridDim.x / args.g.ksplit_n) {
+  GemmParams p = args.g;
+  const int n0 = (unit % tiles_n) * BN;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
@@ -388,14 +417,6 @@ expert_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == CONV_WARPS + 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
-    tmem_relinquish();
-  }
-  if (warp == CONV_WARPS && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
-  }
   if (warp == 1) {
     groups::Tile t = {0, 0, 0, 0};
     const int m_tile = unit / tiles_n;
@@ -404,8 +425,6 @@ expert_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
     groups::group_rows(args.offsets, args.rows, t.expert, p.status, t.lo, t.hi);
     if (lane == 0) { where[0] = t.expert; where[1] = t.lo; where[2] = t.hi; where[3] = t.index; }
   }
-  int inject = 0;
-  if (warp == CONV_WARPS) inject = p.status[3];
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -572,9 +591,17 @@ expert_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_cons
 
   tc_fence_before();
   __syncthreads();
-  if (warp == CONV_WARPS + 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  const bool more = unit + (int)gridDim.x / args.g.ksplit_n < args.units && !*abort_flag;
+  __syncthreads();
+  if (!more) {
+    if (warp == CONV_WARPS + 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, C::TMEM_COLS);
+    }
+    return;
+  }
+  if (threadIdx.x == 0)
+    for (int s = 0; s < 3 * STAGES + 2; ++s) mbar_inval(bar_full + 8 * s);
   }
 }
 
@@ -694,7 +721,7 @@ bool cb200_expert_tc_ok(const void* A, long long lda, const void* B, long long l
 
 int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
                          long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
-                         const int* offsets, const float* bias, int act) {
+                         const int* offsets, const float* bias, int act, const int* only_if) {
   DeviceGuard guard(s->device);
   // how many rows a tile may take: what an even split of the rows over the experts fills
   const long long even = (rows + experts - 1) / experts;
@@ -708,11 +735,11 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   const int forced = s->opt_gemm_k_slices;
   for (int sl = 2; sl <= 8; sl *= 2)
     if ((forced > 0 ? sl <= forced : units * sl <= s->sm_count) && nkb / sl >= 4) slices = sl;
-  if ((nkb + slices - 1) / slices > chunk) slices = 1;
+  if ((nkb + slices - 1) / slices > chunk || only_if) slices = 1;
   RowsArgs a;
   a.C = C; a.ldc = ldc; a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
   a.N = N; a.K = K; a.experts = experts; a.rows = rows; a.w_mn = trans_b ? 0 : 1; a.act = act;
-  a.alpha = alpha; a.beta = beta; a.chunk = chunk; a.slices = slices;
+  a.alpha = alpha; a.beta = beta; a.chunk = chunk; a.slices = slices; a.only_if = only_if;
   const CUtensorMapSwizzle swz = bk == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tmW, tmX;
   int rc = tmap_2d(&tmX, A, rows, K, lda, bk, BN < 64 ? BN : 64, swz);
@@ -720,7 +747,9 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   if (trans_b) rc = tmap_3d(&tmW, B, experts, N, K, ldb, b_stride, bk, BM, swz);
   else rc = tmap_3d(&tmW, B, experts, K, N, ldb, b_stride, 32, bk, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
   if (rc) return rc;
-  const long long ctas = units * slices;
+  CB_REQUIRE(units <= 2147483647LL, "expert_gemm: too many tiles");
+  a.units = (int)units;
+  const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
   if (BN == 256) return launch<RowsArgs, expert_rows_kernel<256, 16>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, slices);
   if (BN == 128) return launch<RowsArgs, expert_rows_kernel<128, 16>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, slices);
   if (BN == 64) return launch<RowsArgs, expert_rows_kernel<64, 32>>(s, RowsCfg<64, 32>::SMEM, tmW, tmX, a, ctas, slices);
@@ -729,19 +758,22 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
 
 int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
                             int M, long long lda, const float* B, int N, long long ldb, int experts, float beta,
-                            const int* offsets) {
+                            const int* offsets, const int* only_if) {
   DeviceGuard guard(s->device);
   Grouped a;
   common(a.g, s, C, ldc, M, N, 0, alpha, beta, nullptr, CB200_ACT_NONE);
   a.g.a_mn_major = a.g.b_mn_major = 1;
-  a.offsets = offsets; a.experts = experts; a.rows = rows; a.chunk = CHUNK; a.c_stride = c_stride;
+  a.offsets = offsets; a.experts = experts; a.rows = rows; a.chunk = CHUNK; a.c_stride = c_stride; a.only_if = only_if;
   a.tiles_m = (M + BM - 1) / BM;
   const long long tiles_m = (long long)a.tiles_m * experts;
   int BN, slices;
-  choose(s, tiles_m, N, (rows / experts + BK) / BK, 16, BN, slices);
+  choose(s, tiles_m, N, (rows / experts + BK) / BK, only_if ? 1 : 16, BN, slices);
   a.g.ksplit_n = slices;
   int rc;
   const long long units = tiles_m * ((N + BN - 1) / BN);
+  CB_REQUIRE(units <= 2147483647LL, "expert_gemm_weights: too many tiles");
+  a.units = (int)units;
+  const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
   if (slices > 1) {
     // slices meet in L2: how long a slice is depends on the groups, so it may take several chunks
     void* ws = nullptr;
@@ -752,7 +784,7 @@ int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long 
   CUtensorMap tmA, tmB;
   if ((rc = tmap_2d(&tmA, A, rows, M, lda, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
   if ((rc = tmap_2d(&tmB, B, rows, N, ldb, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
-  if (BN == 256) return launch<Grouped, expert_weights_kernel<256>>(s, Cfg<256>::SMEM, tmA, tmB, a, units * slices, 1);
-  if (BN == 128) return launch<Grouped, expert_weights_kernel<128>>(s, Cfg<128>::SMEM, tmA, tmB, a, units * slices, 1);
-  return launch<Grouped, expert_weights_kernel<64>>(s, Cfg<64>::SMEM, tmA, tmB, a, units * slices, 1);
+  if (BN == 256) return launch<Grouped, expert_weights_kernel<256>>(s, Cfg<256>::SMEM, tmA, tmB, a, ctas, 1);
+  if (BN == 128) return launch<Grouped, expert_weights_kernel<128>>(s, Cfg<128>::SMEM, tmA, tmB, a, ctas, 1);
+  return launch<Grouped, expert_weights_kernel<64>>(s, Cfg<64>::SMEM, tmA, tmB, a, ctas, 1);
 }

@@ -553,3 +553,52 @@ def test_bias_of_a_layer_may_start_anywhere(stream):
         nn.Linear(ct.to_tensor(W, "float"), bias).forward_fused(ct.to_tensor(X, "float"), Y, "relu")
         want, size = plain.expert_gemm(np.zeros((40, 36)), True, 1.0, X, W[None], 0.0, [0, 40], flat[None, at:at + 36], "relu")
         _within(ct.to_array(Y), want, size, _product_tol("float", 64), at)
+
+
+@pytest.mark.parametrize("route", [0, 1, 2])
+@pytest.mark.parametrize("n,k", [(256, 64), (260, 2600), (500, 129), (33, 40)])
+def test_expert_gemm_scaled_halves(stream, route, n, k):
+    """The three ways an fp32 product can go (by size, never / always through scaled halves), all directions, on data that
+    fits them, that spans too wide a range, that is too large, and with an infinity in one group."""
+    rng = np.random.default_rng(71)
+    stream.set_option("gemm-auto-presplit", route)
+    sizes = [300, 0, 1, 256, 90, 31]
+    rows, e = sum(sizes) + 7, len(sizes)
+    off = ct.to_tensor(_offsets(sizes), "int")
+    for data in ("plain", "scaled", "wide", "large", "inf"):
+        X, dY, W = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (rows, n), (e, n, k)))
+        if data == "scaled":                                   # every row and column at a scale of its own
+            X *= np.exp2(rng.integers(-18, 18, (rows, 1))).astype(np.float32)
+            W *= np.exp2(rng.integers(-12, 12, (e, n, 1))).astype(np.float32)
+            dY *= np.exp2(rng.integers(-12, 12, (1, n))).astype(np.float32)
+        elif data == "wide":                                   # one value that dwarfs its row, and meets a zero
+            X[:, 0], W[:, :, 0], dY[0] = -3e38, 0.0, 0.0
+            X[0] = 0.0
+        elif data == "large":
+            X *= np.float32(1e25)
+        elif data == "inf":
+            X[305, 3] = np.inf                                  # group 3: rows 301 .. 557
+        Y0, W0 = rng.standard_normal((rows, n)).astype(np.float32), rng.standard_normal((e, n, k)).astype(np.float32)
+        Y, dX, dW = ct.to_tensor(Y0, "float"), ct.new_tensor([rows, k], "float"), ct.to_tensor(W0, "float")
+        Xt, dYt, Wt = ct.to_tensor(X, "float"), ct.to_tensor(dY, "float"), ct.to_tensor(W, "float")
+        ct.expert_gemm(Y, True, 0.5, Xt, Wt, 0.5, off)
+        ct.expert_gemm(dX, False, 1.0, dYt, Wt, 0.0, off)
+        ct.expert_gemm_weights(dW, 1.0, dYt, Xt, 1.0, off)
+        stream.sync()
+        keep = np.ones(rows, bool)
+        keep_e = np.ones(e, bool)
+        if data == "inf":
+            keep[305], keep_e[3] = False, False
+        with np.errstate(all="ignore"):
+            want, size = plain.expert_gemm(Y0, True, 0.5, X, W, 0.5, _offsets(sizes))
+            want_x, size_x = plain.expert_gemm(np.zeros((rows, k)), False, 1.0, dY, W, 0.0, _offsets(sizes))
+            want_w, size_w, _, _ = plain.expert_gemm_weights(W0, 1.0, dY, X, 1.0, _offsets(sizes))
+        if data == "wide":
+            size_w[:, :, 0] = np.inf                            # sums of the giant values themselves: anything near them goes
+        _within(ct.to_array(Y).reshape(rows, n)[keep], want[keep], size[keep], _product_tol("float", k), (data, "forward"))
+        _within(ct.to_array(dX), want_x, size_x, _product_tol("float", n), (data, "input"))
+        got_w = ct.to_array(dW).reshape(e, n, k)
+        if data != "wide":
+            _within(got_w[keep_e], want_w[keep_e], size_w[keep_e], _product_tol("float", 300), (data, "weights"))
+        else:
+            _within(got_w[:, :, 1:], want_w[:, :, 1:], size_w[:, :, 1:], _product_tol("float", 300), (data, "weights"))
