@@ -33,7 +33,7 @@ namespace {
 
 constexpr int BM = 128, BN = 256, BK = 32;               // per CTA: 128 lanes, 256 columns of the pair, 32 halves of k
 constexpr int EPI_WARPS = 8;
-constexpr int THREADS = (EPI_WARPS + 3) * 32;
+constexpr int THREADS = (EPI_WARPS + 4) * 32;            // three warpgroups; the last warp only gives its registers up
 constexpr int L_TILE = BM * BK * 2, R_TILE = BN / 2 * BK * 2;       // 8 KiB each
 constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
 constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
@@ -327,23 +327,28 @@ struct PairArgs {
 
 struct Unit { int expert, l0, r0, cols, l_row, kb, nkb; };
 
-__device__ __forceinline__ Unit unit_of(const PairArgs& p, int unit) {
+// The table entry of a unit: requested one unit ahead, so that its latency is not between two tiles.
+__device__ __forceinline__ Entry entry_of(const PairArgs& p, int unit, int n_units) {
+  const int tiles_l = (p.lanes + 2 * BM - 1) / (2 * BM);
+  int row = min(unit, n_units - 1) / tiles_l;
+  if (p.weights) row /= (p.cols + BN - 1) / BN;
+  const int4 v = __ldg(reinterpret_cast<const int4*>(p.table) + row);
+  return {v.x, v.y, v.z, v.w};
+}
+__device__ __forceinline__ Unit unit_of(const PairArgs& p, int unit, const Entry& e) {
   const int tiles_l = (p.lanes + 2 * BM - 1) / (2 * BM);
   Unit u;
   const int row = unit / tiles_l;
+  u.expert = e.expert;
   u.l0 = (unit - row * tiles_l) * 2 * BM;
   if (p.weights) {
     const int tiles_r = (p.cols + BN - 1) / BN;
-    u.expert = row / tiles_r;
-    const Entry e = p.table[u.expert];
-    u.r0 = (row - u.expert * tiles_r) * BN;
+    u.r0 = (row - e.expert * tiles_r) * BN;
     u.cols = min(BN, p.cols - u.r0);
     u.l_row = u.l0;
     u.kb = e.first / BK;
     u.nkb = (e.hi - e.lo + BK - 1) / BK;
   } else {
-    const Entry e = p.table[row];
-    u.expert = e.expert;
     u.r0 = e.lo;
     u.cols = min(BN, e.hi - e.lo);
     u.l_row = e.expert * p.lanes + u.l0;
@@ -415,6 +420,10 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  // Registers: 384 threads are launched with 168 each; an epilogue thread holds 128 accumulators and wants more than the
+  // 40 that leaves, and the third warpgroup needs few: 2 x 216 + 72 = 3 x 168.
+  if (warp >= EPI_WARPS) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == EPI_WARPS || warp == EPI_WARPS + 2) {
     // ---------------- TMA producers (each CTA, its own tiles) ----------------
     if (lane == 0) {
@@ -430,7 +439,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       bool ok = true;
       const bool withhold = (p.status[3] & 1) != 0;     // host-injected fault: arm nothing, load nothing
       for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
-        const Unit u = unit_of(p, unit);
+        const Unit u = unit_of(p, unit, entry_of(p, unit, n_units));
         const int n_half = (u.cols + 31) / 32 * 16;     // columns of the pair's MMA that this CTA stages
         const int row0 = is_l ? u.l_row + (int)rank * BM : u.r0 + (int)rank * n_half;
         for (int i = 0; i < u.nkb; ++i) {
@@ -466,8 +475,10 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       int s = 0;
       uint32_t ph = 0, stage_off = 0, dph = 0;
       bool ok = true, pending_read_out = false;
+      Entry next = n_units > 0 ? entry_of(p, cluster_id, n_units) : Entry{0, 0, 0, 0};
       for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
-        const Unit u = unit_of(p, unit);
+        const Unit u = unit_of(p, unit, next);
+        next = entry_of(p, unit + n_clusters, n_units);
         if (u.nkb == 0) continue;                       // a group without rows: nothing to multiply
         const uint32_t idesc = make_idesc_f16(2 * BM, (u.cols + 31) / 32 * 32);
         uint32_t acc_cross = 0, accumulate = 0;
@@ -513,8 +524,10 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
           if (mbar_try_wait(bar_retired, 0)) break;
       }
     }
-  } else if (warp < EPI_WARPS) {
+  }
+  } else {
     // ---------------- epilogue warps: this CTA's 128 lanes, 128 columns per warp ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int q = warp & 3, half = warp >> 2;
     const uint32_t leader_drained = mapa(bar_drained, 0);
     const uint32_t tmem_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
@@ -522,9 +535,11 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
     float acc[BN / 2];
     uint32_t mph = 0;
     bool ok = true;
+    Entry next = n_units > 0 ? entry_of(p, cluster_id, n_units) : Entry{0, 0, 0, 0};
     for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
-      const Unit u = unit_of(p, unit);
-      const int ncc = min(BN / 2 / 16, max(0, (u.cols - half * (BN / 2) + 15) / 16));    // 16-column pieces of this thread
+      const Unit u = unit_of(p, unit, next);
+      next = entry_of(p, unit + n_clusters, n_units);
+      const int ncc = min(BN / 2 / 32, max(0, (u.cols - half * (BN / 2) + 31) / 32));    // 32-column pieces of this thread
       const int n_mid = u.nkb > 0 ? (u.nkb - 1) / DRAIN : -1;
       const bool none = n_mid < 0;                        // a group without rows: zeros, and no scales
       const int l = u.l0 + (int)rank * BM + q * 32 + lane, left = u.cols - half * (BN / 2);
@@ -548,18 +563,18 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
-        for (int cc = 0; cc < BN / 2 / 16; ++cc) {
+        for (int cc = 0; cc < BN / 2 / 32; ++cc) {
           if (cc < ncc) {
-            uint32_t r[16];
-            tmem_ld_32x16(tmem_lane + cc * 16, r);
+            uint32_t r[32];
+            tmem_ld_32x32(tmem_lane + cc * 32, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[cc * 16 + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 32; ++j) acc[cc * 32 + j] += __uint_as_float(r[j]);
             if (ev == n_mid) {
-              tmem_ld_32x16(tmem_lane + BN + cc * 16, r);
+              tmem_ld_32x32(tmem_lane + BN + cc * 32, r);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) acc[cc * 16 + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, acc[cc * 16 + j]);
+              for (int j = 0; j < 32; ++j) acc[cc * 32 + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, acc[cc * 32 + j]);
             }
           }
         }
