@@ -1,11 +1,11 @@
 // Large fp32 products grouped by expert at twice the rate of 3xTF32: operands as pairs of scaled halves.
 //
 // The tensor core multiplies fp16 at twice the rate of tf32 with the same 11-bit significands, so the split
-//   x * s = h1 + 2^-11 h2,   h1 = half(x * s),  h2 = half(2^11 (x * s - h1)),   s = a power of two per operand row
+//   x * s = h1 + h2,   h1 = half(x * s),  h2 = half(x * s - h1),   s = a power of two per operand row
 // carries 22 bits like hi + lo of 3xTF32 does, and the three products h1 h1, h1 h2, h2 h1 cost half of what they cost
-// there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-29 of
-// it keep their 22 bits, smaller ones an absolute error of 2^-50 of it.  Rows for which that is not good enough -- more
-// than 1 in 64 values (not counting zeros) below 2^-29 of the row's largest, a largest value outside [2^-48, 2^60], an
+// there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-17 of
+// it keep their 22 bits, smaller ones an absolute error of 2^-39 of it.  Rows for which that is not good enough -- more
+// than 1 in 64 values (not counting zeros) below 2^-17 of the row's largest, a largest value outside [2^-48, 2^60], an
 // infinity or a NaN -- raise a flag in device memory; the kernel here then does nothing and the 3xTF32 kernel launched
 // behind it, which otherwise does nothing, does the work.  So results have the accuracy of gemm! whatever the data.
 //
@@ -17,8 +17,13 @@
 // pipeline stages of 32 KB, as the pre-split layer GEMM: every TMA load is a plain one into the issuing CTA, completing on
 // the leader's barrier.  Output features (expert_gemm) or input features (expert_gemm_weights) lie in the lanes, so a warp
 // stores 128 consecutive bytes; the ragged rows (or output features) lie in the columns, in multiples of 32.
-// The tensor core adds with truncation: after every 2048 values of k the epilogue warps add the main accumulator into
-// registers (round to nearest) and it restarts from zero.
+// All three products go to one accumulator of 256 columns, so TMEM holds two: the tensor cores fill one while the epilogue
+// warps empty the other.  (With the cross terms in an accumulator of their own, scaled by 2^11 for range, there was room
+// for one tile, and the read-out and its hand-shakes cost 5 us per tile where the product of a weight gradient takes 3:
+// 125 us against 117 for 8000 rows over 32 experts,
+// 2048 x 1024.)  The tensor core adds with truncation: every 512 values of
+// k -- 96 additions, 3e-6 of an all-positive sum -- the accumulator is added into registers, rounded to nearest, and the
+// other one takes over.
 #include "gemm3x_common.cuh"
 #include "expert_groups.cuh"
 #include <cuda_fp16.h>
@@ -39,7 +44,7 @@ constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
 constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
 constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES;
 constexpr int TMEM_COLS = 2 * BN;
-constexpr int DRAIN = 2048 / BK;
+constexpr int DRAIN = 512 / BK;                         // stages per accumulator filling
 
 // what one warp works out at the start of a call, in device memory
 struct Plan {
@@ -52,8 +57,8 @@ struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); ex
 
 // bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
 // entry per tile of BN rows.
-__global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, const int* offsets, int experts, int rows, int weights,
-                                                  int* status) {
+__global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int* owner, const int* offsets, int experts, int rows,
+                                                  int weights, int* status) {
   const int lane = threadIdx.x;
   int carry_max = 0, carry = 0;
   bool bad = false;
@@ -87,8 +92,10 @@ __global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, cons
     }
     sum += carry;
     if (e < experts) {
-      if (weights) table[e] = {e, lo, hi, sum - mine};
-      else for (int i = 0; i < mine; ++i) table[sum - mine + i] = {e, lo + i * BN, hi, 0};
+      if (weights) {
+        table[e] = {e, lo, hi, sum - mine};
+        for (int i = 0; i < mine; i += BK) owner[(sum - mine + i) / BK] = e;      // whose the next 32 positions are
+      } else for (int i = 0; i < mine; ++i) table[sum - mine + i] = {e, lo + i * BN, hi, 0};
     }
     carry_max = __shfl_sync(0xffffffffu, run, 31);
     carry = __shfl_sync(0xffffffffu, sum, 31);
@@ -114,9 +121,9 @@ __device__ __forceinline__ bool scale_of(uint32_t max_bits, float& up, float& do
 }
 __device__ __forceinline__ void split_half(float y, __half& h1, __half& h2, int& tiny) {
   h1 = __float2half_rn(y);
-  h2 = __float2half_rn((y - __half2float(h1)) * 2048.f);
+  h2 = __float2half_rn(y - __half2float(h1));
   const float a = fabsf(y);
-  tiny += a < 6.103515625e-5f && a > 0.f;                  // below 2^-14: 2^-29 of the row's largest
+  tiny += a < 0.125f && a > 0.f;                           // 2^-17 of the row's largest: h2 leaves the normal halves
 }
 union Half8 { __half h[8]; uint4 v; };
 
@@ -208,24 +215,44 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
 }
 
 // Operands whose reduction runs down their columns, in groups of rows: rows of group g are table[g].lo .. hi (ragged) or
-// g * fixed .. (g + 1) * fixed (the experts' matrices, `stride` apart).
-__device__ __forceinline__ const float* grouped_row(const float* x, long long ld, long long stride, int fixed, int group, int r) {
-  return fixed ? x + group * stride + (long long)r * ld : x + (long long)r * ld;
-}
-
-// maxima[g][c] = bits of the largest magnitude in column c of group g; 64 rows per CTA
+// rows 0 .. fixed of the matrix x + g * stride (the experts' matrices).
+// maxima[g][c] = bits of the largest magnitude in column c of group g.  A CTA: 128 columns of up to 64 rows of one group at a
+// time, four rows side by side and (where the rows are 16-byte aligned) four columns per thread.
+template <int V>
 __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const float* x, long long ld, long long stride, int fixed,
                                                          const Entry* table, int groups_n, int rows, int cols) {
-  const int c = blockIdx.x * 128 + threadIdx.x;
-  if (c >= cols) return;
+  constexpr int LANES = 128 / V, SIDE = 128 / LANES;       // threads per row, rows side by side
+  struct alignas(4 * V) Pack { float e[V]; };
+  __shared__ uint32_t part[SIDE][128];
+  const int tx = threadIdx.x % LANES, ty = threadIdx.x / LANES, c = blockIdx.x * 128 + tx * V;
+  const bool live = c < cols;                              // V = 4: cols is a multiple of 4
+  auto reduce = [&](int g, const float* first, int a, int z) {           // rows a .. z - 1 of group g, row r at first + r * ld
+    uint32_t m[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) m[j] = 0;
+    if (live) {
+#pragma unroll 4
+      for (int r = a + ty; r < z; r += SIDE) {
+        const Pack v = *reinterpret_cast<const Pack*>(first + (long long)r * ld + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) m[j] = max(m[j], __float_as_uint(v.e[j]) & 0x7fffffffu);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[ty][tx * V + j] = m[j];
+    __syncthreads();
+    uint32_t all = part[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < SIDE; ++i) all = max(all, part[i][threadIdx.x]);
+    const int at = blockIdx.x * 128 + threadIdx.x;
+    if (at < cols) atomicMax(maxima + (long long)g * cols + at, all);
+    __syncthreads();
+  };
   if (fixed) {
     const int chunks = (fixed + 63) / 64;
     for (long long b = blockIdx.y; b < (long long)groups_n * chunks; b += gridDim.y) {
-      const int g = (int)(b / chunks), r0 = (int)(b - (long long)g * chunks) * 64, r1 = min(fixed, r0 + 64);
-      uint32_t m = 0;
-#pragma unroll 8
-      for (int r = r0; r < r1; ++r) m = max(m, __float_as_uint(grouped_row(x, ld, stride, fixed, g, r)[c]) & 0x7fffffffu);
-      atomicMax(maxima + (long long)g * cols + c, m);
+      const int g = (int)(b / chunks), r0 = (int)(b - (long long)g * chunks) * 64;
+      reduce(g, x + g * stride, r0, min(fixed, r0 + 64));
     }
     return;
   }
@@ -238,75 +265,82 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const
     }
     for (; g < groups_n && table[g].lo < r1; ++g) {
       const int a = max(r0, table[g].lo), z = min(r1, table[g].hi);
-      uint32_t m = 0;
-#pragma unroll 8
-      for (int r = a; r < z; ++r) m = max(m, __float_as_uint(x[(long long)r * ld + c]) & 0x7fffffffu);
-      if (z > a) atomicMax(maxima + (long long)g * cols + c, m);
+      if (z > a) reduce(g, x, a, z);
     }
   }
 }
 
-// hi / lo [cols (x groups where fixed)][positions]: 32 positions x 64 columns per CTA through shared memory.  Ragged groups
-// start at a multiple of 32 positions and are padded with zeros; fixed ones have rows of their own (pitch kp >= fixed).
+// hi / lo [cols (x groups where fixed)][positions]: 32 positions x 64 columns at a time through shared memory.  Ragged groups
+// start at a multiple of 32 positions and are padded with zeros (owner: which group the next 32 positions belong to); fixed
+// ones have rows of their own (pitch kp >= fixed).  A CTA takes two neighbouring blocks of 64 columns.
 __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* lo, float* down_out, const uint32_t* maxima, const float* x,
-                                                            long long ld, long long stride, int fixed, const Entry* table, int groups_n,
-                                                            int cols, long long kp, Plan* plan) {
-  __shared__ float tile[32][65];
+                                                            long long ld, long long stride, int fixed, const Entry* table,
+                                                            const int* owner, int groups_n, int cols, long long kp, Plan* plan) {
+  __shared__ float tile[2][32][65];
   __shared__ int tiny_all;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int c0 = blockIdx.x * 64;
   const int per = fixed ? (fixed + 31) / 32 : 1;
   const long long blocks = fixed ? (long long)groups_n * per : plan->padded / 32;
   for (long long b = blockIdx.y; b < blocks; b += gridDim.y) {
     int g, r0, end;
     long long pos, row_base;                               // first position written, first row of hi / lo
+    bool begins;                                           // these are the group's first positions
     if (fixed) {
       g = (int)(b / per);
       r0 = (int)(b - (long long)g * per) * 32;
       end = fixed;
       pos = r0;
       row_base = (long long)g * cols;
+      begins = r0 == 0;
     } else {
-      int a = 0, z = groups_n;                             // the group that owns these positions
-      while (z - a > 1) {
-        const int mid = (a + z) >> 1;
-        if (table[mid].first <= b * 32) a = mid; else z = mid;
-      }
-      g = a;                                               // (of groups without rows that start here, the last one: the owner)
+      g = owner[b];
+      const Entry e = table[g];
       pos = b * 32;
-      r0 = table[g].lo + (int)(pos - table[g].first);
-      end = table[g].hi;
+      r0 = e.lo + (int)(pos - e.first);
+      end = e.hi;
       row_base = 0;
+      begins = pos == e.first;
     }
+    const float* src = fixed ? x + g * stride : x;
     __syncthreads();
     if (threadIdx.x == 0) tiny_all = 0;
+    uint32_t m[2] = {0, 0};
+    const int col = threadIdx.x >> 2, p8 = (threadIdx.x & 3) * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = r0 + ty + 4 * i, c = c0 + tx;
-      tile[ty + 4 * i][tx] = (r < end && c < cols) ? grouped_row(x, ld, stride, fixed, g, r)[c] : 0.f;
+    for (int h = 0; h < 2; ++h) {
+      const int mine = blockIdx.x * 128 + h * 64 + col;
+      if (mine < cols) m[h] = maxima[(long long)g * cols + mine];
+      const int c = blockIdx.x * 128 + h * 64 + tx;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + ty + 4 * i;
+        tile[h][ty + 4 * i][tx] = (r < end && c < cols) ? src[(long long)r * ld + c] : 0.f;
+      }
     }
     __syncthreads();
-    // a thread: 8 positions of one column
-    const int col = threadIdx.x >> 2, p8 = (threadIdx.x & 3) * 8, c = c0 + col;
+    // a thread: 8 positions of one column of each block
     int tiny = 0;
-    if (c < cols) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = blockIdx.x * 128 + h * 64 + col;
+      if (c >= cols) continue;
       float up, down;
-      const bool ok = scale_of(maxima[(long long)g * cols + c], up, down);
+      const bool ok = scale_of(m[h], up, down);
       Half8 a, z;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) split_half(tile[p8 + j][col] * up, a.h[j], z.h[j], tiny);
+      for (int j = 0; j < 8; ++j) split_half(tile[h][p8 + j][col] * up, a.h[j], z.h[j], tiny);
       if (pos + p8 < kp) {                                 // kp is a multiple of 8
         *reinterpret_cast<uint4*>(hi + (row_base + c) * kp + pos + p8) = a.v;
         *reinterpret_cast<uint4*>(lo + (row_base + c) * kp + pos + p8) = z.v;
       }
       if (!ok) plan->flag = 1;
-      if (p8 == 0 && pos == (fixed ? 0 : table[g].first)) down_out[(long long)g * cols + c] = down;
+      if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) tiny += __shfl_xor_sync(0xffffffffu, tiny, d);
     if ((threadIdx.x & 31) == 0 && tiny) atomicAdd(&tiny_all, tiny);
     __syncthreads();
-    if (threadIdx.x == 0 && tiny_all * 64 > 32 * 64) plan->flag = 1;
+    if (threadIdx.x == 0 && tiny_all > 64) plan->flag = 1;                // of 32 x 128 values
   }
 }
 
@@ -381,9 +415,9 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = (uint64_t*)(smem + STAGES * STAGE);
   // bars[0..S) full (the leader's copy: its two producers arrive, both CTAs' loads complete bytes), [S..2S) empty,
-  // [2S] accumulators may be read out (each CTA's own), [2S+1] they have been (the leader's: one arrival per epilogue warp
-  // of both CTAs), [2S+2] unwinding only: every MMA issued so far has retired
-  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 3);
+  // [2S..2S+2) accumulator 0 / 1 is filled (each CTA's own), [2S+2..2S+4) it has been read out (the leader's: one arrival
+  // per epilogue warp of both CTAs), [2S+4] unwinding only: every MMA issued so far has retired
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * STAGES + 5);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -395,15 +429,17 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   const int n_units = (p.weights ? p.experts * ((p.cols + BN - 1) / BN) : p.plan->tiles) * tiles_l;
 
   const uint32_t smem_base = smem_u32(smem);
-  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES), bar_mid = smem_u32(bars + 2 * STAGES),
-                 bar_drained = bar_mid + 8, bar_retired = bar_mid + 16;
+  const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + STAGES), bar_filled = smem_u32(bars + 2 * STAGES),
+                 bar_drained = bar_filled + 16, bar_retired = bar_filled + 32;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 2);
       mbar_init(bar_empty + 8 * s, 1);
     }
-    mbar_init(bar_mid, 1);
-    mbar_init(bar_drained, 2 * EPI_WARPS);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_filled + 8 * b, 1);
+      mbar_init(bar_drained + 8 * b, 2 * EPI_WARPS);
+    }
     mbar_init(bar_retired, 1);
     *abort_flag = 0;
     mbar_fence_init();
@@ -470,53 +506,38 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
       const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
       constexpr uint32_t LO_TILE = RAW >> 4, STAGE_STEP = STAGE >> 4;
-      const uint32_t tmem_main = tmem_base, tmem_cross = tmem_base + BN;
-      const uint32_t peer_empty = mapa(bar_empty, 1), peer_mid = mapa(bar_mid, 1);
+      const uint32_t peer_empty = mapa(bar_empty, 1), peer_filled = mapa(bar_filled, 1);
       int s = 0;
-      uint32_t ph = 0, stage_off = 0, dph = 0;
-      bool ok = true, pending_read_out = false;
+      uint32_t ph = 0, stage_off = 0, fill = 0;            // fill: accumulator fillings so far; filling n goes to accumulator n & 1
+      bool ok = true;
       Entry next = n_units > 0 ? entry_of(p, cluster_id, n_units) : Entry{0, 0, 0, 0};
       for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
         const Unit u = unit_of(p, unit, next);
         next = entry_of(p, unit + n_clusters, n_units);
-        if (u.nkb == 0) continue;                       // a group without rows: nothing to multiply
         const uint32_t idesc = make_idesc_f16(2 * BM, (u.cols + 31) / 32 * 32);
-        uint32_t acc_cross = 0, accumulate = 0;
-        int to_drain = DRAIN;
-        for (int i = 0; i < u.nkb; ++i) {
-          if (to_drain == 0) {
-            mma_commit_pair(bar_mid);
-            mma_commit_pair(peer_mid);
-            pending_read_out = true;
-            accumulate = 0;
-            to_drain = DRAIN;
-          }
-          --to_drain;
-          if (!mbar_wait_cluster(bar_full + 8 * s, ph, abort_flag, p.status, 700 + s)) { ok = false; break; }
-          if (pending_read_out) {
-            // the previous read-out must be over before these MMAs overwrite the accumulators
-            if (!mbar_wait_cluster(bar_drained, dph, abort_flag, p.status, 750)) { ok = false; break; }
-            dph ^= 1;
-            pending_read_out = false;
-          }
-          tc_fence_after();
+        for (int i0 = 0; ok && i0 < u.nkb; i0 += DRAIN, ++fill) {      // (a group without rows: nothing to multiply)
+          const int end = min(u.nkb, i0 + DRAIN);
+          const uint32_t acc = tmem_base + (fill & 1) * BN;
+          // the filling before the last one must have been read out of this accumulator (the first two pass at once)
+          if (!mbar_wait_cluster(bar_drained + 8 * (fill & 1), ((fill >> 1) & 1) ^ 1, abort_flag, p.status, 750)) { ok = false; break; }
+          for (int i = i0; i < end; ++i) {
+            if (!mbar_wait_cluster(bar_full + 8 * s, ph, abort_flag, p.status, 700 + s)) { ok = false; break; }
+            tc_fence_after();
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            const uint32_t al = a_low0 + stage_off + kk * 2, bl = b_low0 + stage_off + kk * 2;    // 32 B per k-step
-            mma_f16_pair_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : acc_cross);
-            mma_f16_pair_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
-            mma_f16_pair_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
+            for (int kk = 0; kk < BK / 16; ++kk) {
+              const uint32_t al = a_low0 + stage_off + kk * 2, bl = b_low0 + stage_off + kk * 2;    // 32 B per k-step
+              mma_f16_pair_words(acc, al + LO_TILE, a_hiw, bl, b_hiw, idesc, (i > i0 || kk) ? 1u : 0u);
+              mma_f16_pair_words(acc, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
+              mma_f16_pair_words(acc, al, a_hiw, bl, b_hiw, idesc, 1);
+            }
+            mma_commit_pair(bar_empty + 8 * s);         // stage free in the leader ...
+            mma_commit_pair(peer_empty + 8 * s);        // ... and in the peer
+            if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
           }
-          mma_commit_pair(bar_empty + 8 * s);           // stage free in the leader ...
-          mma_commit_pair(peer_empty + 8 * s);          // ... and in the peer
-          acc_cross = 1;
-          accumulate = 1;
-          if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
+          if (!ok) break;
+          mma_commit_pair(bar_filled + 8 * (fill & 1));
+          mma_commit_pair(peer_filled + 8 * (fill & 1));
         }
-        if (!ok) break;
-        mma_commit_pair(bar_mid);                       // tile finished: last read-out
-        mma_commit_pair(peer_mid);
-        pending_read_out = true;
       }
       if (*abort_flag) {
         mma_commit_pair(bar_retired);
@@ -533,15 +554,14 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
     const uint32_t tmem_lane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
     float* scales = reinterpret_cast<float*>(smem + STAGES * STAGE + 256) + warp * (BN / 2);
     float acc[BN / 2];
-    uint32_t mph = 0;
+    uint32_t fill = 0;
     bool ok = true;
     Entry next = n_units > 0 ? entry_of(p, cluster_id, n_units) : Entry{0, 0, 0, 0};
     for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
       const Unit u = unit_of(p, unit, next);
       next = entry_of(p, unit + n_clusters, n_units);
       const int ncc = min(BN / 2 / 32, max(0, (u.cols - half * (BN / 2) + 31) / 32));    // 32-column pieces of this thread
-      const int n_mid = u.nkb > 0 ? (u.nkb - 1) / DRAIN : -1;
-      const bool none = n_mid < 0;                        // a group without rows: zeros, and no scales
+      const bool none = u.nkb == 0;                        // a group without rows: zeros, and no scales
       const int l = u.l0 + (int)rank * BM + q * 32 + lane, left = u.cols - half * (BN / 2);
       // the scales of this thread's lane and (spread over the warp's lanes) of its columns, requested before the wait
       const float* r_down = (p.weights ? p.r_down + (long long)u.expert * p.cols : p.r_down) + u.r0 + half * (BN / 2);
@@ -554,11 +574,9 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       }
 #pragma unroll
       for (int j = 0; j < BN / 2; ++j) acc[j] = 0.f;
-      // (acc starts from zero and every read-out adds: two ways to define it in this loop cost 80 spilled registers)
 #pragma unroll 1
-      for (int ev = 0; ev <= n_mid; ++ev) {
-        ok = mbar_wait_cluster(bar_mid, mph, abort_flag, p.status, 850);
-        mph ^= 1;
+      for (int i0 = 0; i0 < u.nkb; i0 += DRAIN, ++fill) {
+        ok = mbar_wait_cluster(bar_filled + 8 * (fill & 1), (fill >> 1) & 1, abort_flag, p.status, 850);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -566,21 +584,15 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
         for (int cc = 0; cc < BN / 2 / 32; ++cc) {
           if (cc < ncc) {
             uint32_t r[32];
-            tmem_ld_32x32(tmem_lane + cc * 32, r);
+            tmem_ld_32x32(tmem_lane + (fill & 1) * BN + cc * 32, r);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) acc[cc * 32 + j] += __uint_as_float(r[j]);
-            if (ev == n_mid) {
-              tmem_ld_32x32(tmem_lane + BN + cc * 32, r);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) acc[cc * 32 + j] = fmaf(__uint_as_float(r[j]), 1.f / 2048.f, acc[cc * 32 + j]);
-            }
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_drained);
+        if (lane == 0) mbar_arrive_cluster(leader_drained + 8 * (fill & 1));
       }
       if (!ok) break;
       // out of registers, while the tensor cores work on the pair's next tile
@@ -706,15 +718,18 @@ int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float
 }
 
 int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, const float* x, long long ld, long long stride,
-                  int fixed, const Entry* table, int groups_n, int rows, int cols, long long kp, Plan* plan) {
+                  int fixed, const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
   CB_CUDA(cudaMemsetAsync(maxima, 0, (size_t)groups_n * cols * sizeof(uint32_t), s->stream));
   long long chunks = fixed ? (long long)groups_n * ((fixed + 63) / 64) : (rows + 63) / 64;
-  column_max_kernel<<<dim3((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535)), 128, 0, s->stream>>>(
-      maxima, x, ld, stride, fixed, table, groups_n, rows, cols);
+  const dim3 grid_max((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535));
+  if (((uintptr_t)x & 15) == 0 && ld % 4 == 0 && stride % 4 == 0 && cols % 4 == 0)
+    column_max_kernel<4><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, stride, fixed, table, groups_n, rows, cols);
+  else
+    column_max_kernel<1><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, stride, fixed, table, groups_n, rows, cols);
   CB_LAUNCH_CHECK(s);
   long long blocks = fixed ? (long long)groups_n * ((fixed + 31) / 32) : kp / 32;
-  split_columns_kernel<<<dim3((unsigned)((cols + 63) / 64), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, s->stream>>>(
-      hi, lo, down, maxima, x, ld, stride, fixed, table, groups_n, cols, kp, plan);
+  split_columns_kernel<<<dim3((unsigned)((cols + 127) / 128), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, s->stream>>>(
+      hi, lo, down, maxima, x, ld, stride, fixed, table, owner, groups_n, cols, kp, plan);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
@@ -812,11 +827,11 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   float* l_down = w.take<float>((size_t)l_rows);
   float* r_down = w.take<float>((size_t)rows);
   uint32_t* maxima = w.take<uint32_t>(maxima_n);
-  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, offsets, experts, rows, 0, s->status_dev);
+  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, nullptr, offsets, experts, rows, 0, s->status_dev);
   CB_LAUNCH_CHECK(s);
   if ((rc = split_rows(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan))) return rc;
   if (trans_b) rc = split_rows(s, l_hi, l_lo, l_down, B, ldb, b_stride, N, l_rows, K, (int)kp, plan);
-  else rc = split_columns(s, l_hi, l_lo, l_down, maxima, B, ldb, b_stride, K, table, experts, 0, N, kp, plan);
+  else rc = split_columns(s, l_hi, l_lo, l_down, maxima, B, ldb, b_stride, K, table, nullptr, experts, 0, N, kp, plan);
   if (rc) return rc;
   PairArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = l_down; a.r_down = r_down; a.bias = bias; a.plan = plan; a.table = table;
@@ -833,13 +848,14 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   // C_e[m, n] = sum A[r, m] B[r, n]: n in the lanes, m in the columns
   const long long kp = ((long long)rows + 31LL * (experts < rows ? experts : rows) + 31) / 32 * 32;
   const size_t bytes = up256(sizeof(Plan)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
-                       2 * up256((size_t)M * kp * 2) + 2 * up256((size_t)experts * N * 4) + 2 * up256((size_t)experts * M * 4);
+                       2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / BK) * 4) + 2 * up256((size_t)experts * N * 4) + 2 * up256((size_t)experts * M * 4);
   void* ws = nullptr;
   int rc = cb200_scratch(s, bytes, &ws);
   if (rc) return rc;
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
   Entry* table = w.take<Entry>((size_t)experts + 1);
+  int* owner = w.take<int>((size_t)(kp / BK));
   __half* l_hi = w.take<__half>((size_t)N * kp);
   __half* l_lo = w.take<__half>((size_t)N * kp);
   __half* r_hi = w.take<__half>((size_t)M * kp);
@@ -848,10 +864,10 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   float* r_down = w.take<float>((size_t)experts * M);
   uint32_t* l_max = w.take<uint32_t>((size_t)experts * N);
   uint32_t* r_max = w.take<uint32_t>((size_t)experts * M);
-  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, offsets, experts, rows, 1, s->status_dev);
+  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, owner, offsets, experts, rows, 1, s->status_dev);
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, B, ldb, 0, 0, table, experts, rows, N, kp, plan))) return rc;
-  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, A, lda, 0, 0, table, experts, rows, M, kp, plan))) return rc;
+  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, B, ldb, 0, 0, table, owner, experts, rows, N, kp, plan))) return rc;
+  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, A, lda, 0, 0, table, owner, experts, rows, M, kp, plan))) return rc;
   PairArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.table = table;
   a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
