@@ -16,6 +16,8 @@
 // rows and then over the blocks in order: no atomics, the same bits on every run.
 #include "common.cuh"
 #include <math.h>
+#include <initializer_list>
+#include <mutex>
 
 namespace {
 
@@ -236,43 +238,487 @@ __global__ void __launch_bounds__(128) column_sums_kernel(Backward<T> p, const T
   for (int k = 0; k < SUMS; ++k) parts[((long long)b * SUMS + k) * p.cols + c] = s[k];
 }
 
+// The sum over n rows first, first + pitch, ... of one column: 32 columns x 8 threads each (blockDim 256), added in order.
 template <typename T>
-__global__ void __launch_bounds__(128) column_finish_kernel(Backward<T> p, const T* parts, int blocks) {
-  const long long c = (long long)blockIdx.x * 128 + threadIdx.x;
-  if (c >= p.cols) return;
-  const int k = blockIdx.y;
-  T* to = k == SUM_BEFORE_W ? p.before_w_g : (k == SUM_BEFORE_B ? p.before_b_g : (k == SUM_AFTER_W ? p.after_w_g : p.after_b_g));
-  if (!to) return;
+__device__ __forceinline__ void add_rows(const T* first, long long pitch, int n, T* to, bool live) {
+  __shared__ T part[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int a = n * ty / 8, z = n * (ty + 1) / 8;
   T s = (T)0;
-  for (int b = 0; b < blocks; ++b) s += parts[((long long)b * SUMS + k) * p.cols + c];
-  to[c] = s;
+  if (live) {
+#pragma unroll 8
+    for (int i = a; i < z; ++i) s += first[(long long)i * pitch];
+  }
+  __syncthreads();
+  part[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && live) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += part[i][tx];
+    *to = s;
+  }
 }
 
-// gate groups that more than one row block has a part of; group g = blockIdx.y (strided)
+// blockIdx.y < SUMS: a scale's or bias's gradient.  Behind them: the gate groups that more than one row block has a part of
+// (strided); the first part may be in the second slot of its block, the others are in first slots.
 template <typename T>
-__global__ void __launch_bounds__(128) gate_finish_kernel(Backward<T> p, const T* gate_parts, int blocks) {
-  const long long c = (long long)blockIdx.x * 128 + threadIdx.x;
-  if (c >= p.cols) return;
+__global__ void __launch_bounds__(256) column_finish_kernel(Backward<T> p, const T* parts, const T* gate_parts, int blocks) {
+  const long long c = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
+  if (blockIdx.y < SUMS) {
+    const int k = blockIdx.y;
+    T* to = k == SUM_BEFORE_W ? p.before_w_g : (k == SUM_BEFORE_B ? p.before_b_g : (k == SUM_AFTER_W ? p.after_w_g : p.after_b_g));
+    if (to) add_rows<T>(parts + (long long)k * p.cols + c, (long long)SUMS * p.cols, blocks, to + c, c < p.cols);
+    return;
+  }
   const long long groups = p.rows / p.rows_per_gate;
-  for (long long g = blockIdx.y; g < groups; g += gridDim.y) {
+  for (long long g = blockIdx.y - SUMS; g < groups; g += gridDim.y - SUMS) {
     const long long first = g * p.rows_per_gate, last = first + p.rows_per_gate - 1;
     const int b0 = block_of(p.rows, blocks, first), b1 = block_of(p.rows, blocks, last);
     if (b0 == b1) continue;
-    T s = gate_parts[(2LL * b0 + (first != block_begin(p.rows, blocks, b0))) * p.cols + c];
-    for (int b = b0 + 1; b <= b1; ++b) s += gate_parts[2LL * b * p.cols + c];
-    p.gate_g[g * p.cols + c] = s;
+    T* to = p.gate_g + g * p.cols + c;
+    add_rows<T>(gate_parts + 2LL * (b0 + 1) * p.cols + c, 2 * p.cols, b1 - b0, to, c < p.cols);
+    if (threadIdx.x < 32 && c < p.cols) *to += gate_parts[(2LL * b0 + (first != block_begin(p.rows, blocks, b0))) * p.cols + c];
   }
+}
+
+// ---- rows that fit a CTA's registers: every operand is read once --------------------------------------------------
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T e[VEC]; };
+template <typename T, int VEC> __device__ __forceinline__ Pack<T, VEC> ld_pack(const T* p) { return *reinterpret_cast<const Pack<T, VEC>*>(p); }
+template <typename T, int VEC> __device__ __forceinline__ void st_pack(T* p, const Pack<T, VEC>& v) { *reinterpret_cast<Pack<T, VEC>*>(p) = v; }
+
+// Sums of N values over the threads of a row; every thread gets them.  The values are folded together (each step of the
+// butterfly halves their number: 2^M - 1 + 5 - M shuffles for 2^M values instead of 5 each), the warps' sums go through `part`
+// (2^M x 32), each warp adds those up for itself: one barrier; consecutive calls must use different halves of the buffer.
+template <int N> struct Log2Up { static constexpr int value = N <= 1 ? 0 : 1 + Log2Up<(N + 1) / 2>::value; };
+template <> struct Log2Up<1> { static constexpr int value = 0; };
+template <typename T, int N>
+__device__ __forceinline__ void row_sums(T (&v)[N], T* part, int warps) {
+  constexpr int M = Log2Up<N>::value, G = 32 >> M;         // G lanes end up with the sum of one value
+  const int lane = threadIdx.x & 31;
+  T w[1 << M];
+#pragma unroll
+  for (int k = 0; k < (1 << M); ++k) w[k] = k < N ? v[k < N ? k : 0] : (T)0;
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const int half = (1 << M) >> (m + 1), d = 16 >> m;
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int k = 0; k < half; ++k) {
+      const T give = up ? w[k] : w[k + half], keep = up ? w[k + half] : w[k];
+      w[k] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+    }
+  }
+#pragma unroll
+  for (int d = G >> 1; d > 0; d >>= 1) w[0] += __shfl_xor_sync(0xffffffffu, w[0], d);
+  if (warps > 1) {
+    if ((lane & (G - 1)) == 0) part[(lane / G) * 32 + (threadIdx.x >> 5)] = w[0];
+    __syncthreads();
+    const T* mine = part + (lane / G) * 32;
+    T s = (lane & (G - 1)) < warps ? mine[lane & (G - 1)] : (T)0;
+    if (warps > G)
+      for (int i = (lane & (G - 1)) + G; i < warps; i += G) s += mine[i];
+#pragma unroll
+    for (int d = G >> 1; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    w[0] = s;
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = __shfl_sync(0xffffffffu, w[0], k * G);
+}
+
+// blockDim.x threads per row, ITEMS packs of VEC values each; blockDim.y rows per CTA where a warp holds a row
+template <typename T, int VEC, int ITEMS>
+__global__ void __launch_bounds__(1024) forward_rows_kernel(Forward<T> p) {
+  __shared__ T part[2][32];
+  const long long r = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+  if (r >= p.rows) return;                                 // whole warps: blockDim.y > 1 only with a warp per row
+  const int n = (int)p.cols, warps = blockDim.x >> 5, step = blockDim.x * VEC, c0 = threadIdx.x * VEC;
+  const T inv_n = (T)1 / (T)n;
+  const T* res = p.residual + r * p.ld_residual;
+  const T* x = p.block ? p.block + r * p.ld_block : nullptr;
+  const T* gate = p.gate ? p.gate + (r / p.rows_per_gate) * n : nullptr;
+  Pack<T, VEC> h[ITEMS], u[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = c0 + i * step;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) { h[i].e[e] = (T)0; u[i].e[e] = (T)0; }
+    if (c < n) {
+      h[i] = ld_pack<T, VEC>(res + c);
+      if (x) u[i] = ld_pack<T, VEC>(x + c);
+    }
+  }
+  int turn = 0;
+  // mean and 1 / std of values held in registers (positions behind the row hold zeros)
+  auto stats = [&](const Pack<T, VEC> (&v)[ITEMS], T& mean, T& rstd) {
+    mean = (T)0;
+    if (p.layer) {
+      T s[1] = {(T)0};
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[0] += v[i].e[e];
+      row_sums<T, 1>(s, part[turn], warps);
+      turn ^= 1;
+      mean = s[0] * inv_n;
+    }
+    T q[1] = {(T)0};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (c0 + i * step < n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { const T d = v[i].e[e] - mean; q[0] += d * d; }
+    row_sums<T, 1>(q, part[turn], warps);
+    turn ^= 1;
+    rstd = rsqrt_of(q[0] * inv_n + p.eps);
+  };
+  if (x) {
+    if (p.after_w) {
+      T mean, rstd;
+      stats(u, mean, rstd);
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = c0 + i * step;
+        if (c < n) {
+          const Pack<T, VEC> w = ld_pack<T, VEC>(p.after_w + c);
+          Pack<T, VEC> b;
+          if (p.after_b) b = ld_pack<T, VEC>(p.after_b + c);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) u[i].e[e] = (u[i].e[e] - mean) * rstd * w.e[e] + (p.after_b ? b.e[e] : (T)0);
+        }
+      }
+    }
+    T* total = p.total + r * p.ld_total;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * step;
+      if (c < n) {
+        Pack<T, VEC> g;
+        if (gate) g = ld_pack<T, VEC>(gate + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] += p.scale * (gate ? g.e[e] * u[i].e[e] : u[i].e[e]);
+        st_pack<T, VEC>(total + c, h[i]);
+      }
+    }
+  } else if (p.total) {
+    T* total = p.total + r * p.ld_total;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (c0 + i * step < n) st_pack<T, VEC>(total + c0 + i * step, h[i]);
+  }
+  if (!p.out) return;
+  T mean, rstd;
+  stats(h, mean, rstd);
+  T* out = p.out + r * p.ld_out;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = c0 + i * step;
+    if (c < n) {
+      const Pack<T, VEC> w = ld_pack<T, VEC>(p.before_w + c);
+      Pack<T, VEC> b, y;
+      if (p.before_b) b = ld_pack<T, VEC>(p.before_b + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) y.e[e] = (h[i].e[e] - mean) * rstd * w.e[e] + (p.before_b ? b.e[e] : (T)0);
+      st_pack<T, VEC>(out + c, y);
+    }
+  }
+}
+
+template <int BYTES> __device__ __forceinline__ void copy_async(void* smem, const void* g) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(smem);
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(g) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(g), "n"(BYTES) : "memory");
+}
+
+// The gradients in one pass: a CTA takes a block of consecutive rows; the next row's operands are on their way into shared
+// memory (cp.async; every thread copies what it will read itself, so there is no barrier for data) while a row is worked
+// on, and the column sums of its rows stay in registers.  What bounds it is the issue rate: a row's reductions (three for
+// rms, four for layer) cost a warp as much as 60 of its values, so a thread takes 8 values (with 4, and the reduction for
+// the block's normalisation folded into the other one by linearity -- ten sums at once -- 8192 rows of 2500 took 290 us).
+template <typename T, int VEC, int ITEMS, bool LAYER, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT <= 320 ? 2 : 1) backward_rows_kernel(Backward<T> p, T* parts, T* gate_parts, int blocks) {
+  constexpr int STAGES = 2;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ T part[2][2 * 32];
+  T* const data = reinterpret_cast<T*>(smem_raw);
+  const int n = (int)p.cols, warps = blockDim.x >> 5, step = blockDim.x * VEC, c0 = threadIdx.x * VEC;
+  const int slot = step * ITEMS;                           // elements of one operand's row in shared memory
+  const T inv_n = (T)1 / (T)n;
+  const int b = blockIdx.x, per_gate = (int)p.rows_per_gate;
+  const int r0 = (int)block_begin(p.rows, blocks, b), r1 = (int)block_begin(p.rows, blocks, b + 1);
+  const bool has_y = p.out_g != nullptr, has_t = p.total_g != nullptr, has_x = p.block != nullptr, has_a = p.after_w != nullptr;
+  const bool has_g = p.gate != nullptr, gates = p.gate_g && per_gate > 1, gate_rows = p.gate_g && per_gate == 1;
+
+  auto request = [&](int r) {
+    if (r < r1) {
+      T* to = data + ((r - r0) & 1) * 4 * slot;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = c0 + i * step;
+        if (c < n) {
+          if (has_y) {
+            copy_async<VEC * (int)sizeof(T)>(to + c, p.total + (long long)r * p.ld_total + c);
+            copy_async<VEC * (int)sizeof(T)>(to + slot + c, p.out_g + (long long)r * p.ld_out_g + c);
+          }
+          if (has_t) copy_async<VEC * (int)sizeof(T)>(to + 2 * slot + c, p.total_g + (long long)r * p.ld_total_g + c);
+          if (has_x) copy_async<VEC * (int)sizeof(T)>(to + 3 * slot + c, p.block + (long long)r * p.ld_block + c);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  request(r0);
+
+  Pack<T, VEC> sw[ITEMS], sb[ITEMS], aw[ITEMS], ab[ITEMS], gs[ITEMS];      // column sums of this block's rows
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sw[i].e[e] = sb[i].e[e] = aw[i].e[e] = ab[i].e[e] = gs[i].e[e] = (T)0;
+  int g = r0 / per_gate, g_left = (g + 1) * per_gate - r0;                 // gate row, rows it still serves
+  bool g_whole = g * per_gate == r0;                       // this block has had the group's rows from its first one on
+  int turn = 0, slot_b = 0;                                // slot_b: 1 once the block's first group is over
+
+  for (int r = r0; r < r1; ++r) {
+    request(r + 1);                                        // into the stage that the row before this one was read from
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const T* from = data + ((r - r0) & 1) * 4 * slot;
+    Pack<T, VEC> h[ITEMS], y[ITEMS], x[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * step;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[i].e[e] = y[i].e[e] = x[i].e[e] = (T)0;
+      if (c < n) {
+        if (has_y) { h[i] = ld_pack<T, VEC>(from + c); y[i] = ld_pack<T, VEC>(from + slot + c); }
+        if (has_x) x[i] = ld_pack<T, VEC>(from + 3 * slot + c);
+      }
+    }
+    // ---- statistics of both rows
+    T m[2] = {(T)0, (T)0};
+    if (LAYER) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { m[0] += h[i].e[e]; m[1] += x[i].e[e]; }
+      row_sums<T, 2>(m, part[turn ^= 1], warps);
+      m[0] *= inv_n;
+      m[1] = has_a ? m[1] * inv_n : (T)0;
+    }
+    T q[2] = {(T)0, (T)0};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (c0 + i * step < n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          h[i].e[e] -= m[0];
+          x[i].e[e] -= m[1];
+          q[0] += h[i].e[e] * h[i].e[e];
+          q[1] += x[i].e[e] * x[i].e[e];
+        }
+    row_sums<T, 2>(q, part[turn ^= 1], warps);
+    const T rstd = has_y ? rsqrt_of(q[0] * inv_n + p.eps) : (T)0, rstd_a = has_a ? rsqrt_of(q[1] * inv_n + p.eps) : (T)1;
+    // ---- through the normalisation before the next block: h becomes h_hat, then r
+    T s[2] = {(T)0, (T)0};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * step;
+      if (c < n) {
+        Pack<T, VEC> w;
+        if (has_y) w = ld_pack<T, VEC>(p.before_w + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          h[i].e[e] *= rstd;
+          x[i].e[e] *= rstd_a;
+          sw[i].e[e] += y[i].e[e] * h[i].e[e];
+          sb[i].e[e] += y[i].e[e];
+          if (has_y) y[i].e[e] *= w.e[e];
+          s[0] += y[i].e[e] * h[i].e[e];
+          if (LAYER) s[1] += y[i].e[e];
+        }
+      }
+    }
+    if (LAYER) row_sums<T, 2>(s, part[turn ^= 1], warps);
+    else row_sums<T, 1>(reinterpret_cast<T(&)[1]>(s), part[turn ^= 1], warps);
+    const T m1 = s[0] * inv_n, m2 = s[1] * inv_n;
+    // ---- through the gate and the normalisation after the block
+    --g_left;
+    const bool flush = gates && (g_left == 0 || r + 1 == r1);
+    T a[2] = {(T)0, (T)0};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * step;
+      if (c >= n) continue;
+      if (has_t) {
+        const Pack<T, VEC> t = ld_pack<T, VEC>(from + 2 * slot + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] = t.e[e] + (y[i].e[e] - h[i].e[e] * m1 - m2) * rstd;
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] = (y[i].e[e] - h[i].e[e] * m1 - m2) * rstd;
+      }
+      st_pack<T, VEC>(p.residual_g + (long long)r * p.ld_residual_g + c, h[i]);
+      if (!has_x) continue;
+      Pack<T, VEC> w, wb, ga;
+      if (has_a) w = ld_pack<T, VEC>(p.after_w + c);
+      if (has_g) ga = ld_pack<T, VEC>(p.gate + (long long)g * n + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[i].e[e] *= p.scale;                  // scale * r
+      if (p.gate_g) {
+        if (p.after_b) wb = ld_pack<T, VEC>(p.after_b + c);
+        Pack<T, VEC> u;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          u.e[e] = x[i].e[e];
+          if (has_a) u.e[e] = u.e[e] * w.e[e] + (p.after_b ? wb.e[e] : (T)0);
+          u.e[e] *= h[i].e[e];
+          gs[i].e[e] += u.e[e];
+        }
+        if (gate_rows) st_pack<T, VEC>(p.gate_g + (long long)g * n + c, u);
+        if (flush) {
+          T* to = g_whole && g_left == 0 ? p.gate_g + (long long)g * n : gate_parts + (2LL * b + slot_b) * n;
+          st_pack<T, VEC>(to + c, gs[i]);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) gs[i].e[e] = (T)0;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (has_g) h[i].e[e] *= ga.e[e];                                   // du
+        if (has_a) {
+          aw[i].e[e] += h[i].e[e] * x[i].e[e];
+          ab[i].e[e] += h[i].e[e];
+          h[i].e[e] *= w.e[e];
+          a[0] += h[i].e[e] * x[i].e[e];
+          if (LAYER) a[1] += h[i].e[e];
+        }
+      }
+      if (!has_a) st_pack<T, VEC>(p.block_g + (long long)r * p.ld_block_g + c, h[i]);
+    }
+    if (has_x && has_a) {
+      if (LAYER) row_sums<T, 2>(a, part[turn ^= 1], warps);
+      else row_sums<T, 1>(reinterpret_cast<T(&)[1]>(a), part[turn ^= 1], warps);
+      a[0] *= inv_n;
+      a[1] *= inv_n;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = c0 + i * step;
+        if (c >= n) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] = (h[i].e[e] - x[i].e[e] * a[0] - a[1]) * rstd_a;
+        st_pack<T, VEC>(p.block_g + (long long)r * p.ld_block_g + c, h[i]);
+      }
+    }
+    if (g_left == 0) {
+      ++g;
+      g_left = per_gate;
+      g_whole = true;
+      slot_b = 1;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = c0 + i * step;
+    if (c >= n) continue;
+    T* to = parts + (long long)b * SUMS * n + c;
+    if (p.before_w_g) st_pack<T, VEC>(to + (long long)SUM_BEFORE_W * n, sw[i]);
+    if (p.before_b_g) st_pack<T, VEC>(to + (long long)SUM_BEFORE_B * n, sb[i]);
+    if (p.after_w_g) st_pack<T, VEC>(to + (long long)SUM_AFTER_W * n, aw[i]);
+    if (p.after_b_g) st_pack<T, VEC>(to + (long long)SUM_AFTER_B * n, ab[i]);
+  }
+}
+
+template <typename T> bool packed_ok(int vec, long long cols, std::initializer_list<const void*> ps, std::initializer_list<long long> lds) {
+  if (cols % vec) return false;
+  uintptr_t bits = 0;
+  for (const void* q : ps) bits |= (uintptr_t)q;
+  for (long long ld : lds) if (ld % vec) return false;
+  return (bits & (vec * sizeof(T) - 1)) == 0;
+}
+
+inline int round32(long long v) { return (int)((v + 31) / 32 * 32); }
+
+template <typename T, int VEC, int ITEMS> void launch_forward(cb200_stream* s, const Forward<T>& p) {
+  const int threads = round32((p.cols + VEC * ITEMS - 1) / (VEC * ITEMS));
+  const int side = threads == 32 ? 4 : 1;                  // a warp per row: four rows per CTA
+  forward_rows_kernel<T, VEC, ITEMS><<<(unsigned)((p.rows + side - 1) / side), dim3(threads, side), 0, s->stream>>>(p);
 }
 
 template <typename T> int run_forward(cb200_stream* s, const Forward<T>& p) {
   DeviceGuard guard(s->device);
-  forward_wide_kernel<T><<<(unsigned)p.rows, WIDE_THREADS, 0, s->stream>>>(p);
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = packed_ok<T>(V, p.cols, {p.out, p.total, p.block, p.residual, p.gate, p.after_w, p.after_b, p.before_w, p.before_b},
+                                {p.ld_out, p.ld_total, p.ld_block, p.ld_residual});
+  // few rows: a row is spread over many threads (latency); many: 16 values per thread in flight
+  const bool few = p.rows < 2LL * s->sm_count;
+  if (vec && p.cols <= V * 1024 && (few || p.cols <= V * 32)) launch_forward<T, V, 1>(s, p);
+  else if (vec && p.cols <= V * 2 * 64) launch_forward<T, V, 2>(s, p);
+  else if (vec && p.cols <= V * 4 * 1024) launch_forward<T, V, 4>(s, p);
+  else if (!vec && p.cols <= 1024 && (few || p.cols <= 32)) launch_forward<T, 1, 1>(s, p);
+  else if (!vec && p.cols <= 4 * 1024 && (few || p.cols <= 4 * 128)) launch_forward<T, 1, 4>(s, p);
+  else if (!vec && sizeof(T) == 4 && p.cols <= 16 * 1024) launch_forward<T, 1, sizeof(T) == 4 ? 16 : 4>(s, p);
+  else forward_wide_kernel<T><<<(unsigned)p.rows, WIDE_THREADS, 0, s->stream>>>(p);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+template <typename T, int VEC, int ITEMS, bool LAYER, int MAXT>
+int launch_backward_kernel(cb200_stream* s, const Backward<T>& p, int threads, size_t smem, T* parts, T* gate_parts, int blocks) {
+  static std::once_flag once[64];
+  static cudaError_t result[64];
+  const int dev = s->device & 63;
+  std::call_once(once[dev], [&] {
+    result[dev] = cudaFuncSetAttribute(backward_rows_kernel<T, VEC, ITEMS, LAYER, MAXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 << 10);
+  });
+  if (result[dev] != cudaSuccess) return cb200_cuda_fail(result[dev], "cudaFuncSetAttribute", __FILE__, __LINE__);
+  backward_rows_kernel<T, VEC, ITEMS, LAYER, MAXT><<<(unsigned)blocks, threads, smem, s->stream>>>(p, parts, gate_parts, blocks);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
+template <typename T, int VEC, int ITEMS>
+int launch_backward(cb200_stream* s, const Backward<T>& p, int threads, size_t smem, T* parts, T* gate_parts, int blocks) {
+  if (threads <= 320)
+    return p.layer ? launch_backward_kernel<T, VEC, ITEMS, true, 320>(s, p, threads, smem, parts, gate_parts, blocks)
+                   : launch_backward_kernel<T, VEC, ITEMS, false, 320>(s, p, threads, smem, parts, gate_parts, blocks);
+  return p.layer ? launch_backward_kernel<T, VEC, ITEMS, true, 512>(s, p, threads, smem, parts, gate_parts, blocks)
+                 : launch_backward_kernel<T, VEC, ITEMS, false, 512>(s, p, threads, smem, parts, gate_parts, blocks);
+}
+
+template <typename T> int finish_columns(cb200_stream* s, const Backward<T>& p, const T* parts, const T* gate_parts, int blocks) {
+  const bool gates = p.gate_g && p.rows_per_gate > 1;
+  if (!(p.before_w_g || p.before_b_g || p.after_w_g || p.after_b_g || gates)) return CB200_OK;
+  const long long groups = gates ? p.rows / p.rows_per_gate : 0;
+  column_finish_kernel<T><<<dim3((unsigned)((p.cols + 31) / 32), (unsigned)(SUMS + (groups < 4096 ? groups : 4096))), 256, 0, s->stream>>>(
+      p, parts, gate_parts, blocks);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
 
 template <typename T> int run_backward(cb200_stream* s, const Backward<T>& p) {
   DeviceGuard guard(s->device);
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = packed_ok<T>(V, p.cols, {p.block_g, p.residual_g, p.gate_g, p.out_g, p.total_g, p.total, p.block, p.gate, p.after_w, p.after_b,
+                                            p.before_w}, {p.ld_block_g, p.ld_residual_g, p.ld_out_g, p.ld_total_g, p.ld_total, p.ld_block});
+  // values per thread: its five column sums of each stay in registers (64-bit ones: half as many values)
+  constexpr int VALUES = sizeof(T) == 8 ? 4 : 8;
+  const int threads = round32((p.cols + VALUES - 1) / VALUES);
+  const size_t smem = (size_t)2 * 4 * threads * VALUES * sizeof(T), room = 216 << 10;
+  if (threads <= 512 && smem <= room) {
+    long long per_sm = (long long)(room / smem), by_regs = threads <= 320 ? 65536 / (threads * 96) : 1;
+    if (per_sm > by_regs) per_sm = by_regs;
+    if (per_sm > 16) per_sm = 16;
+    if (per_sm < 1) per_sm = 1;
+    const int blocks = (int)(p.rows < s->sm_count * per_sm ? p.rows : s->sm_count * per_sm);
+    void* ws = nullptr;
+    const size_t parts_n = ((size_t)blocks * SUMS * p.cols + 3) / 4 * 4, gate_n = (size_t)blocks * 2 * p.cols;
+    int rc = cb200_scratch(s, (parts_n + gate_n) * sizeof(T), &ws);
+    if (rc) return rc;
+    T* parts = (T*)ws;
+    T* gate_parts = parts + parts_n;
+    rc = vec ? launch_backward<T, V, VALUES / V>(s, p, threads, smem, parts, gate_parts, blocks)
+             : launch_backward<T, 1, VALUES>(s, p, threads, smem, parts, gate_parts, blocks);
+    if (rc) return rc;
+    return finish_columns<T>(s, p, parts, gate_parts, blocks);
+  }
   const long long col_tiles = (p.cols + 127) / 128;
   long long blocks = (2LL * s->sm_count * 8 + col_tiles - 1) / col_tiles;
   if (blocks > p.rows) blocks = p.rows;
@@ -286,21 +732,12 @@ template <typename T> int run_backward(cb200_stream* s, const Backward<T>& p) {
   T* gate_parts = parts + parts_n;
   backward_wide_kernel<T><<<(unsigned)p.rows, WIDE_THREADS, 0, s->stream>>>(p, stats);
   CB_LAUNCH_CHECK(s);
-  const bool gates = p.gate_g && p.rows_per_gate > 1;
-  if (p.before_w_g || p.before_b_g || p.after_w_g || p.after_b_g || gates) {
+  if (p.before_w_g || p.before_b_g || p.after_w_g || p.after_b_g || (p.gate_g && p.rows_per_gate > 1)) {
     column_sums_kernel<T><<<dim3((unsigned)col_tiles, (unsigned)blocks), 128, 0, s->stream>>>(p, stats, parts, gate_parts,
                                                                                               (int)blocks);
     CB_LAUNCH_CHECK(s);
-    column_finish_kernel<T><<<dim3((unsigned)col_tiles, SUMS), 128, 0, s->stream>>>(p, parts, (int)blocks);
-    CB_LAUNCH_CHECK(s);
   }
-  if (gates) {
-    const long long groups = p.rows / p.rows_per_gate;
-    gate_finish_kernel<T><<<dim3((unsigned)col_tiles, (unsigned)(groups < 1024 ? groups : 1024)), 128, 0, s->stream>>>(
-        p, gate_parts, (int)blocks);
-    CB_LAUNCH_CHECK(s);
-  }
-  return CB200_OK;
+  return finish_columns<T>(s, p, parts, gate_parts, (int)blocks);
 }
 
 int check_desc(const char* what, int dtype, const cb200_block_desc* d) {
