@@ -187,7 +187,7 @@ def call(name, *args):
     """Call a status-returning entry point; a non-zero status becomes B200Error
     (as check-cuda-error turns CUDA statuses into exceptions,
     src/cortex/compute/cuda/driver.clj:40-49)."""
-    rc = getattr(load(), name)(*args)
-    if name not in _NO_CHECK and rc != 0:
+    rc = getattr(_lib or load(), name)(*args)
+    if rc != 0 and name not in _NO_CHECK:
         raise B200Error(rc, last_error())
     return rc

@@ -15,15 +15,17 @@
 
 namespace {
 
-constexpr int TABLE = 512;         // buffers per launch: 24 bytes each in the kernel's parameters
+// Buffers per launch: 28 bytes each in the kernel's parameters.  Two tables, because parameters cost time to pass: a
+// small network's call is bound by its two launches.
+constexpr int SMALL_TABLE = 32, TABLE = 512;
 constexpr int THREADS = 256;
-constexpr int CHUNK = 8192;        // elements
+constexpr int CHUNK = 4096;        // elements
 
-template <typename T> struct Pieces {
-  const T* g[TABLE];
-  T* out[TABLE];
-  long long count[TABLE];
-  int first[TABLE + 1];            // the buffer's first chunk; first[n] = all chunks
+template <typename T, int MOST> struct Pieces {
+  const T* g[MOST];
+  T* out[MOST];
+  long long count[MOST];
+  int first[MOST + 1];             // the buffer's first chunk; first[n] = all chunks
   int n;
 };
 
@@ -31,12 +33,12 @@ template <typename T> struct Pieces {
 struct NormResult { double norm, scale; };
 
 template <typename T> struct Vec;
-template <> struct Vec<float> { typedef float4 type; static constexpr int N = 4; };
-template <> struct Vec<double> { typedef double2 type; static constexpr int N = 2; };
+template <> struct Vec<float> { struct alignas(16) type { float e[4]; }; static constexpr int N = 4; };
+template <> struct Vec<double> { struct alignas(16) type { double e[2]; }; static constexpr int N = 2; };
 
 // Elements [lo, hi) of buffer `p` that chunk `c` covers: chunks are cut at 16-byte boundaries of the buffer.
-template <typename T>
-__device__ __forceinline__ void chunk_range(const Pieces<T>& t, int c, int& p, long long& lo, long long& hi) {
+template <typename T, int MOST>
+__device__ __forceinline__ void chunk_range(const Pieces<T, MOST>& t, int c, int& p, long long& lo, long long& hi) {
   int a = 0, b = t.n;
   while (b - a > 1) {
     const int m = (a + b) >> 1;
@@ -66,10 +68,12 @@ __device__ __forceinline__ double block_sum(double v) {
 
 // partials: one slot per CTA of every launch of the call; `slot0` this launch's first, `slots` all of them.
 // `last` : the call's last launch; its last CTA to finish writes the result.
-template <typename T>
+template <typename T, int MOST>
 __global__ void __launch_bounds__(THREADS)
-square_sum_kernel(const __grid_constant__ Pieces<T> t, double* partials, int slot0, int slots, int last, int* counter,
+square_sum_kernel(const __grid_constant__ Pieces<T, MOST> t, double* partials, int slot0, int slots, int last, int* counter,
                   NormResult* result, T* norm_out, double max_norm) {
+  typedef typename Vec<T>::type V;
+  constexpr int N = Vec<T>::N, WHOLE = CHUNK / N / THREADS;           // 16-byte loads of a whole chunk per thread
   double sum = 0.0;
   const int chunks = t.first[t.n];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -77,9 +81,23 @@ square_sum_kernel(const __grid_constant__ Pieces<T> t, double* partials, int slo
     long long lo, hi;
     chunk_range(t, c, p, lo, hi);
     const T* g = t.g[p];
-    for (long long i = lo + threadIdx.x; i < hi; i += THREADS) {
-      const double v = (double)g[i];
-      sum += v * v;
+    if (hi - lo == CHUNK) {                                // starts on a 16-byte boundary
+      const V* v = reinterpret_cast<const V*>(g + lo);
+      V x[WHOLE];
+#pragma unroll
+      for (int i = 0; i < WHOLE; ++i) x[i] = v[threadIdx.x + i * THREADS];
+      double s[2] = {0.0, 0.0};
+#pragma unroll
+      for (int i = 0; i < WHOLE; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e & 1] += (double)x[i].e[e] * (double)x[i].e[e];
+      sum += s[0] + s[1];
+    } else {
+#pragma unroll 4
+      for (long long i = lo + threadIdx.x; i < hi; i += THREADS) {
+        const double v = (double)g[i];
+        sum += v * v;
+      }
     }
   }
   sum = block_sum(sum);
@@ -104,11 +122,15 @@ square_sum_kernel(const __grid_constant__ Pieces<T> t, double* partials, int slo
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Pieces<T> t, const NormResult* result) {
+// Chunks from the last to the first: what the norm's pass read last is still in L2.  Stores are streaming (they are not
+// read again here), so they do not push it out.
+template <typename T, int MOST>
+__global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Pieces<T, MOST> t, const NormResult* result) {
+  typedef typename Vec<T>::type V;
+  constexpr int N = Vec<T>::N, WHOLE = CHUNK / N / THREADS;
   const T scale = (T)result->scale;
   const int chunks = t.first[t.n];
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+  for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     int p;
     long long lo, hi;
     chunk_range(t, c, p, lo, hi);
@@ -117,14 +139,26 @@ __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ 
     if (scale == (T)1 && g == o) continue;           // within the bound, in place: nothing changes
     if (!(scale >= (T)1e-30)) {                      // a float scale down here would have lost its low bits
       for (long long i = lo + threadIdx.x; i < hi; i += THREADS) o[i] = (T)((double)g[i] * result->scale);
-      continue;
+    } else if (hi - lo == CHUNK && ((uintptr_t)(o + lo) & 15) == 0) {
+      const V* v = reinterpret_cast<const V*>(g + lo);
+      V x[WHOLE];
+#pragma unroll
+      for (int i = 0; i < WHOLE; ++i) x[i] = v[threadIdx.x + i * THREADS];
+#pragma unroll
+      for (int i = 0; i < WHOLE; ++i) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[i].e[e] *= scale;
+        __stcs(reinterpret_cast<float4*>(o + lo) + threadIdx.x + i * THREADS, *reinterpret_cast<const float4*>(&x[i]));
+      }
+    } else {
+#pragma unroll 4
+      for (long long i = lo + threadIdx.x; i < hi; i += THREADS) o[i] = g[i] * scale;
     }
-    for (long long i = lo + threadIdx.x; i < hi; i += THREADS) o[i] = g[i] * scale;
   }
 }
 
-template <typename T>
-int fill(Pieces<T>& t, int n, const void* const* g, void* const* out, const int64_t* counts) {
+template <typename T, int MOST>
+int fill(Pieces<T, MOST>& t, int n, const void* const* g, void* const* out, const int64_t* counts) {
   t.n = 0;
   long long chunks = 0;
   for (int i = 0; i < n; ++i) {
@@ -135,18 +169,18 @@ int fill(Pieces<T>& t, int n, const void* const* g, void* const* out, const int6
     t.count[t.n] = counts[i];
     t.first[t.n] = (int)chunks;
     chunks += (counts[i] + off + CHUNK - 1) / CHUNK;
-    if (chunks > 2000000000LL) { cb200_set_error("global_norm: more than 1.6e13 elements"); return CB200_ERR_INVALID; }
+    if (chunks > 2000000000LL) { cb200_set_error("global_norm: more than 8e12 elements"); return CB200_ERR_INVALID; }
     ++t.n;
   }
   t.first[t.n] = (int)chunks;
   return CB200_OK;
 }
 
-template <typename T>
-int norm_and_clip(cb200_stream* s, int n, const void* const* g, const int64_t* counts, void* const* out, double max_norm,
-                  void* norm) {
+template <typename T, int MOST>
+int norm_and_clip_table(cb200_stream* s, int n, const void* const* g, const int64_t* counts, void* const* out, double max_norm,
+                        void* norm) {
   DeviceGuard guard(s->device);
-  const int launches = n > TABLE ? (n + TABLE - 1) / TABLE : 1;
+  const int launches = n > MOST ? (n + MOST - 1) / MOST : 1;
   const int most = s->sm_count * 8;                  // CTAs of one launch
   void* block = nullptr;
   int* counter = nullptr;
@@ -155,28 +189,35 @@ int norm_and_clip(cb200_stream* s, int n, const void* const* g, const int64_t* c
   if ((rc = cb200_tile_flags(s, 1, &counter))) return rc;
   NormResult* result = (NormResult*)block;
   double* partials = (double*)(result + 1);
-  static thread_local Pieces<T> t;                   // 12 KB: off the caller's stack
+  static thread_local Pieces<T, MOST> t;             // up to 14 KB: off the caller's stack
   int slots = 0;
   for (int l = 0; l < launches; ++l) {
-    const int at = l * TABLE, m = n - at < TABLE ? n - at : TABLE;
-    if ((rc = fill(t, m, g + at, nullptr, counts + at))) return rc;
+    const int at = l * MOST, m = n - at < MOST ? n - at : MOST;
+    if ((rc = fill(t, m, g + at, out ? out + at : nullptr, counts + at))) return rc;
     int grid = t.first[t.n] < most ? t.first[t.n] : most;
     if (grid < 1) grid = 1;
-    square_sum_kernel<T><<<grid, THREADS, 0, s->stream>>>(t, partials, slots, slots + grid, l == launches - 1, counter, result,
-                                                          (T*)norm, out ? max_norm : INFINITY);
+    square_sum_kernel<T, MOST><<<grid, THREADS, 0, s->stream>>>(t, partials, slots, slots + grid, l == launches - 1, counter, result,
+                                                                (T*)norm, out ? max_norm : INFINITY);
     CB_LAUNCH_CHECK(s);
     slots += grid;
   }
   if (!out) return CB200_OK;
-  for (int l = 0; l < launches; ++l) {
-    const int at = l * TABLE, m = n - at < TABLE ? n - at : TABLE;
-    if ((rc = fill(t, m, g + at, out + at, counts + at))) return rc;
+  for (int l = launches - 1; l >= 0; --l) {          // the last launch's table is still filled
+    const int at = l * MOST, m = n - at < MOST ? n - at : MOST;
+    if (l != launches - 1 && (rc = fill(t, m, g + at, out + at, counts + at))) return rc;
     int grid = t.first[t.n] < most ? t.first[t.n] : most;
     if (grid < 1) continue;
-    scale_kernel<T><<<grid, THREADS, 0, s->stream>>>(t, result);
+    scale_kernel<T, MOST><<<grid, THREADS, 0, s->stream>>>(t, result);
     CB_LAUNCH_CHECK(s);
   }
   return CB200_OK;
+}
+
+template <typename T>
+int norm_and_clip(cb200_stream* s, int n, const void* const* g, const int64_t* counts, void* const* out, double max_norm,
+                  void* norm) {
+  return n <= SMALL_TABLE ? norm_and_clip_table<T, SMALL_TABLE>(s, n, g, counts, out, max_norm, norm)
+                          : norm_and_clip_table<T, TABLE>(s, n, g, counts, out, max_norm, norm);
 }
 
 int check_list(const char* what, cb200_stream* s, int dtype, int n, const void* const* g, const int64_t* counts) {

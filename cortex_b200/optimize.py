@@ -14,6 +14,8 @@ it: unary-op! :noop, binary-op! :+, binary-op! :-, binary-op! :+.
 ``global_norm`` and ``clip_gradients`` (no counterpart in the reference) treat the gradient buffers of all layers as
 one vector: they run between the backward pass and the per-buffer steps.
 """
+import math
+
 from . import tensor as ct
 
 
@@ -22,39 +24,43 @@ def _flat(t):
 
 
 def _gradient_list(tensors, name):
-    """(datatype, buffers, element counts) of a list of dense tensors of one type on one device."""
-    ct._require(len(tensors) > 0, "%s: no tensors" % name)
-    first = tensors[0]
-    datatype, device = first.buffer.dtype, first.device
-    ct._require(datatype in ("float", "double"), "%s is only defined for float and double tensors" % name, datatype)
-    buffers, counts = [], []
+    """(datatype, addresses, element counts) of a list of dense tensors of one type on one device.  (A plain loop with one
+    test per tensor: a network has hundreds of buffers, and this runs at every step.)"""
+    if not tensors:
+        raise ct.TensorError("%s: no tensors" % name)
+    datatype, device = tensors[0].buffer.dtype, tensors[0].device
+    if datatype != "float" and datatype != "double":
+        raise ct.TensorError("%s is only defined for float and double tensors: %r" % (name, datatype))
+    addresses, counts = [], []
     for t in tensors:
-        ct._require(t.buffer.dtype == datatype, "Not all arguments match required datatype", t)
-        ct._require(t.device is device, "Tensor arguments are not all on same device", t)
-        shape = t.dimensions["shape"]
-        if len(shape) == 1 and type(shape[0]) is int and t.dimensions["strides"][0] == 1:
+        buffer, dimensions = t.buffer, t.dimensions
+        if buffer.dtype != datatype or t.device is not device:
+            raise ct.TensorError("%s: arguments are not all of one datatype on one device: %r" % (name, t))
+        shape = dimensions["shape"]
+        if len(shape) == 1 and type(shape[0]) is int and dimensions["strides"][0] == 1:
             counts.append(shape[0])
-        else:
-            ct._require(ct._packed(t), "%s needs dense tensors" % name, t)
+        elif ct._packed(t):
             counts.append(t.ecount())
-        buffers.append(t.buffer)
-    return datatype, buffers, counts
+        else:
+            raise ct.TensorError("%s needs dense tensors: %r" % (name, t))
+        addresses.append(buffer.ptr)
+    return datatype, addresses, counts
 
 
 def _norm_tensor(norm, datatype, device):
     if norm is None:
         return ct.new_tensor([1], datatype=datatype, init_value=None)
-    ct._require(norm.ecount() == 1 and norm.get_datatype() == datatype, "norm must be one element of the gradients' datatype", norm)
-    ct._require(norm.device is device, "Tensor arguments are not all on same device", norm)
+    if norm.buffer.dtype != datatype or norm.device is not device or norm.ecount() != 1:
+        raise ct.TensorError("norm must be one element of the gradients' datatype on their device: %r" % (norm,))
     return norm
 
 
 def global_norm(gradients, norm=None):
     """sqrt of the sum of squares over every element of every tensor of the list, as a device tensor [1] of their datatype
     (`norm`, or a new one).  Squares are summed in double, in a fixed order."""
-    datatype, buffers, counts = _gradient_list(gradients, "global-norm")
+    datatype, addresses, counts = _gradient_list(gradients, "global-norm")
     norm = _norm_tensor(norm, datatype, gradients[0].device)
-    ct.check_stream().global_norm(datatype, buffers, counts, norm.buffer)
+    ct.check_stream().global_norm(datatype, addresses, counts, norm.buffer)
     return norm
 
 
@@ -62,15 +68,17 @@ def clip_gradients(gradients, max_norm, clipped=None, norm=None):
     """Scale a list of gradient tensors by max_norm / norm where their global norm exceeds max_norm; otherwise, and when the
     norm is not finite, they stay as they are.  `clipped`: the destinations (the gradients themselves by default).  Returns
     the norm before clipping, a device tensor [1]."""
-    ct._require(0 < max_norm < float("inf"), "The bound must be positive and finite", max_norm)
-    datatype, buffers, counts = _gradient_list(gradients, "clip-gradients")
+    max_norm = float(max_norm)
+    if not 0.0 < max_norm < math.inf:
+        raise ct.TensorError("The bound must be positive and finite: %r" % max_norm)
+    datatype, gradient_addresses, counts = _gradient_list(gradients, "clip-gradients")
     norm = _norm_tensor(norm, datatype, gradients[0].device)
-    destinations = buffers
+    destinations = gradient_addresses
     if clipped is not None:
         c_type, destinations, c_counts = _gradient_list(clipped, "clip-gradients")
-        ct._require(c_type == datatype and c_counts == counts and clipped[0].device is gradients[0].device,
-                    "Destinations must match the gradients in number, size, datatype and device")
-    ct.check_stream().clip_gradients(datatype, buffers, counts, destinations, max_norm, norm.buffer)
+        if c_type != datatype or c_counts != counts or clipped[0].device is not gradients[0].device:
+            raise ct.TensorError("Destinations must match the gradients in number, size, datatype and device")
+    ct.check_stream().clip_gradients(datatype, gradient_addresses, counts, destinations, max_norm, norm.buffer)
     return norm
 
 

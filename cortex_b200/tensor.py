@@ -597,22 +597,25 @@ def gemv(c, trans_a, alpha, A, x, beta):
 def _matrix(t, name):
     """(rows, columns, row pitch) of a 2-d tensor whose columns are adjacent in memory."""
     shp, st = t.dimensions["shape"], t.dimensions["strides"]
-    _require(len(shp) == 2 and type(shp[0]) is int and type(shp[1]) is int, "%s must be a matrix with direct dimensions" % name, t)
-    rows, cols = shp
-    _require(cols == 1 or st[1] == 1, "The columns of %s must be adjacent in memory" % name, t)
-    _require(rows <= 1 or st[0] >= cols, "The rows of %s overlap" % name, t)
-    return rows, cols, st[0] if rows > 1 and st[0] >= cols else cols
+    if len(shp) == 2:
+        rows, cols = shp
+        if type(rows) is int and type(cols) is int and (st[1] == 1 or cols == 1):
+            if rows <= 1:
+                return rows, cols, cols
+            if st[0] >= cols:
+                return rows, cols, st[0]
+    raise TensorError("%s must be a matrix whose columns are adjacent in memory and whose rows do not overlap: %r" % (name, t))
 
 
 def _matrices(t, name):
     """(count, rows, columns, distance, row pitch) of a 3-d tensor of matrices."""
     shp, st = t.dimensions["shape"], t.dimensions["strides"]
-    _require(len(shp) == 3 and dims.direct_shape(shp), "%s must hold one matrix per expert" % name, t)
-    count, rows, cols = shp
-    _require(cols == 1 or st[2] == 1, "The columns of %s must be adjacent in memory" % name, t)
-    pitch = st[1] if rows > 1 else max(st[1], cols)
-    _require(pitch >= cols and (count == 1 or st[0] >= rows * pitch), "The matrices of %s overlap" % name, t)
-    return count, rows, cols, st[0], pitch
+    if len(shp) == 3 and dims.direct_shape(shp) and (st[2] == 1 or shp[2] == 1):
+        count, rows, cols = shp
+        pitch = st[1] if rows > 1 else max(st[1], cols)
+        if pitch >= cols and (count == 1 or st[0] >= rows * pitch):
+            return count, rows, cols, st[0], pitch
+    raise TensorError("%s must hold one matrix per expert, none overlapping, with adjacent columns: %r" % (name, t))
 
 
 def _span(t):
@@ -630,7 +633,8 @@ def _ensure_apart(dest, name, *others):
     for o in others:
         if o is not None:
             a, b = _span(o)
-            _require(hi <= a or b <= lo, "%s overlaps another argument" % name, (dest, o))
+            if hi > a and b > lo:
+                raise TensorError("%s overlaps another argument: %r %r" % (name, dest, o))
 
 
 def _packed(t):
@@ -644,15 +648,24 @@ def _packed(t):
 
 
 def _ensure_dense_vector(t, shape, name):
-    _require(t.dimensions["shape"] == shape and _packed(t), "%s must be a dense tensor of shape %r" % (name, shape), t)
+    if t.dimensions["shape"] != shape or not _packed(t):
+        raise TensorError("%s must be a dense tensor of shape %r: %r" % (name, shape, t))
 
 
-def _expert_checks(name, offsets, experts, *tensors):
-    first = tensors[0]
-    _ensure_datatypes(first.get_datatype(), *[t for t in tensors if t is not None])
-    _ensure_same_device(offsets, *[t for t in tensors if t is not None])
-    _require(first.get_datatype() in ("float", "double"), "%s is only defined for float and double tensors" % name)
-    _require(offsets.get_datatype() == "int", "offsets must be an integer tensor", offsets)
+def _ensure_float_operands(name, *tensors):
+    """One float type and one device; None is skipped.  Returns the datatype."""
+    datatype, device = tensors[0].buffer.dtype, tensors[0].device
+    if datatype != "float" and datatype != "double":
+        raise TensorError("%s is only defined for float and double tensors: %r" % (name, datatype))
+    for t in tensors:
+        if t is not None and (t.buffer.dtype != datatype or t.device is not device):
+            raise TensorError("%s: arguments are not all of one datatype on one device: %r" % (name, t))
+    return datatype
+
+
+def _ensure_offsets(name, offsets, experts, device):
+    if offsets.buffer.dtype != "int" or offsets.device is not device:
+        raise TensorError("%s: offsets must be an integer tensor on the arguments' device: %r" % (name, offsets))
     _ensure_dense_vector(offsets, [experts + 1], "offsets")
 
 
@@ -664,13 +677,15 @@ def expert_gemm(C, trans_b, alpha, A, B, beta, offsets, bias=None, act=None):
     an int tensor on the device; bias [experts, n]; act None, "relu", "tanh" or "logistic".  Groups may be empty; rows outside
     every group keep what C holds.  Offsets that decrease or leave the rows make the next sync of the stream raise."""
     experts, b_rows, b_cols, b_stride, ldb = _matrices(B, "B")
-    _expert_checks("expert-gemm", offsets, experts, C, A, B, bias)
+    _ensure_float_operands("expert-gemm", C, A, B, bias)
+    _ensure_offsets("expert-gemm", offsets, experts, C.device)
     rows, k, lda = _matrix(A, "A")
     c_rows, n, ldc = _matrix(C, "C")
     inner, outer = (b_cols, b_rows) if trans_b else (b_rows, b_cols)
-    _require(k == inner, "A col count doesn't match B row count", ((rows, k), (inner, outer)))
-    _require(c_rows == rows and n == outer, "C shape doesn't match A rows and B columns", ((c_rows, n), (rows, outer)))
-    _require(act in (None, "none", "relu", "tanh", "logistic"), "expert-gemm activation must be relu, tanh or logistic", act)
+    if k != inner or c_rows != rows or n != outer:
+        raise TensorError("Shapes do not fit: C %r, A %r, op(B) %r" % ((c_rows, n), (rows, k), (inner, outer)))
+    if act not in (None, "none", "relu", "tanh", "logistic"):
+        raise TensorError("expert-gemm activation must be relu, tanh or logistic: %r" % (act,))
     if bias is not None:
         _ensure_dense_vector(bias, [experts, n], "bias")
     _ensure_apart(C, "C", A, B, bias, offsets)
@@ -684,11 +699,12 @@ def expert_gemm_weights(C, alpha, A, B, beta, offsets, bias_gradient=None):
     the gradient of the output (A [rows, n]) and the input (B [rows, k]); C [experts, n, k].  bias_gradient [experts, n], when
     given, becomes alpha * (column sums of A_e) + beta * bias_gradient.  offsets as in expert_gemm."""
     experts, c_rows, c_cols, c_stride, ldc = _matrices(C, "C")
-    _expert_checks("expert-gemm-weights", offsets, experts, C, A, B, bias_gradient)
+    _ensure_float_operands("expert-gemm-weights", C, A, B, bias_gradient)
+    _ensure_offsets("expert-gemm-weights", offsets, experts, C.device)
     rows, n, lda = _matrix(A, "A")
     b_rows, k, ldb = _matrix(B, "B")
-    _require(b_rows == rows, "A and B must have the same rows", ((rows, n), (b_rows, k)))
-    _require(c_rows == n and c_cols == k, "C shape doesn't match the columns of A and B", ((c_rows, c_cols), (n, k)))
+    if b_rows != rows or c_rows != n or c_cols != k:
+        raise TensorError("Shapes do not fit: C %r, A %r, B %r" % ((c_rows, c_cols), (rows, n), (b_rows, k)))
     _ensure_apart(C, "C", A, B, bias_gradient, offsets)
     if bias_gradient is not None:
         _ensure_dense_vector(bias_gradient, [experts, n], "bias_gradient")
@@ -701,40 +717,52 @@ def expert_gemm_weights(C, alpha, A, B, beta, offsets, bias_gradient=None):
 # ------------------------------ the normalisations around a residual block --------
 # (no counterpart in the reference, next to its batch and local response normalisation)
 
-def _block_setup(name, matrices, vectors, gate, gate_gradient, residual_scale, epsilon, kind):
-    """Shared checks: returns (datatype, flat (address, pitch) list, addresses of the vectors, descriptor).
-    matrices: name -> tensor or None (the first is there); vectors: name -> tensor or None."""
-    first = next(t for t in matrices.values() if t is not None)
-    datatype = first.get_datatype()
-    there = [t for t in list(matrices.values()) + list(vectors.values()) + [gate, gate_gradient] if t is not None]
-    _require(datatype in ("float", "double"), "%s is only defined for float and double tensors" % name, datatype)
-    _ensure_datatypes(datatype, *there)
-    _ensure_same_device(*there)
-    _require(kind in NORMALIZATIONS, "unknown normalisation", kind)
-    _require(epsilon > 0, "Epsilon must be positive", epsilon)
-    rows, cols, _ = _matrix(first, "input")
+def _block_matrices(shape, *matrices):
+    """(address, pitch) of each matrix in a row, all of the same shape; None: (None, 0)."""
     flat = []
-    for label, t in matrices.items():
+    for t in matrices:
         if t is None:
-            flat += [None, 0]
+            flat += (None, 0)
         else:
-            r, c, pitch = _matrix(t, label)
-            _require(r == rows and c == cols, "Tensor shapes do not match", {label: (r, c), "expected": (rows, cols)})
-            flat += [t.buffer.ptr, pitch]
-    for label, t in vectors.items():
-        if t is not None:
-            _ensure_dense_vector(t, [cols], label)
+            rows, cols, pitch = _matrix(t, "input")
+            if rows != shape[0] or cols != shape[1]:
+                raise TensorError("Tensor shapes do not match: %r, expected %r" % (t, shape))
+            flat += (t.buffer.ptr, pitch)
+    return flat
+
+
+def _block_vectors(cols, *vectors):
+    """Addresses of dense vectors of `cols` elements; None stays."""
+    out = []
+    for t in vectors:
+        if t is None:
+            out.append(None)
+        else:
+            if t.dimensions["shape"] != [cols] or (t.dimensions["strides"][0] != 1 and cols > 1):
+                raise TensorError("scales and biases must be dense vectors of %d elements: %r" % (cols, t))
+            out.append(t.buffer.ptr)
+    return out
+
+
+def _block_desc(shape, gate, gate_gradient, residual_scale, epsilon, kind):
+    if kind not in NORMALIZATIONS:
+        raise TensorError("unknown normalisation: %r" % (kind,))
+    if not epsilon > 0:
+        raise TensorError("Epsilon must be positive: %r" % (epsilon,))
+    rows, cols = shape
     gate_rows = 1
     if gate is not None:
         shp = gate.dimensions["shape"]
-        _require(_packed(gate) and shp[-1] == cols and len(shp) <= 2, "gate must be a dense tensor of columns or rows of columns", gate)
+        if len(shp) > 2 or shp[-1] != cols or not _packed(gate):
+            raise TensorError("gate must be a dense tensor of columns or rows of columns: %r" % (gate,))
         gate_rows = shp[0] if len(shp) == 2 else 1
-        _require(gate_rows >= 1 and rows % gate_rows == 0, "The rows of the gate must divide the rows of the batch", (gate_rows, rows))
-    if gate_gradient is not None:
-        _require(gate is not None and _packed(gate_gradient) and gate_gradient.dimensions["shape"] == gate.dimensions["shape"],
-                 "gate_gradient must be a dense tensor of the gate's shape", gate_gradient)
-    desc = BlockDesc(NORMALIZATIONS[kind], float(epsilon), float(residual_scale), rows, cols, gate_rows)
-    return datatype, flat, [t.buffer.ptr if t is not None else None for t in vectors.values()], desc
+        if gate_rows < 1 or rows % gate_rows:
+            raise TensorError("The rows of the gate must divide the rows of the batch: %r" % ((gate_rows, rows),))
+        if gate_gradient is not None and (gate_gradient.dimensions["shape"] != shp or not _packed(gate_gradient)):
+            raise TensorError("gate_gradient must be a dense tensor of the gate's shape: %r" % (gate_gradient,))
+    elif gate_gradient is not None:
+        raise TensorError("gate_gradient without a gate")
+    return BlockDesc(NORMALIZATIONS[kind], epsilon, residual_scale, rows, cols, gate_rows)
 
 
 def _address(t):
@@ -754,17 +782,21 @@ def block_normalize(output, total, block, residual, gate, residual_scale, after,
     Returns [total, output]."""
     a_scale, a_bias = after if after is not None else (None, None)
     b_scale, b_bias = before if before is not None else (None, None)
-    _require(residual is not None, "A residual is needed")
-    _require((output is not None) == (b_scale is not None), "output and the normalisation before the next block go together")
-    _require(output is not None or total is not None, "Neither output nor total is wanted")
-    _require(block is None or total is not None, "A block needs a total to be added into")
-    _require(block is not None or (gate is None and a_scale is None), "gate and after-normalisation belong to a block")
-    datatype, flat, _, desc = _block_setup(
-        "block-normalize", {"residual": residual, "output": output, "total": total, "block": block},
-        {"after scale": a_scale, "after bias": a_bias, "before scale": b_scale, "before bias": b_bias}, gate, None,
-        residual_scale, epsilon, kind)
-    check_stream().block_normalize(datatype, flat[2:] + flat[:2],
-                                   [_address(t) for t in (gate, a_scale, a_bias, b_scale, b_bias)], desc)
+    if residual is None:
+        raise TensorError("A residual is needed")
+    if (output is None) != (b_scale is None):
+        raise TensorError("output and the normalisation before the next block go together")
+    if total is None and (output is None or block is not None):
+        raise TensorError("A block needs a total to be added into" if block is not None else "Neither output nor total is wanted")
+    if block is None and (gate is not None or a_scale is not None):
+        raise TensorError("gate and after-normalisation belong to a block")
+    datatype = _ensure_float_operands("block-normalize", residual, output, total, block, gate, a_scale, a_bias, b_scale, b_bias)
+    rows, cols, pitch = _matrix(residual, "residual")
+    shape = (rows, cols)
+    check_stream().block_normalize(
+        datatype, _block_matrices(shape, output, total, block) + [residual.buffer.ptr, pitch],
+        [_address(gate)] + _block_vectors(cols, a_scale, a_bias, b_scale, b_bias),
+        _block_desc(shape, gate, None, residual_scale, epsilon, kind))
     return [total, output]
 
 
@@ -780,27 +812,43 @@ def block_normalize_gradients(block_gradient, residual_gradient, gate_gradient, 
     b_scale, _b_bias = before if before is not None else (None, None)
     ga_scale, ga_bias = after_gradients if after_gradients is not None else (None, None)
     gb_scale, gb_bias = before_gradients if before_gradients is not None else (None, None)
-    _require(residual_gradient is not None, "A residual_gradient is needed")
-    _require((output_gradient is not None) == (b_scale is not None), "output_gradient and the normalisation before the next block go together")
-    _require(output_gradient is not None or total_gradient is not None, "No gradient arrives")
-    _require(b_scale is None or total is not None, "The normalisation before the next block needs the total")
-    _require((block is None) == (block_gradient is None), "block and block_gradient go together")
-    _require(block is not None or (gate is None and a_scale is None), "gate and after-normalisation belong to a block")
-    _require(a_scale is not None or (ga_scale is None and ga_bias is None), "after_gradients without an after-normalisation")
-    _require(b_scale is not None or (gb_scale is None and gb_bias is None), "before_gradients without a before-normalisation")
-    matrices = {"residual_gradient": residual_gradient, "block_gradient": block_gradient, "output_gradient": output_gradient,
-                "total_gradient": total_gradient, "total": total, "block": block}
-    vectors = {"after scale": a_scale, "after bias": a_bias, "before scale": b_scale, "after scale gradient": ga_scale,
-               "after bias gradient": ga_bias, "before scale gradient": gb_scale, "before bias gradient": gb_bias}
-    datatype, flat, _, desc = _block_setup("block-normalize-gradients", matrices, vectors, gate, gate_gradient, residual_scale,
-                                           epsilon, kind)
+    if residual_gradient is None:
+        raise TensorError("A residual_gradient is needed")
+    if (output_gradient is None) != (b_scale is None):
+        raise TensorError("output_gradient and the normalisation before the next block go together")
+    if output_gradient is None and total_gradient is None:
+        raise TensorError("No gradient arrives")
+    if b_scale is not None and total is None:
+        raise TensorError("The normalisation before the next block needs the total")
+    if (block is None) != (block_gradient is None):
+        raise TensorError("block and block_gradient go together")
+    if block is None and (gate is not None or a_scale is not None):
+        raise TensorError("gate and after-normalisation belong to a block")
+    if (a_scale is None and (ga_scale is not None or ga_bias is not None)) or (
+            b_scale is None and (gb_scale is not None or gb_bias is not None)):
+        raise TensorError("gradients of a normalisation that is not there")
+    datatype = _ensure_float_operands("block-normalize-gradients", residual_gradient, block_gradient, gate_gradient, ga_scale,
+                                      ga_bias, gb_scale, gb_bias, output_gradient, total_gradient, total, block, gate, a_scale,
+                                      a_bias, b_scale)
+    rows, cols, pitch = _matrix(residual_gradient, "residual_gradient")
+    shape = (rows, cols)
+    desc = _block_desc(shape, gate, gate_gradient, residual_scale, epsilon, kind)
+    vectors = _block_vectors(cols, a_scale, a_bias, b_scale)
     sums = [t for t in (ga_scale, ga_bias, gb_scale, gb_bias) if t is not None]
-    operands = [output_gradient, total_gradient, total, block, gate, a_scale, a_bias, b_scale]
-    for i, t in enumerate(sums):
-        _ensure_apart(t, "A gradient", block_gradient, residual_gradient, gate_gradient, *sums[i + 1:], *operands)
+    sum_addresses = _block_vectors(cols, ga_scale, ga_bias, gb_scale, gb_bias)
+    others = [block_gradient, residual_gradient, gate_gradient, output_gradient, total_gradient, total, block, gate, a_scale,
+              a_bias, b_scale]
+    spans = [_span(t) for t in others if t is not None]
+    for t in sums:                                   # the vectors that are written share no memory with anything else
+        lo, hi = span = _span(t)
+        for a, b in spans:
+            if hi > a and b > lo:
+                raise TensorError("The gradient of a scale or bias overlaps another argument: %r" % (t,))
+        spans.append(span)
     check_stream().block_normalize_gradients(
-        datatype, flat[2:4] + flat[:2], [_address(t) for t in (gate_gradient, ga_scale, ga_bias, gb_scale, gb_bias)], flat[4:],
-        [_address(t) for t in (gate, a_scale, a_bias, b_scale)], desc)
+        datatype, _block_matrices(shape, block_gradient) + [residual_gradient.buffer.ptr, pitch],
+        [_address(gate_gradient)] + sum_addresses,
+        _block_matrices(shape, output_gradient, total_gradient, total, block), [_address(gate)] + vectors, desc)
     return [block_gradient, residual_gradient]
 
 

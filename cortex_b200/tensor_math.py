@@ -8,6 +8,7 @@ objects with ``.ptr`` / ``.dtype`` and dimensions are the dicts of
 ``cortex_b200.dimensions``.
 """
 import ctypes as C
+from array import array
 
 from . import dimensions as dims_mod
 from ._lib import ACTIVATIONS, BINARY_OPS, DTYPE_CODE, REDUCE_OPS, TERNARY_OPS, UNARY_OPS, ConvDesc, Dims
@@ -192,19 +193,15 @@ class CTensorMath:
         self._tm("block_normalize_gradients", DTYPE_CODE[dtype], *gradients, *vector_gradients, *matrices, *vectors,
                  C.byref(desc))
 
-    @staticmethod
-    def _pointer_list(buffers):
-        return (C.c_void_p * len(buffers))(*[b.ptr for b in buffers])
-
     def global_norm(self, dtype, gradients, counts, norm):
-        """norm[0] = sqrt(sum of squares over all buffers)."""
-        n = len(gradients)
-        self._tm("global_norm", DTYPE_CODE[dtype], n, self._pointer_list(gradients), (C.c_int64 * n)(*counts), norm.ptr)
+        """norm[0] = sqrt(sum of squares over all buffers); addresses and counts as lists of integers."""
+        g, n = array("Q", gradients), array("q", counts)
+        self._tm("global_norm", DTYPE_CODE[dtype], len(g), g.buffer_info()[0], n.buffer_info()[0], norm.ptr)
 
     def clip_gradients(self, dtype, gradients, counts, clipped, max_norm, norm):
-        n = len(gradients)
-        self._tm("clip_gradients", DTYPE_CODE[dtype], n, self._pointer_list(gradients), (C.c_int64 * n)(*counts),
-                 self._pointer_list(clipped), float(max_norm), norm.ptr if norm is not None else None)
+        g, n, c = array("Q", gradients), array("q", counts), array("Q", clipped)
+        self._tm("clip_gradients", DTYPE_CODE[dtype], len(g), g.buffer_info()[0], n.buffer_info()[0], c.buffer_info()[0],
+                 max_norm, norm.ptr if norm is not None else None)
 
     def _tm_nostream(self, name, *args):
         from ._lib import call

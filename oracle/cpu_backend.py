@@ -326,20 +326,18 @@ class OracleStream(CTensorMath):
             if to is not None:
                 to[...] = got[name][0]
 
-    def _flat(self, buffer, n):
-        return self._view(buffer.ptr, buffer.dtype, (n,), (1,))
-
     def global_norm(self, dtype, gradients, counts, norm):
-        self._flat(norm, 1)[0] = plain_operators.global_norm([self._flat(g, n) for g, n in zip(gradients, counts)])
+        self._view(norm.ptr, dtype, (1,), (1,))[0] = plain_operators.global_norm(
+            [self._view(g, dtype, (n,), (1,)) for g, n in zip(gradients, counts)])
 
     def clip_gradients(self, dtype, gradients, counts, clipped, max_norm, norm):
-        values = [self._flat(g, n) for g, n in zip(gradients, counts)]
+        values = [self._view(g, dtype, (n,), (1,)) for g, n in zip(gradients, counts)]
         n = plain_operators.global_norm(values)
         scale = plain_operators.clip_scale(n, max_norm)
         for g, c, k in zip(values, clipped, counts):
-            self._flat(c, k)[...] = g.astype(np.float64) * scale
+            self._view(c, dtype, (k,), (1,))[...] = g.astype(np.float64) * scale
         if norm is not None:
-            self._flat(norm, 1)[0] = n
+            self._view(norm.ptr, dtype, (1,), (1,))[0] = n
 
     def choose_convolution_algorithms(self, conv_descriptor, input_width, input_height, output_width, output_height,
                                       batch_size, max_ideal_workspace_size, use_defaults):
