@@ -156,6 +156,101 @@ __global__ void __launch_bounds__(256) expert_weights_simt_kernel(Product<T> p, 
   }
 }
 
+// ---- few rows per expert: the matrices are read once, as fast as memory delivers them ---------------------------------
+// A tile is up to 8 rows of one group; a warp takes 4 rows of its expert's matrix ([out, in]: contiguous along the reduction)
+// and strides over the reduction with 16-byte loads, the rows of A coming from L1.  The 4 x R sums of a lane are folded over
+// the warp (31 shuffles for 32 of them) so that each ends in one lane, which finishes and stores it.
+constexpr int FEW = 8, FEW_OUT = 4, FEW_WARPS = 8;
+
+template <typename T, int V, int R>
+__device__ __forceinline__ void few_rows(const Product<T>& p, const groups::Tile& tile, int t0, int left, int n0) {
+  struct alignas(sizeof(T) * V) Pack { T e[V]; };
+  constexpr int VALUES = FEW_OUT * R;
+  const int lane = threadIdx.x & 31;
+  const T* w = p.B + tile.expert * p.b_stride;
+  const T* a = p.A + (long long)t0 * p.lda;
+  T acc[VALUES];
+#pragma unroll
+  for (int i = 0; i < VALUES; ++i) acc[i] = (T)0;
+  const T* wr[FEW_OUT];
+#pragma unroll
+  for (int j = 0; j < FEW_OUT; ++j) wr[j] = w + (long long)min(n0 + j, p.N - 1) * p.ldb;      // (stores are bounded below)
+#pragma unroll 2
+  for (int k = lane * V; k < p.K; k += 32 * V) {           // V > 1: K is a multiple of V
+    Pack m[FEW_OUT], x[R];
+#pragma unroll
+    for (int j = 0; j < FEW_OUT; ++j) m[j] = *reinterpret_cast<const Pack*>(wr[j] + k);
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = *reinterpret_cast<const Pack*>(a + (long long)min(r, left - 1) * p.lda + k);
+#pragma unroll
+    for (int j = 0; j < FEW_OUT; ++j)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[j * R + r] += m[j].e[e] * x[r].e[e];
+  }
+  // fold: after step d a lane keeps the half of the values that its bit selects
+  int which = 0;
+#pragma unroll
+  for (int half = VALUES / 2, d = 16; d > 0; d >>= 1) {
+    if (half > 0) {
+      const bool up = (lane & d) != 0;
+#pragma unroll
+      for (int i = 0; i < VALUES / 2; ++i)
+        if (i < half) {
+          const T give = up ? acc[i] : acc[i + half], keep = up ? acc[i + half] : acc[i];
+          acc[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+        }
+      which = which * 2 + (up ? 1 : 0);
+      half >>= 1;
+    } else {
+      acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], d);
+    }
+  }
+  const int n = n0 + which / R, r = which % R;
+  constexpr int SAME = 32 / VALUES;                        // lanes that end with the same value
+  if ((lane & (SAME - 1)) == 0 && n < p.N && r < left) {
+    T* c = p.C + (long long)(t0 + r) * p.ldc + n;
+    T o = p.alpha * acc[0];
+    if (p.beta != (T)0) o += p.beta * (*c);
+    if (p.bias) o += p.bias[(long long)tile.expert * p.N + n];
+    *c = act_apply<T>(o, p.act);
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(FEW_WARPS * 32) expert_few_rows_kernel(Product<T> p, int n_blocks) {
+  const int t = (int)blockIdx.x / n_blocks;
+  const int n0 = (((int)blockIdx.x - t * n_blocks) * FEW_WARPS + (threadIdx.x >> 5)) * FEW_OUT;
+  groups::Tile tile;
+  if (!groups::find_tile(p.offsets, p.experts, p.rows, FEW, t, p.status, tile)) return;
+  if (n0 >= p.N) return;
+  const int t0 = tile.lo + tile.index * FEW, left = tile.hi - t0;
+  if (left == 1) few_rows<T, V, 1>(p, tile, t0, left, n0);
+  else if (left == 2) few_rows<T, V, 2>(p, tile, t0, left, n0);
+  else if (left <= 4) few_rows<T, V, 4>(p, tile, t0, left, n0);
+  else few_rows<T, V, 8>(p, tile, t0, left < FEW ? left : FEW, n0);
+}
+
+// By the rows alone (which expert gets how many is not known here).  fp32, 8 experts of 4096 x 1024, rows in all: 2 12 us (the
+// tensor-core kernel 23), 8 25 us (50), 32 47 us (50), 64 68 us (52).
+bool few_rows_ok(const Product<float>& p) { return p.trans_b && p.rows <= 4 * p.experts && p.rows <= 4096; }
+bool few_rows_ok(const Product<double>& p) { return p.trans_b && p.rows <= 8 * p.experts && p.rows <= 4096; }
+
+template <typename T> int run_few_rows(cb200_stream* s, const Product<T>& p) {
+  DeviceGuard guard(s->device);
+  constexpr int V = 16 / sizeof(T);
+  const long long tiles = (p.rows + FEW - 1) / FEW + (p.experts < p.rows ? p.experts : p.rows) - 1;
+  const long long n_blocks = (p.N + FEW_WARPS * FEW_OUT - 1) / (FEW_WARPS * FEW_OUT), ctas = tiles * n_blocks;
+  CB_REQUIRE(ctas <= 2147483647LL, "expert_gemm: too many tiles");
+  if ((((uintptr_t)p.A | (uintptr_t)p.B) & 15) == 0 && p.lda % V == 0 && p.ldb % V == 0 && p.b_stride % V == 0 && p.K % V == 0)
+    expert_few_rows_kernel<T, V><<<(unsigned)ctas, FEW_WARPS * 32, 0, s->stream>>>(p, (int)n_blocks);
+  else
+    expert_few_rows_kernel<T, 1><<<(unsigned)ctas, FEW_WARPS * 32, 0, s->stream>>>(p, (int)n_blocks);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
 // bias_gradient[e, m] = alpha * sum of the group's rows + beta * bias_gradient[e, m]: a warp reads 32 * V columns of a row,
 // the CTA's eight warps take every eighth row with four rows in flight each; fixed order
 template <typename T, int V>
@@ -219,6 +314,7 @@ template <typename T> int run_bias_gradient(cb200_stream* s, const Product<T>& p
 }
 
 template <typename T> int run_rows(cb200_stream* s, const Product<T>& p) {
+  if (!p.only_if && few_rows_ok(p)) return run_few_rows<T>(s, p);
   DeviceGuard guard(s->device);
   const long long tiles = (p.rows + 63) / 64 + (p.experts < p.rows ? p.experts : p.rows);
   expert_rows_simt_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles < 65535 ? tiles : 65535)), 256, 0, s->stream>>>(p);
@@ -258,6 +354,7 @@ int pack(cb200_stream* s, float* dst, const float* src, long long ld, long long 
 }
 
 int rows_tc(cb200_stream* s, Product<float> p) {
+  if (few_rows_ok(p) && s->opt_gemm_auto_presplit != 2 && s->opt_gemm_tile_n == 0) return run_few_rows<float>(s, p);
   const long long b_rows = p.trans_b ? p.N : p.K;
   const int b_cols = p.trans_b ? p.K : p.N;
   if (p.experts == 1) p.b_stride = b_rows * p.ldb;

@@ -70,7 +70,9 @@ struct RowsArgs {
 
 template <int BN, int BK> struct RowsCfg {
   static constexpr int A_TILE = BM * BK * 4, B_TILE = BN * BK * 4, RAW = A_TILE + B_TILE, STAGE = 2 * RAW;
-  static constexpr int STAGES = (196608 / STAGE) > 8 ? 8 : (196608 / STAGE);
+  // narrow tiles: two CTAs per SM, one streaming while the other sets up or stores
+  static constexpr int CTAS = BN <= 64 ? 2 : 1;
+  static constexpr int STAGES = (196608 / CTAS / STAGE) > 8 ? 8 : (196608 / CTAS / STAGE);
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int BOX_ROWS = BN < 64 ? BN : 64;          // rows of one TMA box of the ragged operand
   static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
@@ -105,7 +107,7 @@ __device__ __forceinline__ void store_columns(const RowsArgs& p, const uint32_t 
 }
 
 template <int BN, int BK>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, RowsCfg<BN, BK>::CTAS)
 expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ RowsArgs p) {
   typedef RowsCfg<BN, BK> C;
   constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
@@ -734,7 +736,7 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   int slices = 1;
   const int forced = s->opt_gemm_k_slices;
   for (int sl = 2; sl <= 8; sl *= 2)
-    if ((forced > 0 ? sl <= forced : units * sl <= s->sm_count) && nkb / sl >= 4) slices = sl;
+    if ((forced > 0 ? sl <= forced : units * sl <= s->sm_count * (BN <= 64 ? 2 : 1)) && nkb / sl >= 4) slices = sl;
   if ((nkb + slices - 1) / slices > chunk || only_if) slices = 1;
   RowsArgs a;
   a.C = C; a.ldc = ldc; a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
