@@ -50,68 +50,139 @@ template <typename T> struct Product {
   int* status;
 };
 
-// 64 x 64 tile, 16 x 16 threads, 4 x 4 values per thread, operands of any pitch and alignment.
-// Element (m, k) of the left operand at a[m * sam + k * sak], (k, n) of the right one at b[k * sbk + n * sbn].
+// A 64 x 64 tile by 256 threads, operands of any pitch and alignment.  Element (m, k) of the left operand at
+// a[m * sam + k * sak], (k, n) of the right one at b[k * sbk + n * sbn].  float: 4 x 4 plain FMAs per thread.
+template <typename T> struct Tile64;
+
 template <typename T>
-__device__ __forceinline__ void simt_tile(const T* a, long long sam, long long sak, const T* b, long long sbk, long long sbn,
-                                          int m_left, int n_left, int K, T (&acc)[4][4]) {
-  __shared__ T As[16][64 + 1];
-  __shared__ T Bs[16][64 + 1];
-  const int t = threadIdx.x, tx = t % 16, ty = t / 16;
+__device__ __forceinline__ void finish(T* to, T sum, int n, T alpha, T beta, const T* bias, int act) {
+  T o = alpha * sum;
+  if (beta != (T)0) o += beta * (*to);
+  if (bias) o += bias[n];
+  *to = act_apply<T>(o, act);
+}
+
+template <> struct Tile64<float> {
+  float acc[4][4];
+  __device__ __forceinline__ void run(const float* a, long long sam, long long sak, const float* b, long long sbk, long long sbn, int m_left,
+                                      int n_left, int K) {
+    __shared__ float As[16][64 + 1];
+    __shared__ float Bs[16][64 + 1];
+    const int t = threadIdx.x, tx = t % 16, ty = t / 16;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = (T)0;
-  for (int k0 = 0; k0 < K; k0 += 16) {
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    for (int k0 = 0; k0 < K; k0 += 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int k, m;
+        if (sak == 1) { k = t % 16; m = t / 16 + 16 * i; } else { m = t % 64; k = t / 64 + 4 * i; }
+        As[k][m] = (m < m_left && k0 + k < K) ? a[(long long)m * sam + (long long)(k0 + k) * sak] : 0.f;
+        int kb, n;
+        if (sbn == 1) { n = t % 64; kb = t / 64 + 4 * i; } else { kb = t % 16; n = t / 16 + 16 * i; }
+        Bs[kb][n] = (n < n_left && k0 + kb < K) ? b[(long long)(k0 + kb) * sbk + (long long)n * sbn] : 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        float x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = As[k][ty + 16 * i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = Bs[k][tx + 16 * j];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] += x[i] * y[j];
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void store(float* c, long long ldc, int m_left, int n_left, float alpha, float beta, const float* bias, int act) {
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int m = ty + 16 * i, n = tx + 16 * j;
+        if (m < m_left && n < n_left) finish<float>(c + (long long)m * ldc + n, acc[i][j], n, alpha, beta, bias, act);
+      }
+  }
+};
+
+// double: the fp64 matrix instruction (m8n8k4), 8 warps as 2 x 4 of 32 x 16, the next 16 values of k on their way into
+// registers meanwhile.  Row pitch 68 (4 mod 16): the 16 fragment elements of a half-warp lie in 16 different banks.
+template <> struct Tile64<double> {
+  double acc[4][2][2];
+  __device__ __forceinline__ void run(const double* a, long long sam, long long sak, const double* b, long long sbk, long long sbn, int m_left,
+                                      int n_left, int K) {
+    constexpr int LD = 68;
+    __shared__ double As[16][LD];
+    __shared__ double Bs[16][LD];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, wm = (warp >> 2) * 32, wn = (warp & 3) * 16, fr = lane >> 2, fk = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+    double ra[4], rb[4];
+    auto load = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int k, m;
+        if (sak == 1) { k = t % 16; m = t / 16 + 16 * i; } else { m = t % 64; k = t / 64 + 4 * i; }
+        ra[i] = (m < m_left && k0 + k < K) ? a[(long long)m * sam + (long long)(k0 + k) * sak] : 0.0;
+        int kb, n;
+        if (sbn == 1) { n = t % 64; kb = t / 64 + 4 * i; } else { kb = t % 16; n = t / 16 + 16 * i; }
+        rb[i] = (n < n_left && k0 + kb < K) ? b[(long long)(k0 + kb) * sbk + (long long)n * sbn] : 0.0;
+      }
+    };
+    if (K > 0) load(0);
+    for (int k0 = 0; k0 < K; k0 += 16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (sak == 1) As[t % 16][t / 16 + 16 * i] = ra[i]; else As[t / 64 + 4 * i][t % 64] = ra[i];
+        if (sbn == 1) Bs[t / 64 + 4 * i][t % 64] = rb[i]; else Bs[t % 16][t / 16 + 16 * i] = rb[i];
+      }
+      __syncthreads();
+      if (k0 + 16 < K) load(k0 + 16);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        double x[4], y[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = As[kk * 4 + fk][wm + i * 8 + fr];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) y[j] = Bs[kk * 4 + fk][wn + j * 8 + fr];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
+                         : "+d"(acc[i][j][0]), "+d"(acc[i][j][1])
+                         : "d"(x[i]), "d"(y[j]));
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void store(double* c, long long ldc, int m_left, int n_left, double alpha, double beta, const double* bias, int act) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = (warp >> 2) * 32, wn = (warp & 3) * 16;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      int k, m;
-      if (sak == 1) { k = t % 16; m = t / 16 + 16 * i; } else { m = t % 64; k = t / 64 + 4 * i; }
-      As[k][m] = (m < m_left && k0 + k < K) ? a[(long long)m * sam + (long long)(k0 + k) * sak] : (T)0;
-      int kb, n;
-      if (sbn == 1) { n = t % 64; kb = t / 64 + 4 * i; } else { kb = t % 16; n = t / 16 + 16 * i; }
-      Bs[kb][n] = (n < n_left && k0 + kb < K) ? b[(long long)(k0 + kb) * sbk + (long long)n * sbn] : (T)0;
-    }
-    __syncthreads();
+      const int m = wm + i * 8 + (lane >> 2);
+      if (m >= m_left) continue;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      T x[4], y[4];
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = As[k][ty + 16 * i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = Bs[k][tx + 16 * j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += x[i] * y[j];
-    }
-    __syncthreads();
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void simt_store(T* c, long long ldc, int m_left, int n_left, const T (&acc)[4][4], T alpha, T beta,
-                                           const T* bias, int act) {
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = ty + 16 * i;
-    if (m >= m_left) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = tx + 16 * j;
-      if (n >= n_left) continue;
-      T* to = c + (long long)m * ldc + n;
-      T o = alpha * acc[i][j];
-      if (beta != (T)0) o += beta * (*to);
-      if (bias) o += bias[n];
-      *to = act_apply<T>(o, act);
+        for (int e = 0; e < 2; ++e) {
+          const int n = wn + j * 8 + (lane & 3) * 2 + e;
+          if (n < n_left) finish<double>(c + (long long)m * ldc + n, acc[i][j][e], n, alpha, beta, bias, act);
+        }
     }
   }
-}
+};
 
 template <typename T>
-__global__ void __launch_bounds__(256) expert_rows_simt_kernel(Product<T> p) {
+__global__ void __launch_bounds__(256, 3) expert_rows_tile_kernel(Product<T> p) {
   __shared__ groups::Tile tile;
   __shared__ bool found;
   if (p.only_if && *p.only_if == 0) return;
@@ -126,16 +197,15 @@ __global__ void __launch_bounds__(256) expert_rows_simt_kernel(Product<T> p) {
     if (!found) return;
     const int m0 = tile.lo + tile.index * 64, n0 = (int)blockIdx.x * 64;
     const T* b = p.B + tile.expert * p.b_stride + (p.trans_b ? (long long)n0 * p.ldb : (long long)n0);
-    T acc[4][4];
-    simt_tile<T>(p.A + (long long)m0 * p.lda, p.lda, 1, b, p.trans_b ? 1 : p.ldb, p.trans_b ? p.ldb : 1, tile.hi - m0, p.N - n0,
-                 p.K, acc);
-    simt_store<T>(p.C + (long long)m0 * p.ldc + n0, p.ldc, tile.hi - m0, p.N - n0, acc, p.alpha, p.beta,
-                  p.bias ? p.bias + (long long)tile.expert * p.N + n0 : nullptr, p.act);
+    Tile64<T> c;
+    c.run(p.A + (long long)m0 * p.lda, p.lda, 1, b, p.trans_b ? 1 : p.ldb, p.trans_b ? p.ldb : 1, tile.hi - m0, p.N - n0, p.K);
+    c.store(p.C + (long long)m0 * p.ldc + n0, p.ldc, tile.hi - m0, p.N - n0, p.alpha, p.beta,
+            p.bias ? p.bias + (long long)tile.expert * p.N + n0 : nullptr, p.act);
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) expert_weights_simt_kernel(Product<T> p, int tiles_m) {
+__global__ void __launch_bounds__(256, 3) expert_weights_tile_kernel(Product<T> p, int tiles_m) {
   __shared__ int lo, hi;
   if (p.only_if && *p.only_if == 0) return;
   const int e = (int)blockIdx.z;
@@ -148,11 +218,9 @@ __global__ void __launch_bounds__(256) expert_weights_simt_kernel(Product<T> p, 
   const int n0 = (int)blockIdx.x * 64;
   for (int tm = (int)blockIdx.y; tm < tiles_m; tm += (int)gridDim.y) {
     const int m0 = tm * 64;
-    T acc[4][4];
-    simt_tile<T>(p.A + (long long)lo * p.lda + m0, 1, p.lda, p.B + (long long)lo * p.ldb + n0, p.ldb, 1, p.M - m0, p.N - n0,
-                 hi - lo, acc);
-    simt_store<T>(p.C + e * p.c_stride + (long long)m0 * p.ldc + n0, p.ldc, p.M - m0, p.N - n0, acc, p.alpha, p.beta, nullptr,
-                  CB200_ACT_NONE);
+    Tile64<T> c;
+    c.run(p.A + (long long)lo * p.lda + m0, 1, p.lda, p.B + (long long)lo * p.ldb + n0, p.ldb, 1, p.M - m0, p.N - n0, hi - lo);
+    c.store(p.C + e * p.c_stride + (long long)m0 * p.ldc + n0, p.ldc, p.M - m0, p.N - n0, p.alpha, p.beta, nullptr, CB200_ACT_NONE);
   }
 }
 
@@ -233,8 +301,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32) expert_few_rows_kernel(Product
 }
 
 // By the rows alone (which expert gets how many is not known here).  fp32, 8 experts of 4096 x 1024, rows in all: 2 12 us (the
-// tensor-core kernel 23), 8 25 us (50), 32 47 us (50), 64 68 us (52).
-bool few_rows_ok(const Product<float>& p) { return p.trans_b && p.rows <= 4 * p.experts && p.rows <= 4096; }
+// tensor-core kernel 23), 8 25 us (50), 32 48 us (44), 64 68 us (44).
+bool few_rows_ok(const Product<float>& p) { return p.trans_b && p.rows <= 3 * p.experts && p.rows <= 4096; }
 bool few_rows_ok(const Product<double>& p) { return p.trans_b && p.rows <= 8 * p.experts && p.rows <= 4096; }
 
 template <typename T> int run_few_rows(cb200_stream* s, const Product<T>& p) {
@@ -317,7 +385,7 @@ template <typename T> int run_rows(cb200_stream* s, const Product<T>& p) {
   if (!p.only_if && few_rows_ok(p)) return run_few_rows<T>(s, p);
   DeviceGuard guard(s->device);
   const long long tiles = (p.rows + 63) / 64 + (p.experts < p.rows ? p.experts : p.rows);
-  expert_rows_simt_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles < 65535 ? tiles : 65535)), 256, 0, s->stream>>>(p);
+  expert_rows_tile_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles < 65535 ? tiles : 65535)), 256, 0, s->stream>>>(p);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
@@ -325,7 +393,7 @@ template <typename T> int run_rows(cb200_stream* s, const Product<T>& p) {
 template <typename T> int run_weights(cb200_stream* s, const Product<T>& p) {
   DeviceGuard guard(s->device);
   const int tiles_m = (p.M + 63) / 64;
-  expert_weights_simt_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles_m < 65535 ? tiles_m : 65535), (unsigned)p.experts),
+  expert_weights_tile_kernel<T><<<dim3((unsigned)((p.N + 63) / 64), (unsigned)(tiles_m < 65535 ? tiles_m : 65535), (unsigned)p.experts),
                                   256, 0, s->stream>>>(p, tiles_m);
   CB_LAUNCH_CHECK(s);
   return p.bias_g ? run_bias_gradient<T>(s, p) : CB200_OK;
