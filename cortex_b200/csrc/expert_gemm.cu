@@ -16,7 +16,7 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
 int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
                             int M, long long lda, const float* B, int N, long long ldb, int experts, float beta,
                             const int* offsets, const int* only_if);
-bool cb200_expert_f16_ok(cb200_stream* s, int trans_b, long long rows, long long K, long long N, long long experts);
+bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long N, long long experts);
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts);
 int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
                           long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
@@ -427,7 +427,7 @@ int rows_tc(cb200_stream* s, Product<float> p) {
   const int b_cols = p.trans_b ? p.K : p.N;
   if (p.experts == 1) p.b_stride = b_rows * p.ldb;
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, p.b_stride);
-  if (cb200_expert_f16_ok(s, p.trans_b, p.rows, p.K, p.N, p.experts)) {
+  if (cb200_expert_f16_ok(s, p.rows, p.K, p.N, p.experts)) {
     // products at twice the rate; what follows runs only where the data do not fit scaled halves
     int rc = cb200_expert_rows_f16(s, p.C, p.ldc, p.trans_b, p.alpha, p.A, p.rows, p.K, p.lda, p.B, p.experts, p.N, p.b_stride, p.ldb,
                                    p.beta, p.offsets, p.bias, p.act, &p.only_if);

@@ -21,9 +21,10 @@
 // warps empty the other.  (With the cross terms in an accumulator of their own, scaled by 2^11 for range, there was room
 // for one tile, and the read-out and its hand-shakes cost 5 us per tile where the product of a weight gradient takes 3:
 // 125 us against 117 for 8000 rows over 32 experts,
-// 2048 x 1024.)  The tensor core adds with truncation: every 512 values of
-// k -- 96 additions, 3e-6 of an all-positive sum -- the accumulator is added into registers, rounded to nearest, and the
-// other one takes over.
+// 2048 x 1024.)  The tensor core adds with truncation: every 256 values of
+// k -- 48 additions -- the accumulator is added into registers, rounded to nearest, and the other one takes over.  (Error of
+// normal data against 64 bits, and time of 16384 rows over 8 experts of 4096 x 4096: every 512 1.8e-6 and 1.376 ms, 256
+// 0.93e-6 and 1.382 ms, 128 0.49e-6 and 1.456 ms.)
 #include "gemm3x_common.cuh"
 #include "expert_groups.cuh"
 #include <cuda_fp16.h>
@@ -44,23 +45,24 @@ constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
 constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
 constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES;
 constexpr int TMEM_COLS = 2 * BN;
-constexpr int DRAIN = 512 / BK;                         // stages per accumulator filling
+constexpr int DRAIN = 256 / BK;                         // stages per accumulator filling
 
 // what one warp works out at the start of a call, in device memory
 struct Plan {
   int flag;                    // 1: the operands do not fit scaled halves
   int tiles;                   // expert_gemm: row tiles in the table
   int padded;                  // expert_gemm_weights: padded positions in use
-  int unused;
+  int first_row, end_row;      // rows outside are in no group
+  int unused[3];
 };
 struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); expert_gemm_weights: rows and first padded position
 
 // bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
 // entry per tile of BN rows.
-__global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int* owner, const int* offsets, int experts, int rows,
-                                                  int weights, int* status) {
+__global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int* owner, int* begins, const int* offsets, int experts,
+                                                  int rows, int weights, int* status) {
   const int lane = threadIdx.x;
-  int carry_max = 0, carry = 0;
+  int carry_max = 0, carry = 0, first_row = rows;
   bool bad = false;
   for (int base = 0; base < experts; base += 32) {
     const int e = base + lane;
@@ -83,6 +85,8 @@ __global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int*
     if (lane == 0) before = carry_max;
     lo = max(lo, before);
     hi = max(hi, lo);
+    if (e < experts && begins) begins[e] = lo;
+    if (e < experts && hi > lo) first_row = min(first_row, lo);
     const int mine = e < experts ? (weights ? (hi - lo + BK - 1) / BK * BK : (hi - lo + BN - 1) / BN) : 0;
     int sum = mine;
 #pragma unroll
@@ -101,9 +105,13 @@ __global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int*
     carry = __shfl_sync(0xffffffffu, sum, 31);
   }
   if (__any_sync(0xffffffffu, bad) && lane == 0) groups::report_bad(status);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) first_row = min(first_row, __shfl_xor_sync(0xffffffffu, first_row, d));
   if (lane == 0) {
     plan->flag = 0;
     plan->tiles = plan->padded = carry;
+    plan->first_row = first_row;
+    plan->end_row = carry_max;
     if (weights) table[experts] = {experts, 0, 0, carry};
   }
 }
@@ -137,27 +145,53 @@ __device__ __forceinline__ void load8(const float* p, int left, bool vec, float 
   }
 }
 
-// Rows along which the product reduces: TPR threads per row, 8 values per thread and step, the first HOLD steps in
-// registers between the maximum and the split (longer rows are read again, from L2).
-// Row r of the operand: x + (r / rows_per) * stride + (r % rows_per) * ld.  hi / lo: pitch kp (a multiple of 8).
-template <int TPR>
+// One row of scaled halves: TPR threads per row, 8 values per thread and step, the first HOLD steps in registers between the
+// maximum and the split (longer rows are read again, from L2).  hi / lo: pitch kp (a multiple of 8).
+//   RAGGED = 0  the experts' matrices: row r at x + (r / rows_per) * stride + (r % rows_per) * ld
+//   RAGGED = 1  the ragged rows: rows in no group become zeros and have no say in the flag
+//   RAGGED = 2  the same, every value multiplied by 2^14 fold[expert of the row][column] first: the inverse scales of a matrix
+//               whose rows run along the reduction, which cannot be taken out of the sum behind it
+template <int TPR, int RAGGED>
 __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
-                                                         long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan) {
+                                                         long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan,
+                                                         const float* fold, const int* begins, int experts) {
   constexpr int HOLD = 4;
   __shared__ uint32_t part_max[8];
   __shared__ int part_tiny[8];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * (256 / TPR) + sub;
-  const bool live = r < rows;
-  const float* src = live ? x + (r / rows_per) * stride + (r % rows_per) * ld : x;
+  const bool live = r < rows, grouped = !RAGGED || (r >= plan->first_row && r < plan->end_row);
+  const float* src = live ? (RAGGED ? x + r * ld : x + (r / rows_per) * stride + (r % rows_per) * ld) : x;
   const bool vec = ((uintptr_t)src & 15) == 0;
   const int n = live ? cols : 0;
+  const float* scales = nullptr;
+  if (RAGGED == 2 && live && grouped) {
+    int a = 0, z = experts;                                // the last group that begins at or before this row
+    while (z - a > 1) {
+      const int mid = (a + z) >> 1;
+      if (begins[mid] <= r) a = mid; else z = mid;
+    }
+    scales = fold + (long long)a * cols;
+  }
+  auto fetch = [&](int c, float (&w)[8]) {
+    if (RAGGED && !grouped) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = 0.f;
+      return;
+    }
+    load8(src + c, n - c, vec, w);
+    if (RAGGED == 2) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < n) w[j] *= 16384.f * __ldg(scales + c + j);
+    }
+  };
   float v[HOLD][8];
   uint32_t m = 0;
 #pragma unroll
   for (int it = 0; it < HOLD; ++it) {
     const int c = (it * TPR + t) * 8;
-    if (c < n) load8(src + c, n - c, vec, v[it]);
+    if (c < n) fetch(c, v[it]);
     else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[it][j] = 0.f;
@@ -167,7 +201,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
   }
   for (int c = (HOLD * TPR + t) * 8; c < n; c += TPR * 8) {
     float w[8];
-    load8(src + c, n - c, vec, w);
+    fetch(c, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(w[j]) & 0x7fffffffu);
   }
@@ -196,7 +230,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
   }
   for (int c = (HOLD * TPR + t) * 8; c < n; c += TPR * 8) {
     float w[8];
-    load8(src + c, n - c, vec, w);
+    fetch(c, w);
     put(c, w);
   }
 #pragma unroll
@@ -214,26 +248,25 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
   }
 }
 
-// Operands whose reduction runs down their columns, in groups of rows: rows of group g are table[g].lo .. hi (ragged) or
-// rows 0 .. fixed of the matrix x + g * stride (the experts' matrices).
+// Operands whose reduction runs down their columns, in ragged groups of rows: table[g].lo .. hi.
 // maxima[g][c] = bits of the largest magnitude in column c of group g.  A CTA: 128 columns of up to 64 rows of one group at a
 // time, four rows side by side and (where the rows are 16-byte aligned) four columns per thread.
 template <int V>
-__global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const float* x, long long ld, long long stride, int fixed,
-                                                         const Entry* table, int groups_n, int rows, int cols) {
+__global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const float* x, long long ld, const Entry* table,
+                                                         int groups_n, int rows, int cols) {
   constexpr int LANES = 128 / V, SIDE = 128 / LANES;       // threads per row, rows side by side
   struct alignas(4 * V) Pack { float e[V]; };
   __shared__ uint32_t part[SIDE][128];
   const int tx = threadIdx.x % LANES, ty = threadIdx.x / LANES, c = blockIdx.x * 128 + tx * V;
   const bool live = c < cols;                              // V = 4: cols is a multiple of 4
-  auto reduce = [&](int g, const float* first, int a, int z) {           // rows a .. z - 1 of group g, row r at first + r * ld
+  auto reduce = [&](int g, int a, int z) {                 // rows a .. z - 1 of group g
     uint32_t m[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) m[j] = 0;
     if (live) {
 #pragma unroll 4
       for (int r = a + ty; r < z; r += SIDE) {
-        const Pack v = *reinterpret_cast<const Pack*>(first + (long long)r * ld + c);
+        const Pack v = *reinterpret_cast<const Pack*>(x + (long long)r * ld + c);
 #pragma unroll
         for (int j = 0; j < V; ++j) m[j] = max(m[j], __float_as_uint(v.e[j]) & 0x7fffffffu);
       }
@@ -248,14 +281,6 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const
     if (at < cols) atomicMax(maxima + (long long)g * cols + at, all);
     __syncthreads();
   };
-  if (fixed) {
-    const int chunks = (fixed + 63) / 64;
-    for (long long b = blockIdx.y; b < (long long)groups_n * chunks; b += gridDim.y) {
-      const int g = (int)(b / chunks), r0 = (int)(b - (long long)g * chunks) * 64;
-      reduce(g, x + g * stride, r0, min(fixed, r0 + 64));
-    }
-    return;
-  }
   for (long long b = blockIdx.y; b * 64 < rows; b += gridDim.y) {
     const int r0 = (int)(b * 64), r1 = min(rows, r0 + 64);
     int g = 0, end = groups_n;                              // the last group that begins at or before r0
@@ -265,43 +290,27 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const
     }
     for (; g < groups_n && table[g].lo < r1; ++g) {
       const int a = max(r0, table[g].lo), z = min(r1, table[g].hi);
-      if (z > a) reduce(g, x, a, z);
+      if (z > a) reduce(g, a, z);
     }
   }
 }
 
-// hi / lo [cols (x groups where fixed)][positions]: 32 positions x 64 columns at a time through shared memory.  Ragged groups
-// start at a multiple of 32 positions and are padded with zeros (owner: which group the next 32 positions belong to); fixed
-// ones have rows of their own (pitch kp >= fixed).  A CTA takes two neighbouring blocks of 64 columns.
+// hi / lo [cols][positions]: 32 positions x 64 columns at a time through shared memory.  Groups start at a multiple of 32
+// positions and are padded with zeros (owner: which group the next 32 positions belong to).  A CTA takes two neighbouring
+// blocks of 64 columns.
 __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* lo, float* down_out, const uint32_t* maxima, const float* x,
-                                                            long long ld, long long stride, int fixed, const Entry* table,
-                                                            const int* owner, int groups_n, int cols, long long kp, Plan* plan) {
+                                                            long long ld, const Entry* table, const int* owner, int cols, long long kp,
+                                                            Plan* plan) {
   __shared__ float tile[2][32][65];
   __shared__ int tiny_all;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int per = fixed ? (fixed + 31) / 32 : 1;
-  const long long blocks = fixed ? (long long)groups_n * per : plan->padded / 32;
-  for (long long b = blockIdx.y; b < blocks; b += gridDim.y) {
-    int g, r0, end;
-    long long pos, row_base;                               // first position written, first row of hi / lo
-    bool begins;                                           // these are the group's first positions
-    if (fixed) {
-      g = (int)(b / per);
-      r0 = (int)(b - (long long)g * per) * 32;
-      end = fixed;
-      pos = r0;
-      row_base = (long long)g * cols;
-      begins = r0 == 0;
-    } else {
-      g = owner[b];
-      const Entry e = table[g];
-      pos = b * 32;
-      r0 = e.lo + (int)(pos - e.first);
-      end = e.hi;
-      row_base = 0;
-      begins = pos == e.first;
-    }
-    const float* src = fixed ? x + g * stride : x;
+  const int blocks = plan->padded / 32;
+  for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
+    const int g = owner[b];
+    const Entry e = table[g];
+    const long long pos = (long long)b * 32;               // first position written
+    const int r0 = e.lo + (int)(pos - e.first), end = e.hi;
+    const bool begins = pos == e.first;                    // these are the group's first positions
     __syncthreads();
     if (threadIdx.x == 0) tiny_all = 0;
     uint32_t m[2] = {0, 0};
@@ -314,7 +323,7 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = r0 + ty + 4 * i;
-        tile[h][ty + 4 * i][tx] = (r < end && c < cols) ? src[(long long)r * ld + c] : 0.f;
+        tile[h][ty + 4 * i][tx] = (r < end && c < cols) ? x[(long long)r * ld + c] : 0.f;
       }
     }
     __syncthreads();
@@ -329,10 +338,8 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
       Half8 a, z;
 #pragma unroll
       for (int j = 0; j < 8; ++j) split_half(tile[h][p8 + j][col] * up, a.h[j], z.h[j], tiny);
-      if (pos + p8 < kp) {                                 // kp is a multiple of 8
-        *reinterpret_cast<uint4*>(hi + (row_base + c) * kp + pos + p8) = a.v;
-        *reinterpret_cast<uint4*>(lo + (row_base + c) * kp + pos + p8) = z.v;
-      }
+      *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;             // kp is a multiple of 32
+      *reinterpret_cast<uint4*>(lo + c * kp + pos + p8) = z.v;
       if (!ok) plan->flag = 1;
       if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
     }
@@ -348,13 +355,14 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
 struct PairArgs {
   float* C;                     // element (column c, lane l) of a tile at C + c * ldc + l
   long long ldc, c_stride;
-  const float* l_down; const float* r_down;      // inverse scales
+  const float* l_down; const float* r_down;      // inverse scales (l_down null: the lanes' ones were folded into the columns' values)
   const float* bias;
   const Plan* plan;
   const Entry* table;
   int* status;
   int lanes, cols;              // extents: lanes of one expert's matrix; WEIGHTS: columns of one result
   int K;                        // expert_gemm: reduction length
+  int l_mn;                     // the lanes are contiguous in the lane operand ([k][lane], 64-lane boxes)
   int experts, weights, act;
   float alpha, beta;
 };
@@ -385,7 +393,7 @@ __device__ __forceinline__ Unit unit_of(const PairArgs& p, int unit, const Entry
   } else {
     u.r0 = e.lo;
     u.cols = min(BN, e.hi - e.lo);
-    u.l_row = e.expert * p.lanes + u.l0;
+    u.l_row = p.l_mn ? u.l0 : e.expert * p.lanes + u.l0;
     u.kb = 0;
     u.nkb = (p.K + BK - 1) / BK;
   }
@@ -403,9 +411,9 @@ __device__ __forceinline__ void mma_f16_pair_words(uint32_t d_tmem, uint32_t a_l
       "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// instruction descriptor of kind::f16 with half operands, K-major, fp32 accumulation (the fields of make_idesc_tf32)
-__host__ __device__ __forceinline__ uint32_t make_idesc_f16(int m, int n) {
-  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+// instruction descriptor of kind::f16 with half operands and fp32 accumulation (the fields of make_idesc_tf32)
+__host__ __device__ __forceinline__ uint32_t make_idesc_f16(int m, int n, int a_mn_major) {
+  return (1u << 4) | ((uint32_t)(a_mn_major & 1) << 15) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -484,8 +492,17 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
           const int k0 = (u.kb + i) * BK;
           if (!withhold) {
             if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
-            tma_load_2d_pair(dst, hi_map, k0, row0, leader_full + 8 * s);
-            tma_load_2d_pair(dst + RAW, lo_map, k0, row0, leader_full + 8 * s);
+            if (is_l && p.l_mn) {
+              // [k][lane]: 32 k x 64 lanes per box; k rows behind the expert's meet zeros of the other operand
+              const int k_row = u.expert * p.K + k0;
+              for (int h = 0; h < 2; ++h) {
+                tma_load_2d_pair(dst + h * (L_TILE / 2), hi_map, row0 + 64 * h, k_row, leader_full + 8 * s);
+                tma_load_2d_pair(dst + RAW + h * (L_TILE / 2), lo_map, row0 + 64 * h, k_row, leader_full + 8 * s);
+              }
+            } else {
+              tma_load_2d_pair(dst, hi_map, k0, row0, leader_full + 8 * s);
+              tma_load_2d_pair(dst + RAW, lo_map, k0, row0, leader_full + 8 * s);
+            }
             ++issued;
           }
           if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -501,7 +518,10 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   } else if (warp == EPI_WARPS + 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
     if (leader && lane == 0) {
-      const uint64_t d_a = make_smem_desc(smem_base, 16, 8 * BK * 2, SWZ_64B);
+      // K-major: 64-byte rows, 8-row groups SBO apart, 32 B per k-step.  Lanes contiguous: 64-lane blocks (boxes) LBO apart,
+      // 8-k groups of 128-byte rows SBO apart, 2048 B per k-step.
+      const uint64_t d_a = p.l_mn ? make_smem_desc(smem_base, L_TILE / 2, 1024, SWZ_128B) : make_smem_desc(smem_base, 16, 8 * BK * 2, SWZ_64B);
+      const uint32_t a_step = p.l_mn ? 2048u >> 4 : 32u >> 4;
       const uint64_t d_b = make_smem_desc(smem_base + L_TILE, 16, 8 * BK * 2, SWZ_64B);
       const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
       const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
@@ -514,7 +534,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       for (int unit = cluster_id; ok && unit < n_units; unit += n_clusters) {
         const Unit u = unit_of(p, unit, next);
         next = entry_of(p, unit + n_clusters, n_units);
-        const uint32_t idesc = make_idesc_f16(2 * BM, (u.cols + 31) / 32 * 32);
+        const uint32_t idesc = make_idesc_f16(2 * BM, (u.cols + 31) / 32 * 32, p.l_mn);
         for (int i0 = 0; ok && i0 < u.nkb; i0 += DRAIN, ++fill) {      // (a group without rows: nothing to multiply)
           const int end = min(u.nkb, i0 + DRAIN);
           const uint32_t acc = tmem_base + (fill & 1) * BN;
@@ -525,7 +545,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < BK / 16; ++kk) {
-              const uint32_t al = a_low0 + stage_off + kk * 2, bl = b_low0 + stage_off + kk * 2;    // 32 B per k-step
+              const uint32_t al = a_low0 + stage_off + kk * a_step, bl = b_low0 + stage_off + kk * 2;
               mma_f16_pair_words(acc, al + LO_TILE, a_hiw, bl, b_hiw, idesc, (i > i0 || kk) ? 1u : 0u);
               mma_f16_pair_words(acc, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
               mma_f16_pair_words(acc, al, a_hiw, bl, b_hiw, idesc, 1);
@@ -569,7 +589,8 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
 #pragma unroll
       for (int cc = 0; cc < BN / 2 / 32; ++cc) col_scale[cc] = (!none && cc * 32 + lane < left) ? r_down[cc * 32 + lane] : 1.f;
       if (l < p.lanes) {
-        if (!none) l_scale = p.l_down[(long long)u.expert * p.lanes + l];
+        if (!none && p.l_down) l_scale = p.l_down[(long long)u.expert * p.lanes + l];
+        else if (!none) l_scale = 1.f / 16384.f;           // (2^14 of the folded scales)
         if (p.bias) b = p.bias[(long long)u.expert * p.lanes + l];
       }
 #pragma unroll
@@ -694,48 +715,53 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-int half_map(CUtensorMap* tm, const __half* base, long long rows, long long cols, long long pitch) {
+int half_map(CUtensorMap* tm, const __half* base, long long rows, long long cols, long long pitch, bool mn = false) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) { cb200_set_error("cuTensorMapEncodeTiled is not available from this driver"); return CB200_ERR_CUDA; }
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * 2};
-  const cuuint32_t box[2] = {BK, BM}, ones[2] = {1, 1};
+  const cuuint32_t box[2] = {mn ? 64u : (cuuint32_t)BK, mn ? (cuuint32_t)BK : (cuuint32_t)BM}, ones[2] = {1, 1};
   CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  mn ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { cb200_set_error("cuTensorMapEncodeTiled failed with %d", (int)r); return CB200_ERR_CUDA; }
   return CB200_OK;
 }
 
+template <int RAGGED>
 int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
-               long long rows, int cols, int kp, Plan* plan) {
+               long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0) {
   if (cols <= 1024)
-    split_rows_kernel<32><<<(unsigned)((rows + 7) / 8), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan);
+    split_rows_kernel<32, RAGGED><<<(unsigned)((rows + 7) / 8), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
+                                                                                     plan, fold, begins, experts);
   else if (cols <= 4096)
-    split_rows_kernel<128><<<(unsigned)((rows + 1) / 2), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan);
+    split_rows_kernel<128, RAGGED><<<(unsigned)((rows + 1) / 2), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
+                                                                                      plan, fold, begins, experts);
   else
-    split_rows_kernel<256><<<(unsigned)rows, 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan);
+    split_rows_kernel<256, RAGGED><<<(unsigned)rows, 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan, fold,
+                                                                          begins, experts);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
 
-int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, const float* x, long long ld, long long stride,
-                  int fixed, const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
+int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, const float* x, long long ld, const Entry* table,
+                  const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
   CB_CUDA(cudaMemsetAsync(maxima, 0, (size_t)groups_n * cols * sizeof(uint32_t), s->stream));
-  long long chunks = fixed ? (long long)groups_n * ((fixed + 63) / 64) : (rows + 63) / 64;
+  const long long chunks = (rows + 63) / 64, blocks = kp / 32;
   const dim3 grid_max((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535));
-  if (((uintptr_t)x & 15) == 0 && ld % 4 == 0 && stride % 4 == 0 && cols % 4 == 0)
-    column_max_kernel<4><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, stride, fixed, table, groups_n, rows, cols);
+  if (((uintptr_t)x & 15) == 0 && ld % 4 == 0 && cols % 4 == 0)
+    column_max_kernel<4><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, table, groups_n, rows, cols);
   else
-    column_max_kernel<1><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, stride, fixed, table, groups_n, rows, cols);
+    column_max_kernel<1><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, table, groups_n, rows, cols);
   CB_LAUNCH_CHECK(s);
-  long long blocks = fixed ? (long long)groups_n * ((fixed + 31) / 32) : kp / 32;
   split_columns_kernel<<<dim3((unsigned)((cols + 127) / 128), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, s->stream>>>(
-      hi, lo, down, maxima, x, ld, stride, fixed, table, owner, groups_n, cols, kp, plan);
+      hi, lo, down, maxima, x, ld, table, owner, cols, kp, plan);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
 
-int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long long l_rows, const __half* r_hi, const __half* r_lo,
-                long long r_rows, long long cols, long long l_pitch, long long r_pitch, const PairArgs& a, long long units) {
+int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long long l_rows, long long l_cols, long long l_pitch,
+                const __half* r_hi, const __half* r_lo, long long r_rows, long long r_cols, long long r_pitch, const PairArgs& a,
+                long long units) {
   static std::once_flag once[64];
   static cudaError_t result[64];
   const int dev = s->device & 63;
@@ -743,8 +769,8 @@ int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long lo
   if (result[dev] != cudaSuccess) return cb200_cuda_fail(result[dev], "cudaFuncSetAttribute", __FILE__, __LINE__);
   CUtensorMap tmL, tmLlo, tmR, tmRlo;
   int rc;
-  if ((rc = half_map(&tmL, l_hi, l_rows, cols, l_pitch)) || (rc = half_map(&tmLlo, l_lo, l_rows, cols, l_pitch)) ||
-      (rc = half_map(&tmR, r_hi, r_rows, cols, r_pitch)) || (rc = half_map(&tmRlo, r_lo, r_rows, cols, r_pitch)))
+  if ((rc = half_map(&tmL, l_hi, l_rows, l_cols, l_pitch, a.l_mn)) || (rc = half_map(&tmLlo, l_lo, l_rows, l_cols, l_pitch, a.l_mn)) ||
+      (rc = half_map(&tmR, r_hi, r_rows, r_cols, r_pitch)) || (rc = half_map(&tmRlo, r_lo, r_rows, r_cols, r_pitch)))
     return rc;
   const long long clusters = units < s->sm_count / 2 ? units : s->sm_count / 2;
   cudaLaunchConfig_t cfg = {};
@@ -783,15 +809,15 @@ constexpr size_t MOST_WORKSPACE = (size_t)2 << 30;
 
 }  // namespace
 
-// Is this product better off here?  Both sides' times by the sizes, in microseconds: `split` bytes are read and written
-// once at 5.5 TB/s, and again where the reduction axis is not contiguous.
-bool cb200_expert_f16_ok(cb200_stream* s, int trans_b, long long rows, long long K, long long N, long long experts) {
+// Is this product better off here?  Both sides' times by the sizes, in microseconds: the split reads and writes the operands
+// once.
+bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
   const double l = (double)experts * N * K, r = (double)rows * K;
   if ((l + r) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * K;
-  const double here = 20.0 + (l * (trans_b ? 8 : 12) + r * 8) / 5.5e6 + flops / 330e6, there = flops / 130e6;
+  const double here = 20.0 + (l + r) * 8 / 5.5e6 + flops / 330e6, there = flops / 130e6;
   return rows >= 96 * experts && here < there;
 }
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
@@ -809,36 +835,38 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
                           long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
                           const int* offsets, const float* bias, int act, const int** guard_out) {
   DeviceGuard guard(s->device);
-  const long long kp = up8(K), l_rows = (long long)experts * N;
+  // the matrices' rows as they are stored: [N, K] reduces along them, [K, N] (the gradient of the input) across them
+  const int l_per = trans_b ? N : K, l_cols = trans_b ? K : N;
+  const long long kp = up8(K), lp = up8(l_cols), l_rows = (long long)experts * l_per;
   const size_t tiles = (size_t)((rows + BN - 1) / BN + (experts < rows ? experts : rows));
-  const size_t maxima_n = trans_b ? 0 : (size_t)l_rows;
-  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + 2 * up256((size_t)l_rows * kp * 2) +
-                       2 * up256((size_t)rows * kp * 2) + up256((size_t)l_rows * 4) + up256((size_t)rows * 4) + up256(maxima_n * 4);
+  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)experts * 4) +
+                       2 * up256((size_t)l_rows * lp * 2) + 2 * up256((size_t)rows * kp * 2) + up256((size_t)l_rows * 4) +
+                       up256((size_t)rows * 4);
   void* ws = nullptr;
   int rc = cb200_scratch(s, bytes, &ws);
   if (rc) return rc;
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
   Entry* table = w.take<Entry>(tiles + 1);
-  __half* l_hi = w.take<__half>((size_t)l_rows * kp);
-  __half* l_lo = w.take<__half>((size_t)l_rows * kp);
+  int* begins = w.take<int>((size_t)experts);
+  __half* l_hi = w.take<__half>((size_t)l_rows * lp);
+  __half* l_lo = w.take<__half>((size_t)l_rows * lp);
   __half* r_hi = w.take<__half>((size_t)rows * kp);
   __half* r_lo = w.take<__half>((size_t)rows * kp);
   float* l_down = w.take<float>((size_t)l_rows);
   float* r_down = w.take<float>((size_t)rows);
-  uint32_t* maxima = w.take<uint32_t>(maxima_n);
-  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, nullptr, offsets, experts, rows, 0, s->status_dev);
+  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev);
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_rows(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan))) return rc;
-  if (trans_b) rc = split_rows(s, l_hi, l_lo, l_down, B, ldb, b_stride, N, l_rows, K, (int)kp, plan);
-  else rc = split_columns(s, l_hi, l_lo, l_down, maxima, B, ldb, b_stride, K, table, nullptr, experts, 0, N, kp, plan);
+  if ((rc = split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan))) return rc;
+  if (trans_b) rc = split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan);
+  else rc = split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, l_down, begins, experts);
   if (rc) return rc;
   PairArgs a;
-  a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = l_down; a.r_down = r_down; a.bias = bias; a.plan = plan; a.table = table;
-  a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.experts = experts; a.weights = 0; a.act = act;
-  a.alpha = alpha; a.beta = beta;
+  a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = trans_b ? l_down : nullptr; a.r_down = r_down; a.bias = bias; a.plan = plan;
+  a.table = table; a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.l_mn = trans_b ? 0 : 1; a.experts = experts;
+  a.weights = 0; a.act = act; a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;
-  return launch_pair(s, l_hi, l_lo, l_rows, r_hi, r_lo, rows, K, kp, kp, a, (long long)tiles * ((N + 2 * BM - 1) / (2 * BM)));
+  return launch_pair(s, l_hi, l_lo, l_rows, l_cols, lp, r_hi, r_lo, rows, K, kp, a, (long long)tiles * ((N + 2 * BM - 1) / (2 * BM)));
 }
 
 int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows, int M,
@@ -864,15 +892,15 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   float* r_down = w.take<float>((size_t)experts * M);
   uint32_t* l_max = w.take<uint32_t>((size_t)experts * N);
   uint32_t* r_max = w.take<uint32_t>((size_t)experts * M);
-  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, owner, offsets, experts, rows, 1, s->status_dev);
+  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, owner, nullptr, offsets, experts, rows, 1, s->status_dev);
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, B, ldb, 0, 0, table, owner, experts, rows, N, kp, plan))) return rc;
-  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, A, lda, 0, 0, table, owner, experts, rows, M, kp, plan))) return rc;
+  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, B, ldb, table, owner, experts, rows, N, kp, plan))) return rc;
+  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, A, lda, table, owner, experts, rows, M, kp, plan))) return rc;
   PairArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.table = table;
-  a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
+  a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.l_mn = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
   a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;
-  return launch_pair(s, l_hi, l_lo, N, r_hi, r_lo, M, kp, kp, kp, a,
+  return launch_pair(s, l_hi, l_lo, N, kp, kp, r_hi, r_lo, M, kp, kp, a,
                      (long long)experts * ((M + BN - 1) / BN) * ((N + 2 * BM - 1) / (2 * BM)));
 }

@@ -10,8 +10,8 @@
 //
 // Every CTA finds its tile itself (groups::find_tile, ~1 us, while TMEM and barriers are set up); the grid is the most
 // tiles that the sizes allow, and CTAs without a tile leave at once.
-// Reductions longer than `chunk` k-blocks are cut: the tensor core adds with truncation, so every chunk's sum is rounded
-// to nearest onto C (or onto the slice's parked tile) and the accumulators restart from zero.
+// Long reductions are cut into chunks: the tensor core adds with truncation, so every chunk's sum is rounded to nearest onto
+// C (or onto the slice's parked tile) and the accumulators restart from zero.
 //
 // Warp roles as in gemm_tf32x3_kernel: 0-7 lo tiles and epilogue, 8 TMA producer, 9 TMEM and MMA issue.
 #include "gemm3x_common.cuh"
@@ -64,7 +64,6 @@ struct RowsArgs {
   int act;
   float alpha, beta;
   const int* only_if;          // null, or a device word: do nothing while it is zero
-  int chunk;                   // k-blocks between roundings of the accumulators
   int slices;                  // CTAs of a cluster that share a tile, each over a slice of K
 };
 
@@ -73,7 +72,11 @@ template <int BN, int BK> struct RowsCfg {
   // narrow tiles: two CTAs per SM, one streaming while the other sets up or stores
   static constexpr int CTAS = BN <= 64 ? 2 : 1;
   static constexpr int STAGES = (196608 / CTAS / STAGE) > 8 ? 8 : (196608 / CTAS / STAGE);
-  static constexpr int TMEM_COLS = 2 * BN;
+  // The tensor core adds with truncation, so a long run of additions shrinks a sum.  Tiles that leave TMEM room take turns
+  // between several main accumulators, joined in the epilogue; a reduction longer than a chunk goes out to C in between.
+  static constexpr int MAINS = BN == 32 ? 4 : (BN == 256 ? 1 : 3);
+  static constexpr int CHUNK = MAINS == 1 ? 1024 / BK : MAINS * 512 / BK;      // k-blocks
+  static constexpr int TMEM_COLS = BN == 32 ? 256 : (MAINS + 1) * BN;          // mains, then the cross terms
   static constexpr int BOX_ROWS = BN < 64 ? BN : 64;          // rows of one TMA box of the ragged operand
   static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
   static_assert(BM * BN * 4 <= STAGES * STAGE, "a parked tile must fit the pipeline stages");
@@ -174,7 +177,8 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   const int nkb_all = (p.K + BK - 1) / BK;
   const int kb_begin = (int)((long long)nkb_all * slice / p.slices);
   const int nkb = (int)((long long)nkb_all * (slice + 1) / p.slices) - kb_begin;
-  const int n_chunks = (nkb + p.chunk - 1) / p.chunk, per = (nkb + n_chunks - 1) / n_chunks;
+  const int n_chunks = (nkb + C::CHUNK - 1) / C::CHUNK, per = (nkb + n_chunks - 1) / n_chunks;
+  const int run = max((per + C::MAINS - 1) / C::MAINS, 256 / BK);              // k-blocks into one main accumulator
   const float* bias = p.bias ? p.bias + (long long)expert * p.N : nullptr;
 
   if (warp == CONV_WARPS) {
@@ -213,14 +217,14 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       constexpr uint32_t K_SWZ = BK == 32 ? SWZ_128B : SWZ_64B, K_SBO = 8 * BK * 4;
       const uint32_t a_step = (p.w_mn ? 1024u : 32u) >> 4;
       constexpr uint32_t b_step = 32u >> 4;
-      const uint32_t tmem_main = tmem_base, tmem_cross = tmem_base + BN;
+      const uint32_t tmem_cross = tmem_base + C::MAINS * BN;
       const uint64_t d_a = p.w_mn ? make_smem_desc(smem_base, W_BOX, 512, SWZ_128B_BASE32B) : make_smem_desc(smem_base, 16, K_SBO, K_SWZ);
       const uint64_t d_b = make_smem_desc(smem_base + A_TILE, 16, K_SBO, K_SWZ);
       const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
       const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
       constexpr uint32_t LO_TILE = C::RAW >> 4, STAGE_STEP = C::STAGE >> 4;
-      uint32_t accumulate = 0, ph = 0, stage_off = 0, rph = 0;
-      int s = 0, in_chunk = 0, commits = 0;
+      uint32_t accumulate = 0, cross = 0, ph = 0, stage_off = 0, rph = 0, tmem_main = tmem_base;
+      int s = 0, in_chunk = 0, in_run = 0, commits = 0;
       for (int i = 0; i < nkb; ++i) {
         if (in_chunk == per) {
           // the chunk's sums go out before its accumulators are overwritten
@@ -230,23 +234,30 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
           if (!mbar_wait(bar_read, rph, abort_flag, p.status, 250)) break;
           rph ^= 1;
           tc_fence_after();
-          in_chunk = 0;
+          in_chunk = in_run = 0;
+          accumulate = cross = 0;
+          tmem_main = tmem_base;
+        }
+        if (C::MAINS > 1 && in_run == run) {
+          in_run = 0;
           accumulate = 0;
+          tmem_main += BN;
         }
         ++in_chunk;
+        ++in_run;
         if (!mbar_wait(bar_conv + 8 * s, ph, abort_flag, p.status, 200 + s)) break;
         tc_fence_after();
         if (!MMA_WHOLE || elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BK / 8; ++kk) {
             const uint32_t al = a_low0 + stage_off + kk * a_step, bl = b_low0 + stage_off + kk * b_step;
-            mma_tf32_ss_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
+            mma_tf32_ss_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : cross);
             mma_tf32_ss_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
             mma_tf32_ss_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
           }
           mma_commit(bar_empty + 8 * s);
         }
-        accumulate = 1;
+        accumulate = cross = 1;
         if (MMA_WHOLE) __syncwarp();
         if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
       }
@@ -295,14 +306,22 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       const bool last = c + 1 == n_chunks;
+      const int mains = (end - c * per + run - 1) / run;     // main accumulators in use
 #pragma unroll 1
       for (int cc = half; cc * 32 < cols; cc += 2) {
         uint32_t r[32], rc[32];
         tmem_ld_32x32(lane_base + (uint32_t)(cc * 32), r);
-        tmem_ld_32x32(lane_base + (uint32_t)(BN + cc * 32), rc);
+        tmem_ld_32x32(lane_base + (uint32_t)(C::MAINS * BN + cc * 32), rc);
         tmem_ld_wait();
 #pragma unroll
         for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
+#pragma unroll 1
+        for (int m = 1; m < mains; ++m) {
+          tmem_ld_32x32(lane_base + (uint32_t)(m * BN + cc * 32), rc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
+        }
         if (p.slices > 1) {
           // parked in this CTA's own shared memory ([columns / 4][128 lanes] float4); one chunk only, so the stages are free
           float4* slot = reinterpret_cast<float4*>(smem) + (q * 32 + lane);
@@ -711,8 +730,8 @@ void common(GemmParams& g, cb200_stream* s, float* C, long long ldc, int M, int 
   for (int d = 0; d < MAX_PEERS; ++d) g.peers[d] = nullptr;
 }
 
-// k-blocks between roundings: 2048 values of k, where the truncating additions have shrunk a sum by 1.4e-5 at most
-constexpr int CHUNK = 2048 / BK;
+// k-blocks between roundings: 1024 values of k, where the truncating additions have shrunk a sum by 7e-6 at most
+constexpr int CHUNK = 1024 / BK;
 
 }  // namespace
 
@@ -730,7 +749,8 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   int BN = s->opt_gemm_tile_n > 0 ? s->opt_gemm_tile_n : (even <= 32 ? 32 : (even <= 64 ? 64 : (even <= 128 ? 128 : 256)));
   const int bk = BN <= 64 ? 32 : 16;
   const long long tiles = (rows + BN - 1) / BN + (experts < rows ? experts : rows) - 1, units = tiles * ((N + BM - 1) / BM);
-  const int nkb = (K + bk - 1) / bk, chunk = 2048 / bk;
+  const int nkb = (K + bk - 1) / bk;
+  const int chunk = BN == 256 ? RowsCfg<256, 16>::CHUNK : (BN == 128 ? RowsCfg<128, 16>::CHUNK : (BN == 64 ? RowsCfg<64, 32>::CHUNK : RowsCfg<32, 32>::CHUNK));
   // K slices (the CTAs of a cluster) where the tiles leave SMs free; a slice is one chunk, since its parked tile lies in
   // shared memory that the next chunk's stages would need
   int slices = 1;
@@ -741,7 +761,7 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   RowsArgs a;
   a.C = C; a.ldc = ldc; a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
   a.N = N; a.K = K; a.experts = experts; a.rows = rows; a.w_mn = trans_b ? 0 : 1; a.act = act;
-  a.alpha = alpha; a.beta = beta; a.chunk = chunk; a.slices = slices; a.only_if = only_if;
+  a.alpha = alpha; a.beta = beta; a.slices = slices; a.only_if = only_if;
   const CUtensorMapSwizzle swz = bk == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tmW, tmX;
   int rc = tmap_2d(&tmX, A, rows, K, lda, bk, BN < 64 ? BN : 64, swz);
