@@ -13,8 +13,8 @@
 // (HBM-bound; operands whose reduction axis is not contiguous get a pass for the column maxima first); the product; the
 // guarded 3xTF32 kernel.
 //
-// The product runs on CTA pairs (tcgen05.mma.cta_group::2, 256 lanes x up to 256 columns per pair), persistent, six
-// pipeline stages of 32 KB, as the pre-split layer GEMM: every TMA load is a plain one into the issuing CTA, completing on
+// The product runs on CTA pairs (tcgen05.mma.cta_group::2, 256 lanes x up to 256 columns per pair), persistent, three
+// pipeline stages of 64 KB (128-byte rows), as the pre-split layer GEMM: every TMA load is a plain one into the issuing CTA, completing on
 // the leader's barrier.  Output features (expert_gemm) or input features (expert_gemm_weights) lie in the lanes, so a warp
 // stores 128 consecutive bytes; the ragged rows (or output features) lie in the columns, in multiples of 32.
 // All three products go to one accumulator of 256 columns, so TMEM holds two: the tensor cores fill one while the epilogue
@@ -37,10 +37,12 @@ using namespace gemm3x;
 
 namespace {
 
-constexpr int BM = 128, BN = 256, BK = 32;               // per CTA: 128 lanes, 256 columns of the pair, 32 halves of k
+constexpr int BM = 128, BN = 256, BK = 64;               // per CTA: 128 lanes, 256 columns of the pair, 64 halves of k
+constexpr int POS = 32;                                  // padded positions that the column pass writes at a time
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = (EPI_WARPS + 4) * 32;            // three warpgroups; the last warp only gives its registers up
-constexpr int L_TILE = BM * BK * 2, R_TILE = BN / 2 * BK * 2;       // 8 KiB each
+constexpr int L_TILE = BM * BK * 2, R_TILE = BN / 2 * BK * 2;       // 16 KiB each
+constexpr int R_BOX = 64;                                // rows of one box of the column operand
 constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
 constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
 constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES;
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int*
     if (e < experts) {
       if (weights) {
         table[e] = {e, lo, hi, sum - mine};
-        for (int i = 0; i < mine; i += BK) owner[(sum - mine + i) / BK] = e;      // whose the next 32 positions are
+        for (int i = 0; i < mine; i += POS) owner[(sum - mine + i) / POS] = e;      // whose the next 32 positions are
       } else for (int i = 0; i < mine; ++i) table[sum - mine + i] = {e, lo + i * BN, hi, 0};
     }
     carry_max = __shfl_sync(0xffffffffu, run, 31);
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const
   }
 }
 
-// hi / lo [cols][positions]: 32 positions x 64 columns at a time through shared memory.  Groups start at a multiple of 32
+// hi / lo [cols][positions]: 32 positions x 64 columns at a time through shared memory.  Groups start at a multiple of 64
 // positions and are padded with zeros (owner: which group the next 32 positions belong to).  A CTA takes two neighbouring
 // blocks of 64 columns.
 __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* lo, float* down_out, const uint32_t* maxima, const float* x,
@@ -304,11 +306,11 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
   __shared__ float tile[2][32][65];
   __shared__ int tiny_all;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-  const int blocks = plan->padded / 32;
+  const int blocks = plan->padded / POS;
   for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
     const int g = owner[b];
     const Entry e = table[g];
-    const long long pos = (long long)b * 32;               // first position written
+    const long long pos = (long long)b * POS;              // first position written
     const int r0 = e.lo + (int)(pos - e.first), end = e.hi;
     const bool begins = pos == e.first;                    // these are the group's first positions
     __syncthreads();
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
       Half8 a, z;
 #pragma unroll
       for (int j = 0; j < 8; ++j) split_half(tile[h][p8 + j][col] * up, a.h[j], z.h[j], tiny);
-      *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;             // kp is a multiple of 32
+      *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;             // kp is a multiple of 64
       *reinterpret_cast<uint4*>(lo + c * kp + pos + p8) = z.v;
       if (!ok) plan->flag = 1;
       if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
@@ -475,7 +477,6 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       const CUtensorMap* hi_map = is_l ? &tmL : &tmR;
       const CUtensorMap* lo_map = is_l ? &tmLlo : &tmRlo;
       const uint32_t tile_off = is_l ? 0u : (uint32_t)L_TILE;
-      const uint32_t bytes = 2u * (is_l ? 2u * L_TILE : 2u * R_TILE);         // this CTA's tiles and the peer's
       const uint32_t leader_full = mapa(bar_full, 0);
       long long issued = 0;
       int s = 0;
@@ -486,6 +487,8 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
         const Unit u = unit_of(p, unit, entry_of(p, unit, n_units));
         const int n_half = (u.cols + 31) / 32 * 16;     // columns of the pair's MMA that this CTA stages
         const int row0 = is_l ? u.l_row + (int)rank * BM : u.r0 + (int)rank * n_half;
+        const int boxes = (n_half + R_BOX - 1) / R_BOX;
+        const uint32_t bytes = 4u * (is_l ? (uint32_t)L_TILE : (uint32_t)(boxes * R_BOX * BK * 2));      // hi and lo, this CTA's and the peer's
         for (int i = 0; i < u.nkb; ++i) {
           if (!mbar_wait_cluster(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 500 + s)) { ok = false; break; }
           const uint32_t dst = smem_base + s * STAGE + tile_off;
@@ -493,15 +496,20 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
           if (!withhold) {
             if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
             if (is_l && p.l_mn) {
-              // [k][lane]: 32 k x 64 lanes per box; k rows behind the expert's meet zeros of the other operand
+              // [k][lane]: 64 k x 64 lanes per box; k rows behind the expert's meet zeros of the other operand
               const int k_row = u.expert * p.K + k0;
               for (int h = 0; h < 2; ++h) {
                 tma_load_2d_pair(dst + h * (L_TILE / 2), hi_map, row0 + 64 * h, k_row, leader_full + 8 * s);
                 tma_load_2d_pair(dst + RAW + h * (L_TILE / 2), lo_map, row0 + 64 * h, k_row, leader_full + 8 * s);
               }
-            } else {
+            } else if (is_l) {
               tma_load_2d_pair(dst, hi_map, k0, row0, leader_full + 8 * s);
               tma_load_2d_pair(dst + RAW, lo_map, k0, row0, leader_full + 8 * s);
+            } else {
+              for (int h = 0; h < boxes; ++h) {
+                tma_load_2d_pair(dst + h * (R_BOX * BK * 2), hi_map, k0, row0 + h * R_BOX, leader_full + 8 * s);
+                tma_load_2d_pair(dst + RAW + h * (R_BOX * BK * 2), lo_map, k0, row0 + h * R_BOX, leader_full + 8 * s);
+              }
             }
             ++issued;
           }
@@ -518,11 +526,11 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   } else if (warp == EPI_WARPS + 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
     if (leader && lane == 0) {
-      // K-major: 64-byte rows, 8-row groups SBO apart, 32 B per k-step.  Lanes contiguous: 64-lane blocks (boxes) LBO apart,
+      // K-major: 128-byte rows, 8-row groups SBO apart, 32 B per k-step.  Lanes contiguous: 64-lane blocks (boxes) LBO apart,
       // 8-k groups of 128-byte rows SBO apart, 2048 B per k-step.
-      const uint64_t d_a = p.l_mn ? make_smem_desc(smem_base, L_TILE / 2, 1024, SWZ_128B) : make_smem_desc(smem_base, 16, 8 * BK * 2, SWZ_64B);
+      const uint64_t d_a = p.l_mn ? make_smem_desc(smem_base, L_TILE / 2, 1024, SWZ_128B) : make_smem_desc(smem_base, 16, 8 * BK * 2, SWZ_128B);
       const uint32_t a_step = p.l_mn ? 2048u >> 4 : 32u >> 4;
-      const uint64_t d_b = make_smem_desc(smem_base + L_TILE, 16, 8 * BK * 2, SWZ_64B);
+      const uint64_t d_b = make_smem_desc(smem_base + L_TILE, 16, 8 * BK * 2, SWZ_128B);
       const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
       const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
       constexpr uint32_t LO_TILE = RAW >> 4, STAGE_STEP = STAGE >> 4;
@@ -715,13 +723,13 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-int half_map(CUtensorMap* tm, const __half* base, long long rows, long long cols, long long pitch, bool mn = false) {
+int half_map(CUtensorMap* tm, const __half* base, long long rows, long long cols, long long pitch, int box_cols, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) { cb200_set_error("cuTensorMapEncodeTiled is not available from this driver"); return CB200_ERR_CUDA; }
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * 2};
-  const cuuint32_t box[2] = {mn ? 64u : (cuuint32_t)BK, mn ? (cuuint32_t)BK : (cuuint32_t)BM}, ones[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows}, ones[2] = {1, 1};
   CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  mn ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) { cb200_set_error("cuTensorMapEncodeTiled failed with %d", (int)r); return CB200_ERR_CUDA; }
   return CB200_OK;
@@ -746,7 +754,7 @@ int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float
 int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, const float* x, long long ld, const Entry* table,
                   const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
   CB_CUDA(cudaMemsetAsync(maxima, 0, (size_t)groups_n * cols * sizeof(uint32_t), s->stream));
-  const long long chunks = (rows + 63) / 64, blocks = kp / 32;
+  const long long chunks = (rows + 63) / 64, blocks = kp / POS;
   const dim3 grid_max((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535));
   if (((uintptr_t)x & 15) == 0 && ld % 4 == 0 && cols % 4 == 0)
     column_max_kernel<4><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, table, groups_n, rows, cols);
@@ -769,8 +777,9 @@ int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long lo
   if (result[dev] != cudaSuccess) return cb200_cuda_fail(result[dev], "cudaFuncSetAttribute", __FILE__, __LINE__);
   CUtensorMap tmL, tmLlo, tmR, tmRlo;
   int rc;
-  if ((rc = half_map(&tmL, l_hi, l_rows, l_cols, l_pitch, a.l_mn)) || (rc = half_map(&tmLlo, l_lo, l_rows, l_cols, l_pitch, a.l_mn)) ||
-      (rc = half_map(&tmR, r_hi, r_rows, r_cols, r_pitch)) || (rc = half_map(&tmRlo, r_lo, r_rows, r_cols, r_pitch)))
+  const int l_box = a.l_mn ? BK : BM;                      // 64 halves wide either way
+  if ((rc = half_map(&tmL, l_hi, l_rows, l_cols, l_pitch, 64, l_box)) || (rc = half_map(&tmLlo, l_lo, l_rows, l_cols, l_pitch, 64, l_box)) ||
+      (rc = half_map(&tmR, r_hi, r_rows, r_cols, r_pitch, 64, R_BOX)) || (rc = half_map(&tmRlo, r_lo, r_rows, r_cols, r_pitch, 64, R_BOX)))
     return rc;
   const long long clusters = units < s->sm_count / 2 ? units : s->sm_count / 2;
   cudaLaunchConfig_t cfg = {};
@@ -822,7 +831,7 @@ bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long
 }
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
-  const double operands = (double)(rows + 32 * experts) * (M + N);
+  const double operands = (double)(rows + BK * experts) * (M + N);
   if (operands * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * M;
@@ -874,16 +883,16 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
                              const int** guard_out) {
   DeviceGuard guard(s->device);
   // C_e[m, n] = sum A[r, m] B[r, n]: n in the lanes, m in the columns
-  const long long kp = ((long long)rows + 31LL * (experts < rows ? experts : rows) + 31) / 32 * 32;
+  const long long kp = ((long long)rows + (BK - 1LL) * (experts < rows ? experts : rows) + BK - 1) / BK * BK;
   const size_t bytes = up256(sizeof(Plan)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
-                       2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / BK) * 4) + 2 * up256((size_t)experts * N * 4) + 2 * up256((size_t)experts * M * 4);
+                       2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / POS) * 4) + 2 * up256((size_t)experts * N * 4) + 2 * up256((size_t)experts * M * 4);
   void* ws = nullptr;
   int rc = cb200_scratch(s, bytes, &ws);
   if (rc) return rc;
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
   Entry* table = w.take<Entry>((size_t)experts + 1);
-  int* owner = w.take<int>((size_t)(kp / BK));
+  int* owner = w.take<int>((size_t)(kp / POS));
   __half* l_hi = w.take<__half>((size_t)N * kp);
   __half* l_lo = w.take<__half>((size_t)N * kp);
   __half* r_hi = w.take<__half>((size_t)M * kp);
