@@ -23,7 +23,7 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
                           const int* offsets, const float* bias, int act, const int** guard);
 int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows, int M,
                              long long lda, const float* B, int N, long long ldb, int experts, float beta, const int* offsets,
-                             const int** guard);
+                             float* bias_gradient, const int** guard);
 
 namespace {
 
@@ -456,17 +456,18 @@ int rows_tc(cb200_stream* s, Product<float> p) {
 }
 
 int weights_tc(cb200_stream* s, Product<float> p) {
-  if (p.bias_g) {
+  const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
+  const bool halves = cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts);
+  if (!halves && p.bias_g) {
     DeviceGuard guard(s->device);
     int rc = run_bias_gradient<float>(s, p);
     if (rc) return rc;
   }
-  const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
-  if (cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts)) {
+  if (halves) {
     int rc = cb200_expert_weights_f16(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta,
-                                      p.offsets, &p.only_if);
+                                      p.offsets, p.bias_g, &p.only_if);
     if (rc) return rc;
-    p.bias_g = nullptr;                                          // done above
+    p.bias_g = nullptr;                                          // done with the column pass
     if (pack_a || pack_b) return run_weights<float>(s, p);
   } else if (pack_a || pack_b) {
     DeviceGuard guard(s->device);

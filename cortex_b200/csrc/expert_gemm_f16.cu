@@ -61,8 +61,14 @@ struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); ex
 
 // bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
 // entry per tile of BN rows.
-__global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int* owner, int* begins, const int* offsets, int experts,
-                                                  int rows, int weights, int* status) {
+// (CTA 0, one warp; the other CTAs zero the words that the next kernels take maxima into)
+__global__ void __launch_bounds__(128) plan_kernel(Plan* plan, Entry* table, int* owner, int* begins, const int* offsets, int experts,
+                                                   int rows, int weights, int* status, uint32_t* zero, long long zero_n) {
+  if (blockIdx.x > 0) {
+    for (long long i = (blockIdx.x - 1LL) * 128 + threadIdx.x; i < zero_n; i += (gridDim.x - 1LL) * 128) zero[i] = 0;
+    return;
+  }
+  if (threadIdx.x >= 32) return;
   const int lane = threadIdx.x;
   int carry_max = 0, carry = 0, first_row = rows;
   bool bad = false;
@@ -118,6 +124,10 @@ __global__ void __launch_bounds__(32) plan_kernel(Plan* plan, Entry* table, int*
   }
 }
 
+// The kernels of a call are launched so that each may be set up while its predecessor ends; nothing of the predecessors'
+// results is touched before this.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- scaled halves ---------------------------------------------------------------------------------------------
 // Scale of a row (or column) whose largest magnitude has these bits: 2^up; its inverse; false: outside the range.
 __device__ __forceinline__ bool scale_of(uint32_t max_bits, float& up, float& down) {
@@ -158,6 +168,7 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
                                                          long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan,
                                                          const float* fold, const int* begins, int experts) {
   constexpr int HOLD = 4;
+  wait_for_previous_kernel();
   __shared__ uint32_t part_max[8];
   __shared__ int part_tiny[8];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, warp = threadIdx.x >> 5;
@@ -183,9 +194,10 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
     }
     load8(src + c, n - c, vec, w);
     if (RAGGED == 2) {
+      float f[8];
+      load8(scales + c, n - c, ((uintptr_t)scales & 15) == 0, f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < n) w[j] *= 16384.f * __ldg(scales + c + j);
+      for (int j = 0; j < 8; ++j) w[j] *= 16384.f * f[j];
     }
   };
   float v[HOLD][8];
@@ -252,35 +264,45 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
 
 // Operands whose reduction runs down their columns, in ragged groups of rows: table[g].lo .. hi.
 // maxima[g][c] = bits of the largest magnitude in column c of group g.  A CTA: 128 columns of up to 64 rows of one group at a
-// time, four rows side by side and (where the rows are 16-byte aligned) four columns per thread.
+// time, four rows side by side and (where the rows are 16-byte aligned) four columns per thread.  `sums`, where given, gets
+// those rows' column sums, in row b + g for the rows of block b that belong to group g (a pair of its own for every such row).
 template <int V>
-__global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const float* x, long long ld, const Entry* table,
+__global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, float* sums, const float* x, long long ld, const Entry* table,
                                                          int groups_n, int rows, int cols) {
   constexpr int LANES = 128 / V, SIDE = 128 / LANES;       // threads per row, rows side by side
+  wait_for_previous_kernel();
   struct alignas(4 * V) Pack { float e[V]; };
   __shared__ uint32_t part[SIDE][128];
+  __shared__ float part_sum[SIDE][128];
   const int tx = threadIdx.x % LANES, ty = threadIdx.x / LANES, c = blockIdx.x * 128 + tx * V;
   const bool live = c < cols;                              // V = 4: cols is a multiple of 4
-  auto reduce = [&](int g, int a, int z) {                 // rows a .. z - 1 of group g
+  auto reduce = [&](long long b, int g, int a, int z) {    // rows a .. z - 1 of block b, all of group g
     uint32_t m[V];
+    float s[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) m[j] = 0;
+    for (int j = 0; j < V; ++j) { m[j] = 0; s[j] = 0.f; }
     if (live) {
 #pragma unroll 4
       for (int r = a + ty; r < z; r += SIDE) {
         const Pack v = *reinterpret_cast<const Pack*>(x + (long long)r * ld + c);
 #pragma unroll
-        for (int j = 0; j < V; ++j) m[j] = max(m[j], __float_as_uint(v.e[j]) & 0x7fffffffu);
+        for (int j = 0; j < V; ++j) { m[j] = max(m[j], __float_as_uint(v.e[j]) & 0x7fffffffu); s[j] += v.e[j]; }
       }
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) part[ty][tx * V + j] = m[j];
+    for (int j = 0; j < V; ++j) { part[ty][tx * V + j] = m[j]; part_sum[ty][tx * V + j] = s[j]; }
     __syncthreads();
     uint32_t all = part[0][threadIdx.x];
 #pragma unroll
     for (int i = 1; i < SIDE; ++i) all = max(all, part[i][threadIdx.x]);
     const int at = blockIdx.x * 128 + threadIdx.x;
     if (at < cols) atomicMax(maxima + (long long)g * cols + at, all);
+    if (sums && at < cols) {
+      float sum = part_sum[0][threadIdx.x];
+#pragma unroll
+      for (int i = 1; i < SIDE; ++i) sum += part_sum[i][threadIdx.x];
+      sums[(b + g) * cols + at] = sum;
+    }
     __syncthreads();
   };
   for (long long b = blockIdx.y; b * 64 < rows; b += gridDim.y) {
@@ -292,9 +314,27 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, const
     }
     for (; g < groups_n && table[g].lo < r1; ++g) {
       const int a = max(r0, table[g].lo), z = min(r1, table[g].hi);
-      if (z > a) reduce(g, a, z);
+      if (z > a) reduce(b, g, a, z);
     }
   }
+}
+
+// bias_gradient[g, c] = alpha * (the sums of group g's rows, block by block) + beta * bias_gradient[g, c]
+__global__ void __launch_bounds__(128) column_sum_kernel(float* out, const float* sums, const Entry* table, int cols, float alpha, float beta) {
+  wait_for_previous_kernel();
+  const int c = blockIdx.x * 128 + threadIdx.x, g = blockIdx.y;
+  if (c >= cols) return;
+  const Entry e = table[g];
+  float s = 0.f;
+  if (e.hi > e.lo) {
+    const long long first = e.lo / 64, last = (e.hi - 1) / 64;
+#pragma unroll 8
+    for (long long b = first; b <= last; ++b) s += sums[(b + g) * cols + c];
+  }
+  float* to = out + (long long)g * cols + c;
+  float v = alpha * s;
+  if (beta != 0.f) v += beta * (*to);
+  *to = v;
 }
 
 // hi / lo [cols][positions]: 32 positions x 64 columns at a time through shared memory.  Groups start at a multiple of 64
@@ -305,6 +345,7 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
                                                             Plan* plan) {
   __shared__ float tile[2][32][65];
   __shared__ int tiny_all;
+  wait_for_previous_kernel();
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   const int blocks = plan->padded / POS;
   for (int b = blockIdx.y; b < blocks; b += gridDim.y) {
@@ -434,6 +475,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   const bool leader = rank == 0;
   const int n_clusters = (int)gridDim.x >> 1, cluster_id = (int)blockIdx.x >> 1;
 
+  wait_for_previous_kernel();
   if (p.plan->flag) return;               // both CTAs of every pair: nothing has been set up yet
   const int tiles_l = (p.lanes + 2 * BM - 1) / (2 * BM);
   const int n_units = (p.weights ? p.experts * ((p.cols + BN - 1) / BN) : p.plan->tiles) * tiles_l;
@@ -735,36 +777,52 @@ int half_map(CUtensorMap* tm, const __half* base, long long rows, long long cols
   return CB200_OK;
 }
 
-template <int RAGGED>
-int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
-               long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0) {
-  if (cols <= 1024)
-    split_rows_kernel<32, RAGGED><<<(unsigned)((rows + 7) / 8), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
-                                                                                     plan, fold, begins, experts);
-  else if (cols <= 4096)
-    split_rows_kernel<128, RAGGED><<<(unsigned)((rows + 1) / 2), 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
-                                                                                      plan, fold, begins, experts);
-  else
-    split_rows_kernel<256, RAGGED><<<(unsigned)rows, 256, 0, s->stream>>>(hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan, fold,
-                                                                          begins, experts);
+// Launch `kernel` behind what the stream holds, set up while its predecessor ends (it waits by itself).
+template <typename... P, typename... A>
+int launch_next(cb200_stream* s, void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaLaunchKernelEx(expert product)", __FILE__, __LINE__);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
 
-int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, const float* x, long long ld, const Entry* table,
-                  const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
-  CB_CUDA(cudaMemsetAsync(maxima, 0, (size_t)groups_n * cols * sizeof(uint32_t), s->stream));
+template <int RAGGED>
+int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
+               long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0) {
+  if (cols <= 1024)
+    return launch_next(s, split_rows_kernel<32, RAGGED>, dim3((unsigned)((rows + 7) / 8)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
+                       rows, cols, kp, plan, fold, begins, experts);
+  if (cols <= 4096)
+    return launch_next(s, split_rows_kernel<128, RAGGED>, dim3((unsigned)((rows + 1) / 2)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
+                       rows, cols, kp, plan, fold, begins, experts);
+  return launch_next(s, split_rows_kernel<256, RAGGED>, dim3((unsigned)rows), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
+                     plan, fold, begins, experts);
+}
+
+// `sums` (may be null): workspace for the column sums of 64-row blocks, ((rows + 63) / 64 + groups_n) x cols
+int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, float* sums, const float* x, long long ld,
+                  const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
   const long long chunks = (rows + 63) / 64, blocks = kp / POS;
   const dim3 grid_max((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535));
-  if (((uintptr_t)x & 15) == 0 && ld % 4 == 0 && cols % 4 == 0)
-    column_max_kernel<4><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, table, groups_n, rows, cols);
-  else
-    column_max_kernel<1><<<grid_max, 128, 0, s->stream>>>(maxima, x, ld, table, groups_n, rows, cols);
-  CB_LAUNCH_CHECK(s);
-  split_columns_kernel<<<dim3((unsigned)((cols + 127) / 128), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, s->stream>>>(
-      hi, lo, down, maxima, x, ld, table, owner, cols, kp, plan);
-  CB_LAUNCH_CHECK(s);
-  return CB200_OK;
+  const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0 && cols % 4 == 0;
+  int rc = launch_next(s, vec ? column_max_kernel<4> : column_max_kernel<1>, grid_max, 128, 0, 1, maxima, sums, x, ld, table, groups_n, rows, cols);
+  if (rc) return rc;
+  return launch_next(s, split_columns_kernel, dim3((unsigned)((cols + 127) / 128), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, 1, hi,
+                     lo, down, maxima, x, ld, table, owner, cols, kp, plan);
 }
 
 int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long long l_rows, long long l_cols, long long l_pitch,
@@ -782,22 +840,7 @@ int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long lo
       (rc = half_map(&tmR, r_hi, r_rows, r_cols, r_pitch, 64, R_BOX)) || (rc = half_map(&tmRlo, r_lo, r_rows, r_cols, r_pitch, 64, R_BOX)))
     return rc;
   const long long clusters = units < s->sm_count / 2 ? units : s->sm_count / 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * clusters), 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
-  cfg.dynamicSmemBytes = SMEM;
-  cfg.stream = s->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, expert_pair_kernel, tmL, tmLlo, tmR, tmRlo, a);
-  if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaLaunchKernelEx(expert_pair_kernel)", __FILE__, __LINE__);
-  CB_LAUNCH_CHECK(s);
-  return CB200_OK;
+  return launch_next(s, expert_pair_kernel, dim3((unsigned)(2 * clusters)), THREADS, SMEM, 2, tmL, tmLlo, tmR, tmRlo, a);
 }
 
 inline long long up8(long long v) { return (v + 7) / 8 * 8; }
@@ -864,7 +907,7 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   __half* r_lo = w.take<__half>((size_t)rows * kp);
   float* l_down = w.take<float>((size_t)l_rows);
   float* r_down = w.take<float>((size_t)rows);
-  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev);
+  plan_kernel<<<1, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev, nullptr, 0);
   CB_LAUNCH_CHECK(s);
   if ((rc = split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan))) return rc;
   if (trans_b) rc = split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan);
@@ -880,12 +923,14 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
 
 int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows, int M,
                              long long lda, const float* B, int N, long long ldb, int experts, float beta, const int* offsets,
-                             const int** guard_out) {
+                             float* bias_gradient, const int** guard_out) {
   DeviceGuard guard(s->device);
   // C_e[m, n] = sum A[r, m] B[r, n]: n in the lanes, m in the columns
   const long long kp = ((long long)rows + (BK - 1LL) * (experts < rows ? experts : rows) + BK - 1) / BK * BK;
+  const size_t sums_n = bias_gradient ? ((size_t)(rows + 63) / 64 + experts) * M : 0;
   const size_t bytes = up256(sizeof(Plan)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
-                       2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / POS) * 4) + 2 * up256((size_t)experts * N * 4) + 2 * up256((size_t)experts * M * 4);
+                       2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / POS) * 4) + up256((size_t)experts * N * 4) + up256((size_t)experts * M * 4) +
+                       up256((size_t)experts * (M + N) * 4) + up256(sums_n * 4);
   void* ws = nullptr;
   int rc = cb200_scratch(s, bytes, &ws);
   if (rc) return rc;
@@ -899,12 +944,17 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   __half* r_lo = w.take<__half>((size_t)M * kp);
   float* l_down = w.take<float>((size_t)experts * N);
   float* r_down = w.take<float>((size_t)experts * M);
-  uint32_t* l_max = w.take<uint32_t>((size_t)experts * N);
-  uint32_t* r_max = w.take<uint32_t>((size_t)experts * M);
-  plan_kernel<<<1, 32, 0, s->stream>>>(plan, table, owner, nullptr, offsets, experts, rows, 1, s->status_dev);
+  uint32_t* l_max = w.take<uint32_t>((size_t)experts * (M + N));
+  uint32_t* r_max = l_max + (size_t)experts * N;
+  float* sums = bias_gradient ? w.take<float>(sums_n) : nullptr;
+  plan_kernel<<<129, 128, 0, s->stream>>>(plan, table, owner, nullptr, offsets, experts, rows, 1, s->status_dev, l_max,
+                                          (long long)experts * (M + N));
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, B, ldb, table, owner, experts, rows, N, kp, plan))) return rc;
-  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, A, lda, table, owner, experts, rows, M, kp, plan))) return rc;
+  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, nullptr, B, ldb, table, owner, experts, rows, N, kp, plan))) return rc;
+  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, sums, A, lda, table, owner, experts, rows, M, kp, plan))) return rc;
+  if (bias_gradient && (rc = launch_next(s, column_sum_kernel, dim3((unsigned)((M + 127) / 128), (unsigned)experts), 128, 0, 1, bias_gradient,
+                                         sums, table, M, alpha, beta)))
+    return rc;
   PairArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.table = table;
   a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.l_mn = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
