@@ -238,12 +238,12 @@ __global__ void __launch_bounds__(128) column_sums_kernel(Backward<T> p, const T
   for (int k = 0; k < SUMS; ++k) parts[((long long)b * SUMS + k) * p.cols + c] = s[k];
 }
 
-// The sum over n rows first, first + pitch, ... of one column: 32 columns x 8 threads each (blockDim 256), added in order.
+// The sum over n rows first, first + pitch, ... of one column: 32 columns x 32 threads each (blockDim 1024), added in order.
 template <typename T>
 __device__ __forceinline__ void add_rows(const T* first, long long pitch, int n, T* to, bool live) {
-  __shared__ T part[8][33];
+  __shared__ T part[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int a = n * ty / 8, z = n * (ty + 1) / 8;
+  const int a = (int)((long long)n * ty / 32), z = (int)((long long)n * (ty + 1) / 32);
   T s = (T)0;
   if (live) {
 #pragma unroll 8
@@ -254,7 +254,7 @@ __device__ __forceinline__ void add_rows(const T* first, long long pitch, int n,
   __syncthreads();
   if (ty == 0 && live) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += part[i][tx];
+    for (int i = 1; i < 32; ++i) s += part[i][tx];
     *to = s;
   }
 }
@@ -262,7 +262,7 @@ __device__ __forceinline__ void add_rows(const T* first, long long pitch, int n,
 // blockIdx.y < SUMS: a scale's or bias's gradient.  Behind them: the gate groups that more than one row block has a part of
 // (strided); the first part may be in the second slot of its block, the others are in first slots.
 template <typename T>
-__global__ void __launch_bounds__(256) column_finish_kernel(Backward<T> p, const T* parts, const T* gate_parts, int blocks) {
+__global__ void __launch_bounds__(1024) column_finish_kernel(Backward<T> p, const T* parts, const T* gate_parts, int blocks) {
   const long long c = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
   if (blockIdx.y < SUMS) {
     const int k = blockIdx.y;
@@ -687,7 +687,7 @@ template <typename T> int finish_columns(cb200_stream* s, const Backward<T>& p, 
   const bool gates = p.gate_g && p.rows_per_gate > 1;
   if (!(p.before_w_g || p.before_b_g || p.after_w_g || p.after_b_g || gates)) return CB200_OK;
   const long long groups = gates ? p.rows / p.rows_per_gate : 0;
-  column_finish_kernel<T><<<dim3((unsigned)((p.cols + 31) / 32), (unsigned)(SUMS + (groups < 4096 ? groups : 4096))), 256, 0, s->stream>>>(
+  column_finish_kernel<T><<<dim3((unsigned)((p.cols + 31) / 32), (unsigned)(SUMS + (groups < 4096 ? groups : 4096))), 1024, 0, s->stream>>>(
       p, parts, gate_parts, blocks);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;

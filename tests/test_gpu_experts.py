@@ -602,3 +602,130 @@ def test_expert_gemm_scaled_halves(stream, route, n, k):
             _within(got_w[keep_e], want_w[keep_e], size_w[keep_e], _product_tol("float", 300), (data, "weights"))
         else:
             _within(got_w[:, :, 1:], want_w[:, :, 1:], size_w[:, :, 1:], _product_tol("float", 300), (data, "weights"))
+
+
+@pytest.mark.parametrize("way", ["forward", "input", "weights"])
+@pytest.mark.parametrize("route,sizes,n,k", [(1, [200, 0, 56], 264, 512), (1, [20, 4, 8], 264, 512), (2, [200, 0, 56], 264, 512)])
+def test_expert_gemm_waits_that_run_out(b200_driver, way, route, sizes, n, k):
+    """Producers that deliver nothing (a setting, not a fault): every role gives up in time, the sync raises, and the next call
+    on the stream is right."""
+    s = b200_driver.default_device().create_stream()
+    s.set_option("gemm-auto-presplit", route)
+    if route == 1:
+        s.set_option("gemm-tile-n", 128)            # (the tensor-core kernel also where there are few rows)
+    rng = np.random.default_rng(5)
+    rows, off = sum(sizes), _offsets(sizes)
+    X, dY, W = (rng.standard_normal(sh).astype(np.float32) for sh in ((rows, k), (rows, n), (3, n, k)))
+    with ct.with_stream(s):
+        o, Xt, dYt, Wt = ct.to_tensor(off, "int"), ct.to_tensor(X, "float"), ct.to_tensor(dY, "float"), ct.to_tensor(W, "float")
+        out = {"forward": ct.new_tensor([rows, n], "float"), "input": ct.new_tensor([rows, k], "float"),
+               "weights": ct.new_tensor([3, n, k], "float")}[way]
+
+        def run():
+            if way == "forward":
+                ct.expert_gemm(out, True, 1.0, Xt, Wt, 0.0, o)
+            elif way == "input":
+                ct.expert_gemm(out, False, 1.0, dYt, Wt, 0.0, o)
+            else:
+                ct.expert_gemm_weights(out, 1.0, dYt, Xt, 0.0, o)
+
+        run()
+        s.sync()
+        s.set_option("wait-limit-cycles", 1 << 20)
+        s.set_option("inject-fault", 1)
+        run()
+        with pytest.raises(_lib.B200Error) as err:
+            s.sync()
+        assert err.value.code == 4
+        s.set_option("inject-fault", 0)
+        s.set_option("wait-limit-cycles", 0)
+        run()
+        s.sync()
+        want = {"forward": lambda: plain.expert_gemm(np.zeros((rows, n)), True, 1.0, X, W, 0.0, off),
+                "input": lambda: plain.expert_gemm(np.zeros((rows, k)), False, 1.0, dY, W, 0.0, off),
+                "weights": lambda: plain.expert_gemm_weights(np.zeros((3, n, k)), 1.0, dY, X, 0.0, off)[:2]}[way]()
+        _within(ct.to_array(out), *want, _product_tol("float", max(k, n)), way)
+
+
+@pytest.mark.parametrize("offsets", [[0, 500, 300, 640], [-5, 100, 200, 640], [0, 10, 20, 900], [0, 10, 2147483647, -2147483648]])
+def test_expert_gemm_scaled_halves_reports_bad_offsets(b200_driver, offsets):
+    s = b200_driver.default_device().create_stream()
+    s.set_option("gemm-auto-presplit", 2)
+    rows, n, k = 640, 72, 104
+    rng = np.random.default_rng(3)
+    X, dY, W = (rng.standard_normal(sh).astype(np.float32) for sh in ((rows, k), (rows, n), (3, n, k)))
+    with ct.with_stream(s):
+        off = ct.to_tensor(np.array(offsets, np.int32), "int")
+        Xt, dYt, Wt = ct.to_tensor(X, "float"), ct.to_tensor(dY, "float"), ct.to_tensor(W, "float")
+        Y, dX, dW, db = ct.new_tensor([rows, n], "float"), ct.new_tensor([rows, k], "float"), ct.new_tensor([3, n, k], "float"), ct.new_tensor([3, n], "float")
+        ct.expert_gemm(Y, True, 1.0, Xt, Wt, 0.0, off)
+        with pytest.raises(_lib.B200Error):
+            s.sync()
+        ct.expert_gemm(dX, False, 1.0, dYt, Wt, 0.0, off)
+        with pytest.raises(_lib.B200Error):
+            s.sync()
+        ct.expert_gemm_weights(dW, 1.0, dYt, Xt, 0.0, off, bias_gradient=db)
+        with pytest.raises(_lib.B200Error):
+            s.sync()
+        _within(ct.to_array(Y), *plain.expert_gemm(np.zeros((rows, n)), True, 1.0, X, W, 0.0, offsets), _product_tol("float", k), "y")
+        _within(ct.to_array(dX), *plain.expert_gemm(np.zeros((rows, k)), False, 1.0, dY, W, 0.0, offsets), _product_tol("float", n), "x")
+        w, ws, b, bs = plain.expert_gemm_weights(np.zeros((3, n, k)), 1.0, dY, X, 0.0, offsets, np.zeros((3, n)))
+        _within(ct.to_array(dW), w, ws, _product_tol("float", rows), "w")
+        _within(ct.to_array(db), b, bs, (rows + 8) * U["float"], "b")
+    s.sync()
+
+
+def test_no_rows(stream):
+    """A batch without rows: nothing to compute, gradients of zero."""
+    off = ct.to_tensor(np.zeros(4, np.int32), "int")
+    W = ct.new_tensor([3, 8, 4], "float")
+    X, Y, D = (ct.new_tensor([0, c], "float") for c in (4, 8, 4))
+    ct.expert_gemm(Y, True, 1.0, X, W, 0.0, off)
+    ct.expert_gemm(D, False, 1.0, Y, W, 0.0, off)
+    dW, db = ct.to_tensor(np.ones((3, 8, 4)), "float"), ct.to_tensor(np.ones((3, 8)), "float")
+    ct.expert_gemm_weights(dW, 1.0, Y, X, 0.5, off, bias_gradient=db)
+    assert np.all(ct.to_array(dW) == 0.5) and np.all(ct.to_array(db) == 0.5)
+    ct.expert_gemm_weights(dW, 1.0, Y, X, 0.0, off, bias_gradient=db)
+    assert not ct.to_array(dW).any() and not ct.to_array(db).any()
+    w, e = ct.to_tensor(np.ones(4), "float"), [ct.new_tensor([0, 4], "float") for _ in range(7)]
+    ct.block_normalize(e[0], e[1], e[2], e[3], None, 1.0, (w, None), (w, None), 1e-5)
+    ga, gb = ct.to_tensor(np.ones(4), "float"), ct.to_tensor(np.ones(4), "float")
+    ct.block_normalize_gradients(e[4], e[5], None, (ga, None), (gb, None), e[0], e[1], e[2], e[3], None, 1.0, (w, None), (w, None), 1e-5)
+    assert not ct.to_array(ga).any() and not ct.to_array(gb).any()
+
+
+def test_offsets_beyond_32_bits(stream):
+    """Matrices of more than 2^31 elements: the last rows are found and right."""
+    rows, d = (1 << 19) + 5, 4100
+    rng = np.random.default_rng(81)
+    last, w = rng.standard_normal((3, d)).astype(np.float32), rng.standard_normal(d).astype(np.float32)
+    x, y = ct.new_tensor([rows, d], "float", init_value=None), ct.new_tensor([rows, d], "float", init_value=None)
+
+    def fill(value):                                 # (memset takes fewer than 2^31 elements at a time)
+        for first in (0, rows // 2):
+            n = (rows // 2 if first == 0 else rows - rows // 2) * d
+            ct.assign(ct.Tensor(x.device, {"shape": [n], "strides": [1]}, x.buffer.sub_buffer(first * d, n)), value)
+
+    fill(1.0)
+    tail = lambda t: ct.Tensor(t.device, {"shape": [3, d], "strides": [d, 1]}, t.buffer.sub_buffer((rows - 3) * d, 3 * d))
+    ct.assign(tail(x), ct.to_tensor(last, "float"))
+    wt, gate = ct.to_tensor(w, "float"), ct.to_tensor(w[None], "float")
+    ct.block_normalize(y, x, x, x, gate, 0.5, (wt, None), (wt, None), 1e-5, "layer")
+    total, t_size, out, o_size = plain.block_normalize(last, last, w[None], 0.5, (w, None), (w, None), 1e-5, "layer")
+    _within(ct.to_array(tail(x)), total, t_size, _norm_tol("float", d), "total")
+    _within(ct.to_array(tail(y)), out, o_size, 2 * _norm_tol("float", d), "output")
+    # the product: all rows are one expert's but the last three
+    A, W = ct.new_tensor([rows, 8], "float"), rng.standard_normal((2, d, 8)).astype(np.float32)
+    a_last = rng.standard_normal((3, 8)).astype(np.float32)
+    at = ct.Tensor(A.device, {"shape": [3, 8], "strides": [8, 1]}, A.buffer.sub_buffer((rows - 3) * 8, 24))
+    ct.assign(at, ct.to_tensor(a_last, "float"))
+    ct.expert_gemm(y, True, 1.0, A, ct.to_tensor(W, "float"), 0.0, ct.to_tensor(np.array([0, rows - 3, rows], np.int32), "int"))
+    want, size = plain.expert_gemm(np.zeros((3, d)), True, 1.0, a_last, W, 0.0, [0, 0, 3])
+    _within(ct.to_array(tail(y)), want, size, _product_tol("float", 8), "product")
+    # the norm, and a piece behind 2^31 elements
+    fill(0.5)
+    flat = ct.as_vector(x)
+    norm = ct.to_array(optimize.clip_gradients([flat], 1.0))[0]
+    n = rows * d
+    assert abs(norm - 0.5 * np.sqrt(n)) <= norm * 2.0 ** -23
+    np.testing.assert_allclose(ct.to_array(tail(x)), 1.0 / np.sqrt(n), rtol=2.0 ** -22)
