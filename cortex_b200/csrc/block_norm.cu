@@ -653,7 +653,8 @@ template <typename T> int run_forward(cb200_stream* s, const Forward<T>& p) {
   else if (vec && p.cols <= V * 2 * 64) launch_forward<T, V, 2>(s, p);
   else if (vec && p.cols <= V * 4 * 1024) launch_forward<T, V, 4>(s, p);
   else if (!vec && p.cols <= 1024 && (few || p.cols <= 32)) launch_forward<T, 1, 1>(s, p);
-  else if (!vec && p.cols <= 4 * 1024 && (few || p.cols <= 4 * 128)) launch_forward<T, 1, 4>(s, p);
+  else if (!vec && p.cols <= 4 * 1024) launch_forward<T, 1, 4>(s, p);
+  else if (!vec && p.cols <= 8 * 1024) launch_forward<T, 1, 8>(s, p);
   else if (!vec && sizeof(T) == 4 && p.cols <= 16 * 1024) launch_forward<T, 1, sizeof(T) == 4 ? 16 : 4>(s, p);
   else forward_wide_kernel<T><<<(unsigned)p.rows, WIDE_THREADS, 0, s->stream>>>(p);
   CB_LAUNCH_CHECK(s);

@@ -111,10 +111,10 @@ template <> struct Tile64<float> {
   }
 };
 
-// double: the fp64 matrix instruction (m8n8k4), 8 warps as 2 x 4 of 32 x 16, the next 16 values of k on their way into
+// double: the fp64 matrix instruction (m16n8k8), 8 warps as 2 x 4 of 32 x 16, the next 16 values of k on their way into
 // registers meanwhile.  Row pitch 68 (4 mod 16): the 16 fragment elements of a half-warp lie in 16 different banks.
 template <> struct Tile64<double> {
-  double acc[4][2][2];
+  double acc[2][2][4];
   __device__ __forceinline__ void run(const double* a, long long sam, long long sak, const double* b, long long sbk, long long sbn, int m_left,
                                       int n_left, int K) {
     constexpr int LD = 68;
@@ -122,9 +122,11 @@ template <> struct Tile64<double> {
     __shared__ double Bs[16][LD];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, wm = (warp >> 2) * 32, wn = (warp & 3) * 16, fr = lane >> 2, fk = lane & 3;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.0;
     double ra[4], rb[4];
     auto load = [&](int k0) {
 #pragma unroll
@@ -147,19 +149,28 @@ template <> struct Tile64<double> {
       __syncthreads();
       if (k0 + 16 < K) load(k0 + 16);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        double x[4], y[2];
+      for (int kk = 0; kk < 2; ++kk) {
+        double x[2][4], y[2][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = As[kk * 4 + fk][wm + i * 8 + fr];
+        for (int i = 0; i < 2; ++i) {
+          const int m = wm + i * 16 + fr, k = kk * 8 + fk;
+          x[i][0] = As[k][m];
+          x[i][1] = As[k][m + 8];
+          x[i][2] = As[k + 4][m];
+          x[i][3] = As[k + 4][m + 8];
+        }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) y[j] = Bs[kk * 4 + fk][wn + j * 8 + fr];
+        for (int j = 0; j < 2; ++j) {
+          y[j][0] = Bs[kk * 8 + fk][wn + j * 8 + fr];
+          y[j][1] = Bs[kk * 8 + fk + 4][wn + j * 8 + fr];
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
-                         : "+d"(acc[i][j][0]), "+d"(acc[i][j][1])
-                         : "d"(x[i]), "d"(y[j]));
+            asm volatile("mma.sync.aligned.m16n8k8.row.col.f64.f64.f64.f64 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                         : "+d"(acc[i][j][0]), "+d"(acc[i][j][1]), "+d"(acc[i][j][2]), "+d"(acc[i][j][3])
+                         : "d"(x[i][0]), "d"(x[i][1]), "d"(x[i][2]), "d"(x[i][3]), "d"(y[j][0]), "d"(y[j][1]));
       }
       __syncthreads();
     }
@@ -167,7 +178,7 @@ template <> struct Tile64<double> {
   __device__ __forceinline__ void store(double* c, long long ldc, int m_left, int n_left, double alpha, double beta, const double* bias, int act) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = (warp >> 2) * 32, wn = (warp & 3) * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {                            // 16-row tile i / 2, its upper or lower 8 rows
       const int m = wm + i * 8 + (lane >> 2);
       if (m >= m_left) continue;
 #pragma unroll
@@ -175,7 +186,7 @@ template <> struct Tile64<double> {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int n = wn + j * 8 + (lane & 3) * 2 + e;
-          if (n < n_left) finish<double>(c + (long long)m * ldc + n, acc[i][j][e], n, alpha, beta, bias, act);
+          if (n < n_left) finish<double>(c + (long long)m * ldc + n, acc[i >> 1][j][(i & 1) * 2 + e], n, alpha, beta, bias, act);
         }
     }
   }
@@ -320,12 +331,12 @@ template <typename T> int run_few_rows(cb200_stream* s, const Product<T>& p) {
 }
 
 // bias_gradient[e, m] = alpha * sum of the group's rows + beta * bias_gradient[e, m]: a warp reads 32 * V columns of a row,
-// the CTA's eight warps take every eighth row with four rows in flight each; fixed order
+// the CTA's 32 warps take every 32nd row with four rows in flight each; fixed order
 template <typename T, int V>
-__global__ void __launch_bounds__(256) expert_bias_gradient_kernel(Product<T> p) {
+__global__ void __launch_bounds__(1024) expert_bias_gradient_kernel(Product<T> p) {
   struct alignas(sizeof(T) * V) Pack { T e[V]; };
   __shared__ int lo, hi;
-  __shared__ T part[8][32 * V + 1];
+  __shared__ T part[32][32 * V];
   const int e = (int)blockIdx.y;
   if (threadIdx.x < 32) {
     int a, b;
@@ -340,16 +351,16 @@ __global__ void __launch_bounds__(256) expert_bias_gradient_kernel(Product<T> p)
   if (m < p.M) {
     const T* a = p.A + m;
     int r = lo + ty;
-    for (; r + 24 < hi; r += 32) {
+    for (; r + 96 < hi; r += 128) {
       Pack v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const Pack*>(a + (long long)(r + 8 * i) * p.lda);
+      for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const Pack*>(a + (long long)(r + 32 * i) * p.lda);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] += v[i].e[j];
     }
-    for (; r < hi; r += 8) {
+    for (; r < hi; r += 32) {
       const Pack v = *reinterpret_cast<const Pack*>(a + (long long)r * p.lda);
 #pragma unroll
       for (int j = 0; j < V; ++j) s[j] += v.e[j];
@@ -358,25 +369,23 @@ __global__ void __launch_bounds__(256) expert_bias_gradient_kernel(Product<T> p)
 #pragma unroll
   for (int j = 0; j < V; ++j) part[ty][tx * V + j] = s[j];
   __syncthreads();
-  for (int c = threadIdx.x; c < 32 * V; c += 256) {
-    const int at = (int)blockIdx.x * 32 * V + c;
-    if (at >= p.M) break;
-    T sum = part[0][c];
+  const int at = (int)blockIdx.x * 32 * V + threadIdx.x;
+  if (threadIdx.x >= 32 * V || at >= p.M) return;
+  T sum = part[0][threadIdx.x];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) sum += part[w][c];
-    T* to = p.bias_g + (long long)e * p.M + at;
-    T o = p.alpha * sum;
-    if (p.beta != (T)0) o += p.beta * (*to);
-    *to = o;
-  }
+  for (int w = 1; w < 32; ++w) sum += part[w][threadIdx.x];
+  T* to = p.bias_g + (long long)e * p.M + at;
+  T o = p.alpha * sum;
+  if (p.beta != (T)0) o += p.beta * (*to);
+  *to = o;
 }
 
 template <typename T> int run_bias_gradient(cb200_stream* s, const Product<T>& p) {
   constexpr int V = 16 / sizeof(T);
   if (((uintptr_t)p.A & 15) == 0 && p.lda % V == 0 && p.M % V == 0)
-    expert_bias_gradient_kernel<T, V><<<dim3((unsigned)((p.M + 32 * V - 1) / (32 * V)), (unsigned)p.experts), 256, 0, s->stream>>>(p);
+    expert_bias_gradient_kernel<T, V><<<dim3((unsigned)((p.M + 32 * V - 1) / (32 * V)), (unsigned)p.experts), 1024, 0, s->stream>>>(p);
   else
-    expert_bias_gradient_kernel<T, 1><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 256, 0, s->stream>>>(p);
+    expert_bias_gradient_kernel<T, 1><<<dim3((unsigned)((p.M + 31) / 32), (unsigned)p.experts), 1024, 0, s->stream>>>(p);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }

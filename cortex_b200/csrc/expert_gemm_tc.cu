@@ -2,11 +2,8 @@
 // which the tensor core reads the top 19 bits, lo = x - trunc(x); main and cross terms in two TMEM accumulators) over
 // ragged groups whose bounds are read from device memory.
 //
-//   expert_rows_kernel      C[r, :] for the rows r of a group, the group's matrix as the other operand (a 3-d tensor map, so
-//                           a tile that ends behind its expert's matrix reads zeros).
-//   expert_weights_kernel   128 x BN tile of C_e [M, N] = A_e^T B_e: the reduction runs over the group's rows.  Both operands
-//                           are MN-major; rows of the last k-block that belong to the next group are zeroed, hi tile
-//                           included, by the warps that compute the lo tiles (an infinity or a NaN there does not matter).
+// One kernel: C[r, :] for the rows r of a group, the group's matrix as the other operand (a 3-d tensor map, so a tile that ends
+// behind its expert's matrix reads zeros); and C_e = A_e^T B_e, reduced over the group's rows.
 //
 // Every CTA finds its tile itself (groups::find_tile, ~1 us, while TMEM and barriers are set up); the grid is the most
 // tiles that the sizes allow, and CTAs without a tile leave at once.
@@ -23,28 +20,9 @@ using namespace gemm3x;
 
 namespace {
 
-constexpr int BM = 128, BK = 16;
+constexpr int BM = 128;
 constexpr int CONV_WARPS = 8;
 constexpr int THREADS = (CONV_WARPS + 2) * 32;
-constexpr int BOX = BK * 128;                             // bytes of one 32 x BK MN-major TMA box
-
-template <int BN> struct Cfg {
-  static constexpr int A_TILE = BM * BK * 4, B_TILE = BN * BK * 4, RAW = A_TILE + B_TILE, STAGE = 2 * RAW;
-  static constexpr int STAGES = (196608 / STAGE) > 8 ? 8 : (196608 / STAGE);
-  static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
-};
-
-struct Grouped {
-  GemmParams g;
-  const int* offsets;
-  const int* only_if;      // null, or a device word: do nothing while it is zero
-  int experts, rows;
-  int units;               // tiles
-  int chunk;               // k-blocks between roundings of the accumulators
-  long long c_stride;      // WEIGHTS: distance of the experts' results
-  int tiles_m;             // WEIGHTS: row tiles of one result
-};
 
 // ---- C[r, :] for the rows of every group ------------------------------------------------------------------------
 // The expert's matrix is the operand with 128 rows (its N output features, whole tiles but the last) and the ragged
@@ -52,9 +30,20 @@ struct Grouped {
 // 30 rows costs 32 columns of accumulator, not 128 lanes.  A tile's columns that belong to the next group are computed
 // (columns of an accumulator are independent) and not stored.  Lane = output feature in TMEM, so the 32 lanes of a warp
 // store 128 consecutive bytes of a row of C whatever its pitch and alignment.
+//
+// ---- C_e = A_e^T B_e over the rows of every group (WEIGHTS) -------------------------------------------------------
+// The same kernel with the columns of B in the lanes (128 consecutive values of a row of C_e) and the columns of A, up
+// to BN of them, in the accumulator's columns: both operands reduce down their columns (MN-major), over the group's
+// rows; rows of the last k-block that belong to the next group are zeroed by the warps that compute the lo tiles.
+// K slices meet in L2 (how long a slice is depends on the group): the CTA that arrives last adds them in order and
+// stores; nobody waits.
 struct RowsArgs {
   float* C;
   long long ldc;
+  long long c_stride;          // WEIGHTS: distance of the experts' results
+  int cols, tiles_r;           // WEIGHTS: rows of a result (columns of A), tiles of BN of them
+  float* park;                 // WEIGHTS with slices: parked tiles
+  int* arrived;                // and arrival counts, zero between launches
   const float* bias;           // [experts, N] or null
   const int* offsets;
   int* status;
@@ -83,10 +72,10 @@ template <int BN, int BK> struct RowsCfg {
 };
 
 // 32 accumulator columns (rows first .. first + 31 of C) of one output feature per lane
-__device__ __forceinline__ void store_columns(const RowsArgs& p, const uint32_t (&r)[32], int first, int hi, int n, const float* bias,
-                                              float beta, bool last) {
+__device__ __forceinline__ void store_columns(const RowsArgs& p, float* C, const uint32_t (&r)[32], int first, int hi, int n,
+                                              const float* bias, float beta, bool last) {
   if (n >= p.N) return;
-  float* c = p.C + (long long)first * p.ldc + n;
+  float* c = C + (long long)first * p.ldc + n;
   const float b = (bias && last) ? bias[n] : 0.f;
   const int left = hi - first;
   if (beta != 0.f) {
@@ -109,9 +98,9 @@ __device__ __forceinline__ void store_columns(const RowsArgs& p, const uint32_t 
   }
 }
 
-template <int BN, int BK>
+template <int BN, int BK, bool WEIGHTS>
 __global__ void __launch_bounds__(THREADS, RowsCfg<BN, BK>::CTAS)
-expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ RowsArgs p) {
+expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ RowsArgs p) {
   typedef RowsCfg<BN, BK> C;
   constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
   constexpr int W_BOX = BK * 128;                            // bytes of one 32 x BK box of an MN-major matrix
@@ -122,7 +111,7 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   // bars[0..S) full, [S..2S) conv, [2S..3S) empty, [3S] accumulators ready, [3S+1] accumulators read out
   uint32_t* tmem_slot = (uint32_t*)(bars + 3 * STAGES + 2);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  int* where = (int*)(tmem_slot + 2);                        // {found, expert, lo, hi, index}
+  int* where = (int*)(tmem_slot + 2);                        // {found, expert, lo, hi, index}, then a word for arrivals
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (p.only_if && *p.only_if == 0) return;
@@ -158,7 +147,15 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   }
   if (warp == 1) {
     groups::Tile t = {0, 0, 0, 0};
-    const bool found = groups::find_tile(p.offsets, p.experts, p.rows, BN, unit / tiles_n, p.status, t);
+    bool found = true;
+    if (WEIGHTS) {
+      const int rest = unit / tiles_n;
+      t.expert = rest / p.tiles_r;
+      t.index = rest - t.expert * p.tiles_r;
+      groups::group_rows(p.offsets, p.rows, t.expert, p.status, t.lo, t.hi);
+    } else {
+      found = groups::find_tile(p.offsets, p.experts, p.rows, BN, unit / tiles_n, p.status, t);
+    }
     if (lane == 0) { where[0] = found; where[1] = t.expert; where[2] = t.lo; where[3] = t.hi; where[4] = t.index; }
   }
   tc_fence_before();
@@ -170,13 +167,19 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     if (warp == CONV_WARPS + 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
     return;
   }
-  const int expert = where[1], hi = where[3], t0 = where[2] + where[4] * BN;
-  const int cols = min(BN, hi - t0);                         // rows of C in this tile = accumulator columns
-  const int boxes = (cols + C::BOX_ROWS - 1) / C::BOX_ROWS;
-  const int raw_bytes = A_TILE + boxes * C::BOX_ROWS * BK * 4;
-  const int nkb_all = (p.K + BK - 1) / BK;
+  // rows t0 .. hi - 1 of C (of C_e) belong to this tile, as far as its columns go
+  const int expert = where[1], g_lo = where[2], g_hi = where[3];
+  const int t0 = WEIGHTS ? where[4] * BN : g_lo + where[4] * BN, hi = WEIGHTS ? p.cols : g_hi;
+  const int cols = min(BN, hi - t0);                         // accumulator columns
+  const int boxes = WEIGHTS ? (cols + 31) / 32 : (cols + C::BOX_ROWS - 1) / C::BOX_ROWS;
+  const int raw_bytes = A_TILE + boxes * (WEIGHTS ? W_BOX : C::BOX_ROWS * BK * 4);
+  float* const out = WEIGHTS ? p.C + expert * p.c_stride : p.C;
+  const int nkb_all = ((WEIGHTS ? g_hi - g_lo : p.K) + BK - 1) / BK;
   const int kb_begin = (int)((long long)nkb_all * slice / p.slices);
-  const int nkb = (int)((long long)nkb_all * (slice + 1) / p.slices) - kb_begin;
+  int nkb = (int)((long long)nkb_all * (slice + 1) / p.slices) - kb_begin;
+  // an empty reduction (a group without rows, a slice without k-blocks): one k-block of zeros
+  const bool empty = WEIGHTS && nkb == 0;
+  if (empty) nkb = 1;
   const int n_chunks = (nkb + C::CHUNK - 1) / C::CHUNK, per = (nkb + n_chunks - 1) / n_chunks;
   const int run = max((per + C::MAINS - 1) / C::MAINS, 256 / BK);              // k-blocks into one main accumulator
   const float* bias = p.bias ? p.bias + (long long)expert * p.N : nullptr;
@@ -193,13 +196,18 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
       const int k0 = (kb_begin + i) * BK;
       if (!withhold && elect_one()) {
         mbar_arrive_expect_tx(full, (uint32_t)raw_bytes);
-        if (!p.w_mn) {
+        if (WEIGHTS) {
+#pragma unroll
+          for (int j = 0; j < BM / 32; ++j) tma_load_2d(w_dst + j * W_BOX, &tmW, n0 + 32 * j, g_lo + k0, full);
+          for (int j = 0; j < boxes; ++j) tma_load_2d(x_dst + j * W_BOX, &tmX, t0 + 32 * j, g_lo + k0, full);
+        } else if (!p.w_mn) {
           tma_load_3d(w_dst, &tmW, k0, n0, expert, full);
         } else {
 #pragma unroll
           for (int j = 0; j < BM / 32; ++j) tma_load_3d(w_dst + j * W_BOX, &tmW, n0 + 32 * j, k0, expert, full);
         }
-        for (int j = 0; j < boxes; ++j) tma_load_2d(x_dst + j * C::BOX_ROWS * BK * 4, &tmX, k0, t0 + j * C::BOX_ROWS, full);
+        if (!WEIGHTS)
+          for (int j = 0; j < boxes; ++j) tma_load_2d(x_dst + j * C::BOX_ROWS * BK * 4, &tmX, k0, t0 + j * C::BOX_ROWS, full);
       }
       if (!withhold) issued = i + 1;
       if (++s == STAGES) { s = 0; ph ^= 1; }
@@ -213,13 +221,15 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
   } else if (warp == CONV_WARPS + 1) {
     // ------------------------------ MMA issuer --------------------------------
     if (MMA_WHOLE || lane == 0) {
-      const uint32_t idesc = make_idesc_tf32(BM, (cols + 15) / 16 * 16, p.w_mn, 0);
+      const bool a_mn = WEIGHTS || p.w_mn;
+      const uint32_t idesc = make_idesc_tf32(BM, (cols + 15) / 16 * 16, a_mn, WEIGHTS);
       constexpr uint32_t K_SWZ = BK == 32 ? SWZ_128B : SWZ_64B, K_SBO = 8 * BK * 4;
-      const uint32_t a_step = (p.w_mn ? 1024u : 32u) >> 4;
-      constexpr uint32_t b_step = 32u >> 4;
+      const uint32_t a_step = (a_mn ? 1024u : 32u) >> 4;
+      constexpr uint32_t b_step = (WEIGHTS ? 1024u : 32u) >> 4;
       const uint32_t tmem_cross = tmem_base + C::MAINS * BN;
-      const uint64_t d_a = p.w_mn ? make_smem_desc(smem_base, W_BOX, 512, SWZ_128B_BASE32B) : make_smem_desc(smem_base, 16, K_SBO, K_SWZ);
-      const uint64_t d_b = make_smem_desc(smem_base + A_TILE, 16, K_SBO, K_SWZ);
+      const uint64_t d_a = a_mn ? make_smem_desc(smem_base, W_BOX, 512, SWZ_128B_BASE32B) : make_smem_desc(smem_base, 16, K_SBO, K_SWZ);
+      const uint64_t d_b = WEIGHTS ? make_smem_desc(smem_base + A_TILE, W_BOX, 512, SWZ_128B_BASE32B)
+                                   : make_smem_desc(smem_base + A_TILE, 16, K_SBO, K_SWZ);
       const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
       const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
       constexpr uint32_t LO_TILE = C::RAW >> 4, STAGE_STEP = C::STAGE >> 4;
@@ -289,6 +299,15 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
           *reinterpret_cast<float4*>(low + off) = l;
         };
         constexpr int PASS = CONV_WARPS * 32 * 16;
+        if (WEIGHTS) {
+          const int valid = empty ? 0 : g_hi - g_lo - (kb_begin + i) * BK;       // rows of this k-block inside the group
+          if (valid < BK) {
+            // (the 16-byte pieces that this thread reads itself below; a k row is 128 bytes of every box)
+#pragma unroll 1
+            for (int off = tid * 16; off < raw_bytes; off += PASS)
+              if (((off & (W_BOX - 1)) >> 7) >= valid) *reinterpret_cast<float4*>(raw + off) = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
         if (raw_bytes == C::RAW) {
 #pragma unroll
           for (int k = 0; k < C::RAW / PASS; ++k) split(tid * 16 + k * PASS);
@@ -322,7 +341,19 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
         }
-        if (p.slices > 1) {
+        if (WEIGHTS && p.slices > 1) {
+          float4* slot = reinterpret_cast<float4*>(p.park + ((long long)unit * p.slices + slice) * (BM * BN)) + (q * 32 + lane);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            float4* to = slot + (cc * 8 + (j >> 2)) * 128;
+            float4 v = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
+            if (c > 0) {                                     // the slice's earlier chunks: this thread's own values
+              const float4 o = __ldcg(to);
+              v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+            }
+            __stcg(to, v);
+          }
+        } else if (p.slices > 1) {
           // parked in this CTA's own shared memory ([columns / 4][128 lanes] float4); one chunk only, so the stages are free
           float4* slot = reinterpret_cast<float4*>(smem) + (q * 32 + lane);
 #pragma unroll
@@ -330,7 +361,7 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             slot[(cc * 8 + (j >> 2)) * 128] = make_float4(__uint_as_float(r[j]), __uint_as_float(r[j + 1]), __uint_as_float(r[j + 2]),
                                                           __uint_as_float(r[j + 3]));
         } else {
-          store_columns(p, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, c == 0 ? p.beta : 1.f, last);
+          store_columns(p, out, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, c == 0 ? p.beta : 1.f, last);
         }
       }
       if (!last) {
@@ -339,11 +370,42 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         if (lane == 0) mbar_arrive(bar_read);
       }
     }
+    if (WEIGHTS && p.slices > 1) {
+      if (ok) __threadfence();
+      asm volatile("bar.sync 1, %0;" ::"n"(CONV_WARPS * 32) : "memory");
+      if (threadIdx.x == 0) where[5] = *abort_flag ? -1 : atomicAdd(p.arrived + unit, 1);
+      asm volatile("bar.sync 1, %0;" ::"n"(CONV_WARPS * 32) : "memory");
+      if (where[5] == p.slices - 1) {
+        __threadfence();
+#pragma unroll 1
+        for (int cc = half; cc * 32 < cols; cc += 2) {
+          const float4* from = reinterpret_cast<const float4*>(p.park + (long long)unit * p.slices * (BM * BN)) + (cc * 8 * 128 + q * 32 + lane);
+          float4 a[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[j] = __ldcg(from + j * 128);
+          for (int sl = 1; sl < p.slices; ++sl) {
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __ldcg(from + (long long)sl * (BM * BN / 4) + j * 128);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { a[j].x += v[j].x; a[j].y += v[j].y; a[j].z += v[j].z; a[j].w += v[j].w; }
+          }
+          uint32_t r[32];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            r[4 * j] = __float_as_uint(a[j].x); r[4 * j + 1] = __float_as_uint(a[j].y);
+            r[4 * j + 2] = __float_as_uint(a[j].z); r[4 * j + 3] = __float_as_uint(a[j].w);
+          }
+          store_columns(p, out, r, t0 + cc * 32, hi, n0 + q * 32 + lane, nullptr, p.beta, true);
+        }
+        if (threadIdx.x == 0) p.arrived[unit] = 0;           // left zero for the next launch
+      }
+    }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (p.slices > 1) {
+  if (!WEIGHTS && p.slices > 1) {
     // Every thread of every CTA takes both barriers.  Between them the tile's 32 x 32 pieces are dealt round the cluster's
     // CTAs and warps, each summed in slice order whoever does it.
     cluster_sync_all();
@@ -369,250 +431,12 @@ expert_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
           r[4 * j] = __float_as_uint(a[j].x); r[4 * j + 1] = __float_as_uint(a[j].y);
           r[4 * j + 2] = __float_as_uint(a[j].z); r[4 * j + 3] = __float_as_uint(a[j].w);
         }
-        store_columns(p, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, p.beta, true);
+        store_columns(p, out, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, p.beta, true);
       }
     }
     cluster_sync_all();
   }
   const bool more = unit + (int)gridDim.x / p.slices < p.units && !*abort_flag;
-  __syncthreads();
-  if (!more) {
-    if (warp == CONV_WARPS + 1) {
-      tc_fence_after();
-      tmem_dealloc(tmem_base, C::TMEM_COLS);
-    }
-    return;
-  }
-  if (threadIdx.x == 0)
-    for (int s = 0; s < 3 * STAGES + 2; ++s) mbar_inval(bar_full + 8 * s);
-  }
-}
-
-// ---- C_e = A_e^T B_e over the rows of every group ------------------------------------------------------------------
-template <int BN>
-__global__ void __launch_bounds__(THREADS, 1)
-expert_weights_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const __grid_constant__ Grouped args) {
-  typedef Cfg<BN> C;
-  constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
-  constexpr bool MMA_WHOLE = BN < 256;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* bars = (uint64_t*)(smem + STAGES * C::STAGE);
-  // bars[0..S) full, [S..2S) conv, [2S..3S) empty, [3S] accumulators ready, [3S+1] accumulators read out
-  uint32_t* tmem_slot = (uint32_t*)(bars + 3 * STAGES + 2);
-  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  int* where = (int*)(tmem_slot + 3);                      // {found, expert, lo, hi, index}
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (args.only_if && *args.only_if == 0) return;
-  const int tiles_n = (args.g.N + BN - 1) / BN;
-  const int first_unit = (int)blockIdx.x / args.g.ksplit_n, k_slice = (int)blockIdx.x - first_unit * args.g.ksplit_n;
-
-  const uint32_t smem_base = smem_u32(smem);
-  const uint32_t bar_full = smem_u32(bars), bar_conv = smem_u32(bars + STAGES), bar_empty = smem_u32(bars + 2 * STAGES),
-                 bar_acc = smem_u32(bars + 3 * STAGES), bar_read = bar_acc + 8;
-  if (warp == CONV_WARPS + 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
-    tmem_relinquish();
-  }
-  if (warp == CONV_WARPS && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
-  }
-  int inject = 0;
-  if (warp == CONV_WARPS) inject = args.g.status[3];
-  // One tile per CTA; a guarded launch (only_if) has a small grid whose CTAs take tiles in turn.
-#pragma unroll 1
-  for (int unit = first_unit; unit < args.units; unit += (int)gridDim.x / args.g.ksplit_n) {
-  GemmParams p = args.g;
-  const int n0 = (unit % tiles_n) * BN;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
-      mbar_init(bar_conv + 8 * s, CONV_WARPS);
-      mbar_init(bar_empty + 8 * s, 1);
-    }
-    mbar_init(bar_acc, 1);
-    mbar_init(bar_read, CONV_WARPS);
-    *abort_flag = 0;
-    mbar_fence_init();
-  }
-  if (warp == 1) {
-    groups::Tile t = {0, 0, 0, 0};
-    const int m_tile = unit / tiles_n;
-    t.expert = m_tile / args.tiles_m;
-    t.index = m_tile - t.expert * args.tiles_m;
-    groups::group_rows(args.offsets, args.rows, t.expert, p.status, t.lo, t.hi);
-    if (lane == 0) { where[0] = t.expert; where[1] = t.lo; where[2] = t.hi; where[3] = t.index; }
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  const int lo = where[1], hi = where[2], m0 = where[3] * BM;
-  p.C += where[0] * args.c_stride;
-  const int nkb_all = (hi - lo + BK - 1) / BK;
-  const int kb_begin = (int)((long long)nkb_all * k_slice / p.ksplit_n);
-  int nkb = (int)((long long)nkb_all * (k_slice + 1) / p.ksplit_n) - kb_begin;
-  // an empty reduction (a group without rows, a slice without k-blocks): one k-block of zeros
-  const bool empty = nkb == 0;
-  if (empty) nkb = 1;
-  const int n_chunks = (nkb + args.chunk - 1) / args.chunk, per = (nkb + n_chunks - 1) / n_chunks;
-
-  if (warp == CONV_WARPS) {
-    // ------------------------------ TMA producer ------------------------------
-    {
-      int issued = 0, s = 0;
-      uint32_t ph = 0;
-      const bool withhold = (inject & 1) != 0;              // host-injected fault: arm nothing, load nothing
-      for (int i = 0; i < nkb; ++i) {
-        if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 100 + s)) break;
-        const uint32_t full = bar_full + 8 * s;
-        const uint32_t a_dst = smem_base + s * C::STAGE, b_dst = a_dst + A_TILE;
-        const int k0 = (kb_begin + i) * BK;
-        if (withhold) {
-          if (++s == STAGES) { s = 0; ph ^= 1; }
-          continue;
-        }
-        if (elect_one()) {
-          mbar_arrive_expect_tx(full, C::RAW);
-#pragma unroll
-          for (int j = 0; j < BM / 32; ++j) tma_load_2d(a_dst + j * BOX, &tmA, m0 + 32 * j, lo + k0, full);
-#pragma unroll
-          for (int j = 0; j < BN / 32; ++j) tma_load_2d(b_dst + j * BOX, &tmB, n0 + 32 * j, lo + k0, full);
-        }
-        issued = i + 1;
-        if (++s == STAGES) { s = 0; ph ^= 1; }
-      }
-      if (*abort_flag) {
-        for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
-          for (int it = 0; it < (1 << 16); ++it)
-            if (mbar_try_wait(bar_full + 8 * (i % STAGES), (i / STAGES) & 1)) break;
-      }
-    }
-  } else if (warp == CONV_WARPS + 1) {
-    // ------------------------------ MMA issuer --------------------------------
-    if (MMA_WHOLE || lane == 0) {
-      // both operands MN-major: 32-element blocks one TMA box apart, 4-k-row atoms 512 B apart, 1024 B per k-step
-      const uint32_t idesc = make_idesc_tf32(BM, BN, 1, 1);
-      constexpr uint32_t STEP = 1024u >> 4;
-      const uint32_t tmem_main = tmem_base, tmem_cross = tmem_base + BN;
-      const uint64_t d_a = make_smem_desc(smem_base, BOX, 512, SWZ_128B_BASE32B);
-      const uint64_t d_b = make_smem_desc(smem_base + A_TILE, BOX, 512, SWZ_128B_BASE32B);
-      const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
-      const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
-      constexpr uint32_t LO_TILE = C::RAW >> 4, STAGE_STEP = C::STAGE >> 4;
-      uint32_t accumulate = 0, ph = 0, stage_off = 0, rph = 0;
-      int s = 0, in_chunk = 0;
-      int commits = 0;
-      for (int i = 0; i < nkb; ++i) {
-        if (in_chunk == per) {
-          // the chunk's sums go out before its accumulators are overwritten
-          if (!MMA_WHOLE || elect_one()) mma_commit(bar_acc);
-          if (MMA_WHOLE) __syncwarp();
-          ++commits;
-          if (!mbar_wait(bar_read, rph, abort_flag, p.status, 250)) break;
-          rph ^= 1;
-          tc_fence_after();
-          in_chunk = 0;
-          accumulate = 0;
-        }
-        ++in_chunk;
-        if (!mbar_wait(bar_conv + 8 * s, ph, abort_flag, p.status, 200 + s)) break;
-        tc_fence_after();
-        if (!MMA_WHOLE || elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < BK / 8; ++kk) {
-            const uint32_t al = a_low0 + stage_off + kk * STEP, bl = b_low0 + stage_off + kk * STEP;
-            mma_tf32_ss_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
-            mma_tf32_ss_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
-            mma_tf32_ss_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
-          }
-          mma_commit(bar_empty + 8 * s);
-        }
-        accumulate = 1;
-        if (MMA_WHOLE) __syncwarp();
-        if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
-      }
-      if (!MMA_WHOLE || elect_one()) mma_commit(bar_acc);
-      if (MMA_WHOLE) __syncwarp();
-      if (*abort_flag) {
-        // every MMA issued must have retired before TMEM is freed: the phase of the commit above
-        for (int it = 0; it < (1 << 16); ++it)
-          if (mbar_try_wait(bar_acc, (uint32_t)(commits & 1))) break;
-      }
-    }
-  } else {
-    // ------------------- hi / lo split, then epilogue (warps 0-7) ---------------
-    const int tid = threadIdx.x;
-    bool ok = true;
-    int i = 0;
-    for (int c = 0; ok && c < n_chunks; ++c) {
-      const int end = min(nkb, (c + 1) * per);
-      for (; i < end; ++i) {
-        const int s = i % STAGES, ph = (i / STAGES) & 1;
-        if (!mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 300 + s)) { ok = false; break; }
-        uint8_t* raw = smem + s * C::STAGE;
-        uint8_t* low = raw + C::RAW;
-        const int valid = empty ? 0 : hi - lo - (kb_begin + i) * BK;      // rows of this k-block inside the group
-        if (valid < BK) {
-#pragma unroll 1
-          for (int off = tid * 16; off < C::RAW; off += CONV_WARPS * 32 * 16)
-            if (((off & (BOX - 1)) >> 7) >= valid) *reinterpret_cast<float4*>(raw + off) = make_float4(0.f, 0.f, 0.f, 0.f);
-          // every thread zeroed 16-byte pieces that it reads itself below
-        }
-#pragma unroll
-        for (int k = 0; k < C::RAW / 16 / (CONV_WARPS * 32); ++k) {
-          const int off = (tid + k * CONV_WARPS * 32) * 16;
-          const float4 v = *reinterpret_cast<const float4*>(raw + off);
-          float4 l;
-          l.x = lo_part(v.x); l.y = lo_part(v.y); l.z = lo_part(v.z); l.w = lo_part(v.w);
-          *reinterpret_cast<float4*>(low + off) = l;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_conv + 8 * s);
-      }
-      if (ok) ok = mbar_wait(bar_acc, (uint32_t)(c & 1), abort_flag, p.status, 400);
-      ok = __all_sync(0xffffffffu, ok);                      // tcgen05.ld below is warp-collective
-      if (!ok) break;
-      tc_fence_after();
-      const bool last = c + 1 == n_chunks;
-      if (p.ksplit_n > 1) {
-        float* park = p.ksplit_ws + ((long long)unit * p.ksplit_n + k_slice) * (BM * BN);
-        if (c == 0) dump_tile<BN>(p, tmem_base, park, warp, lane);
-        else add_tile<BN>(tmem_base, park, warp, lane);
-      } else {
-        // staging lies in the pipeline stages, which are free only behind the last k-block
-        epilogue_tile<BN>(p, tmem_base, m0, n0, warp, lane, last ? reinterpret_cast<float*>(smem) : nullptr,
-                          c == 0 ? p.beta : 1.f, last, c > 0);
-      }
-      if (!last) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_read);
-      }
-    }
-    if (p.ksplit_n > 1) {
-      // slices parked in L2: the CTA that arrives last sums them in slice order and stores; nobody waits
-      if (ok) __threadfence();
-      asm volatile("bar.sync 1, %0;" ::"n"(CONV_WARPS * 32) : "memory");
-      int* arrived = reinterpret_cast<int*>(tmem_slot + 2);
-      if (threadIdx.x == 0) *arrived = *abort_flag ? -1 : atomicAdd(p.tile_flags + unit, 1);
-      asm volatile("bar.sync 1, %0;" ::"n"(CONV_WARPS * 32) : "memory");
-      if (*arrived == p.ksplit_n - 1) {
-        __threadfence();
-        epilogue_tile<BN>(p, tmem_base, m0, n0, warp, lane, reinterpret_cast<float*>(smem), p.beta, true, false, nullptr,
-                          p.ksplit_ws + (long long)unit * p.ksplit_n * (BM * BN), p.ksplit_n);
-        if (threadIdx.x == 0) p.tile_flags[unit] = 0;        // left zero for the next launch
-      }
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  const bool more = unit + (int)gridDim.x / args.g.ksplit_n < args.units && !*abort_flag;
   __syncthreads();
   if (!more) {
     if (warp == CONV_WARPS + 1) {
@@ -719,20 +543,6 @@ void choose(const cb200_stream* s, long long tiles_m, int N, int nkb, int max_sl
   }
 }
 
-void common(GemmParams& g, cb200_stream* s, float* C, long long ldc, int M, int N, int K, float alpha, float beta, const float* bias,
-            int act) {
-  g.C = C; g.ldc = ldc; g.M = M; g.N = N; g.K = K; g.alpha = alpha; g.beta = beta; g.bias = bias; g.act = act;
-  g.a_mn_major = g.b_mn_major = 0;
-  g.store_mode = STORE_ROW_MAJOR; g.hw = 1; g.flags = 0; g.group_n = 1; g.drain_every = 0; g.C_lo = nullptr;
-  g.k_split = 1; g.split_from = 0; g.partials = nullptr; g.split_block = 1;
-  g.ksplit_n = 1; g.ksplit_cluster = 0; g.ksplit_ws = nullptr; g.tile_flags = nullptr; g.status = s->status_dev;
-  g.n_peers = 0;
-  for (int d = 0; d < MAX_PEERS; ++d) g.peers[d] = nullptr;
-}
-
-// k-blocks between roundings: 1024 values of k, where the truncating additions have shrunk a sum by 7e-6 at most
-constexpr int CHUNK = 1024 / BK;
-
 }  // namespace
 
 // Operands that TMA can address: 16-byte bases, pitches and distances that are multiples of 4 elements.
@@ -747,6 +557,8 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   // how many rows a tile may take: what an even split of the rows over the experts fills
   const long long even = (rows + experts - 1) / experts;
   int BN = s->opt_gemm_tile_n > 0 ? s->opt_gemm_tile_n : (even <= 32 ? 32 : (even <= 64 ? 64 : (even <= 128 ? 128 : 256)));
+  // short reductions are all set-up and stores: narrow tiles, two to an SM, overlap them
+  if (s->opt_gemm_tile_n == 0 && BN > 64 && K <= 128) BN = 64;
   const int bk = BN <= 64 ? 32 : 16;
   const long long tiles = (rows + BN - 1) / BN + (experts < rows ? experts : rows) - 1, units = tiles * ((N + BM - 1) / BM);
   const int nkb = (K + bk - 1) / bk;
@@ -759,7 +571,8 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
     if ((forced > 0 ? sl <= forced : units * sl <= s->sm_count * (BN <= 64 ? 2 : 1)) && nkb / sl >= 4) slices = sl;
   if ((nkb + slices - 1) / slices > chunk || only_if) slices = 1;
   RowsArgs a;
-  a.C = C; a.ldc = ldc; a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
+  a.C = C; a.ldc = ldc; a.c_stride = 0; a.cols = a.tiles_r = 0; a.park = nullptr; a.arrived = nullptr;
+  a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
   a.N = N; a.K = K; a.experts = experts; a.rows = rows; a.w_mn = trans_b ? 0 : 1; a.act = act;
   a.alpha = alpha; a.beta = beta; a.slices = slices; a.only_if = only_if;
   const CUtensorMapSwizzle swz = bk == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -772,41 +585,39 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   CB_REQUIRE(units <= 2147483647LL, "expert_gemm: too many tiles");
   a.units = (int)units;
   const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
-  if (BN == 256) return launch<RowsArgs, expert_rows_kernel<256, 16>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, slices);
-  if (BN == 128) return launch<RowsArgs, expert_rows_kernel<128, 16>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, slices);
-  if (BN == 64) return launch<RowsArgs, expert_rows_kernel<64, 32>>(s, RowsCfg<64, 32>::SMEM, tmW, tmX, a, ctas, slices);
-  return launch<RowsArgs, expert_rows_kernel<32, 32>>(s, RowsCfg<32, 32>::SMEM, tmW, tmX, a, ctas, slices);
+  if (BN == 256) return launch<RowsArgs, expert_tf32x3_kernel<256, 16, false>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, slices);
+  if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, false>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, slices);
+  if (BN == 64) return launch<RowsArgs, expert_tf32x3_kernel<64, 32, false>>(s, RowsCfg<64, 32>::SMEM, tmW, tmX, a, ctas, slices);
+  return launch<RowsArgs, expert_tf32x3_kernel<32, 32, false>>(s, RowsCfg<32, 32>::SMEM, tmW, tmX, a, ctas, slices);
 }
 
 int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
                             int M, long long lda, const float* B, int N, long long ldb, int experts, float beta,
                             const int* offsets, const int* only_if) {
   DeviceGuard guard(s->device);
-  Grouped a;
-  common(a.g, s, C, ldc, M, N, 0, alpha, beta, nullptr, CB200_ACT_NONE);
-  a.g.a_mn_major = a.g.b_mn_major = 1;
-  a.offsets = offsets; a.experts = experts; a.rows = rows; a.chunk = CHUNK; a.c_stride = c_stride; a.only_if = only_if;
-  a.tiles_m = (M + BM - 1) / BM;
-  const long long tiles_m = (long long)a.tiles_m * experts;
+  const long long tiles_l = (N + BM - 1) / BM;
   int BN, slices;
-  choose(s, tiles_m, N, (rows / experts + BK) / BK, only_if ? 1 : 16, BN, slices);
-  a.g.ksplit_n = slices;
-  int rc;
-  const long long units = tiles_m * ((N + BN - 1) / BN);
-  CB_REQUIRE(units <= 2147483647LL, "expert_gemm_weights: too many tiles");
+  choose(s, tiles_l * experts, M, (rows / experts + 16) / 16, only_if ? 1 : 16, BN, slices);
+  RowsArgs a;
+  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.cols = M; a.tiles_r = (M + BN - 1) / BN; a.park = nullptr; a.arrived = nullptr;
+  a.bias = nullptr; a.offsets = offsets; a.status = s->status_dev;
+  a.N = N; a.K = 0; a.experts = experts; a.rows = rows; a.w_mn = 1; a.act = CB200_ACT_NONE;
+  a.alpha = alpha; a.beta = beta; a.slices = slices; a.only_if = only_if;
+  const long long units = tiles_l * a.tiles_r * experts;
+  CB_REQUIRE(units * slices <= 2147483647LL, "expert_gemm_weights: too many tiles");
   a.units = (int)units;
   const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
+  int rc;
   if (slices > 1) {
-    // slices meet in L2: how long a slice is depends on the groups, so it may take several chunks
     void* ws = nullptr;
     if ((rc = cb200_partials(s, (size_t)units * slices * BM * BN * sizeof(float), &ws))) return rc;
-    if ((rc = cb200_tile_flags(s, (size_t)units, &a.g.tile_flags))) return rc;
-    a.g.ksplit_ws = (float*)ws;
+    if ((rc = cb200_tile_flags(s, (size_t)units, &a.arrived))) return rc;
+    a.park = (float*)ws;
   }
-  CUtensorMap tmA, tmB;
-  if ((rc = tmap_2d(&tmA, A, rows, M, lda, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
-  if ((rc = tmap_2d(&tmB, B, rows, N, ldb, 32, BK, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
-  if (BN == 256) return launch<Grouped, expert_weights_kernel<256>>(s, Cfg<256>::SMEM, tmA, tmB, a, ctas, 1);
-  if (BN == 128) return launch<Grouped, expert_weights_kernel<128>>(s, Cfg<128>::SMEM, tmA, tmB, a, ctas, 1);
-  return launch<Grouped, expert_weights_kernel<64>>(s, Cfg<64>::SMEM, tmA, tmB, a, ctas, 1);
+  CUtensorMap tmW, tmX;
+  if ((rc = tmap_2d(&tmW, B, rows, N, ldb, 32, 16, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
+  if ((rc = tmap_2d(&tmX, A, rows, M, lda, 32, 16, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
+  if (BN == 256) return launch<RowsArgs, expert_tf32x3_kernel<256, 16, true>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, 1);
+  if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, true>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1);
+  return launch<RowsArgs, expert_tf32x3_kernel<64, 16, true>>(s, RowsCfg<64, 16>::SMEM, tmW, tmX, a, ctas, 1);
 }

@@ -132,32 +132,6 @@ __device__ __forceinline__ void dump_tile(const GemmParams& p, uint32_t tmem_bas
   }
 }
 
-// Round this CTA's accumulators to nearest onto a tile that dump_tile parked earlier (the same thread's values).
-template <int BN>
-__device__ __forceinline__ void add_tile(uint32_t tmem_base, float* dst, int warp, int lane) {
-  const int q = warp & 3, half = warp >> 2;
-  constexpr int COLS_PER_HALF = BN / 2;
-  float4* slot = reinterpret_cast<float4*>(dst) + (q * 32 + lane);
-#pragma unroll 1
-  for (int cc = 0; cc < COLS_PER_HALF / 32; ++cc) {
-    const int col0 = half * COLS_PER_HALF + cc * 32;
-    uint32_t r[32], rc[32];
-    tmem_ld_32x32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)col0, r);
-    tmem_ld_32x32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(BN + col0), rc);
-    tmem_ld_wait();
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      float4* to = slot + ((col0 + j) >> 2) * 128;
-      float4 v = __ldcg(to);
-      v.x += __uint_as_float(r[j]) + __uint_as_float(rc[j]);
-      v.y += __uint_as_float(r[j + 1]) + __uint_as_float(rc[j + 1]);
-      v.z += __uint_as_float(r[j + 2]) + __uint_as_float(rc[j + 2]);
-      v.w += __uint_as_float(r[j + 3]) + __uint_as_float(rc[j + 3]);
-      __stcg(to, v);
-    }
-  }
-}
-
 // The same parked tile ([BN / 4][128 rows] float4) in this CTA's own shared memory: the cluster form of the hand-over.
 template <int BN>
 __device__ __forceinline__ void dump_tile_smem(const GemmParams& p, uint32_t tmem_base, float* dst, int warp, int lane) {
