@@ -118,8 +118,8 @@ template <> struct Tile64<double> {
   __device__ __forceinline__ void run(const double* a, long long sam, long long sak, const double* b, long long sbk, long long sbn, int m_left,
                                       int n_left, int K) {
     constexpr int LD = 68;
-    __shared__ double As[16][LD];
-    __shared__ double Bs[16][LD];
+    __shared__ double As2[2][16][LD];
+    __shared__ double Bs2[2][16][LD];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, wm = (warp >> 2) * 32, wn = (warp & 3) * 16, fr = lane >> 2, fk = lane & 3;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -140,7 +140,11 @@ template <> struct Tile64<double> {
       }
     };
     if (K > 0) load(0);
+    __syncthreads();                                         // (the tile before has been read)
     for (int k0 = 0; k0 < K; k0 += 16) {
+      // two buffers in turn: one barrier per step
+      double (&As)[16][LD] = As2[(k0 >> 4) & 1];
+      double (&Bs)[16][LD] = Bs2[(k0 >> 4) & 1];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (sak == 1) As[t % 16][t / 16 + 16 * i] = ra[i]; else As[t / 64 + 4 * i][t % 64] = ra[i];
@@ -172,7 +176,6 @@ template <> struct Tile64<double> {
                          : "+d"(acc[i][j][0]), "+d"(acc[i][j][1]), "+d"(acc[i][j][2]), "+d"(acc[i][j][3])
                          : "d"(x[i][0]), "d"(x[i][1]), "d"(x[i][2]), "d"(x[i][3]), "d"(y[j][0]), "d"(y[j][1]));
       }
-      __syncthreads();
     }
   }
   __device__ __forceinline__ void store(double* c, long long ldc, int m_left, int n_left, double alpha, double beta, const double* bias, int act) {
