@@ -383,6 +383,108 @@ __global__ void __launch_bounds__(1024) expert_bias_gradient_kernel(Product<T> p
   *to = o;
 }
 
+// ---- weight gradients of few rows per expert: the results are written once, as fast as memory takes them --------------
+// A warp has 8 rows of C_e (columns of A) and 128 columns, four to a lane: V of them adjacent where B and C take 16-byte
+// accesses, else 32 apart, so that a warp's stores are whole lines whatever the pitch.  The group's rows are added in order with
+// FMAs; A's values are the same for all lanes.  The CTAs of the first columns add up the bias gradient beside.
+constexpr int FEW_M = 8;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256, sizeof(T) == 8 ? 2 : (V == 1 ? 3 : 4)) expert_few_weights_kernel(Product<T> p, int tiles_m) {
+  constexpr int PACKS = 4 / V;
+  struct alignas(sizeof(T) * V) Pack { T e[V]; };
+  __shared__ int bounds[2];
+  const int e = (int)blockIdx.z, lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+  if (warp == 0) {
+    int a, b;
+    groups::group_rows(p.offsets, p.rows, e, p.status, a, b);
+    if (lane == 0) { bounds[0] = a; bounds[1] = b; }
+  }
+  __syncthreads();
+  const int lo = bounds[0], hi = bounds[1];
+  const long long n0 = (long long)blockIdx.x * 128 + lane * V;
+  for (int tm = (int)blockIdx.y; tm < tiles_m; tm += (int)gridDim.y) {
+    const int m0 = tm * (8 * FEW_M) + warp * FEW_M, m_left = p.M - m0;
+    if (m_left <= 0) return;
+    T acc[FEW_M][PACKS * V], sum[FEW_M];
+#pragma unroll
+    for (int i = 0; i < FEW_M; ++i) {
+      sum[i] = (T)0;
+#pragma unroll
+      for (int j = 0; j < PACKS * V; ++j) acc[i][j] = (T)0;
+    }
+    const T* a = p.A + m0;
+#pragma unroll 2
+    for (int r = lo; r < hi; ++r) {
+      Pack b[PACKS];
+      T x[FEW_M];
+#pragma unroll
+      for (int j = 0; j < PACKS; ++j) {
+        const long long n = n0 + j * 32 * V;
+        if (n < p.N) b[j] = *reinterpret_cast<const Pack*>(p.B + (long long)r * p.ldb + n);      // V > 1: N is a multiple of V
+        else
+#pragma unroll
+          for (int v = 0; v < V; ++v) b[j].e[v] = (T)0;
+      }
+#pragma unroll
+      for (int i = 0; i < FEW_M; i += V) {                   // (V > 1: M is a multiple of V; stores are bounded below)
+        const Pack from = *reinterpret_cast<const Pack*>(a + (long long)r * p.lda + (i < m_left ? i : 0));
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[i + v] = from.e[v];
+      }
+#pragma unroll
+      for (int i = 0; i < FEW_M; ++i) {
+        sum[i] += x[i];
+#pragma unroll
+        for (int j = 0; j < PACKS; ++j)
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[i][j * V + v] += x[i] * b[j].e[v];
+      }
+    }
+    T* c = p.C + e * p.c_stride + (long long)m0 * p.ldc;
+#pragma unroll
+    for (int i = 0; i < FEW_M; ++i) {
+      if (i >= m_left) break;
+#pragma unroll
+      for (int j = 0; j < PACKS; ++j) {
+        const long long n = n0 + j * 32 * V;
+        if (n >= p.N) continue;
+        Pack* to = reinterpret_cast<Pack*>(c + (long long)i * p.ldc + n);
+        Pack o;
+        if (p.beta != (T)0) o = *to;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o.e[v] = p.beta != (T)0 ? p.alpha * acc[i][j * V + v] + p.beta * o.e[v] : p.alpha * acc[i][j * V + v];
+        *to = o;
+      }
+      if (p.bias_g && blockIdx.x == 0 && lane == 0) {
+        T* to = p.bias_g + (long long)e * p.M + m0 + i;
+        *to = p.beta != (T)0 ? p.alpha * sum[i] + p.beta * *to : p.alpha * sum[i];
+      }
+    }
+  }
+}
+
+// Measured, this kernel / the tile kernels: 8 experts of 1024 x 4096 (134 MB, 20 us) with 1, 8, 16, 24 rows each 27, 53, 84,
+// 115 / 111, 113, 115, 119 us; 3 of 1506 x 1291 (operands that TMA cannot address) 10, 19, 31, 43 / 41, 41, 42, 43 us;
+// doubles, 8 of 1024 x 4096 with 1, 8, 16 rows 49, 101, 159 / 106, 118, 135 us.  The limit on all rows is for routings that
+// send everything to one expert, whose few CTAs then walk all of them one after another.
+template <typename T> bool few_weights_ok(const Product<T>& p) {
+  return p.rows <= (sizeof(T) == 4 ? 16LL : 8LL) * p.experts && p.rows <= 512;
+}
+
+template <typename T> int run_few_weights(cb200_stream* s, const Product<T>& p) {
+  DeviceGuard guard(s->device);
+  constexpr int V = 16 / sizeof(T);
+  const int tiles_m = (p.M + 8 * FEW_M - 1) / (8 * FEW_M);
+  const dim3 grid((unsigned)((p.N + 127) / 128), (unsigned)(tiles_m < 65535 ? tiles_m : 65535), (unsigned)p.experts);
+  const bool wide = (((uintptr_t)p.A | (uintptr_t)p.B | (uintptr_t)p.C) & 15) == 0 && p.M % V == 0 && p.N % V == 0 && p.lda % V == 0 &&
+                    p.ldb % V == 0 && p.ldc % V == 0 && p.c_stride % V == 0;
+  if (wide) expert_few_weights_kernel<T, V><<<grid, 256, 0, s->stream>>>(p, tiles_m);
+  else expert_few_weights_kernel<T, 1><<<grid, 256, 0, s->stream>>>(p, tiles_m);
+  CB_LAUNCH_CHECK(s);
+  return CB200_OK;
+}
+
 template <typename T> int run_bias_gradient(cb200_stream* s, const Product<T>& p) {
   constexpr int V = 16 / sizeof(T);
   if (((uintptr_t)p.A & 15) == 0 && p.lda % V == 0 && p.M % V == 0)
@@ -412,23 +514,37 @@ template <typename T> int run_weights(cb200_stream* s, const Product<T>& p) {
 }
 
 // ---- fp32: the tensor-core kernels, behind a copy of operands that TMA cannot address -----------------------------------
-__global__ void __launch_bounds__(256) pack_rows_kernel(float* dst, long long ld_dst, const float* src, long long ld, long long stride,
-                                                        long long rows_per, long long rows, int cols) {
-  const long long total = rows * ld_dst;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long r = i / ld_dst;
-    const int c = (int)(i - r * ld_dst);
-    if (c < cols) dst[i] = src[(r / rows_per) * stride + (r % rows_per) * ld + c];
+// A warp (eight lanes where rows are short) takes a row at a time; blockIdx.y is the matrix.
+template <int LANES>
+__global__ void __launch_bounds__(256) pack_rows_kernel(float* __restrict__ dst, long long ld_dst, const float* __restrict__ src,
+                                                        long long ld, long long stride, long long rows, int cols) {
+  const int sub = (int)threadIdx.x % LANES;
+  src += (long long)blockIdx.y * stride;
+  dst += (long long)blockIdx.y * rows * ld_dst;
+  for (long long r = (long long)blockIdx.x * (256 / LANES) + (int)threadIdx.x / LANES; r < rows; r += (long long)gridDim.x * (256 / LANES)) {
+    const float* from = src + r * ld;
+    float* to = dst + r * ld_dst;
+    for (int c = sub; c < cols; c += 8 * LANES) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j * LANES < cols) v[j] = from[c + j * LANES];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j * LANES < cols) to[c + j * LANES] = v[j];
+    }
   }
 }
 
-// rows x cols (rows_per of them per matrix, matrices `stride` apart) into dense rows of a multiple of 4
-int pack(cb200_stream* s, float* dst, const float* src, long long ld, long long stride, long long rows_per, long long rows, int cols) {
+// `matrices` of rows x cols, `stride` apart, into dense rows of a multiple of 4 (32 x 2894 x 226, 168 MB read
+// and written: 24 us, all eight loads of a lane's turn in flight)
+int pack(cb200_stream* s, float* dst, const float* src, long long ld, long long stride, int matrices, long long rows, int cols) {
+  const int lanes = cols <= 64 ? 8 : 32;
+  const long long need = (rows + 256 / lanes - 1) / (256 / lanes), cap = ((long long)s->sm_count * 32 + matrices - 1) / matrices;
+  const dim3 grid((unsigned)(need < cap ? need : cap), (unsigned)matrices);
   const long long ld_dst = (cols + 3) / 4 * 4;
-  long long blocks = (rows * ld_dst + 1023) / 1024;
-  const long long cap = (long long)s->sm_count * 16;
-  if (blocks > cap) blocks = cap;
-  pack_rows_kernel<<<(unsigned)blocks, 256, 0, s->stream>>>(dst, ld_dst, src, ld, stride, rows_per, rows, cols);
+  if (lanes == 8) pack_rows_kernel<8><<<grid, 256, 0, s->stream>>>(dst, ld_dst, src, ld, stride, rows, cols);
+  else pack_rows_kernel<32><<<grid, 256, 0, s->stream>>>(dst, ld_dst, src, ld, stride, rows, cols);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
@@ -455,11 +571,11 @@ int rows_tc(cb200_stream* s, Product<float> p) {
     float* a = (float*)ws;
     float* b = a + a_n;
     if (pack_a) {
-      if ((rc = pack(s, a, p.A, p.lda, 0, p.rows, p.rows, p.K))) return rc;
+      if ((rc = pack(s, a, p.A, p.lda, 0, 1, p.rows, p.K))) return rc;
       p.A = a; p.lda = lda;
     }
     if (pack_b) {
-      if ((rc = pack(s, b, p.B, p.ldb, p.b_stride, b_rows, p.experts * b_rows, b_cols))) return rc;
+      if ((rc = pack(s, b, p.B, p.ldb, p.b_stride, p.experts, b_rows, b_cols))) return rc;
       p.B = b; p.ldb = ldb; p.b_stride = b_rows * ldb;
     }
   }
@@ -468,6 +584,7 @@ int rows_tc(cb200_stream* s, Product<float> p) {
 }
 
 int weights_tc(cb200_stream* s, Product<float> p) {
+  if (few_weights_ok(p) && s->opt_gemm_auto_presplit != 2 && s->opt_gemm_tile_n == 0) return run_few_weights<float>(s, p);
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
   const bool halves = cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts);
   if (!halves && p.bias_g) {
@@ -491,11 +608,11 @@ int weights_tc(cb200_stream* s, Product<float> p) {
     float* a = (float*)ws;
     float* b = a + a_n;
     if (pack_a) {
-      if ((rc = pack(s, a, p.A, p.lda, 0, p.rows, p.rows, p.M))) return rc;
+      if ((rc = pack(s, a, p.A, p.lda, 0, 1, p.rows, p.M))) return rc;
       p.A = a; p.lda = lda;
     }
     if (pack_b) {
-      if ((rc = pack(s, b, p.B, p.ldb, 0, p.rows, p.rows, p.N))) return rc;
+      if ((rc = pack(s, b, p.B, p.ldb, 0, 1, p.rows, p.N))) return rc;
       p.B = b; p.ldb = ldb;
     }
   }
@@ -563,10 +680,11 @@ int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_str
   if (dtype == CB200_FLOAT) {
     const Product<float> p = product<float>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb, beta,
                                             offsets, nullptr, bias_gradient, CB200_ACT_NONE);
-    return rows > 0 ? weights_tc(s, p) : run_weights<float>(s, p);
+    return weights_tc(s, p);
   }
-  return run_weights<double>(s, product<double>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb,
-                                                beta, offsets, nullptr, bias_gradient, CB200_ACT_NONE));
+  const Product<double> p = product<double>(s, C, c_stride, ldc, 0, alpha, A, rows, a_cols, 0, lda, B, experts, b_cols, 0, ldb, beta,
+                                            offsets, nullptr, bias_gradient, CB200_ACT_NONE);
+  return few_weights_ok(p) ? run_few_weights<double>(s, p) : run_weights<double>(s, p);
 }
 
 }  // extern "C"
