@@ -861,15 +861,19 @@ constexpr size_t MOST_WORKSPACE = (size_t)2 << 30;
 
 }  // namespace
 
-// Is this product better off here?  Both sides' times by the sizes, in microseconds: the split reads and writes the operands
-// once.
+// Is this product better off here?  Both sides' times by the sizes, in microseconds (the split reads and writes the operands
+// once).  Measured, here / 3xTF32: 8 experts of 2048 x 1024 with 96, 256, 1024 rows each 56, 75, 122 / 60, 87, 203; 32 of 512 x
+// 512 43, 56, 97 / 41, 53, 119; weight gradients of 8 experts of 1024 x 4096 with 96, 256, 512 rows 81, 107, 164 / 81, 146, 229;
+// 32 of 512 x 512 52, 79, 119 / 48, 72, 134.
 bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
   const double l = (double)experts * N * K, r = (double)rows * K;
   if ((l + r) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * K;
-  const double here = 20.0 + (l + r) * 8 / 5.5e6 + flops / 330e6, there = flops / 130e6;
+  // (halves that do not stay in L2 between the split and the product are read from memory)
+  const double beyond = l + r > 60e6 ? l + r - 60e6 : 0.0;
+  const double here = 25.0 + (l + r) * 1.7e-6 + beyond * 2.3e-6 + flops / 590e6, there = 15.0 + l * 1.7e-6 + flops / 190e6;
   return rows >= 96 * experts && here < there;
 }
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
@@ -877,9 +881,9 @@ bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, l
   const double operands = (double)(rows + BK * experts) * (M + N);
   if (operands * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
-  const double flops = 2.0 * rows * N * M;
-  const double here = 25.0 + operands * 12 / 4.5e6 + flops / 330e6, there = flops / 85e6;
-  return rows >= 64 * experts && here < there;
+  const double flops = 2.0 * rows * N * M, results = (double)experts * N * M;
+  const double here = 28.0 + operands * 1.85e-6 + results * 0.67e-6 + flops / 300e6, there = 12.0 + results * 1e-6 + flops / 150e6;
+  return rows >= 96 * experts && here < there;
 }
 
 // The flag that the guarded 3xTF32 launch reads is returned through `guard`.

@@ -24,6 +24,11 @@ constexpr int BM = 128;
 constexpr int CONV_WARPS = 8;
 constexpr int THREADS = (CONV_WARPS + 2) * 32;
 
+// The whole warp waits, and agrees: lanes that gave up never leave others behind in a warp-wide operation.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, site));
+}
+
 // ---- C[r, :] for the rows of every group ------------------------------------------------------------------------
 // The expert's matrix is the operand with 128 rows (its N output features, whole tiles but the last) and the ragged
 // rows of the group are the other one, up to BN of them: the tensor core takes any multiple of 16 there, so a group of
@@ -71,8 +76,10 @@ template <int BN, int BK> struct RowsCfg {
   static_assert(BM * BN * 4 <= STAGES * STAGE, "a parked tile must fit the pipeline stages");
 };
 
-// 32 accumulator columns (rows first .. first + 31 of C) of one output feature per lane
-__device__ __forceinline__ void store_columns(const RowsArgs& p, float* C, const uint32_t (&r)[32], int first, int hi, int n,
+// 32 accumulator columns (rows first .. first + 31 of C) of one output feature per lane.  No branch between the values: one
+// per value (the activation's) keeps a warp from having more than one in flight (42 cycles a store; a weight gradient of 8
+// experts of 1024 x 4096 with 32 rows each 121 us, 68 without).
+__device__ __forceinline__ void store_columns(const RowsArgs& p, float* C, uint32_t (&r)[32], int first, int hi, int n,
                                               const float* bias, float beta, bool last) {
   if (n >= p.N) return;
   float* c = C + (long long)first * p.ldc + n;
@@ -83,18 +90,25 @@ __device__ __forceinline__ void store_columns(const RowsArgs& p, float* C, const
 #pragma unroll
     for (int j = 0; j < 32; ++j) old[j] = j < left ? c[(long long)j * p.ldc] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      float v = p.alpha * __uint_as_float(r[j]) + beta * old[j] + b;
-      if (last) v = apply_act(v, p.act);
-      if (j < left) c[(long long)j * p.ldc] = v;
-    }
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(p.alpha * __uint_as_float(r[j]) + beta * old[j] + b);
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      float v = p.alpha * __uint_as_float(r[j]) + b;
-      if (last) v = apply_act(v, p.act);
-      if (j < left) c[(long long)j * p.ldc] = v;
-    }
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(p.alpha * __uint_as_float(r[j]) + b);
+  }
+  if (last && p.act == CB200_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(apply_act(__uint_as_float(r[j]), CB200_ACT_RELU));
+  } else if (last && p.act != CB200_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(apply_act(__uint_as_float(r[j]), p.act));
+  }
+  if (left >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) c[(long long)j * p.ldc] = __uint_as_float(r[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < left) c[(long long)j * p.ldc] = __uint_as_float(r[j]);
   }
 }
 
@@ -190,7 +204,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     uint32_t ph = 0;
     const bool withhold = (inject & 1) != 0;                 // host-injected fault: arm nothing, load nothing
     for (int i = 0; i < nkb; ++i) {
-      if (!mbar_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 100 + s)) break;
+      if (!warp_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 100 + s)) break;
       const uint32_t full = bar_full + 8 * s;
       const uint32_t w_dst = smem_base + s * C::STAGE, x_dst = w_dst + A_TILE;
       const int k0 = (kb_begin + i) * BK;
@@ -289,7 +303,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       const int end = min(nkb, (c + 1) * per);
       for (; i < end; ++i) {
         const int s = i % STAGES, ph = (i / STAGES) & 1;
-        if (!mbar_wait(bar_full + 8 * s, ph, abort_flag, p.status, 300 + s)) { ok = false; break; }
+        if (!warp_wait(bar_full + 8 * s, ph, abort_flag, p.status, 300 + s)) { ok = false; break; }
         uint8_t* raw = smem + s * C::STAGE;
         uint8_t* low = raw + C::RAW;
         auto split = [&](int off) {
@@ -320,8 +334,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_conv + 8 * s);
       }
-      if (ok) ok = mbar_wait(bar_acc, (uint32_t)(c & 1), abort_flag, p.status, 400);
-      ok = __all_sync(0xffffffffu, ok);                      // tcgen05.ld below is warp-collective
+      if (ok) ok = warp_wait(bar_acc, (uint32_t)(c & 1), abort_flag, p.status, 400);
       if (!ok) break;
       tc_fence_after();
       const bool last = c + 1 == n_chunks;
@@ -450,6 +463,309 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   }
 }
 
+// ---- many tiles of short reductions -------------------------------------------------------------------------------
+// Where a tile is a few k-blocks, setting up a CTA, filling its pipeline and storing its sums take longer than the products.
+// Here a CTA stays (one to an SM) and takes tiles in turn: the producer finds the next tile, says in a ring which it is and
+// loads on; four more warps store a tile's sums from one set of accumulators while the next tile's go into the other.
+// The arithmetic is that of the kernel above; a chunk of a long reduction is an entry of the ring like a tile.
+constexpr int EPI_WARPS = 4, STREAM_THREADS = (CONV_WARPS + 2 + EPI_WARPS) * 32, RING = 8;
+
+template <int BN, int BK> struct StreamCfg {
+  static constexpr int A_TILE = BM * BK * 4, B_TILE = BN * BK * 4, RAW = A_TILE + B_TILE, STAGE = 2 * RAW;
+  static constexpr int STAGES = (196608 / STAGE) > 8 ? 8 : (196608 / STAGE);
+  static constexpr int MAINS = BN == 128 ? 1 : 3, SET = (MAINS + 1) * BN;      // TMEM columns of a set of accumulators
+  static constexpr int CHUNK = MAINS == 1 ? 1024 / BK : MAINS * 512 / BK;      // k-blocks
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 1024;
+  static_assert(2 * SET == 512, "two sets of accumulators");
+};
+
+struct Entry { int more, expert, g_lo, g_hi, t0, n0, kb_begin, nkb, chunk, last; };
+
+template <int BN, int BK, bool WEIGHTS>
+__global__ void __launch_bounds__(STREAM_THREADS, 1)
+expert_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ RowsArgs p) {
+  typedef StreamCfg<BN, BK> C;
+  constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
+  constexpr int W_BOX = BK * 128;                            // bytes of one 32 x BK box of an MN-major matrix
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = (uint64_t*)(smem + STAGES * C::STAGE);
+  // bars: full, conv, empty [STAGES each]; sums ready, sums read [2 each]; entry written, entry done [RING each]; MMAs retired
+  uint32_t* tmem_slot = (uint32_t*)(bars + 3 * STAGES + 5 + 2 * RING);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  Entry* ring = (Entry*)(tmem_slot + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.only_if && *p.only_if == 0) return;
+  const int tiles_n = (p.N + BM - 1) / BM;
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bar_full = smem_u32(bars), bar_conv = smem_u32(bars + STAGES), bar_empty = smem_u32(bars + 2 * STAGES),
+                 bar_acc = smem_u32(bars + 3 * STAGES), bar_read = bar_acc + 16, bar_entry = bar_read + 16, bar_done = bar_entry + 8 * RING,
+                 bar_retired = bar_done + 8 * RING;
+  if (warp == CONV_WARPS + 1) {
+    tmem_alloc(smem_u32(tmem_slot), 2 * C::SET);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_conv + 8 * s, CONV_WARPS);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_acc + 8 * b, 1);
+      mbar_init(bar_read + 8 * b, EPI_WARPS);
+    }
+    for (int e = 0; e < RING; ++e) {
+      mbar_init(bar_entry + 8 * e, 1);
+      mbar_init(bar_done + 8 * e, EPI_WARPS);
+    }
+    mbar_init(bar_retired, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == CONV_WARPS && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmX);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // columns of the accumulator and bytes of a stage for an entry
+  auto columns = [&](const Entry& e) { return min(BN, (WEIGHTS ? p.cols : e.g_hi) - e.t0); };
+  auto boxes_of = [&](int cols) { return WEIGHTS ? (cols + 31) / 32 : (cols + 63) / 64; };
+  auto bytes_of = [&](int cols) { return A_TILE + boxes_of(cols) * (WEIGHTS ? W_BOX : 64 * BK * 4); };
+
+  if (warp == CONV_WARPS) {
+    // ------------------------------ tiles and TMA -----------------------------
+    const bool withhold = (p.status[3] & 1) != 0;            // host-injected fault: arm nothing, load nothing
+    int issued = 0, s = 0, it = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int unit = (int)blockIdx.x; ok; unit += (int)gridDim.x) {
+      Entry e;
+      e.more = unit < p.units;
+      int chunks = 1, per = 0, nkb = 0;
+      if (e.more) {
+        groups::Tile t = {0, 0, 0, 0};
+        e.n0 = (unit % tiles_n) * BM;
+        if (WEIGHTS) {
+          const int rest = unit / tiles_n;
+          t.expert = rest / p.tiles_r;
+          t.index = rest - t.expert * p.tiles_r;
+          groups::group_rows(p.offsets, p.rows, t.expert, p.status, t.lo, t.hi);
+        } else {
+          e.more = groups::find_tile(p.offsets, p.experts, p.rows, BN, unit / tiles_n, p.status, t);
+        }
+        e.expert = t.expert; e.g_lo = t.lo; e.g_hi = t.hi;
+        e.t0 = WEIGHTS ? t.index * BN : t.lo + t.index * BN;
+        nkb = max(((WEIGHTS ? t.hi - t.lo : p.K) + BK - 1) / BK, 1);           // (a group without rows: a k-block of zeros)
+        chunks = (nkb + C::CHUNK - 1) / C::CHUNK;
+        per = (nkb + chunks - 1) / chunks;
+      }
+      for (int c = 0; c < chunks; ++c, ++it) {
+        const int slot = it % RING;
+        if (!warp_wait(bar_done + 8 * slot, ((it / RING) & 1) ^ 1, abort_flag, p.status, 500 + slot)) { ok = false; break; }
+        e.kb_begin = c * per;
+        e.nkb = min(per, nkb - c * per);
+        e.chunk = c;
+        e.last = c + 1 == chunks;
+        if (lane == 0) {
+          ring[slot] = e;
+          mbar_arrive(bar_entry + 8 * slot);
+        }
+        __syncwarp();
+        if (!e.more) { ok = false; break; }
+        const int boxes = boxes_of(columns(e)), raw_bytes = bytes_of(columns(e));
+        for (int i = 0; i < e.nkb; ++i) {
+          if (!warp_wait(bar_empty + 8 * s, ph ^ 1, abort_flag, p.status, 100 + s)) { ok = false; break; }
+          const uint32_t full = bar_full + 8 * s;
+          const uint32_t w_dst = smem_base + s * C::STAGE, x_dst = w_dst + A_TILE;
+          const int k0 = (e.kb_begin + i) * BK;
+          if (!withhold && elect_one()) {
+            mbar_arrive_expect_tx(full, (uint32_t)raw_bytes);
+            if (WEIGHTS) {
+#pragma unroll
+              for (int j = 0; j < BM / 32; ++j) tma_load_2d(w_dst + j * W_BOX, &tmW, e.n0 + 32 * j, e.g_lo + k0, full);
+              for (int j = 0; j < boxes; ++j) tma_load_2d(x_dst + j * W_BOX, &tmX, e.t0 + 32 * j, e.g_lo + k0, full);
+            } else {
+              if (!p.w_mn) {
+                tma_load_3d(w_dst, &tmW, k0, e.n0, e.expert, full);
+              } else {
+#pragma unroll
+                for (int j = 0; j < BM / 32; ++j) tma_load_3d(w_dst + j * W_BOX, &tmW, e.n0 + 32 * j, k0, e.expert, full);
+              }
+              for (int j = 0; j < boxes; ++j) tma_load_2d(x_dst + j * 64 * BK * 4, &tmX, k0, e.t0 + j * 64, full);
+            }
+          }
+          if (!withhold) ++issued;
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+      }
+    }
+    if (*abort_flag) {
+      // copies already issued land before this CTA gives its shared memory back
+      for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+        for (int n = 0; n < (1 << 16); ++n)
+          if (mbar_try_wait(bar_full + 8 * (i % STAGES), (i / STAGES) & 1)) break;
+    }
+  } else if (warp == CONV_WARPS + 1) {
+    // ------------------------------ MMA issuer --------------------------------
+    const bool a_mn = WEIGHTS || p.w_mn;
+    constexpr uint32_t K_SWZ = BK == 32 ? SWZ_128B : SWZ_64B, K_SBO = 8 * BK * 4;
+    const uint32_t a_step = (a_mn ? 1024u : 32u) >> 4;
+    constexpr uint32_t b_step = (WEIGHTS ? 1024u : 32u) >> 4;
+    const uint64_t d_a = a_mn ? make_smem_desc(smem_base, W_BOX, 512, SWZ_128B_BASE32B) : make_smem_desc(smem_base, 16, K_SBO, K_SWZ);
+    const uint64_t d_b = WEIGHTS ? make_smem_desc(smem_base + A_TILE, W_BOX, 512, SWZ_128B_BASE32B)
+                                 : make_smem_desc(smem_base + A_TILE, 16, K_SBO, K_SWZ);
+    const uint32_t a_hiw = (uint32_t)(d_a >> 32), b_hiw = (uint32_t)(d_b >> 32);
+    const uint32_t a_low0 = (uint32_t)d_a, b_low0 = (uint32_t)d_b;
+    constexpr uint32_t LO_TILE = C::RAW >> 4, STAGE_STEP = C::STAGE >> 4;
+    uint32_t ph = 0, stage_off = 0;
+    int s = 0;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int slot = it % RING, set = it & 1;
+      if (!warp_wait(bar_entry + 8 * slot, (it / RING) & 1, abort_flag, p.status, 520 + slot)) break;
+      const Entry e = ring[slot];
+      if (!e.more) break;
+      if (!warp_wait(bar_read + 8 * set, ((it >> 1) & 1) ^ 1, abort_flag, p.status, 250 + set)) break;
+      tc_fence_after();
+      const uint32_t idesc = make_idesc_tf32(BM, (columns(e) + 15) / 16 * 16, a_mn, WEIGHTS);
+      const int run = max((e.nkb + C::MAINS - 1) / C::MAINS, 256 / BK);        // k-blocks into one main accumulator
+      uint32_t tmem_main = tmem_base + set * C::SET, accumulate = 0, cross = 0;
+      const uint32_t tmem_cross = tmem_main + C::MAINS * BN;
+      int in_run = 0;
+      for (int i = 0; i < e.nkb; ++i) {
+        if (C::MAINS > 1 && in_run == run) {
+          in_run = 0;
+          accumulate = 0;
+          tmem_main += BN;
+        }
+        ++in_run;
+        if (!warp_wait(bar_conv + 8 * s, ph, abort_flag, p.status, 200 + s)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < BK / 8; ++kk) {
+            const uint32_t al = a_low0 + stage_off + kk * a_step, bl = b_low0 + stage_off + kk * b_step;
+            mma_tf32_ss_words(tmem_cross, al + LO_TILE, a_hiw, bl, b_hiw, idesc, kk ? 1u : cross);
+            mma_tf32_ss_words(tmem_cross, al, a_hiw, bl + LO_TILE, b_hiw, idesc, 1);
+            mma_tf32_ss_words(tmem_main, al, a_hiw, bl, b_hiw, idesc, kk ? 1u : accumulate);
+          }
+          mma_commit(bar_empty + 8 * s);
+        }
+        accumulate = cross = 1;
+        __syncwarp();
+        if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
+      }
+      if (ok && elect_one()) mma_commit(bar_acc + 8 * set);
+      __syncwarp();
+    }
+    if (*abort_flag) {
+      // every MMA issued must have retired before TMEM is freed
+      if (elect_one()) mma_commit(bar_retired);
+      __syncwarp();
+      for (int n = 0; n < (1 << 16); ++n)
+        if (mbar_try_wait(bar_retired, 0)) break;
+    }
+  } else if (warp < CONV_WARPS) {
+    // ------------------------------ hi / lo split ------------------------------
+    constexpr int PASS = CONV_WARPS * 32 * 16;
+    const int tid = threadIdx.x;
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int slot = it % RING;
+      if (!warp_wait(bar_entry + 8 * slot, (it / RING) & 1, abort_flag, p.status, 540 + slot)) break;
+      const Entry e = ring[slot];
+      if (!e.more) break;
+      const int raw_bytes = bytes_of(columns(e));
+      for (int i = 0; i < e.nkb; ++i) {
+        if (!warp_wait(bar_full + 8 * s, ph, abort_flag, p.status, 300 + s)) { ok = false; break; }
+        uint8_t* raw = smem + s * C::STAGE;
+        uint8_t* low = raw + C::RAW;
+        auto split = [&](int off) {
+          const float4 v = *reinterpret_cast<const float4*>(raw + off);
+          float4 l;
+          l.x = lo_part(v.x); l.y = lo_part(v.y); l.z = lo_part(v.z); l.w = lo_part(v.w);
+          *reinterpret_cast<float4*>(low + off) = l;
+        };
+        if (WEIGHTS) {
+          const int valid = e.g_hi - e.g_lo - (e.kb_begin + i) * BK;             // rows of this k-block inside the group
+          if (valid < BK) {
+            // (the 16-byte pieces that this thread reads itself below; a k row is 128 bytes of every box)
+#pragma unroll 1
+            for (int off = tid * 16; off < raw_bytes; off += PASS)
+              if (((off & (W_BOX - 1)) >> 7) >= valid) *reinterpret_cast<float4*>(raw + off) = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+        if (raw_bytes == C::RAW) {
+#pragma unroll
+          for (int k = 0; k < C::RAW / PASS; ++k) split(tid * 16 + k * PASS);
+        } else {
+#pragma unroll
+          for (int k = 0; k < A_TILE / PASS; ++k) split(tid * 16 + k * PASS);
+          for (int off = A_TILE + tid * 16; off < raw_bytes; off += PASS) split(off);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_conv + 8 * s);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+  } else {
+    // ------------------------------ epilogue -----------------------------------
+    const int q = warp & 3;                                  // the TMEM lanes of this warp
+    for (int it = 0;; ++it) {
+      const int slot = it % RING, set = it & 1;
+      if (!warp_wait(bar_entry + 8 * slot, (it / RING) & 1, abort_flag, p.status, 560 + slot)) break;
+      const Entry e = ring[slot];
+      if (!e.more) break;
+      if (!warp_wait(bar_acc + 8 * set, (uint32_t)((it >> 1) & 1), abort_flag, p.status, 400 + set)) break;
+      tc_fence_after();
+      const int cols = columns(e), run = max((e.nkb + C::MAINS - 1) / C::MAINS, 256 / BK), mains = (e.nkb + run - 1) / run;
+      const uint32_t lane_base = tmem_base + set * C::SET + ((uint32_t)(q * 32) << 16);
+      float* const out = WEIGHTS ? p.C + e.expert * p.c_stride : p.C;
+      const float* bias = p.bias ? p.bias + (long long)e.expert * p.N : nullptr;
+#pragma unroll 1
+      for (int cc = 0; cc * 32 < cols; ++cc) {
+        uint32_t r[32], rc[32];
+        tmem_ld_32x32(lane_base + (uint32_t)(cc * 32), r);
+        tmem_ld_32x32(lane_base + (uint32_t)(C::MAINS * BN + cc * 32), rc);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
+#pragma unroll 1
+        for (int m = 1; m < mains; ++m) {
+          tmem_ld_32x32(lane_base + (uint32_t)(m * BN + cc * 32), rc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
+        }
+        store_columns(p, out, r, e.t0 + cc * 32, WEIGHTS ? p.cols : e.g_hi, e.n0 + q * 32 + lane, bias, e.chunk == 0 ? p.beta : 1.f, e.last);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar_read + 8 * set);
+        mbar_arrive(bar_done + 8 * slot);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == CONV_WARPS + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * C::SET);
+  }
+}
+
 // ------------------------------ host side -------------------------------------
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -496,7 +812,8 @@ int tmap_3d(CUtensorMap* tm, const float* base, long long count, long long rows,
 }
 
 template <typename A, void (*KERNEL)(CUtensorMap, CUtensorMap, A)>
-int launch(cb200_stream* s, int smem, const CUtensorMap& tmA, const CUtensorMap& tmB, const A& a, long long ctas, int cluster) {
+int launch(cb200_stream* s, int smem, const CUtensorMap& tmA, const CUtensorMap& tmB, const A& a, long long ctas, int cluster,
+           int threads = THREADS) {
   static std::once_flag once[64];
   static cudaError_t result[64];
   const int dev = s->device & 63;
@@ -505,7 +822,7 @@ int launch(cb200_stream* s, int smem, const CUtensorMap& tmA, const CUtensorMap&
   CB_REQUIRE(ctas <= 2147483647LL, "expert_gemm: too many tiles");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas, 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s->stream;
   cudaLaunchAttribute attr[1];
@@ -556,20 +873,32 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   DeviceGuard guard(s->device);
   // how many rows a tile may take: what an even split of the rows over the experts fills
   const long long even = (rows + experts - 1) / experts;
-  int BN = s->opt_gemm_tile_n > 0 ? s->opt_gemm_tile_n : (even <= 32 ? 32 : (even <= 64 ? 64 : (even <= 128 ? 128 : 256)));
-  // short reductions are all set-up and stores: narrow tiles, two to an SM, overlap them
-  if (s->opt_gemm_tile_n == 0 && BN > 64 && K <= 128) BN = 64;
-  const int bk = BN <= 64 ? 32 : 16;
-  const long long tiles = (rows + BN - 1) / BN + (experts < rows ? experts : rows) - 1, units = tiles * ((N + BM - 1) / BM);
-  const int nkb = (K + bk - 1) / bk;
-  const int chunk = BN == 256 ? RowsCfg<256, 16>::CHUNK : (BN == 128 ? RowsCfg<128, 16>::CHUNK : (BN == 64 ? RowsCfg<64, 32>::CHUNK : RowsCfg<32, 32>::CHUNK));
+  int BN = even <= 32 ? 32 : (even <= 64 ? 64 : (even <= 128 ? 128 : 256));
+  if (s->opt_gemm_tile_n > 0) BN = s->opt_gemm_tile_n;
+  const bool forced = s->opt_gemm_tile_n > 0 || s->opt_gemm_k_slices > 0;
+  int bk = 0;
+  long long units = 0;
+  auto cut = [&] {
+    bk = BN <= 64 ? 32 : 16;
+    units = ((rows + BN - 1) / BN + (experts < rows ? experts : rows) - 1) * ((N + BM - 1) / BM);
+  };
+  cut();
   // K slices (the CTAs of a cluster) where the tiles leave SMs free; a slice is one chunk, since its parked tile lies in
   // shared memory that the next chunk's stages would need
+  const int chunk = BN == 256 ? RowsCfg<256, 16>::CHUNK : (BN == 128 ? RowsCfg<128, 16>::CHUNK : (BN == 64 ? RowsCfg<64, 32>::CHUNK : RowsCfg<32, 32>::CHUNK));
+  const int nkb = (K + bk - 1) / bk, wanted = s->opt_gemm_k_slices;
   int slices = 1;
-  const int forced = s->opt_gemm_k_slices;
   for (int sl = 2; sl <= 8; sl *= 2)
-    if ((forced > 0 ? sl <= forced : units * sl <= s->sm_count * (BN <= 64 ? 2 : 1)) && nkb / sl >= 4) slices = sl;
+    if ((wanted > 0 ? sl <= wanted : units * sl <= s->sm_count * (BN <= 64 ? 2 : 1)) && nkb / sl >= 4) slices = sl;
   if ((nkb + slices - 1) / slices > chunk || only_if) slices = 1;
+  // Short reductions in tiles that follow one another (this / the kernel of one tile a CTA, us): 16 experts of 2048 x 128 with
+  // 64, 256 rows each 18, 33 / 22, 39; 32 of 1024 x 1024 with 32, 64, 128, 256 rows 53, 76, 109, 175 / 77, 89, 121, 151; 64 of
+  // 1024 x 4096 with 32, 64 rows 406, 559 / 406, 467.
+  const bool stream = !forced && slices == 1 && (K <= 256 || (K <= 1024 && even <= 128));
+  if (stream) {
+    BN = even <= 64 ? 64 : 128;
+    cut();
+  }
   RowsArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = 0; a.cols = a.tiles_r = 0; a.park = nullptr; a.arrived = nullptr;
   a.bias = bias; a.offsets = offsets; a.status = s->status_dev;
@@ -584,6 +913,11 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   if (rc) return rc;
   CB_REQUIRE(units <= 2147483647LL, "expert_gemm: too many tiles");
   a.units = (int)units;
+  if (stream) {
+    const long long ctas = units < s->sm_count ? units : s->sm_count;
+    if (BN == 128) return launch<RowsArgs, expert_stream_kernel<128, 16, false>>(s, StreamCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
+    return launch<RowsArgs, expert_stream_kernel<64, 32, false>>(s, StreamCfg<64, 32>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
+  }
   const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
   if (BN == 256) return launch<RowsArgs, expert_tf32x3_kernel<256, 16, false>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, slices);
   if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, false>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, slices);
@@ -598,6 +932,10 @@ int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long 
   const long long tiles_l = (N + BM - 1) / BM;
   int BN, slices;
   choose(s, tiles_l * experts, M, (rows / experts + 16) / 16, only_if ? 1 : 16, BN, slices);
+  // short reductions in tiles that follow one another (this / the kernel of one tile a CTA, us): 8 experts of 1024 x 4096 with
+  // 20, 64, 96, 160 rows each 43, 65, 81, 114 / 64, 80, 92, 113; 32 of 512 x 512 with 64, 96 rows 37, 47 / 35, 39
+  const bool stream = s->opt_gemm_tile_n == 0 && s->opt_gemm_k_slices == 0 && slices == 1 && rows <= 96LL * experts;
+  if (stream) BN = M > 64 ? 128 : 64;
   RowsArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.cols = M; a.tiles_r = (M + BN - 1) / BN; a.park = nullptr; a.arrived = nullptr;
   a.bias = nullptr; a.offsets = offsets; a.status = s->status_dev;
@@ -617,6 +955,11 @@ int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long 
   CUtensorMap tmW, tmX;
   if ((rc = tmap_2d(&tmW, B, rows, N, ldb, 32, 16, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
   if ((rc = tmap_2d(&tmX, A, rows, M, lda, 32, 16, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
+  if (stream) {
+    const long long ctas = units < s->sm_count ? units : s->sm_count;
+    if (BN == 128) return launch<RowsArgs, expert_stream_kernel<128, 16, true>>(s, StreamCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
+    return launch<RowsArgs, expert_stream_kernel<64, 16, true>>(s, StreamCfg<64, 16>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
+  }
   if (BN == 256) return launch<RowsArgs, expert_tf32x3_kernel<256, 16, true>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, 1);
   if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, true>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1);
   return launch<RowsArgs, expert_tf32x3_kernel<64, 16, true>>(s, RowsCfg<64, 16>::SMEM, tmW, tmX, a, ctas, 1);
