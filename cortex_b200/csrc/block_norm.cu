@@ -204,46 +204,49 @@ __global__ void __launch_bounds__(128) column_sums_kernel(Backward<T> p, const T
   const T aw = p.after_w ? p.after_w[c] : (T)1, ab = p.after_b ? p.after_b[c] : (T)0;
   T s[SUMS] = {(T)0, (T)0, (T)0, (T)0};
   T gs = (T)0;
-  long long seg = r0;                                      // first row of the current gate group inside this block
-  for (long long r = r0; r < r1; ++r) {
-    if (p.out_g) {
-      const T dy = p.out_g[r * p.ld_out_g + c];
-      s[SUM_BEFORE_W] += dy * ((p.total[r * p.ld_total + c] - stats[4 * r]) * stats[4 * r + 1]);
-      s[SUM_BEFORE_B] += dy;
-    }
-    if (p.block) {
-      const T d = p.scale * p.residual_g[r * p.ld_residual_g + c];
-      const T x = p.block[r * p.ld_block + c];
-      const T hat = (x - stats[4 * r + 2]) * stats[4 * r + 3];
-      const long long g = r / p.rows_per_gate;
-      const T du = p.gate ? d * p.gate[g * p.cols + c] : d;
-      if (p.after_w) {
+  // the rows that share a gate row make a segment; without such groups the whole block does
+  const long long per = p.rows_per_gate;
+  const bool grouped = p.gate && per > 1;
+  const long long gate_step = p.gate && per == 1 ? p.cols : 0;
+  for (long long r = r0; r < r1;) {
+    const long long g = grouped ? r / per : 0, end = grouped ? (g + 1) * per : r1, stop = end < r1 ? end : r1;
+    const T* gate = p.gate ? p.gate + (grouped ? g : (per == 1 ? r : 0)) * p.cols + c : nullptr;
+    const long long first = r;
+#pragma unroll 4
+    for (; r < stop; ++r) {
+      if (p.out_g) {
+        const T dy = p.out_g[r * p.ld_out_g + c];
+        s[SUM_BEFORE_W] += dy * ((p.total[r * p.ld_total + c] - stats[4 * r]) * stats[4 * r + 1]);
+        s[SUM_BEFORE_B] += dy;
+      }
+      if (p.block) {
+        const T d = p.scale * p.residual_g[r * p.ld_residual_g + c];
+        const T x = p.block[r * p.ld_block + c];
+        const T hat = (x - stats[4 * r + 2]) * stats[4 * r + 3];
+        const T du = gate ? d * gate[(r - first) * gate_step] : d;
         s[SUM_AFTER_W] += du * hat;
         s[SUM_AFTER_B] += du;
-      }
-      if (gates) {
         gs += d * (p.after_w ? hat * aw + ab : x);
-        const long long end = (g + 1) * p.rows_per_gate;
-        if (r + 1 == end || r + 1 == r1) {
-          const bool whole = seg == g * p.rows_per_gate && r + 1 == end;
-          T* to = whole ? p.gate_g + g * p.cols : gate_parts + (2LL * b + (seg != r0)) * p.cols;
-          to[c] = gs;
-          gs = (T)0;
-          seg = r + 1;
-        }
       }
     }
+    if (gates) {
+      const bool whole = first == g * per && r == end;
+      T* to = whole ? p.gate_g + g * p.cols : gate_parts + (2LL * b + (first != r0)) * p.cols;
+      to[c] = gs;
+    }
+    gs = (T)0;
   }
 #pragma unroll
   for (int k = 0; k < SUMS; ++k) parts[((long long)b * SUMS + k) * p.cols + c] = s[k];
 }
 
-// The sum over n rows first, first + pitch, ... of one column: 32 columns x 32 threads each (blockDim 1024), added in order.
-template <typename T>
+// The sum over n rows first, first + pitch, ... of one column: COLUMNS columns x blockDim.x / COLUMNS threads each, added in order.
+template <typename T, int COLUMNS, int THREADS>
 __device__ __forceinline__ void add_rows(const T* first, long long pitch, int n, T* to, bool live) {
-  __shared__ T part[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int a = (int)((long long)n * ty / 32), z = (int)((long long)n * (ty + 1) / 32);
+  constexpr int DEEP = THREADS / COLUMNS;
+  __shared__ T part[DEEP][COLUMNS + 1];
+  const int tx = threadIdx.x % COLUMNS, ty = threadIdx.x / COLUMNS;
+  const int a = (int)((long long)n * ty / DEEP), z = (int)((long long)n * (ty + 1) / DEEP);
   T s = (T)0;
   if (live) {
 #pragma unroll 8
@@ -254,30 +257,33 @@ __device__ __forceinline__ void add_rows(const T* first, long long pitch, int n,
   __syncthreads();
   if (ty == 0 && live) {
 #pragma unroll
-    for (int i = 1; i < 32; ++i) s += part[i][tx];
+    for (int i = 1; i < DEEP; ++i) s += part[i][tx];
     *to = s;
   }
 }
 
-// blockIdx.y < SUMS: a scale's or bias's gradient.  Behind them: the gate groups that more than one row block has a part of
-// (strided); the first part may be in the second slot of its block, the others are in first slots.
+// blockIdx.y: a scale's or bias's gradient
 template <typename T>
-__global__ void __launch_bounds__(1024) column_finish_kernel(Backward<T> p, const T* parts, const T* gate_parts, int blocks) {
+__global__ void __launch_bounds__(1024) column_finish_kernel(Backward<T> p, const T* parts, int blocks) {
   const long long c = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
-  if (blockIdx.y < SUMS) {
-    const int k = blockIdx.y;
-    T* to = k == SUM_BEFORE_W ? p.before_w_g : (k == SUM_BEFORE_B ? p.before_b_g : (k == SUM_AFTER_W ? p.after_w_g : p.after_b_g));
-    if (to) add_rows<T>(parts + (long long)k * p.cols + c, (long long)SUMS * p.cols, blocks, to + c, c < p.cols);
-    return;
-  }
-  const long long groups = p.rows / p.rows_per_gate;
-  for (long long g = blockIdx.y - SUMS; g < groups; g += gridDim.y - SUMS) {
+  const int k = blockIdx.y;
+  T* to = k == SUM_BEFORE_W ? p.before_w_g : (k == SUM_BEFORE_B ? p.before_b_g : (k == SUM_AFTER_W ? p.after_w_g : p.after_b_g));
+  if (to) add_rows<T, 32, 1024>(parts + (long long)k * p.cols + c, (long long)SUMS * p.cols, blocks, to + c, c < p.cols);
+}
+
+// The gate groups that more than one row block has a part of: the first part may be in the second slot of its block, the
+// others are in first slots.  As many threads to a column as there are parts to add (64 groups of 2500 columns over 296 row
+// blocks, five parts each: with 32 threads to a column, most of them idle, this took 25 us of 33 for the column sums).
+template <typename T, int COLUMNS>
+__global__ void __launch_bounds__(256) gate_finish_kernel(Backward<T> p, const T* gate_parts, int blocks) {
+  const long long c = (long long)blockIdx.x * COLUMNS + threadIdx.x % COLUMNS, groups = p.rows / p.rows_per_gate;
+  for (long long g = blockIdx.y; g < groups; g += gridDim.y) {
     const long long first = g * p.rows_per_gate, last = first + p.rows_per_gate - 1;
     const int b0 = block_of(p.rows, blocks, first), b1 = block_of(p.rows, blocks, last);
     if (b0 == b1) continue;
     T* to = p.gate_g + g * p.cols + c;
-    add_rows<T>(gate_parts + 2LL * (b0 + 1) * p.cols + c, 2 * p.cols, b1 - b0, to, c < p.cols);
-    if (threadIdx.x < 32 && c < p.cols) *to += gate_parts[(2LL * b0 + (first != block_begin(p.rows, blocks, b0))) * p.cols + c];
+    add_rows<T, COLUMNS, 256>(gate_parts + 2LL * (b0 + 1) * p.cols + c, 2 * p.cols, b1 - b0, to, c < p.cols);
+    if (threadIdx.x < COLUMNS && c < p.cols) *to += gate_parts[(2LL * b0 + (first != block_begin(p.rows, blocks, b0))) * p.cols + c];
   }
 }
 
@@ -422,6 +428,8 @@ __global__ void __launch_bounds__(1024) forward_rows_kernel(Forward<T> p) {
     }
   }
 }
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 template <int BYTES> __device__ __forceinline__ void copy_async(void* smem, const void* g) {
   const uint32_t d = (uint32_t)__cvta_generic_to_shared(smem);
@@ -626,6 +634,187 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 320 ? 2 : 1) backward_rows_kerne
   }
 }
 
+// Rows too wide for that: the row in registers, read once; the column sums of the CTA's rows in shared memory, where every
+// thread adds to its own columns only (no barrier).  The next row is asked for into L2 while a row is worked on.  4097 to 8192
+// fp32 columns; 5286 rows of 6564 254 us, where a pass over the rows and one over the columns took 480 (127 at HBM's rate).
+template <typename T, int VEC, int ITEMS, bool LAYER>
+__global__ void __launch_bounds__(1024) backward_hold_kernel(Backward<T> p, T* parts, T* gate_parts, int blocks) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ T part[2][2 * 32];
+  const int n = (int)p.cols, warps = blockDim.x >> 5, step = blockDim.x * VEC, c0 = threadIdx.x * VEC, slot = step * ITEMS;
+  T* const sums = reinterpret_cast<T*>(smem_raw);          // before_w, before_b, after_w, after_b, gate: [5][slot]
+  const T inv_n = (T)1 / (T)n;
+  const int b = blockIdx.x, per_gate = (int)p.rows_per_gate;
+  const int r0 = (int)block_begin(p.rows, blocks, b), r1 = (int)block_begin(p.rows, blocks, b + 1);
+  const bool has_y = p.out_g != nullptr, has_x = p.block != nullptr, has_a = p.after_w != nullptr;
+  const bool gates = p.gate_g && per_gate > 1, gate_rows = p.gate_g && per_gate == 1;
+  const Pack<T, VEC> zero = {};
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int k = 0; k <= SUMS; ++k) st_pack<T, VEC>(sums + k * slot + c0 + i * step, zero);
+  int g = r0 / per_gate, g_left = (g + 1) * per_gate - r0;                 // gate row, rows it still serves
+  bool g_whole = g * per_gate == r0;                       // this block has had the group's rows from its first one on
+  int turn = 0, slot_b = 0;                                // slot_b: 1 once the block's first group is over
+
+#pragma unroll 1
+  for (int r = r0; r < r1; ++r) {
+    Pack<T, VEC> h[ITEMS], y[ITEMS], x[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * step;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) h[i].e[e] = y[i].e[e] = x[i].e[e] = (T)0;
+      if (c < n) {
+        if (has_y) { h[i] = ld_pack<T, VEC>(p.total + (long long)r * p.ld_total + c); y[i] = ld_pack<T, VEC>(p.out_g + (long long)r * p.ld_out_g + c); }
+        if (has_x) x[i] = ld_pack<T, VEC>(p.block + (long long)r * p.ld_block + c);
+        if (r + 1 < r1 && (threadIdx.x * VEC * (int)sizeof(T)) % 128 == 0) {
+          const long long q = r + 1;
+          if (has_y) { prefetch_l2(p.total + q * p.ld_total + c); prefetch_l2(p.out_g + q * p.ld_out_g + c); }
+          if (has_x) prefetch_l2(p.block + q * p.ld_block + c);
+          if (p.total_g) prefetch_l2(p.total_g + q * p.ld_total_g + c);
+        }
+      }
+    }
+    T m[2] = {(T)0, (T)0}, q[2] = {(T)0, (T)0}, d[2] = {(T)0, (T)0}, a[2] = {(T)0, (T)0};
+    if (LAYER) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { m[0] += h[i].e[e]; m[1] += x[i].e[e]; }
+      row_sums<T, 2>(m, part[turn ^= 1], warps);
+      m[0] *= inv_n;
+      m[1] = has_a ? m[1] * inv_n : (T)0;
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (c0 + i * step < n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          h[i].e[e] -= m[0];
+          x[i].e[e] -= m[1];
+          q[0] += h[i].e[e] * h[i].e[e];
+          q[1] += x[i].e[e] * x[i].e[e];
+        }
+    row_sums<T, 2>(q, part[turn ^= 1], warps);
+    const T rstd = has_y ? rsqrt_of(q[0] * inv_n + p.eps) : (T)1, rstd_a = has_a ? rsqrt_of(q[1] * inv_n + p.eps) : (T)1;
+    if (has_y) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = c0 + i * step;
+        if (c >= n) continue;
+        const Pack<T, VEC> w = ld_pack<T, VEC>(p.before_w + c);
+        Pack<T, VEC> sw = ld_pack<T, VEC>(sums + SUM_BEFORE_W * slot + c), sb = ld_pack<T, VEC>(sums + SUM_BEFORE_B * slot + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          h[i].e[e] *= rstd;
+          sw.e[e] += y[i].e[e] * h[i].e[e];
+          sb.e[e] += y[i].e[e];
+          y[i].e[e] *= w.e[e];
+          d[0] += y[i].e[e] * h[i].e[e];
+          if (LAYER) d[1] += y[i].e[e];
+        }
+        st_pack<T, VEC>(sums + SUM_BEFORE_W * slot + c, sw);
+        st_pack<T, VEC>(sums + SUM_BEFORE_B * slot + c, sb);
+      }
+      row_sums<T, 2>(d, part[turn ^= 1], warps);
+      d[0] *= inv_n;
+      d[1] *= inv_n;
+    }
+    --g_left;
+    const bool flush = gates && (g_left == 0 || r + 1 == r1);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int c = c0 + i * step;
+      if (c >= n) continue;
+      if (has_y)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] = (y[i].e[e] - h[i].e[e] * d[0] - d[1]) * rstd;
+      if (p.total_g) {
+        const Pack<T, VEC> t = ld_pack<T, VEC>(p.total_g + (long long)r * p.ld_total_g + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] += t.e[e];
+      }
+      st_pack<T, VEC>(p.residual_g + (long long)r * p.ld_residual_g + c, h[i]);
+      if (!has_x) continue;
+      Pack<T, VEC> w, wb, ga;
+      if (has_a) w = ld_pack<T, VEC>(p.after_w + c);
+      if (p.gate) ga = ld_pack<T, VEC>(p.gate + (long long)g * n + c);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        h[i].e[e] *= p.scale;
+        x[i].e[e] *= rstd_a;
+      }
+      if (p.gate_g) {
+        if (p.after_b) wb = ld_pack<T, VEC>(p.after_b + c);
+        Pack<T, VEC> u;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) u.e[e] = (has_a ? x[i].e[e] * w.e[e] + (p.after_b ? wb.e[e] : (T)0) : x[i].e[e]) * h[i].e[e];
+        if (gate_rows) {
+          st_pack<T, VEC>(p.gate_g + (long long)g * n + c, u);
+        } else {
+          const Pack<T, VEC> before = ld_pack<T, VEC>(sums + SUMS * slot + c);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) u.e[e] += before.e[e];
+          if (flush) {
+            T* to = g_whole && g_left == 0 ? p.gate_g + (long long)g * n : gate_parts + (2LL * b + slot_b) * n;
+            st_pack<T, VEC>(to + c, u);
+          }
+          st_pack<T, VEC>(sums + SUMS * slot + c, flush ? zero : u);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (p.gate) h[i].e[e] *= ga.e[e];
+      if (has_a) {
+        Pack<T, VEC> sw = ld_pack<T, VEC>(sums + SUM_AFTER_W * slot + c), sb = ld_pack<T, VEC>(sums + SUM_AFTER_B * slot + c);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          sw.e[e] += h[i].e[e] * x[i].e[e];
+          sb.e[e] += h[i].e[e];
+          h[i].e[e] *= w.e[e];
+          a[0] += h[i].e[e] * x[i].e[e];
+          if (LAYER) a[1] += h[i].e[e];
+        }
+        st_pack<T, VEC>(sums + SUM_AFTER_W * slot + c, sw);
+        st_pack<T, VEC>(sums + SUM_AFTER_B * slot + c, sb);
+      } else {
+        st_pack<T, VEC>(p.block_g + (long long)r * p.ld_block_g + c, h[i]);
+      }
+    }
+    if (has_x && has_a) {
+      row_sums<T, 2>(a, part[turn ^= 1], warps);
+      a[0] *= inv_n;
+      a[1] *= inv_n;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = c0 + i * step;
+        if (c >= n) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[i].e[e] = (h[i].e[e] - x[i].e[e] * a[0] - a[1]) * rstd_a;
+        st_pack<T, VEC>(p.block_g + (long long)r * p.ld_block_g + c, h[i]);
+      }
+    }
+    if (g_left == 0) {
+      ++g;
+      g_left = per_gate;
+      g_whole = true;
+      slot_b = 1;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int c = c0 + i * step;
+    if (c >= n) continue;
+    T* to = parts + (long long)b * SUMS * n + c;
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) st_pack<T, VEC>(to + (long long)k * n, ld_pack<T, VEC>(sums + k * slot + c));
+  }
+}
+
+inline int round32(long long v) { return (int)((v + 31) / 32 * 32); }
+
+
 template <typename T> bool packed_ok(int vec, long long cols, std::initializer_list<const void*> ps, std::initializer_list<long long> lds) {
   if (cols % vec) return false;
   uintptr_t bits = 0;
@@ -634,7 +823,6 @@ template <typename T> bool packed_ok(int vec, long long cols, std::initializer_l
   return (bits & (vec * sizeof(T) - 1)) == 0;
 }
 
-inline int round32(long long v) { return (int)((v + 31) / 32 * 32); }
 
 template <typename T, int VEC, int ITEMS> void launch_forward(cb200_stream* s, const Forward<T>& p) {
   const int threads = round32((p.cols + VEC * ITEMS - 1) / (VEC * ITEMS));
@@ -661,16 +849,14 @@ template <typename T> int run_forward(cb200_stream* s, const Forward<T>& p) {
   return CB200_OK;
 }
 
-template <typename T, int VEC, int ITEMS, bool LAYER, int MAXT>
+template <typename T, void (*KERNEL)(Backward<T>, T*, T*, int)>
 int launch_backward_kernel(cb200_stream* s, const Backward<T>& p, int threads, size_t smem, T* parts, T* gate_parts, int blocks) {
   static std::once_flag once[64];
   static cudaError_t result[64];
   const int dev = s->device & 63;
-  std::call_once(once[dev], [&] {
-    result[dev] = cudaFuncSetAttribute(backward_rows_kernel<T, VEC, ITEMS, LAYER, MAXT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 << 10);
-  });
+  std::call_once(once[dev], [&] { result[dev] = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 << 10); });
   if (result[dev] != cudaSuccess) return cb200_cuda_fail(result[dev], "cudaFuncSetAttribute", __FILE__, __LINE__);
-  backward_rows_kernel<T, VEC, ITEMS, LAYER, MAXT><<<(unsigned)blocks, threads, smem, s->stream>>>(p, parts, gate_parts, blocks);
+  KERNEL<<<(unsigned)blocks, threads, smem, s->stream>>>(p, parts, gate_parts, blocks);
   CB_LAUNCH_CHECK(s);
   return CB200_OK;
 }
@@ -678,19 +864,29 @@ int launch_backward_kernel(cb200_stream* s, const Backward<T>& p, int threads, s
 template <typename T, int VEC, int ITEMS>
 int launch_backward(cb200_stream* s, const Backward<T>& p, int threads, size_t smem, T* parts, T* gate_parts, int blocks) {
   if (threads <= 320)
-    return p.layer ? launch_backward_kernel<T, VEC, ITEMS, true, 320>(s, p, threads, smem, parts, gate_parts, blocks)
-                   : launch_backward_kernel<T, VEC, ITEMS, false, 320>(s, p, threads, smem, parts, gate_parts, blocks);
-  return p.layer ? launch_backward_kernel<T, VEC, ITEMS, true, 512>(s, p, threads, smem, parts, gate_parts, blocks)
-                 : launch_backward_kernel<T, VEC, ITEMS, false, 512>(s, p, threads, smem, parts, gate_parts, blocks);
+    return p.layer ? launch_backward_kernel<T, backward_rows_kernel<T, VEC, ITEMS, true, 320>>(s, p, threads, smem, parts, gate_parts, blocks)
+                   : launch_backward_kernel<T, backward_rows_kernel<T, VEC, ITEMS, false, 320>>(s, p, threads, smem, parts, gate_parts, blocks);
+  if (threads <= 512)
+    return p.layer ? launch_backward_kernel<T, backward_rows_kernel<T, VEC, ITEMS, true, 512>>(s, p, threads, smem, parts, gate_parts, blocks)
+                   : launch_backward_kernel<T, backward_rows_kernel<T, VEC, ITEMS, false, 512>>(s, p, threads, smem, parts, gate_parts, blocks);
+  return p.layer ? launch_backward_kernel<T, backward_hold_kernel<T, VEC, ITEMS, true>>(s, p, threads, smem, parts, gate_parts, blocks)
+                 : launch_backward_kernel<T, backward_hold_kernel<T, VEC, ITEMS, false>>(s, p, threads, smem, parts, gate_parts, blocks);
 }
 
 template <typename T> int finish_columns(cb200_stream* s, const Backward<T>& p, const T* parts, const T* gate_parts, int blocks) {
-  const bool gates = p.gate_g && p.rows_per_gate > 1;
-  if (!(p.before_w_g || p.before_b_g || p.after_w_g || p.after_b_g || gates)) return CB200_OK;
-  const long long groups = gates ? p.rows / p.rows_per_gate : 0;
-  column_finish_kernel<T><<<dim3((unsigned)((p.cols + 31) / 32), (unsigned)(SUMS + (groups < 4096 ? groups : 4096))), 1024, 0, s->stream>>>(
-      p, parts, gate_parts, blocks);
-  CB_LAUNCH_CHECK(s);
+  if (p.before_w_g || p.before_b_g || p.after_w_g || p.after_b_g) {
+    column_finish_kernel<T><<<dim3((unsigned)((p.cols + 31) / 32), SUMS), 1024, 0, s->stream>>>(p, parts, blocks);
+    CB_LAUNCH_CHECK(s);
+  }
+  if (p.gate_g && p.rows_per_gate > 1 && blocks > 1) {
+    const long long groups = p.rows / p.rows_per_gate, each = blocks / groups;
+    const unsigned y = (unsigned)(groups < 4096 ? groups : 4096);
+    auto grid = [&](int columns) { return dim3((unsigned)((p.cols + columns - 1) / columns), y); };
+    if (each >= 64) gate_finish_kernel<T, 8><<<grid(8), 256, 0, s->stream>>>(p, gate_parts, blocks);
+    else if (each >= 16) gate_finish_kernel<T, 32><<<grid(32), 256, 0, s->stream>>>(p, gate_parts, blocks);
+    else gate_finish_kernel<T, 128><<<grid(128), 256, 0, s->stream>>>(p, gate_parts, blocks);
+    CB_LAUNCH_CHECK(s);
+  }
   return CB200_OK;
 }
 
@@ -702,8 +898,9 @@ template <typename T> int run_backward(cb200_stream* s, const Backward<T>& p) {
   // values per thread: its five column sums of each stay in registers (64-bit ones: half as many values)
   constexpr int VALUES = sizeof(T) == 8 ? 4 : 8;
   const int threads = round32((p.cols + VALUES - 1) / VALUES);
-  const size_t smem = (size_t)2 * 4 * threads * VALUES * sizeof(T), room = 216 << 10;
-  if (threads <= 512 && smem <= room) {
+  // two rows of four operands, or (wider rows) the five column sums
+  const size_t smem = (size_t)(threads <= 512 ? 2 * 4 : SUMS + 1) * threads * VALUES * sizeof(T), room = 216 << 10;
+  if (threads <= 1024) {
     long long per_sm = (long long)(room / smem), by_regs = threads <= 320 ? 65536 / (threads * 96) : 1;
     if (per_sm > by_regs) per_sm = by_regs;
     if (per_sm > 16) per_sm = 16;

@@ -873,7 +873,10 @@ bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long
   const double flops = 2.0 * rows * N * K;
   // (halves that do not stay in L2 between the split and the product are read from memory)
   const double beyond = l + r > 60e6 ? l + r - 60e6 : 0.0;
-  const double here = 25.0 + (l + r) * 1.7e-6 + beyond * 2.3e-6 + flops / 590e6, there = 15.0 + l * 1.7e-6 + flops / 190e6;
+  // (whole reductions: a tile of 256 x 256 takes 0.85 us per 64 values of k, fewer rows less, on a pair of SMs)
+  const double even = (double)rows / experts, tiles = (double)((N + 255) / 256) * (rows / 256 + experts / 2 + 1), waves = ceil(tiles / (s->sm_count / 2));
+  const double tile = K * (0.85 / 64) * (even < 256 ? even / 256 : 1.0), product = waves * tile > flops / 590e6 ? waves * tile : flops / 590e6;
+  const double here = 25.0 + (l + r) * 1.7e-6 + beyond * 2.3e-6 + product, there = 15.0 + l * 1.2e-6 + flops / 120e6;
   return rows >= 96 * experts && here < there;
 }
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
@@ -882,7 +885,7 @@ bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, l
   if (operands * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * M, results = (double)experts * N * M;
-  const double here = 28.0 + operands * 1.85e-6 + results * 0.67e-6 + flops / 300e6, there = 12.0 + results * 1e-6 + flops / 150e6;
+  const double here = 28.0 + operands * 1.85e-6 + results * 0.67e-6 + flops / 300e6, there = 12.0 + results * 1e-6 + flops / 125e6;
   return rows >= 96 * experts && here < there;
 }
 

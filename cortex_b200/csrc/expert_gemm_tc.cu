@@ -7,8 +7,9 @@
 //
 // Every CTA finds its tile itself (groups::find_tile, ~1 us, while TMEM and barriers are set up); the grid is the most
 // tiles that the sizes allow, and CTAs without a tile leave at once.
-// Long reductions are cut into chunks: the tensor core adds with truncation, so every chunk's sum is rounded to nearest onto
-// C (or onto the slice's parked tile) and the accumulators restart from zero.
+// The tensor core adds with truncation, which shrinks a sum by about 2e-9 of itself for every value of k it runs over: an
+// accumulator takes RUN of them at most (512: 1.5e-6 of error against 64 bits, 256: 0.9e-6), several take turns, and what is
+// longer is cut into chunks whose sums are rounded to nearest onto C (or onto the slice's parked tile).
 //
 // Warp roles as in gemm_tf32x3_kernel: 0-7 lo tiles and epilogue, 8 TMA producer, 9 TMEM and MMA issue.
 #include "gemm3x_common.cuh"
@@ -21,6 +22,7 @@ using namespace gemm3x;
 namespace {
 
 constexpr int BM = 128;
+constexpr int RUN = 256;                                  // values of k that one main accumulator adds up at most
 constexpr int CONV_WARPS = 8;
 constexpr int THREADS = (CONV_WARPS + 2) * 32;
 
@@ -40,14 +42,14 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // The same kernel with the columns of B in the lanes (128 consecutive values of a row of C_e) and the columns of A, up
 // to BN of them, in the accumulator's columns: both operands reduce down their columns (MN-major), over the group's
 // rows; rows of the last k-block that belong to the next group are zeroed by the warps that compute the lo tiles.
-// K slices meet in L2 (how long a slice is depends on the group): the CTA that arrives last adds them in order and
-// stores; nobody waits.
+// K slices meet in L2 (how long a slice is depends on the group; products whose slices are longer than a chunk do it too):
+// the CTA that arrives last adds them in order and stores; nobody waits.
 struct RowsArgs {
   float* C;
   long long ldc;
   long long c_stride;          // WEIGHTS: distance of the experts' results
   int cols, tiles_r;           // WEIGHTS: rows of a result (columns of A), tiles of BN of them
-  float* park;                 // WEIGHTS with slices: parked tiles
+  float* park;                 // K slices that meet in L2: parked tiles
   int* arrived;                // and arrival counts, zero between launches
   const float* bias;           // [experts, N] or null
   const int* offsets;
@@ -66,10 +68,9 @@ template <int BN, int BK> struct RowsCfg {
   // narrow tiles: two CTAs per SM, one streaming while the other sets up or stores
   static constexpr int CTAS = BN <= 64 ? 2 : 1;
   static constexpr int STAGES = (196608 / CTAS / STAGE) > 8 ? 8 : (196608 / CTAS / STAGE);
-  // The tensor core adds with truncation, so a long run of additions shrinks a sum.  Tiles that leave TMEM room take turns
-  // between several main accumulators, joined in the epilogue; a reduction longer than a chunk goes out to C in between.
-  static constexpr int MAINS = BN == 32 ? 4 : (BN == 256 ? 1 : 3);
-  static constexpr int CHUNK = MAINS == 1 ? 1024 / BK : MAINS * 512 / BK;      // k-blocks
+  // main accumulators that take turns, joined in the epilogue; a reduction longer than a chunk goes out to C in between
+  static constexpr int MAINS = BN == 32 ? 4 : 3;
+  static constexpr int CHUNK = MAINS * RUN / BK;                               // k-blocks
   static constexpr int TMEM_COLS = BN == 32 ? 256 : (MAINS + 1) * BN;          // mains, then the cross terms
   static constexpr int BOX_ROWS = BN < 64 ? BN : 64;          // rows of one TMA box of the ragged operand
   static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
@@ -118,7 +119,6 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   typedef RowsCfg<BN, BK> C;
   constexpr int STAGES = C::STAGES, A_TILE = C::A_TILE;
   constexpr int W_BOX = BK * 128;                            // bytes of one 32 x BK box of an MN-major matrix
-  constexpr bool MMA_WHOLE = BN < 256;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = (uint64_t*)(smem + STAGES * C::STAGE);
@@ -195,7 +195,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   const bool empty = WEIGHTS && nkb == 0;
   if (empty) nkb = 1;
   const int n_chunks = (nkb + C::CHUNK - 1) / C::CHUNK, per = (nkb + n_chunks - 1) / n_chunks;
-  const int run = max((per + C::MAINS - 1) / C::MAINS, 256 / BK);              // k-blocks into one main accumulator
+  const int run = max((per + C::MAINS - 1) / C::MAINS, RUN / BK);              // k-blocks into one main accumulator
   const float* bias = p.bias ? p.bias + (long long)expert * p.N : nullptr;
 
   if (warp == CONV_WARPS) {
@@ -234,7 +234,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
     }
   } else if (warp == CONV_WARPS + 1) {
     // ------------------------------ MMA issuer --------------------------------
-    if (MMA_WHOLE || lane == 0) {
+    {
       const bool a_mn = WEIGHTS || p.w_mn;
       const uint32_t idesc = make_idesc_tf32(BM, (cols + 15) / 16 * 16, a_mn, WEIGHTS);
       constexpr uint32_t K_SWZ = BK == 32 ? SWZ_128B : SWZ_64B, K_SBO = 8 * BK * 4;
@@ -252,10 +252,10 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       for (int i = 0; i < nkb; ++i) {
         if (in_chunk == per) {
           // the chunk's sums go out before its accumulators are overwritten
-          if (!MMA_WHOLE || elect_one()) mma_commit(bar_acc);
-          if (MMA_WHOLE) __syncwarp();
+          if (elect_one()) mma_commit(bar_acc);
+          __syncwarp();
           ++commits;
-          if (!mbar_wait(bar_read, rph, abort_flag, p.status, 250)) break;
+          if (!warp_wait(bar_read, rph, abort_flag, p.status, 250)) break;
           rph ^= 1;
           tc_fence_after();
           in_chunk = in_run = 0;
@@ -269,9 +269,9 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         }
         ++in_chunk;
         ++in_run;
-        if (!mbar_wait(bar_conv + 8 * s, ph, abort_flag, p.status, 200 + s)) break;
+        if (!warp_wait(bar_conv + 8 * s, ph, abort_flag, p.status, 200 + s)) break;
         tc_fence_after();
-        if (!MMA_WHOLE || elect_one()) {
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BK / 8; ++kk) {
             const uint32_t al = a_low0 + stage_off + kk * a_step, bl = b_low0 + stage_off + kk * b_step;
@@ -282,11 +282,11 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
           mma_commit(bar_empty + 8 * s);
         }
         accumulate = cross = 1;
-        if (MMA_WHOLE) __syncwarp();
+        __syncwarp();
         if (++s == STAGES) { s = 0; ph ^= 1; stage_off = 0; } else { stage_off += STAGE_STEP; }
       }
-      if (!MMA_WHOLE || elect_one()) mma_commit(bar_acc);
-      if (MMA_WHOLE) __syncwarp();
+      if (elect_one()) mma_commit(bar_acc);
+      __syncwarp();
       if (*abort_flag) {
         // every MMA issued must have retired before TMEM is freed: the phase of the commit above
         for (int it = 0; it < (1 << 16); ++it)
@@ -354,7 +354,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(rc[j]));
         }
-        if (WEIGHTS && p.slices > 1) {
+        if (p.park) {
           float4* slot = reinterpret_cast<float4*>(p.park + ((long long)unit * p.slices + slice) * (BM * BN)) + (q * 32 + lane);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
@@ -383,7 +383,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
         if (lane == 0) mbar_arrive(bar_read);
       }
     }
-    if (WEIGHTS && p.slices > 1) {
+    if (p.park) {
       if (ok) __threadfence();
       asm volatile("bar.sync 1, %0;" ::"n"(CONV_WARPS * 32) : "memory");
       if (threadIdx.x == 0) where[5] = *abort_flag ? -1 : atomicAdd(p.arrived + unit, 1);
@@ -409,7 +409,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
             r[4 * j] = __float_as_uint(a[j].x); r[4 * j + 1] = __float_as_uint(a[j].y);
             r[4 * j + 2] = __float_as_uint(a[j].z); r[4 * j + 3] = __float_as_uint(a[j].w);
           }
-          store_columns(p, out, r, t0 + cc * 32, hi, n0 + q * 32 + lane, nullptr, p.beta, true);
+          store_columns(p, out, r, t0 + cc * 32, hi, n0 + q * 32 + lane, bias, p.beta, true);
         }
         if (threadIdx.x == 0) p.arrived[unit] = 0;           // left zero for the next launch
       }
@@ -418,7 +418,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
 
   tc_fence_before();
   __syncthreads();
-  if (!WEIGHTS && p.slices > 1) {
+  if (!WEIGHTS && p.slices > 1 && !p.park) {
     // Every thread of every CTA takes both barriers.  Between them the tile's 32 x 32 pieces are dealt round the cluster's
     // CTAs and warps, each summed in slice order whoever does it.
     cluster_sync_all();
@@ -474,7 +474,7 @@ template <int BN, int BK> struct StreamCfg {
   static constexpr int A_TILE = BM * BK * 4, B_TILE = BN * BK * 4, RAW = A_TILE + B_TILE, STAGE = 2 * RAW;
   static constexpr int STAGES = (196608 / STAGE) > 8 ? 8 : (196608 / STAGE);
   static constexpr int MAINS = BN == 128 ? 1 : 3, SET = (MAINS + 1) * BN;      // TMEM columns of a set of accumulators
-  static constexpr int CHUNK = MAINS == 1 ? 1024 / BK : MAINS * 512 / BK;      // k-blocks
+  static constexpr int CHUNK = MAINS * RUN / BK;      // k-blocks
   static constexpr int SMEM = STAGES * STAGE + 1024 + 1024;
   static_assert(2 * SET == 512, "two sets of accumulators");
 };
@@ -635,7 +635,7 @@ expert_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       if (!warp_wait(bar_read + 8 * set, ((it >> 1) & 1) ^ 1, abort_flag, p.status, 250 + set)) break;
       tc_fence_after();
       const uint32_t idesc = make_idesc_tf32(BM, (columns(e) + 15) / 16 * 16, a_mn, WEIGHTS);
-      const int run = max((e.nkb + C::MAINS - 1) / C::MAINS, 256 / BK);        // k-blocks into one main accumulator
+      const int run = max((e.nkb + C::MAINS - 1) / C::MAINS, RUN / BK);        // k-blocks into one main accumulator
       uint32_t tmem_main = tmem_base + set * C::SET, accumulate = 0, cross = 0;
       const uint32_t tmem_cross = tmem_main + C::MAINS * BN;
       int in_run = 0;
@@ -728,7 +728,7 @@ expert_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
       if (!e.more) break;
       if (!warp_wait(bar_acc + 8 * set, (uint32_t)((it >> 1) & 1), abort_flag, p.status, 400 + set)) break;
       tc_fence_after();
-      const int cols = columns(e), run = max((e.nkb + C::MAINS - 1) / C::MAINS, 256 / BK), mains = (e.nkb + run - 1) / run;
+      const int cols = columns(e), run = max((e.nkb + C::MAINS - 1) / C::MAINS, RUN / BK), mains = (e.nkb + run - 1) / run;
       const uint32_t lane_base = tmem_base + set * C::SET + ((uint32_t)(q * 32) << 16);
       float* const out = WEIGHTS ? p.C + e.expert * p.c_stride : p.C;
       const float* bias = p.bias ? p.bias + (long long)e.expert * p.N : nullptr;
@@ -838,17 +838,25 @@ int launch(cb200_stream* s, int smem, const CUtensorMap& tmA, const CUtensorMap&
   return CB200_OK;
 }
 
+// room for the slices of `units` tiles that meet in L2
+int get_park(cb200_stream* s, RowsArgs& a, long long units, int BN) {
+  void* ws = nullptr;
+  const int rc = cb200_partials(s, (size_t)units * a.slices * BM * BN * sizeof(float), &ws);
+  a.park = (float*)ws;
+  return rc ? rc : cb200_tile_flags(s, (size_t)units, &a.arrived);
+}
+
 // Tile width and K slices for `tiles_m` row tiles (an estimate for ragged groups) of N columns reduced over `nkb`
 // k-blocks: the timing model of gemm!, t = waves x (5 us + k-blocks per slice x c[BN]) + hand-over.
 void choose(const cb200_stream* s, long long tiles_m, int N, int nkb, int max_slices, int& bn_out, int& slices_out) {
-  const int bn_max = N > 128 ? 256 : (N > 64 ? 128 : 64);
+  const int bn_max = N > 64 ? 128 : 64;
   double best = 1e30;
   bn_out = bn_max;
   slices_out = 1;
-  for (int bn = 256; bn >= 64; bn >>= 1) {
+  for (int bn = 128; bn >= 64; bn >>= 1) {
     if (bn > bn_max) continue;
     if (s->opt_gemm_tile_n > 0 && bn != s->opt_gemm_tile_n && s->opt_gemm_tile_n <= bn_max) continue;
-    const double c = bn == 256 ? 0.56 : (bn == 128 ? 0.455 : 0.39);
+    const double c = bn == 128 ? 0.455 : 0.39;
     const long long tiles = tiles_m * ((N + bn - 1) / bn);
     for (int sl = 1; sl <= max_slices; ++sl) {
       if (sl > 1 && (tiles * sl > s->sm_count || nkb / sl < 4)) break;
@@ -873,8 +881,8 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   DeviceGuard guard(s->device);
   // how many rows a tile may take: what an even split of the rows over the experts fills
   const long long even = (rows + experts - 1) / experts;
-  int BN = even <= 32 ? 32 : (even <= 64 ? 64 : (even <= 128 ? 128 : 256));
-  if (s->opt_gemm_tile_n > 0) BN = s->opt_gemm_tile_n;
+  int BN = even <= 32 ? 32 : (even <= 64 ? 64 : 128);
+  if (s->opt_gemm_tile_n > 0) BN = s->opt_gemm_tile_n < 128 ? s->opt_gemm_tile_n : 128;
   const bool forced = s->opt_gemm_tile_n > 0 || s->opt_gemm_k_slices > 0;
   int bk = 0;
   long long units = 0;
@@ -883,18 +891,25 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
     units = ((rows + BN - 1) / BN + (experts < rows ? experts : rows) - 1) * ((N + BM - 1) / BM);
   };
   cut();
-  // K slices (the CTAs of a cluster) where the tiles leave SMs free; a slice is one chunk, since its parked tile lies in
-  // shared memory that the next chunk's stages would need
-  const int chunk = BN == 256 ? RowsCfg<256, 16>::CHUNK : (BN == 128 ? RowsCfg<128, 16>::CHUNK : (BN == 64 ? RowsCfg<64, 32>::CHUNK : RowsCfg<32, 32>::CHUNK));
+  // K slices where the tiles leave SMs free: the CTAs of a cluster if a slice is one chunk (its parked tile lies in shared
+  // memory that the next chunk's stages would need), else CTAs that meet in L2 (3 experts of 600 x 4000 with 300 rows each
+  // 155 us uncut)
+  const int chunk = BN == 128 ? RowsCfg<128, 16>::CHUNK : (BN == 64 ? RowsCfg<64, 32>::CHUNK : RowsCfg<32, 32>::CHUNK);
   const int nkb = (K + bk - 1) / bk, wanted = s->opt_gemm_k_slices;
+  const long long room = s->sm_count * (BN <= 64 ? 2 : 1);
   int slices = 1;
+  bool meet = false;
   for (int sl = 2; sl <= 8; sl *= 2)
-    if ((wanted > 0 ? sl <= wanted : units * sl <= s->sm_count * (BN <= 64 ? 2 : 1)) && nkb / sl >= 4) slices = sl;
-  if ((nkb + slices - 1) / slices > chunk || only_if) slices = 1;
-  // Short reductions in tiles that follow one another (this / the kernel of one tile a CTA, us): 16 experts of 2048 x 128 with
-  // 64, 256 rows each 18, 33 / 22, 39; 32 of 1024 x 1024 with 32, 64, 128, 256 rows 53, 76, 109, 175 / 77, 89, 121, 151; 64 of
-  // 1024 x 4096 with 32, 64 rows 406, 559 / 406, 467.
-  const bool stream = !forced && slices == 1 && (K <= 256 || (K <= 1024 && even <= 128));
+    if ((wanted > 0 ? sl <= wanted : units * sl <= room) && nkb / sl >= 4) slices = sl;
+  if ((nkb + slices - 1) / slices > chunk) {
+    meet = slices > 1;
+    if (meet && wanted == 0) slices = (int)(room / units < 16 ? room / units : 16);
+  }
+  if (only_if) { slices = 1; meet = false; }
+  // Tiles that follow one another where nothing is sliced (this / the kernel of one tile a CTA, us): 16 experts of 2048 x 128
+  // with 64, 256 rows each 18, 33 / 22, 39; 32 of 1024 x 1024 with 32, 64, 128 rows 53, 76, 109 / 77, 89, 121; but two narrow
+  // tiles to an SM are faster at long reductions: 64 of 1024 x 4096 with 20, 64 rows 417, 559 / 285, 467.
+  const bool stream = !forced && slices == 1 && (K <= 1024 || even > 64);
   if (stream) {
     BN = even <= 64 ? 64 : 128;
     cut();
@@ -906,23 +921,24 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   a.alpha = alpha; a.beta = beta; a.slices = slices; a.only_if = only_if;
   const CUtensorMapSwizzle swz = bk == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tmW, tmX;
-  int rc = tmap_2d(&tmX, A, rows, K, lda, bk, BN < 64 ? BN : 64, swz);
-  if (rc) return rc;
+  int rc;
+  CB_REQUIRE(units * slices <= 2147483647LL, "expert_gemm: too many tiles");
+  if (meet && (rc = get_park(s, a, units, BN))) return rc;
+  if ((rc = tmap_2d(&tmX, A, rows, K, lda, bk, BN < 64 ? BN : 64, swz))) return rc;
   if (trans_b) rc = tmap_3d(&tmW, B, experts, N, K, ldb, b_stride, bk, BM, swz);
   else rc = tmap_3d(&tmW, B, experts, K, N, ldb, b_stride, 32, bk, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B);
   if (rc) return rc;
-  CB_REQUIRE(units <= 2147483647LL, "expert_gemm: too many tiles");
   a.units = (int)units;
+  const int cluster = meet ? 1 : slices;
   if (stream) {
     const long long ctas = units < s->sm_count ? units : s->sm_count;
     if (BN == 128) return launch<RowsArgs, expert_stream_kernel<128, 16, false>>(s, StreamCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
     return launch<RowsArgs, expert_stream_kernel<64, 32, false>>(s, StreamCfg<64, 32>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
   }
   const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
-  if (BN == 256) return launch<RowsArgs, expert_tf32x3_kernel<256, 16, false>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, slices);
-  if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, false>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, slices);
-  if (BN == 64) return launch<RowsArgs, expert_tf32x3_kernel<64, 32, false>>(s, RowsCfg<64, 32>::SMEM, tmW, tmX, a, ctas, slices);
-  return launch<RowsArgs, expert_tf32x3_kernel<32, 32, false>>(s, RowsCfg<32, 32>::SMEM, tmW, tmX, a, ctas, slices);
+  if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, false>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, cluster);
+  if (BN == 64) return launch<RowsArgs, expert_tf32x3_kernel<64, 32, false>>(s, RowsCfg<64, 32>::SMEM, tmW, tmX, a, ctas, cluster);
+  return launch<RowsArgs, expert_tf32x3_kernel<32, 32, false>>(s, RowsCfg<32, 32>::SMEM, tmW, tmX, a, ctas, cluster);
 }
 
 int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows,
@@ -946,12 +962,7 @@ int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long 
   a.units = (int)units;
   const long long ctas = only_if && units > s->sm_count ? s->sm_count : units * slices;
   int rc;
-  if (slices > 1) {
-    void* ws = nullptr;
-    if ((rc = cb200_partials(s, (size_t)units * slices * BM * BN * sizeof(float), &ws))) return rc;
-    if ((rc = cb200_tile_flags(s, (size_t)units, &a.arrived))) return rc;
-    a.park = (float*)ws;
-  }
+  if (slices > 1 && (rc = get_park(s, a, units, BN))) return rc;
   CUtensorMap tmW, tmX;
   if ((rc = tmap_2d(&tmW, B, rows, N, ldb, 32, 16, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
   if ((rc = tmap_2d(&tmX, A, rows, M, lda, 32, 16, CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))) return rc;
@@ -960,7 +971,6 @@ int cb200_expert_weights_tc(cb200_stream* s, float* C, long long c_stride, long 
     if (BN == 128) return launch<RowsArgs, expert_stream_kernel<128, 16, true>>(s, StreamCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
     return launch<RowsArgs, expert_stream_kernel<64, 16, true>>(s, StreamCfg<64, 16>::SMEM, tmW, tmX, a, ctas, 1, STREAM_THREADS);
   }
-  if (BN == 256) return launch<RowsArgs, expert_tf32x3_kernel<256, 16, true>>(s, RowsCfg<256, 16>::SMEM, tmW, tmX, a, ctas, 1);
   if (BN == 128) return launch<RowsArgs, expert_tf32x3_kernel<128, 16, true>>(s, RowsCfg<128, 16>::SMEM, tmW, tmX, a, ctas, 1);
   return launch<RowsArgs, expert_tf32x3_kernel<64, 16, true>>(s, RowsCfg<64, 16>::SMEM, tmW, tmX, a, ctas, 1);
 }

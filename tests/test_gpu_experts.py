@@ -70,6 +70,12 @@ PRODUCTS = [
     (40, [9, 8, 7, 6, 5, 4], 500, 784), (600, [64, 65, 63, 128, 192, 1, 87], 68, 1028), (1000, [700, 200], 132, 516),
     (3, [1, 1, 1], 1001, 333), (512, [511, 1], 257, 129), (96, [3] * 32, 40, 2052), (33, [16, 17], 4, 8),
     (70, [1] * 70, 20, 12),
+    # few rows with long reductions (K slices), a group that outgrows the estimate its kernel was chosen by, short reductions in
+    # many tiles, few tiles with long reductions
+    (8, [1] * 8, 260, 1028), (14, [8, 0, 3, 1], 129, 2051), (4, [2, 2], 40, 4096), (99, [60, 1, 0, 35], 300, 520), (180, [90, 90], 1000, 68),
+    (9, [0, 0, 7], 64, 64), (16, [0, 0, 16, 0], 257, 130), (515, [500, 0, 0, 0, 0, 12], 132, 260), (2103, [0, 2100, 3], 72, 100),
+    (1320, [1300] + [1] * 14, 200, 136), (1200, [40] * 30, 516, 250), (450, [64, 65, 63, 1, 128, 129], 260, 256), (932, [400, 532], 20, 3332),
+    (3000, [1000, 2000], 32, 36), (1040, [1024, 5, 11], 200, 1400),
 ]
 
 
@@ -256,7 +262,8 @@ def test_expert_gemm_many_experts_and_no_rows(stream):
 
 # rows, cols, gate rows (0 = none)
 BLOCKS = [(1, 1, 0), (1, 5, 1), (3, 8, 3), (4, 100, 2), (7, 129, 7), (16, 1024, 4), (12, 2500, 3), (5, 4096, 1), (300, 64, 1),
-          (257, 36, 257), (1000, 40, 125), (90, 513, 9), (2, 9000, 1), (3, 20001, 3), (6, 8192, 2), (640, 260, 5), (2000, 16, 2)]
+          (257, 36, 257), (1000, 40, 125), (90, 513, 9), (2, 9000, 1), (3, 20001, 3), (6, 8192, 2), (640, 260, 5), (2000, 16, 2),
+          (700, 4100, 7), (5, 4101, 5), (4, 6001, 1), (301, 2101, 1), (9, 4097, 0)]
 
 
 def _block_inputs(rows, d, gate_rows, with_after, with_bias, datatype, seed):
