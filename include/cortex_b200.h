@@ -429,8 +429,14 @@ int cb200_graph_destroy(cb200_graph* g);
  *     A is the gradient of the layer's output, B its input.  Empty groups: beta * C_e.
  * float / double, at most 4096 experts; with beta = 0 what C held is not read.  C must not overlap the other operands.
  * Offsets that decrease or leave [0, rows] are clamped on the device (nothing outside the operands is touched, rows are
- * never computed twice) and the call is reported as CB200_ERR_CUDA by the next cb200_stream_sync.  fp32 operands are
- * multiplied on the tensor cores with the split arithmetic of gemm!. */
+ * never computed twice) and the call is reported as CB200_ERR_CUDA by the next cb200_stream_sync.
+ * fp32 arithmetic, by the sizes: plain FMAs (few rows per expert), the split arithmetic of gemm!, or (large products) operands as
+ * two fp16 halves of values scaled by a power of two per row or column, where the data allow it: a value's place below its row's
+ * largest is checked on the device, and a call whose data do not fit falls back to the former inside its own launches.  Either
+ * way results of data of one magnitude are within about 1e-6 of the 64-bit ones (relative to their norm).  A row with an infinity or a
+ * NaN gives no finite result, but may give NaN where exact arithmetic gives an infinity.  Of the options below, gemm-auto-presplit
+ * (1: never halves, 2: always), gemm-tile-n (32, 64, 128: rows or result rows per tile; larger values mean 128) and gemm-k-slices
+ * steer these calls too. */
 int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int trans_b, double alpha, const void* A,
                       int64_t rows, int64_t a_cols, int64_t lda, const void* B, int64_t experts, int64_t b_cols,
                       int64_t b_stride, int64_t ldb, double beta, const int32_t* offsets, const void* bias, int act);
