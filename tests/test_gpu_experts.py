@@ -614,12 +614,22 @@ def test_expert_gemm_scaled_halves(stream, route, n, k):
 @pytest.mark.parametrize("way", ["forward", "input", "weights"])
 @pytest.mark.parametrize("route,sizes,n,k", [(1, [200, 0, 56], 264, 512), (1, [20, 4, 8], 264, 512), (2, [200, 0, 56], 264, 512)])
 def test_expert_gemm_waits_that_run_out(b200_driver, way, route, sizes, n, k):
+    _waits_that_run_out(b200_driver, way, route, sizes, n, k, 128 if route == 1 else 0)  # (tensor cores also where there are few rows)
+
+
+# tiles that follow one another, 128 and 64 wide; slices that meet in L2, of a product and of a weight gradient
+@pytest.mark.parametrize("way,sizes,n,k", [("forward", [200, 0, 56], 264, 512), ("input", [20, 9, 8], 264, 512), ("weights", [100, 0, 56], 264, 512),
+                                           ("forward", [200, 0, 56], 264, 16000), ("weights", [400, 0, 112], 264, 512)])
+def test_expert_gemm_waits_that_run_out_by_sizes(b200_driver, way, sizes, n, k):
+    _waits_that_run_out(b200_driver, way, 1, sizes, n, k, 0)
+
+
+def _waits_that_run_out(b200_driver, way, route, sizes, n, k, tile_n):
     """Producers that deliver nothing (a setting, not a fault): every role gives up in time, the sync raises, and the next call
     on the stream is right."""
     s = b200_driver.default_device().create_stream()
     s.set_option("gemm-auto-presplit", route)
-    if route == 1:
-        s.set_option("gemm-tile-n", 128)            # (the tensor-core kernel also where there are few rows)
+    s.set_option("gemm-tile-n", tile_n)
     rng = np.random.default_rng(5)
     rows, off = sum(sizes), _offsets(sizes)
     X, dY, W = (rng.standard_normal(sh).astype(np.float32) for sh in ((rows, k), (rows, n), (3, n, k)))
