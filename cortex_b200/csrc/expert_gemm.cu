@@ -820,11 +820,14 @@ int weights_tc(cb200_stream* s, Product<float> p) {
   return cb200_expert_weights_tc(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta, p.offsets, p.only_if);
 }
 
+// kernels step 32-bit indexes past the last row and column, by a tile or a warp's stride at most
+constexpr int64_t MAX_EXTENT = 2147483647LL - 65535;
+
 int check_common(const char* what, cb200_stream* s, int dtype, const void* C, const void* A, const void* B, int64_t rows,
                  int64_t experts, const int32_t* offsets) {
   CB_REQUIRE(s && C && A && B && offsets, "%s: null argument", what);
   CB_REQUIRE(dtype == CB200_FLOAT || dtype == CB200_DOUBLE, "%s: only defined for float and double tensors", what);
-  CB_REQUIRE(rows >= 0 && rows <= 2147483647LL, "%s: bad row count", what);
+  CB_REQUIRE(rows >= 0 && rows <= MAX_EXTENT, "%s: bad row count", what);
   CB_REQUIRE(experts >= 1 && experts <= groups::MAX_EXPERTS, "%s: %lld experts outside [1, %d]", what, (long long)experts,
              (int)groups::MAX_EXPERTS);
   const uintptr_t size = cb200_dtype_size(dtype);
@@ -858,7 +861,7 @@ int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int tran
                       double beta, const int32_t* offsets, const void* bias, int act) {
   int rc = check_common("expert_gemm", s, dtype, C, A, B, rows, experts, offsets);
   if (rc) return rc;
-  CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= 2147483647LL && b_cols <= 2147483647LL, "expert_gemm: bad extents");
+  CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= MAX_EXTENT && b_cols <= MAX_EXTENT, "expert_gemm: bad extents");
   CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= (trans_b ? a_cols : b_cols), "expert_gemm: pitch smaller than the row");
   CB_REQUIRE(b_stride >= (trans_b ? b_cols : a_cols) * ldb || experts == 1, "expert_gemm: the experts' matrices overlap");
   CB_REQUIRE(act >= CB200_ACT_NONE && act <= CB200_ACT_LOGISTIC, "expert_gemm: unknown activation %d", act);
@@ -875,7 +878,7 @@ int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_str
                               int64_t experts, double beta, const int32_t* offsets, void* bias_gradient) {
   int rc = check_common("expert_gemm_weights", s, dtype, C, A, B, rows, experts, offsets);
   if (rc) return rc;
-  CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= 2147483647LL && b_cols <= 2147483647LL, "expert_gemm_weights: bad extents");
+  CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= MAX_EXTENT && b_cols <= MAX_EXTENT, "expert_gemm_weights: bad extents");
   CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= b_cols, "expert_gemm_weights: pitch smaller than the row");
   CB_REQUIRE(c_stride >= a_cols * ldc || experts == 1, "expert_gemm_weights: the experts' matrices overlap");
   if (dtype == CB200_FLOAT) {

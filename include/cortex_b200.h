@@ -427,7 +427,7 @@ int cb200_graph_destroy(cb200_graph* g);
  *   expert_gemm_weights:  C_e = alpha * sum_{r in group e} A[r, :]^T B[r, :] + beta * C_e   (C_e [a_cols, b_cols])
  *     and, where bias_gradient is not NULL, bias_gradient[e, :] = alpha * sum_{r in group e} A[r, :] + beta * bias_gradient[e, :]
  *     A is the gradient of the layer's output, B its input.  Empty groups: beta * C_e.
- * float / double, at most 4096 experts; with beta = 0 what C held is not read.  C must not overlap the other operands.
+ * float / double, at most 4096 experts, extents of at most 2^31 - 65536; with beta = 0 what C held is not read.  C must not overlap the other operands.
  * Offsets that decrease or leave [0, rows] are clamped on the device (nothing outside the operands is touched, rows are
  * never computed twice) and the call is reported as CB200_ERR_CUDA by the next cb200_stream_sync.
  * fp32 arithmetic, by the sizes: plain FMAs (few rows per expert), the split arithmetic of gemm!, or (large products) operands as

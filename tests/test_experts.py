@@ -188,6 +188,17 @@ def test_c_abi_expert_refusals():
         _refused(c[0], *c[1:], match=text)
 
 
+@pytest.mark.parametrize("extent", [2 ** 31 - 65535, 2 ** 31 - 1, 2 ** 31])
+def test_c_abi_expert_extents_leave_room_for_the_kernels_indexes(extent):
+    """Kernels step 32-bit indexes past the last row and column by a tile at most."""
+    big = 2 ** 33
+    _refused("cb200_expert_gemm", 4, P, big, 1, 1.0, P + 4096, 4, extent, big, P + 8192, 1, 8, 64, big, 0.0, P + 16384, None, 0, match="extents")
+    _refused("cb200_expert_gemm", 4, P, big, 1, 1.0, P + 4096, 4, 8, big, P + 8192, 1, extent, 64, big, 0.0, P + 16384, None, 0, match="extents")
+    _refused("cb200_expert_gemm", 4, P, big, 1, 1.0, P + 4096, extent, 8, big, P + 8192, 1, 8, 64, big, 0.0, P + 16384, None, 0, match="row count")
+    for m, n in ((extent, 8), (8, extent)):
+        _refused("cb200_expert_gemm_weights", 4, P, 64, big, 1.0, P + 4096, 4, m, big, P + 8192, n, big, 1, 0.0, P + 16384, None, match="extents")
+
+
 def test_c_abi_block_refusals():
     M = [P + i * 65536 for i in range(12)]
 
