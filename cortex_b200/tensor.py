@@ -628,13 +628,35 @@ def _span(t):
     return t.buffer.ptr, t.buffer.ptr + (last + 1) * DTYPE_SIZE[t.buffer.dtype]
 
 
+def _overlap(x, y):
+    """Do two tensors share memory?  Most live in buffers of their own, which the buffers' bounds tell."""
+    p, q = x.buffer, y.buffer
+    if p.ptr + p.n * DTYPE_SIZE[p.dtype] <= q.ptr or q.ptr + q.n * DTYPE_SIZE[q.dtype] <= p.ptr:
+        return False
+    (lo, hi), (a, b) = _span(x), _span(y)
+    return hi > a and b > lo
+
+
+def _buffers_apart(written, others):
+    """Do the buffers of `written` lie apart from one another and from those of `others` (None is skipped), as far as the
+    buffers' bounds tell?  (False: the tensors themselves may still be apart.)"""
+    spans = list({(b.ptr, b.ptr + b.n * DTYPE_SIZE[b.dtype]) for b in [t.buffer for t in others if t is not None]})
+    for t in written:
+        b = t.buffer
+        spans.append((b.ptr, b.ptr + b.n * DTYPE_SIZE[b.dtype]))
+    spans.sort()
+    end = 0
+    for lo, hi in spans:
+        if lo < end:
+            return False
+        end = hi
+    return True
+
+
 def _ensure_apart(dest, name, *others):
-    lo, hi = _span(dest)
     for o in others:
-        if o is not None:
-            a, b = _span(o)
-            if hi > a and b > lo:
-                raise TensorError("%s overlaps another argument: %r %r" % (name, dest, o))
+        if o is not None and _overlap(dest, o):
+            raise TensorError("%s overlaps another argument: %r %r" % (name, dest, o))
 
 
 def _packed(t):
@@ -838,13 +860,15 @@ def block_normalize_gradients(block_gradient, residual_gradient, gate_gradient, 
     sum_addresses = _block_vectors(cols, ga_scale, ga_bias, gb_scale, gb_bias)
     others = [block_gradient, residual_gradient, gate_gradient, output_gradient, total_gradient, total, block, gate, a_scale,
               a_bias, b_scale]
-    spans = [_span(t) for t in others if t is not None]
-    for t in sums:                                   # the vectors that are written share no memory with anything else
-        lo, hi = span = _span(t)
-        for a, b in spans:
-            if hi > a and b > lo:
-                raise TensorError("The gradient of a scale or bias overlaps another argument: %r" % (t,))
-        spans.append(span)
+    # the vectors that are written share no memory with anything else
+    if sums and not _buffers_apart(sums, others):
+        spans = [_span(t) for t in others if t is not None]
+        for t in sums:
+            lo, hi = span = _span(t)
+            for a, b in spans:
+                if hi > a and b > lo:
+                    raise TensorError("The gradient of a scale or bias overlaps another argument: %r" % (t,))
+            spans.append(span)
     check_stream().block_normalize_gradients(
         datatype, _block_matrices(shape, block_gradient) + [residual_gradient.buffer.ptr, pitch],
         [_address(gate_gradient)] + sum_addresses,
