@@ -162,11 +162,12 @@ __device__ __forceinline__ void load8(const float* p, int left, bool vec, float 
 //   RAGGED = 0  the experts' matrices: row r at x + (r / rows_per) * stride + (r % rows_per) * ld
 //   RAGGED = 1  the ragged rows: rows in no group become zeros and have no say in the flag
 //   RAGGED = 2  the same, every value multiplied by 2^14 fold[expert of the row][column] first: the inverse scales of a matrix
-//               whose rows run along the reduction, which cannot be taken out of the sum behind it
+//               whose rows run across the reduction, which cannot be taken out of the sum behind it
+// zero_scale: a row of zeros gets the inverse scale 0, not 1
 template <int TPR, int RAGGED>
 __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
                                                          long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan,
-                                                         const float* fold, const int* begins, int experts) {
+                                                         const float* fold, const int* begins, int experts, bool zero_scale) {
   constexpr int HOLD = 4;
   wait_for_previous_kernel();
   __shared__ uint32_t part_max[8];
@@ -257,7 +258,9 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
     for (int w = 0; w < TPR / 32; ++w) tiny += part_tiny[sub * (TPR / 32) + w];
   }
   if (t == 0 && live) {
-    down_out[r] = down;
+    // (a scale of 0 that is folded into the other operand takes what meets a row of zeros out of its row's maximum, but for
+    // infinities and NaN)
+    down_out[r] = zero_scale && m == 0 ? 0.f : down;
     if (!ok || (long long)tiny * 64 > cols) plan->flag = 1;
   }
 }
@@ -802,15 +805,16 @@ int launch_next(cb200_stream* s, void (*kernel)(P...), dim3 grid, int threads, s
 
 template <int RAGGED>
 int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
-               long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0) {
+               long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0,
+               bool zero_scale = false) {
   if (cols <= 1024)
     return launch_next(s, split_rows_kernel<32, RAGGED>, dim3((unsigned)((rows + 7) / 8)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
-                       rows, cols, kp, plan, fold, begins, experts);
+                       rows, cols, kp, plan, fold, begins, experts, zero_scale);
   if (cols <= 4096)
     return launch_next(s, split_rows_kernel<128, RAGGED>, dim3((unsigned)((rows + 1) / 2)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
-                       rows, cols, kp, plan, fold, begins, experts);
+                       rows, cols, kp, plan, fold, begins, experts, zero_scale);
   return launch_next(s, split_rows_kernel<256, RAGGED>, dim3((unsigned)rows), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
-                     plan, fold, begins, experts);
+                     plan, fold, begins, experts, zero_scale);
 }
 
 // `sums` (may be null): workspace for the column sums of 64-row blocks, ((rows + 63) / 64 + groups_n) x cols
@@ -916,7 +920,9 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   float* r_down = w.take<float>((size_t)rows);
   plan_kernel<<<1, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev, nullptr, 0);
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan))) return rc;
+  if ((rc = split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, nullptr, nullptr, 0,
+                          !trans_b)))
+    return rc;
   if (trans_b) rc = split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan);
   else rc = split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, l_down, begins, experts);
   if (rc) return rc;

@@ -1,0 +1,111 @@
+"""Products grouped by expert on data that is hard on their arithmetic: values far below the largest of their row or column,
+alone where the other operand is not zero; zeros; infinities and NaN under an activation.  Tolerances: test_gpu_experts."""
+import numpy as np
+import pytest
+
+from cortex_b200 import tensor as ct
+from oracle import plain_operators as plain
+from test_gpu_experts import _offsets, _product_tol, _within, stream  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# by size and always through scaled halves; the first sizes take them by themselves, the others are no multiple of anything
+SHAPES = [(0, [700, 600, 0, 748], 2048, 1024), (2, [300, 0, 1, 130, 3, 31], 258, 129), (2, [90, 200], 130, 514)]
+
+
+def _data(seed, sizes, n, k, tail=3):
+    rng = np.random.default_rng(seed)
+    rows = sum(sizes) + tail
+    X, dY, W = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (rows, n), (len(sizes), n, k)))
+    return rng, X, dY, W
+
+
+def _forward(X, W, sizes, act=None, bias=None):
+    Y = ct.new_tensor([len(X), W.shape[1]], "float")
+    ct.expert_gemm(Y, True, 1.0, ct.to_tensor(X, "float"), ct.to_tensor(W, "float"), 0.0, ct.to_tensor(_offsets(sizes), "int"), act=act)
+    return ct.to_array(Y).reshape(len(X), W.shape[1])
+
+
+def _input(dY, W, sizes):
+    dX = ct.new_tensor([len(dY), W.shape[2]], "float")
+    ct.expert_gemm(dX, False, 1.0, ct.to_tensor(dY, "float"), ct.to_tensor(W, "float"), 0.0, ct.to_tensor(_offsets(sizes), "int"))
+    return ct.to_array(dX).reshape(len(dY), W.shape[2])
+
+
+def _weights(dY, X, sizes):
+    e, n, k = len(sizes), dY.shape[1], X.shape[1]
+    dW, db = ct.new_tensor([e, n, k], "float"), ct.new_tensor([e, n], "float")
+    ct.expert_gemm_weights(dW, 1.0, ct.to_tensor(dY, "float"), ct.to_tensor(X, "float"), 0.0, ct.to_tensor(_offsets(sizes), "int"),
+                           bias_gradient=db)
+    return ct.to_array(dW).reshape(e, n, k)
+
+
+def _hold(way, sizes, X, dY, W):
+    """The product against 64 bits, every element within the bound of its own terms."""
+    zeros = np.zeros
+    if way == "forward":
+        want, size = plain.expert_gemm(zeros((len(X), W.shape[1])), True, 1.0, X, W, 0.0, _offsets(sizes))
+        _within(_forward(X, W, sizes), want, size, _product_tol("float", W.shape[2]), way)
+    elif way == "input":
+        want, size = plain.expert_gemm(zeros((len(dY), W.shape[2])), False, 1.0, dY, W, 0.0, _offsets(sizes))
+        _within(_input(dY, W, sizes), want, size, _product_tol("float", W.shape[1]), way)
+    else:
+        want, size = plain.expert_gemm_weights(zeros(W.shape), 1.0, dY, X, 0.0, _offsets(sizes))[:2]
+        _within(_weights(dY, X, sizes), want, size, _product_tol("float", max(sizes)), way)
+
+
+# ---- which way a call went: the fallback leaves the bits of a call that is certain to fall back ---------------------------
+
+def _fell_back(way, sizes, X, dY, W):
+    """Appends a group with a row outside the halves' range, which sends the whole call to the other kernels; were the other
+    groups' results the same bits without it?"""
+    more = sizes + [1]
+    at = sum(sizes)
+    big = lambda a: np.concatenate([a[:at], np.full((1, a.shape[1]), 1e25, np.float32), a[at:]])
+    W2 = np.concatenate([W, W[:1]])
+    run = {"forward": lambda s, x, d, w: _forward(x, w, s)[:at], "input": lambda s, x, d, w: _input(d, w, s)[:at],
+           "weights": lambda s, x, d, w: _weights(d, x, s)[:len(sizes)]}[way]
+    return np.array_equal(run(sizes, X, dY, W), run(more, big(X), big(dY), W2))
+
+
+def _relu(x):
+    return np.maximum(x, 0.0)
+
+
+@pytest.mark.parametrize("way", ["forward", "input", "weights"])
+def test_ordinary_data_stays_on_halves(stream, way):  # noqa: F811
+    stream.set_option("gemm-auto-presplit", 2)
+    sizes, n, k = [300, 1, 256, 90, 0, 31], 260, 520
+    rng, X, dY, W = _data(23, sizes, n, k)
+    assert not _fell_back(way, sizes, X, dY, W)
+    if way == "forward":
+        assert not _fell_back(way, sizes, _relu(X), dY, W)
+    elif way == "input":
+        assert not _fell_back(way, sizes, X, dY * (rng.random(dY.shape) < 0.5), W)
+    else:
+        assert not _fell_back(way, sizes, _relu(X), dY, W)
+        assert not _fell_back(way, sizes, X, dY * (rng.random(dY.shape) < 0.5), W)
+    large = np.float32(1e25)
+    assert _fell_back(way, sizes, X * (large if way == "forward" else 1), dY * (large if way != "forward" else 1), W)
+
+
+def test_a_row_of_zeros_stays_on_halves_input(stream):  # noqa: F811
+    """An output feature without weights (pruned, or padding) in one matrix, and a NaN that meets it."""
+    stream.set_option("gemm-auto-presplit", 2)
+    sizes, n, k = [300, 1, 256], 260, 520
+    rng, X, dY, W = _data(29, sizes, n, k)
+    W[0, 17] = 0.0
+    W[2, :5] = 0.0
+    assert not _fell_back("input", sizes, X, dY, W)
+    _hold("input", sizes, X, dY, W)
+    W[:, :, 33] = 0.0                                           # and an input feature without any
+    assert not _fell_back("input", sizes, X, dY, W)
+    _hold("input", sizes, X, dY, W)
+    W[2] = 0.0
+    assert not _fell_back("input", sizes, X, dY, W)
+    _hold("input", sizes, X, dY, W)
+    for bad in (np.nan, np.inf):                                # 0 * NaN and 0 * infinity are NaN
+        dY2 = dY.copy()
+        dY2[4, 17] = bad
+        got = _input(dY2, W, sizes)
+        assert np.isnan(got[4]).all() and np.isfinite(np.delete(got[:sum(sizes)], 4, 0)).all()
