@@ -4,10 +4,10 @@
 //   x * s = h1 + h2,   h1 = half(x * s),  h2 = half(x * s - h1),   s = a power of two per operand row
 // carries 22 bits like hi + lo of 3xTF32 does, and the three products h1 h1, h1 h2, h2 h1 cost half of what they cost
 // there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-17 of
-// it keep their 22 bits, smaller ones an absolute error of 2^-39 of it.  Rows for which that is not good enough -- more
-// than 1 in 64 values (not counting zeros) below 2^-17 of the row's largest, a largest value outside [2^-48, 2^60], an
-// infinity or a NaN -- raise a flag in device memory; the kernel here then does nothing and the 3xTF32 kernel launched
-// behind it, which otherwise does nothing, does the work.  So results have the accuracy of gemm! whatever the data.
+// it keep their 22 bits, smaller ones an absolute error of 2^-39 of it.  Where that could show in an element of the result
+// (fits() has the condition and the proof: what is lost stays below 2^-18 of the sum of the element's |a||b|), where a
+// row's largest value is outside [2^-48, 2^60], and where there is an infinity or a NaN, a flag is raised in device memory;
+// the kernel here then does nothing and the 3xTF32 kernel launched behind it, which otherwise does nothing, does the work.
 //
 // Steps of a call: group bounds and the table of tiles (one warp); the operands' halves, K-contiguous, with their scales
 // (HBM-bound; operands whose reduction axis is not contiguous get a pass for the column maxima first); the product; the
@@ -57,6 +57,17 @@ struct Plan {
   int first_row, end_row;      // rows outside are in no group
   int unused[3];
 };
+// How an expert's rows of halves (of either operand, along the reduction) lie in the halves' range, rows of zeros apart.  All
+// zero at the start of a call.
+struct alignas(16) Fit {
+  int bad;                     // a row's largest value is outside the range of the scales
+  int deep;                    // a value is below DEEP, and not 0
+  int thin[2];                 // most values below BIG in a row, zeros too: of the lanes' operand, of the columns'
+  int tiny[2];                 // most values below TINY in a row, without the zeros
+  int unused[2];
+};
+// of a scaled value (a row's largest: 2^14 to 2^15)
+constexpr float BIG = 16.f, TINY = 0.125f, DEEP = 1.f / 64;
 struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); expert_gemm_weights: rows and first padded position
 
 // bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
@@ -93,7 +104,10 @@ __global__ void __launch_bounds__(128) plan_kernel(Plan* plan, Entry* table, int
     if (lane == 0) before = carry_max;
     lo = max(lo, before);
     hi = max(hi, lo);
-    if (e < experts && begins) begins[e] = lo;
+    if (e < experts && begins) {
+      begins[e] = lo;
+      if (e == experts - 1) begins[experts] = hi;
+    }
     if (e < experts && hi > lo) first_row = min(first_row, lo);
     const int mine = e < experts ? (weights ? (hi - lo + BK - 1) / BK * BK : (hi - lo + BN - 1) / BN) : 0;
     int sum = mine;
@@ -139,13 +153,28 @@ __device__ __forceinline__ bool scale_of(uint32_t max_bits, float& up, float& do
   down = __uint_as_float((uint32_t)(127 - e) << 23);
   return ok;
 }
-__device__ __forceinline__ void split_half(float y, __half& h1, __half& h2, int& tiny) {
+__device__ __forceinline__ void split_half(float y, __half& h1, __half& h2) {
   h1 = __float2half_rn(y);
   h2 = __float2half_rn(y - __half2float(h1));
-  const float a = fabsf(y);
-  tiny += a < 0.125f && a > 0.f;                           // 2^-17 of the row's largest: h2 leaves the normal halves
 }
-union Half8 { __half h[8]; uint4 v; };
+__device__ __forceinline__ void split_half(float y, __half& h1, __half& h2, int& tiny) {
+  split_half(y, h1, h2);
+  const float a = fabsf(y);
+  tiny += a < TINY && a > 0.f;                             // 2^-17 of the row's largest: h2 leaves the normal halves
+}
+// Fewer than this in a row count as this many, and are not written down.
+__host__ __device__ __forceinline__ int thin_floor(int K) { return K / 16; }
+__host__ __device__ __forceinline__ int tiny_floor(int K) { return K / 32; }
+// May the expert's product of reduction length K run on halves?  A value y of a row is off by 2^-22 |y|, or, below TINY, by
+// 2^-25.  Without values below DEEP that is 2^-19 of every value, and 2^-18 sum |a||b| in every element of the result.  With
+// them, at least K - thin - thin terms of a sum are products of two values of BIG or more, 2^8; and the values below TINY add
+// at most 2^-25 2^15 (tiny + tiny) to its error: 2^-18 of the former if their number is no larger.
+__device__ __forceinline__ bool fits(const Fit& f, int K) {
+  const long long both = (long long)K - max(f.thin[0], thin_floor(K)) - max(f.thin[1], thin_floor(K));
+  const long long tiny = (long long)max(f.tiny[0], tiny_floor(K)) + max(f.tiny[1], tiny_floor(K));
+  return !f.bad && (!f.deep || (both >= 1 && both >= tiny));
+}
+union Half8 { __half h[8]; __half2 h2[4]; uint4 v; };
 
 __device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
   if (vec && left >= 8) {
@@ -164,29 +193,34 @@ __device__ __forceinline__ void load8(const float* p, int left, bool vec, float 
 //   RAGGED = 2  the same, every value multiplied by 2^14 fold[expert of the row][column] first: the inverse scales of a matrix
 //               whose rows run across the reduction, which cannot be taken out of the sum behind it
 // zero_scale: a row of zeros gets the inverse scale 0, not 1
+// fit: null, or what the rows look like goes there (rows along the reduction); else rows with more than 1 in 64 values below
+// TINY raise the flag.
 template <int TPR, int RAGGED>
-__global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
+__global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
                                                          long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan,
-                                                         const float* fold, const int* begins, int experts, bool zero_scale) {
+                                                         const float* fold, const int* begins, int experts, bool zero_scale,
+                                                         Fit* fit) {
   constexpr int HOLD = 4;
   wait_for_previous_kernel();
   __shared__ uint32_t part_max[8];
-  __shared__ int part_tiny[8];
+  __shared__ int part_tiny[8], part_thin[8];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * (256 / TPR) + sub;
   const bool live = r < rows, grouped = !RAGGED || (r >= plan->first_row && r < plan->end_row);
   const float* src = live ? (RAGGED ? x + r * ld : x + (r / rows_per) * stride + (r % rows_per) * ld) : x;
   const bool vec = ((uintptr_t)src & 15) == 0;
   const int n = live ? cols : 0;
-  const float* scales = nullptr;
-  if (RAGGED == 2 && live && grouped) {
+  auto expert_of_row = [&]() {
+    if (!RAGGED) return (int)(r / rows_per);
     int a = 0, z = experts;                                // the last group that begins at or before this row
     while (z - a > 1) {
       const int mid = (a + z) >> 1;
       if (begins[mid] <= r) a = mid; else z = mid;
     }
-    scales = fold + (long long)a * cols;
-  }
+    return a;
+  };
+  const float* scales = nullptr;
+  if (RAGGED == 2 && live && grouped) scales = fold + (long long)expert_of_row() * cols;
   auto fetch = [&](int c, float (&w)[8]) {
     if (RAGGED && !grouped) {
 #pragma unroll
@@ -230,13 +264,32 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
   }
   float up, down;
   const bool ok = scale_of(m, up, down);
-  int tiny = 0;
+  if (!ok) up = 0.f;
+  int tiny = 0, thin = 0;
+  bool deep = false;
   auto put = [&](int c, const float (&w)[8]) {
     Half8 a, b;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j], tiny);
+    for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j]);
     *reinterpret_cast<uint4*>(hi + r * kp + c) = a.v;      // pitch and position are multiples of 8 halves
     *reinterpret_cast<uint4*>(lo + r * kp + c) = b.v;
+    // two at a time
+    __half2 small = __float2half2_rn(0.f), least = __float2half2_rn(65504.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 q = __habs2(a.h2[j]);
+      small = __hadd2(small, __hlt2(q, __float2half2_rn(BIG)));
+      least = __hmin2(least, q);
+    }
+    thin += (int)__half2float(__hadd(__low2half(small), __high2half(small)));
+    if (n - c < 8) thin -= 8 - (n - c);
+    if (__half2float(__hmin(__low2half(least), __high2half(least))) < TINY)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = fabsf(w[j] * up);
+        tiny += w[j] != 0.f && y < TINY;
+        deep = deep || (w[j] != 0.f && y < DEEP);
+      }
   };
 #pragma unroll
   for (int it = 0; it < HOLD; ++it) {
@@ -248,20 +301,29 @@ __global__ void __launch_bounds__(256) split_rows_kernel(__half* hi, __half* lo,
     fetch(c, w);
     put(c, w);
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) tiny += __shfl_xor_sync(0xffffffffu, tiny, d);
+  tiny = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiny);
+  thin = (int)__reduce_add_sync(0xffffffffu, (unsigned)thin);
+  deep = __any_sync(0xffffffffu, deep);
+  if (fit && deep && ok && (threadIdx.x & 31) == 0) fit[expert_of_row()].deep = 1;
   if (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) part_tiny[warp] = tiny;
+    if ((threadIdx.x & 31) == 0) { part_tiny[warp] = tiny; part_thin[warp] = thin; }
     __syncthreads();
-    tiny = 0;
+    tiny = thin = 0;
 #pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) tiny += part_tiny[sub * (TPR / 32) + w];
+    for (int w = 0; w < TPR / 32; ++w) { tiny += part_tiny[sub * (TPR / 32) + w]; thin += part_thin[sub * (TPR / 32) + w]; }
   }
   if (t == 0 && live) {
     // (a scale of 0 that is folded into the other operand takes what meets a row of zeros out of its row's maximum, but for
     // infinities and NaN)
     down_out[r] = zero_scale && m == 0 ? 0.f : down;
-    if (!ok || (long long)tiny * 64 > cols) plan->flag = 1;
+    if (!fit) {
+      if (!ok || (long long)tiny * 64 > cols) plan->flag = 1;
+    } else if (m != 0 && (!ok || thin > thin_floor(cols) || tiny > tiny_floor(cols))) {      // (ordinary rows: none of it)
+      Fit* f = fit + expert_of_row();
+      if (!ok) f->bad = 1;
+      else if (thin > thin_floor(cols)) atomicMax(&f->thin[RAGGED ? 1 : 0], thin);
+      if (ok && tiny > tiny_floor(cols)) atomicMax(&f->tiny[RAGGED ? 1 : 0], tiny);
+    }
   }
 }
 
@@ -403,7 +465,9 @@ struct PairArgs {
   long long ldc, c_stride;
   const float* l_down; const float* r_down;      // inverse scales (l_down null: the lanes' ones were folded into the columns' values)
   const float* bias;
-  const Plan* plan;
+  Plan* plan;
+  const Fit* fit;               // per expert, or null
+  const int* begins;            // with fit: the groups' first rows, and the last one's end
   const Entry* table;
   int* status;
   int lanes, cols;              // extents: lanes of one expert's matrix; WEIGHTS: columns of one result
@@ -479,7 +543,17 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   const int n_clusters = (int)gridDim.x >> 1, cluster_id = (int)blockIdx.x >> 1;
 
   wait_for_previous_kernel();
-  if (p.plan->flag) return;               // both CTAs of every pair: nothing has been set up yet
+  int no_fit = p.plan->flag;
+  if (p.fit)
+    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+      const Fit f = p.fit[e];
+      const int first = p.begins[e], end = p.begins[e + 1];
+      no_fit |= f.bad | (end > first && !fits(f, p.K));
+    }
+  if (__syncthreads_or(no_fit)) {         // every CTA comes to the same: nothing has been set up yet
+    if (threadIdx.x == 0) p.plan->flag = 1;
+    return;
+  }
   const int tiles_l = (p.lanes + 2 * BM - 1) / (2 * BM);
   const int n_units = (p.weights ? p.experts * ((p.cols + BN - 1) / BN) : p.plan->tiles) * tiles_l;
 
@@ -806,15 +880,15 @@ int launch_next(cb200_stream* s, void (*kernel)(P...), dim3 grid, int threads, s
 template <int RAGGED>
 int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
                long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0,
-               bool zero_scale = false) {
+               bool zero_scale = false, Fit* fit = nullptr) {
   if (cols <= 1024)
     return launch_next(s, split_rows_kernel<32, RAGGED>, dim3((unsigned)((rows + 7) / 8)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
-                       rows, cols, kp, plan, fold, begins, experts, zero_scale);
+                       rows, cols, kp, plan, fold, begins, experts, zero_scale, fit);
   if (cols <= 4096)
     return launch_next(s, split_rows_kernel<128, RAGGED>, dim3((unsigned)((rows + 1) / 2)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
-                       rows, cols, kp, plan, fold, begins, experts, zero_scale);
+                       rows, cols, kp, plan, fold, begins, experts, zero_scale, fit);
   return launch_next(s, split_rows_kernel<256, RAGGED>, dim3((unsigned)rows), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
-                     plan, fold, begins, experts, zero_scale);
+                     plan, fold, begins, experts, zero_scale, fit);
 }
 
 // `sums` (may be null): workspace for the column sums of 64-row blocks, ((rows + 63) / 64 + groups_n) x cols
@@ -902,7 +976,7 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   const int l_per = trans_b ? N : K, l_cols = trans_b ? K : N;
   const long long kp = up8(K), lp = up8(l_cols), l_rows = (long long)experts * l_per;
   const size_t tiles = (size_t)((rows + BN - 1) / BN + (experts < rows ? experts : rows));
-  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)experts * 4) +
+  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)(experts + 1) * 4) + up256((size_t)experts * sizeof(Fit)) +
                        2 * up256((size_t)l_rows * lp * 2) + 2 * up256((size_t)rows * kp * 2) + up256((size_t)l_rows * 4) +
                        up256((size_t)rows * 4);
   void* ws = nullptr;
@@ -911,23 +985,26 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
   Entry* table = w.take<Entry>(tiles + 1);
-  int* begins = w.take<int>((size_t)experts);
+  int* begins = w.take<int>((size_t)experts + 1);
+  Fit* fit = w.take<Fit>((size_t)experts);
   __half* l_hi = w.take<__half>((size_t)l_rows * lp);
   __half* l_lo = w.take<__half>((size_t)l_rows * lp);
   __half* r_hi = w.take<__half>((size_t)rows * kp);
   __half* r_lo = w.take<__half>((size_t)rows * kp);
   float* l_down = w.take<float>((size_t)l_rows);
   float* r_down = w.take<float>((size_t)rows);
-  plan_kernel<<<1, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev, nullptr, 0);
+  plan_kernel<<<1 + (experts + 63) / 64, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev,
+                                                              (uint32_t*)fit, (long long)experts * (sizeof(Fit) / 4));
   CB_LAUNCH_CHECK(s);
   if ((rc = split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, nullptr, nullptr, 0,
-                          !trans_b)))
+                          !trans_b, trans_b ? fit : nullptr)))
     return rc;
-  if (trans_b) rc = split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan);
+  if (trans_b) rc = split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, nullptr, begins, experts, false, fit);
   else rc = split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, l_down, begins, experts);
   if (rc) return rc;
   PairArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = trans_b ? l_down : nullptr; a.r_down = r_down; a.bias = bias; a.plan = plan;
+  a.fit = trans_b ? fit : nullptr; a.begins = begins;
   a.table = table; a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.l_mn = trans_b ? 0 : 1; a.experts = experts;
   a.weights = 0; a.act = act; a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;
@@ -969,7 +1046,7 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
                                          sums, table, M, alpha, beta)))
     return rc;
   PairArgs a;
-  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.table = table;
+  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.fit = nullptr; a.begins = nullptr; a.table = table;
   a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.l_mn = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
   a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;

@@ -54,6 +54,20 @@ def _hold(way, sizes, X, dY, W):
         _within(_weights(dY, X, sizes), want, size, _product_tol("float", max(sizes)), way)
 
 
+@pytest.mark.parametrize("route,sizes,n,k", SHAPES)
+@pytest.mark.parametrize("small", [-22, -28, -34, -45])
+@pytest.mark.parametrize("side", ["rows", "matrices"])
+def test_small_values_that_alone_meet_others_forward(stream, route, sizes, n, k, small, side):  # noqa: F811
+    """Up to 1 in 64 values of a row far below its largest, and a row of the other operand that is zero everywhere else."""
+    stream.set_option("gemm-auto-presplit", route)
+    rng, X, dY, W = _data(7, sizes, n, k)
+    at = rng.choice(k, max(1, k // 64), replace=False)
+    one, other = (X[:1], W[0, 3:4]) if side == "rows" else (W[0, 3:4], X[:1])
+    one[:, at] *= np.float32(2.0 ** small)
+    other[:, np.setdiff1d(np.arange(k), at)] = 0.0
+    _hold("forward", sizes, X, dY, W)
+
+
 # ---- which way a call went: the fallback leaves the bits of a call that is certain to fall back ---------------------------
 
 def _fell_back(way, sizes, X, dY, W):
