@@ -157,11 +157,6 @@ __device__ __forceinline__ void split_half(float y, __half& h1, __half& h2) {
   h1 = __float2half_rn(y);
   h2 = __float2half_rn(y - __half2float(h1));
 }
-__device__ __forceinline__ void split_half(float y, __half& h1, __half& h2, int& tiny) {
-  split_half(y, h1, h2);
-  const float a = fabsf(y);
-  tiny += a < TINY && a > 0.f;                             // 2^-17 of the row's largest: h2 leaves the normal halves
-}
 // Fewer than this in a row count as this many, and are not written down.
 __host__ __device__ __forceinline__ int thin_floor(int K) { return K / 16; }
 __host__ __device__ __forceinline__ int tiny_floor(int K) { return K / 32; }
@@ -175,6 +170,29 @@ __device__ __forceinline__ bool fits(const Fit& f, int K) {
   return !f.bad && (!f.deep || (both >= 1 && both >= tiny));
 }
 union Half8 { __half h[8]; __half2 h2[4]; uint4 v; };
+
+// Eight values times `up` as halves; of the first `n` of them: how many are below BIG, how many of those that are not 0 below
+// TINY (added to what is there), and whether one is below DEEP.
+__device__ __forceinline__ void split8(const float (&w)[8], float up, int n, Half8& a, Half8& b, int& thin, int& tiny, bool& deep) {
+  __half2 small = __float2half2_rn(0.f), least = __float2half2_rn(65504.f);        // two at a time
+#pragma unroll
+  for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __half2 q = __habs2(a.h2[j]);
+    small = __hadd2(small, __hlt2(q, __float2half2_rn(BIG)));
+    least = __hmin2(least, q);
+  }
+  thin += (int)__half2float(__hadd(__low2half(small), __high2half(small)));
+  if (n < 8) thin -= 8 - n;                                // (the others are zeros)
+  if (__half2float(__hmin(__low2half(least), __high2half(least))) < TINY)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = fabsf(w[j] * up);
+      tiny += w[j] != 0.f && y < TINY;
+      deep = deep || (w[j] != 0.f && y < DEEP);
+    }
+}
 
 __device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
   if (vec && left >= 8) {
@@ -269,27 +287,9 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
   bool deep = false;
   auto put = [&](int c, const float (&w)[8]) {
     Half8 a, b;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j]);
+    split8(w, up, n - c, a, b, thin, tiny, deep);
     *reinterpret_cast<uint4*>(hi + r * kp + c) = a.v;      // pitch and position are multiples of 8 halves
     *reinterpret_cast<uint4*>(lo + r * kp + c) = b.v;
-    // two at a time
-    __half2 small = __float2half2_rn(0.f), least = __float2half2_rn(65504.f);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __half2 q = __habs2(a.h2[j]);
-      small = __hadd2(small, __hlt2(q, __float2half2_rn(BIG)));
-      least = __hmin2(least, q);
-    }
-    thin += (int)__half2float(__hadd(__low2half(small), __high2half(small)));
-    if (n - c < 8) thin -= 8 - (n - c);
-    if (__half2float(__hmin(__low2half(least), __high2half(least))) < TINY)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float y = fabsf(w[j] * up);
-        tiny += w[j] != 0.f && y < TINY;
-        deep = deep || (w[j] != 0.f && y < DEEP);
-      }
   };
 #pragma unroll
   for (int it = 0; it < HOLD; ++it) {
@@ -384,19 +384,36 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, float
   }
 }
 
-// bias_gradient[g, c] = alpha * (the sums of group g's rows, block by block) + beta * bias_gradient[g, c]
-__global__ void __launch_bounds__(128) column_sum_kernel(float* out, const float* sums, const Entry* table, int cols, float alpha, float beta) {
+// What split_columns_kernel counted in the columns of an operand, one word per group and column.
+struct ColumnCounts { const uint32_t* maxima; int* thin; int* tiny; int cols; };
+
+// The counts of both operands' columns into the groups' Fit: columns of r first, then those of l, 128 a CTA.  Beside, where `out`
+// is given,  out[g, c] = alpha * (the sums of the rows of group g in column c of r, block by block) + beta * out[g, c]
+__global__ void __launch_bounds__(128) column_fit_kernel(Fit* fit, ColumnCounts l, ColumnCounts r, const Entry* table, float* out, const float* sums,
+                                                         float alpha, float beta) {
   wait_for_previous_kernel();
-  const int c = blockIdx.x * 128 + threadIdx.x, g = blockIdx.y;
-  if (c >= cols) return;
+  const int blocks_r = (r.cols + 127) / 128, g = blockIdx.y;
+  const bool is_r = (int)blockIdx.x < blocks_r;
+  const ColumnCounts& p = is_r ? r : l;
+  const int c = ((int)blockIdx.x - (is_r ? 0 : blocks_r)) * 128 + (int)threadIdx.x;
   const Entry e = table[g];
+  const int n = e.hi - e.lo;
+  const long long at = (long long)g * p.cols + c;
+  const bool counts = n > 0 && c < p.cols && p.maxima[at] != 0;
+  const unsigned thin = __reduce_max_sync(0xffffffffu, counts ? (unsigned)p.thin[at] : 0u);
+  const unsigned tiny = __reduce_max_sync(0xffffffffu, counts ? (unsigned)p.tiny[at] : 0u);
+  if ((threadIdx.x & 31) == 0) {
+    if ((int)thin > thin_floor(n)) atomicMax(&fit[g].thin[is_r ? 1 : 0], (int)thin);
+    if ((int)tiny > tiny_floor(n)) atomicMax(&fit[g].tiny[is_r ? 1 : 0], (int)tiny);
+  }
+  if (!out || !is_r || c >= p.cols) return;
   float s = 0.f;
-  if (e.hi > e.lo) {
+  if (n > 0) {
     const long long first = e.lo / 64, last = (e.hi - 1) / 64;
 #pragma unroll 8
-    for (long long b = first; b <= last; ++b) s += sums[(b + g) * cols + c];
+    for (long long b = first; b <= last; ++b) s += sums[(b + g) * p.cols + c];
   }
-  float* to = out + (long long)g * cols + c;
+  float* to = out + at;
   float v = alpha * s;
   if (beta != 0.f) v += beta * (*to);
   *to = v;
@@ -407,9 +424,8 @@ __global__ void __launch_bounds__(128) column_sum_kernel(float* out, const float
 // blocks of 64 columns.
 __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* lo, float* down_out, const uint32_t* maxima, const float* x,
                                                             long long ld, const Entry* table, const int* owner, int cols, long long kp,
-                                                            Plan* plan) {
+                                                            const Plan* plan, Fit* fit, int* thin_out, int* tiny_out) {
   __shared__ float tile[2][32][65];
-  __shared__ int tiny_all;
   wait_for_previous_kernel();
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   const int blocks = plan->padded / POS;
@@ -420,7 +436,6 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
     const int r0 = e.lo + (int)(pos - e.first), end = e.hi;
     const bool begins = pos == e.first;                    // these are the group's first positions
     __syncthreads();
-    if (threadIdx.x == 0) tiny_all = 0;
     uint32_t m[2] = {0, 0};
     const int col = threadIdx.x >> 2, p8 = (threadIdx.x & 3) * 8;
 #pragma unroll
@@ -436,26 +451,33 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
     }
     __syncthreads();
     // a thread: 8 positions of one column of each block
-    int tiny = 0;
+    const int valid = max(0, min(8, end - (r0 + p8)));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = blockIdx.x * 128 + h * 64 + col;
-      if (c >= cols) continue;
-      float up, down;
+      float up, down, w[8];
       const bool ok = scale_of(m[h], up, down);
       Half8 a, z;
+      int thin = 0, tiny = 0;
+      bool deep = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) split_half(tile[h][p8 + j][col] * up, a.h[j], z.h[j], tiny);
-      *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;             // kp is a multiple of 64
-      *reinterpret_cast<uint4*>(lo + c * kp + pos + p8) = z.v;
-      if (!ok) plan->flag = 1;
-      if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
+      for (int j = 0; j < 8; ++j) w[j] = tile[h][p8 + j][col];
+      split8(w, up, valid, a, z, thin, tiny, deep);
+      if (c < cols) {
+        *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;           // kp is a multiple of 64
+        *reinterpret_cast<uint4*>(lo + c * kp + pos + p8) = z.v;
+        if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
+        if (!ok) fit[g].bad = 1;
+        else if (deep) fit[g].deep = 1;
+      }
+      int both = thin | tiny << 8;                         // at most 32 each in the column's four threads
+      both += __shfl_xor_sync(0xffffffffu, both, 1);
+      both += __shfl_xor_sync(0xffffffffu, both, 2);
+      if (p8 == 0 && c < cols && ok && m[h] != 0) {
+        if (both & 255) atomicAdd(thin_out + (long long)g * cols + c, both & 255);
+        if (both >> 8) atomicAdd(tiny_out + (long long)g * cols + c, both >> 8);
+      }
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) tiny += __shfl_xor_sync(0xffffffffu, tiny, d);
-    if ((threadIdx.x & 31) == 0 && tiny) atomicAdd(&tiny_all, tiny);
-    __syncthreads();
-    if (threadIdx.x == 0 && tiny_all > 64) plan->flag = 1;                // of 32 x 128 values
   }
 }
 
@@ -467,7 +489,7 @@ struct PairArgs {
   const float* bias;
   Plan* plan;
   const Fit* fit;               // per expert, or null
-  const int* begins;            // with fit: the groups' first rows, and the last one's end
+  const int* begins;            // with fit, expert_gemm: the groups' first rows, and the last one's end
   const Entry* table;
   int* status;
   int lanes, cols;              // extents: lanes of one expert's matrix; WEIGHTS: columns of one result
@@ -547,8 +569,15 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   if (p.fit)
     for (int e = threadIdx.x; e < p.experts; e += THREADS) {
       const Fit f = p.fit[e];
-      const int first = p.begins[e], end = p.begins[e + 1];
-      no_fit |= f.bad | (end > first && !fits(f, p.K));
+      int n, K = p.K;                                      // the group's rows, the length of its reduction
+      if (p.weights) {
+        const Entry t = p.table[e];
+        n = K = t.hi - t.lo;
+      } else {
+        const int first = p.begins[e];
+        n = p.begins[e + 1] - first;
+      }
+      no_fit |= f.bad | (n > 0 && !fits(f, K));
     }
   if (__syncthreads_or(no_fit)) {         // every CTA comes to the same: nothing has been set up yet
     if (threadIdx.x == 0) p.plan->flag = 1;
@@ -893,14 +922,15 @@ int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float
 
 // `sums` (may be null): workspace for the column sums of 64-row blocks, ((rows + 63) / 64 + groups_n) x cols
 int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, float* sums, const float* x, long long ld,
-                  const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, Plan* plan) {
+                  const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, const Plan* plan, Fit* fit, int* thin,
+                  int* tiny) {
   const long long chunks = (rows + 63) / 64, blocks = kp / POS;
   const dim3 grid_max((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535));
   const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0 && cols % 4 == 0;
   int rc = launch_next(s, vec ? column_max_kernel<4> : column_max_kernel<1>, grid_max, 128, 0, 1, maxima, sums, x, ld, table, groups_n, rows, cols);
   if (rc) return rc;
   return launch_next(s, split_columns_kernel, dim3((unsigned)((cols + 127) / 128), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, 1, hi,
-                     lo, down, maxima, x, ld, table, owner, cols, kp, plan);
+                     lo, down, maxima, x, ld, table, owner, cols, kp, plan, fit, thin, tiny);
 }
 
 int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long long l_rows, long long l_cols, long long l_pitch,
@@ -959,8 +989,8 @@ bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long
 }
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
-  const double operands = (double)(rows + BK * experts) * (M + N);
-  if (operands * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
+  const double operands = (double)(rows + BK * experts) * (M + N), counts = 3.0 * experts * (M + N);
+  if ((operands + counts) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * M, results = (double)experts * N * M;
   const double here = 28.0 + operands * 1.85e-6 + results * 0.67e-6 + flops / 300e6, there = 12.0 + results * 1e-6 + flops / 125e6;
@@ -1020,7 +1050,7 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   const size_t sums_n = bias_gradient ? ((size_t)(rows + 63) / 64 + experts) * M : 0;
   const size_t bytes = up256(sizeof(Plan)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
                        2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / POS) * 4) + up256((size_t)experts * N * 4) + up256((size_t)experts * M * 4) +
-                       up256((size_t)experts * (M + N) * 4) + up256(sums_n * 4);
+                       up256(((size_t)experts * (M + N) * 3 + (size_t)experts * (sizeof(Fit) / 4)) * 4) + up256(sums_n * 4);
   void* ws = nullptr;
   int rc = cb200_scratch(s, bytes, &ws);
   if (rc) return rc;
@@ -1034,19 +1064,28 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   __half* r_lo = w.take<__half>((size_t)M * kp);
   float* l_down = w.take<float>((size_t)experts * N);
   float* r_down = w.take<float>((size_t)experts * M);
-  uint32_t* l_max = w.take<uint32_t>((size_t)experts * (M + N));
-  uint32_t* r_max = l_max + (size_t)experts * N;
+  // (one block, so that it is zeroed in one go)
+  const size_t l_n = (size_t)experts * N, r_n = (size_t)experts * M, fit_words = (size_t)experts * (sizeof(Fit) / 4);
+  uint32_t* zeroed = w.take<uint32_t>((l_n + r_n) * 3 + fit_words);
+  Fit* fit = (Fit*)zeroed;
+  uint32_t* l_max = zeroed + fit_words;
+  uint32_t* r_max = l_max + l_n;
+  int* l_thin = (int*)(r_max + r_n);
+  int* r_thin = l_thin + l_n;
+  int* l_tiny = r_thin + r_n;
+  int* r_tiny = l_tiny + l_n;
   float* sums = bias_gradient ? w.take<float>(sums_n) : nullptr;
-  plan_kernel<<<129, 128, 0, s->stream>>>(plan, table, owner, nullptr, offsets, experts, rows, 1, s->status_dev, l_max,
-                                          (long long)experts * (M + N));
+  plan_kernel<<<129, 128, 0, s->stream>>>(plan, table, owner, nullptr, offsets, experts, rows, 1, s->status_dev, zeroed,
+                                          (long long)((l_n + r_n) * 3 + fit_words));
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, nullptr, B, ldb, table, owner, experts, rows, N, kp, plan))) return rc;
-  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, sums, A, lda, table, owner, experts, rows, M, kp, plan))) return rc;
-  if (bias_gradient && (rc = launch_next(s, column_sum_kernel, dim3((unsigned)((M + 127) / 128), (unsigned)experts), 128, 0, 1, bias_gradient,
-                                         sums, table, M, alpha, beta)))
+  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, nullptr, B, ldb, table, owner, experts, rows, N, kp, plan, fit, l_thin, l_tiny))) return rc;
+  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, sums, A, lda, table, owner, experts, rows, M, kp, plan, fit, r_thin, r_tiny))) return rc;
+  const ColumnCounts l_counts = {l_max, l_thin, l_tiny, N}, r_counts = {r_max, r_thin, r_tiny, M};
+  if ((rc = launch_next(s, column_fit_kernel, dim3((unsigned)((M + 127) / 128 + (N + 127) / 128), (unsigned)experts), 128, 0, 1, fit, l_counts, r_counts,
+                        table, bias_gradient, sums, alpha, beta)))
     return rc;
   PairArgs a;
-  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.fit = nullptr; a.begins = nullptr; a.table = table;
+  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.fit = fit; a.begins = nullptr; a.table = table;
   a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.l_mn = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
   a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;

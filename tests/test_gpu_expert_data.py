@@ -68,6 +68,41 @@ def test_small_values_that_alone_meet_others_forward(stream, route, sizes, n, k,
     _hold("forward", sizes, X, dY, W)
 
 
+@pytest.mark.parametrize("route,sizes,n,k", SHAPES)
+@pytest.mark.parametrize("small", [-22, -28, -34, -45])
+@pytest.mark.parametrize("columns", [1, 2, 20])
+def test_one_large_value_that_meets_zeros_weights(stream, route, sizes, n, k, small, columns):  # noqa: F811
+    """Columns of one operand with a single large value, and rows of the other that are zero there."""
+    stream.set_option("gemm-auto-presplit", route)
+    for swap in (False, True):
+        rng, X, dY, W = _data(11, sizes, n, k)
+        one, other = (X, dY) if swap else (dY, X)
+        at = rng.choice(one.shape[1], columns, replace=False)
+        at[-1] = one.shape[1] - 1                               # (the last of a width that is no multiple of 128)
+        one[:, at] *= np.float32(2.0 ** small)
+        for lo, hi in zip(_offsets(sizes)[:-1], _offsets(sizes)[1:]):
+            if hi > lo:
+                r = int(rng.integers(lo, hi))
+                one[r, at] = 1.0
+                other[r] = 0.0
+        _hold("weights", sizes, X, dY, W)
+
+
+@pytest.mark.parametrize("small", [-28, -45])
+def test_sparse_columns_with_few_values_weights(stream, small):  # noqa: F811
+    """The same where a column has few values at all: one large and some small ones among zeros."""
+    stream.set_option("gemm-auto-presplit", 2)
+    sizes, n, k = [512, 3, 200], 129, 70
+    rng, X, dY, W = _data(13, sizes, n, k)
+    for lo, hi in ((0, 512), (512, 515), (515, 715)):
+        rows = rng.choice(np.arange(lo, hi), 3, replace=False)
+        column = np.zeros(hi - lo, np.float32)
+        column[rows - lo] = [1.0, 2.0 ** small, -1.5 * 2.0 ** small]
+        dY[lo:hi, 5] = column
+        X[rows[0]] = 0.0
+    _hold("weights", sizes, X, dY, W)
+
+
 # ---- which way a call went: the fallback leaves the bits of a call that is certain to fall back ---------------------------
 
 def _fell_back(way, sizes, X, dY, W):
