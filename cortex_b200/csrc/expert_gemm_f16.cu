@@ -57,17 +57,19 @@ struct Plan {
   int first_row, end_row;      // rows outside are in no group
   int unused[3];
 };
-// How an expert's rows of halves (of either operand, along the reduction) lie in the halves' range, rows of zeros apart.  All
-// zero at the start of a call.
+// How an expert's vectors of halves (rows or columns of either operand, along the reduction) lie in the halves' range, vectors
+// of zeros apart.  All zero at the start of a call.
 struct alignas(16) Fit {
-  int bad;                     // a row's largest value is outside the range of the scales
+  int bad;                     // a scaled row's (column's) largest value is outside the range of the scales
   int deep;                    // a value is below DEEP, and not 0
-  int thin[2];                 // most values below BIG in a row, zeros too: of the lanes' operand, of the columns'
-  int tiny[2];                 // most values below TINY in a row, without the zeros
-  int unused[2];
+  int thin[2];                 // most values below BIG in a vector, zeros too: of the lanes' operand, of the columns'
+  int tiny[2];                 // most values below TINY in a vector, without the zeros
+  int zero_rows;               // a matrix scaled across the reduction: rows of zeros
+  int sparse;                  // and whether there is a row with too many values below BIG to count them by columns
 };
-// of a scaled value (a row's largest: 2^14 to 2^15)
-constexpr float BIG = 16.f, TINY = 0.125f, DEEP = 1.f / 64;
+// of a scaled value (the largest of what was scaled together: 2^14 to 2^15)
+// (ACROSS: of matrices that are scaled across the reduction, where counting costs more)
+constexpr float BIG = 16.f, BIG_ACROSS = 4.f, TINY = 0.125f, DEEP = 1.f / 64;
 struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); expert_gemm_weights: rows and first padded position
 
 // bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
@@ -157,22 +159,31 @@ __device__ __forceinline__ void split_half(float y, __half& h1, __half& h2) {
   h1 = __float2half_rn(y);
   h2 = __float2half_rn(y - __half2float(h1));
 }
-// Fewer than this in a row count as this many, and are not written down.
+// Fewer than this in a vector count as this many, and are not written down.
 __host__ __device__ __forceinline__ int thin_floor(int K) { return K / 16; }
-__host__ __device__ __forceinline__ int tiny_floor(int K) { return K / 32; }
-// May the expert's product of reduction length K run on halves?  A value y of a row is off by 2^-22 |y|, or, below TINY, by
+__host__ __device__ __forceinline__ int tiny_floor(int K) { return K / 128; }
+// May the expert's product of reduction length K run on halves?  A scaled value y is off by 2^-22 |y|, or, below TINY, by
 // 2^-25.  Without values below DEEP that is 2^-19 of every value, and 2^-18 sum |a||b| in every element of the result.  With
 // them, at least K - thin - thin terms of a sum are products of two values of BIG or more, 2^8; and the values below TINY add
-// at most 2^-25 2^15 (tiny + tiny) to its error: 2^-18 of the former if their number is no larger.
-__device__ __forceinline__ bool fits(const Fit& f, int K) {
+// at most 2^-25 2^15 (tiny + tiny) to its error: 2^-18 of the former if their number is no larger (with BIG_ACROSS on one side:
+// products of 2^6, no more than a quarter of their number).
+__device__ __forceinline__ bool fits(const Fit& f, int K, bool across) {
   const long long both = (long long)K - max(f.thin[0], thin_floor(K)) - max(f.thin[1], thin_floor(K));
   const long long tiny = (long long)max(f.tiny[0], tiny_floor(K)) + max(f.tiny[1], tiny_floor(K));
-  return !f.bad && (!f.deep || (both >= 1 && both >= tiny));
+  return !f.bad && (!f.deep || (both >= 1 && both >= (across ? 4 : 1) * tiny));
 }
 union Half8 { __half h[8]; __half2 h2[4]; uint4 v; };
 
-// Eight values times `up` as halves; of the first `n` of them: how many are below BIG, how many of those that are not 0 below
-// TINY (added to what is there), and whether one is below DEEP.
+// Eight values times `up` as halves.  split8_least: the smallest magnitude of them; split8: of the first n of them, how many are
+// below BIG and how many that are not 0 below TINY (added to what is there), and whether one is below DEEP.
+__device__ __forceinline__ float split8_least(const float (&w)[8], float up, Half8& a, Half8& b) {
+  __half2 least = __float2half2_rn(65504.f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) least = __hmin2(least, __habs2(a.h2[j]));
+  return __half2float(__hmin(__low2half(least), __high2half(least)));
+}
 __device__ __forceinline__ void split8(const float (&w)[8], float up, int n, Half8& a, Half8& b, int& thin, int& tiny, bool& deep) {
   __half2 small = __float2half2_rn(0.f), least = __float2half2_rn(65504.f);        // two at a time
 #pragma unroll
@@ -207,29 +218,41 @@ __device__ __forceinline__ void load8(const float* p, int left, bool vec, float 
 // One row of scaled halves: TPR threads per row, 8 values per thread and step, the first HOLD steps in registers between the
 // maximum and the split (longer rows are read again, from L2).  hi / lo: pitch kp (a multiple of 8).
 //   RAGGED = 0  the experts' matrices: row r at x + (r / rows_per) * stride + (r % rows_per) * ld
-//   RAGGED = 1  the ragged rows: rows in no group become zeros and have no say in the flag
+//   RAGGED = 3  the same, of rows that run across the reduction: what lies low is counted by columns, in `across`; a row of
+//               zeros gets the inverse scale 0
+//   RAGGED = 1  the ragged rows: rows in no group become zeros
 //   RAGGED = 2  the same, every value multiplied by 2^14 fold[expert of the row][column] first: the inverse scales of a matrix
 //               whose rows run across the reduction, which cannot be taken out of the sum behind it
-// zero_scale: a row of zeros gets the inverse scale 0, not 1
-// fit: null, or what the rows look like goes there (rows along the reduction); else rows with more than 1 in 64 values below
-// TINY raise the flag.
+// `fit` is told what the rows look like.  Behind the CTAs of the rows (row_ctas) those of RAGGED = 2 turn the column counts of
+// the matrices before into their Fit.
+struct Across { int* zeros; int* small; int* tiny; int cols; };      // per expert and column: 0; else below BIG_ACROSS; below TINY
 template <int TPR, int RAGGED>
 __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
-                                                         long long stride, int rows_per, long long rows, int cols, int kp, Plan* plan,
-                                                         const float* fold, const int* begins, int experts, bool zero_scale,
-                                                         Fit* fit) {
+                                                         long long stride, int rows_per, long long rows, int cols, int kp,
+                                                         const Plan* plan, Fit* fit, const float* fold, const int* begins, int experts,
+                                                         Across across, unsigned row_ctas) {
   constexpr int HOLD = 4;
+  constexpr bool MATRICES = RAGGED == 0 || RAGGED == 3;
   wait_for_previous_kernel();
+  if (RAGGED == 2 && blockIdx.x >= row_ctas) {
+    const long long i = (long long)(blockIdx.x - row_ctas) * 256 + threadIdx.x;
+    if (i >= (long long)experts * across.cols) return;
+    Fit* f = fit + i / across.cols;
+    const int zeros = across.zeros[i], thin = f->sparse ? cols : (zeros == cols - f->zero_rows ? 0 : zeros + across.small[i]), tiny = across.tiny[i];
+    if (thin > thin_floor(cols)) atomicMax(&f->thin[0], thin);
+    if (tiny > tiny_floor(cols)) atomicMax(&f->tiny[0], tiny);
+    return;
+  }
   __shared__ uint32_t part_max[8];
   __shared__ int part_tiny[8], part_thin[8];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * (256 / TPR) + sub;
-  const bool live = r < rows, grouped = !RAGGED || (r >= plan->first_row && r < plan->end_row);
-  const float* src = live ? (RAGGED ? x + r * ld : x + (r / rows_per) * stride + (r % rows_per) * ld) : x;
+  const bool live = r < rows, grouped = MATRICES || (r >= plan->first_row && r < plan->end_row);
+  const float* src = live ? (!MATRICES ? x + r * ld : x + (r / rows_per) * stride + (r % rows_per) * ld) : x;
   const bool vec = ((uintptr_t)src & 15) == 0;
   const int n = live ? cols : 0;
   auto expert_of_row = [&]() {
-    if (!RAGGED) return (int)(r / rows_per);
+    if (MATRICES) return (int)(r / rows_per);
     int a = 0, z = experts;                                // the last group that begins at or before this row
     while (z - a > 1) {
       const int mid = (a + z) >> 1;
@@ -237,10 +260,11 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
     }
     return a;
   };
+  const int sparse = RAGGED == 3 && live ? __ldcg(&fit[r / rows_per].sparse) : 0;      // (set: the counts do not matter any more)
   const float* scales = nullptr;
   if (RAGGED == 2 && live && grouped) scales = fold + (long long)expert_of_row() * cols;
   auto fetch = [&](int c, float (&w)[8]) {
-    if (RAGGED && !grouped) {
+    if (!MATRICES && !grouped) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = 0.f;
       return;
@@ -283,11 +307,24 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
   float up, down;
   const bool ok = scale_of(m, up, down);
   if (!ok) up = 0.f;
+  const long long by_expert = RAGGED == 3 && live ? r / rows_per * cols : 0;
+  const bool by_column = RAGGED == 3 && live && !sparse;
   int tiny = 0, thin = 0;
   bool deep = false;
   auto put = [&](int c, const float (&w)[8]) {
     Half8 a, b;
-    split8(w, up, n - c, a, b, thin, tiny, deep);
+    if (RAGGED != 3) {
+      split8(w, up, n - c, a, b, thin, tiny, deep);
+    } else if (split8_least(w, up, a, b) < BIG_ACROSS && m != 0 && ok) {     // (one step of eight warps in fifty)
+      for (int j = 0; j < min(8, n - c); ++j) {
+        const float x = src[c + j], y = fabsf(x * up);
+        if (y >= BIG_ACROSS) continue;
+        ++thin;
+        if (by_column) atomicAdd((x == 0.f ? across.zeros : across.small) + by_expert + c + j, 1);
+        if (by_column && x != 0.f && y < TINY) atomicAdd(across.tiny + by_expert + c + j, 1);
+        deep = deep || (x != 0.f && y < DEEP);
+      }
+    }
     *reinterpret_cast<uint4*>(hi + r * kp + c) = a.v;      // pitch and position are multiples of 8 halves
     *reinterpret_cast<uint4*>(lo + r * kp + c) = b.v;
   };
@@ -304,7 +341,7 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
   tiny = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiny);
   thin = (int)__reduce_add_sync(0xffffffffu, (unsigned)thin);
   deep = __any_sync(0xffffffffu, deep);
-  if (fit && deep && ok && (threadIdx.x & 31) == 0) fit[expert_of_row()].deep = 1;
+  if (deep && ok && (threadIdx.x & 31) == 0) fit[expert_of_row()].deep = 1;
   if (TPR > 32) {
     if ((threadIdx.x & 31) == 0) { part_tiny[warp] = tiny; part_thin[warp] = thin; }
     __syncthreads();
@@ -315,14 +352,18 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
   if (t == 0 && live) {
     // (a scale of 0 that is folded into the other operand takes what meets a row of zeros out of its row's maximum, but for
     // infinities and NaN)
-    down_out[r] = zero_scale && m == 0 ? 0.f : down;
-    if (!fit) {
-      if (!ok || (long long)tiny * 64 > cols) plan->flag = 1;
-    } else if (m != 0 && (!ok || thin > thin_floor(cols) || tiny > tiny_floor(cols))) {      // (ordinary rows: none of it)
+    down_out[r] = RAGGED == 3 && m == 0 ? 0.f : down;
+    const bool many = thin > thin_floor(cols), many_tiny = tiny > tiny_floor(cols);
+    if (RAGGED == 3 && m == 0) {
+      atomicAdd(&fit[expert_of_row()].zero_rows, 1);
+    } else if (m != 0 && (!ok || many || (RAGGED != 3 && many_tiny))) {      // (ordinary rows: none of it)
       Fit* f = fit + expert_of_row();
       if (!ok) f->bad = 1;
-      else if (thin > thin_floor(cols)) atomicMax(&f->thin[RAGGED ? 1 : 0], thin);
-      if (ok && tiny > tiny_floor(cols)) atomicMax(&f->tiny[RAGGED ? 1 : 0], tiny);
+      else if (RAGGED == 3) f->sparse = 1;
+      else {
+        if (many) atomicMax(&f->thin[RAGGED ? 1 : 0], thin);
+        if (many_tiny) atomicMax(&f->tiny[RAGGED ? 1 : 0], tiny);
+      }
     }
   }
 }
@@ -488,8 +529,8 @@ struct PairArgs {
   const float* l_down; const float* r_down;      // inverse scales (l_down null: the lanes' ones were folded into the columns' values)
   const float* bias;
   Plan* plan;
-  const Fit* fit;               // per expert, or null
-  const int* begins;            // with fit, expert_gemm: the groups' first rows, and the last one's end
+  const Fit* fit;               // per expert
+  const int* begins;            // expert_gemm: the groups' first rows, and the last one's end
   const Entry* table;
   int* status;
   int lanes, cols;              // extents: lanes of one expert's matrix; WEIGHTS: columns of one result
@@ -565,20 +606,19 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   const int n_clusters = (int)gridDim.x >> 1, cluster_id = (int)blockIdx.x >> 1;
 
   wait_for_previous_kernel();
-  int no_fit = p.plan->flag;
-  if (p.fit)
-    for (int e = threadIdx.x; e < p.experts; e += THREADS) {
-      const Fit f = p.fit[e];
-      int n, K = p.K;                                      // the group's rows, the length of its reduction
-      if (p.weights) {
-        const Entry t = p.table[e];
-        n = K = t.hi - t.lo;
-      } else {
-        const int first = p.begins[e];
-        n = p.begins[e + 1] - first;
-      }
-      no_fit |= f.bad | (n > 0 && !fits(f, K));
+  int no_fit = 0;
+  for (int e = threadIdx.x; e < p.experts; e += THREADS) {
+    const Fit f = p.fit[e];
+    int n, K = p.K;                                        // the group's rows, the length of its reduction
+    if (p.weights) {
+      const Entry t = p.table[e];
+      n = K = t.hi - t.lo;
+    } else {
+      const int first = p.begins[e];
+      n = p.begins[e + 1] - first;
     }
+    no_fit |= f.bad | (n > 0 && !fits(f, K, p.l_mn));
+  }
   if (__syncthreads_or(no_fit)) {         // every CTA comes to the same: nothing has been set up yet
     if (threadIdx.x == 0) p.plan->flag = 1;
     return;
@@ -908,16 +948,13 @@ int launch_next(cb200_stream* s, void (*kernel)(P...), dim3 grid, int threads, s
 
 template <int RAGGED>
 int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
-               long long rows, int cols, int kp, Plan* plan, const float* fold = nullptr, const int* begins = nullptr, int experts = 0,
-               bool zero_scale = false, Fit* fit = nullptr) {
-  if (cols <= 1024)
-    return launch_next(s, split_rows_kernel<32, RAGGED>, dim3((unsigned)((rows + 7) / 8)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
-                       rows, cols, kp, plan, fold, begins, experts, zero_scale, fit);
-  if (cols <= 4096)
-    return launch_next(s, split_rows_kernel<128, RAGGED>, dim3((unsigned)((rows + 1) / 2)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per,
-                       rows, cols, kp, plan, fold, begins, experts, zero_scale, fit);
-  return launch_next(s, split_rows_kernel<256, RAGGED>, dim3((unsigned)rows), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows, cols, kp,
-                     plan, fold, begins, experts, zero_scale, fit);
+               long long rows, int cols, int kp, const Plan* plan, Fit* fit, const int* begins, int experts, Across across, const float* fold) {
+  const long long more = RAGGED == 2 ? ((long long)experts * across.cols + 255) / 256 : 0;
+  const int rows_a_cta = cols <= 1024 ? 8 : (cols <= 4096 ? 2 : 1);
+  const unsigned ctas = (unsigned)((rows + rows_a_cta - 1) / rows_a_cta);
+  auto* kernel = cols <= 1024 ? split_rows_kernel<32, RAGGED> : (cols <= 4096 ? split_rows_kernel<128, RAGGED> : split_rows_kernel<256, RAGGED>);
+  return launch_next(s, kernel, dim3((unsigned)(ctas + more)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan, fit, fold,
+                     begins, experts, across, ctas);
 }
 
 // `sums` (may be null): workspace for the column sums of 64-row blocks, ((rows + 63) / 64 + groups_n) x cols
@@ -976,7 +1013,7 @@ constexpr size_t MOST_WORKSPACE = (size_t)2 << 30;
 bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
   const double l = (double)experts * N * K, r = (double)rows * K;
-  if ((l + r) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
+  if ((l + r + 3.0 * experts * N) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * K;
   // (halves that do not stay in L2 between the split and the product are read from memory)
@@ -1005,8 +1042,10 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   // the matrices' rows as they are stored: [N, K] reduces along them, [K, N] (the gradient of the input) across them
   const int l_per = trans_b ? N : K, l_cols = trans_b ? K : N;
   const long long kp = up8(K), lp = up8(l_cols), l_rows = (long long)experts * l_per;
+  // zero at the start of the call: the experts' Fit, and the counts by columns of matrices that are scaled across the reduction
+  const size_t fit_words = (size_t)experts * (sizeof(Fit) / 4), columns = trans_b ? 0 : (size_t)experts * N, zeroed_n = fit_words + 3 * columns;
   const size_t tiles = (size_t)((rows + BN - 1) / BN + (experts < rows ? experts : rows));
-  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)(experts + 1) * 4) + up256((size_t)experts * sizeof(Fit)) +
+  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)(experts + 1) * 4) + up256(zeroed_n * 4) +
                        2 * up256((size_t)l_rows * lp * 2) + 2 * up256((size_t)rows * kp * 2) + up256((size_t)l_rows * 4) +
                        up256((size_t)rows * 4);
   void* ws = nullptr;
@@ -1016,25 +1055,28 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   Plan* plan = w.take<Plan>(1);
   Entry* table = w.take<Entry>(tiles + 1);
   int* begins = w.take<int>((size_t)experts + 1);
-  Fit* fit = w.take<Fit>((size_t)experts);
+  uint32_t* zeroed = w.take<uint32_t>(zeroed_n);
+  Fit* fit = (Fit*)zeroed;
+  int* counts = (int*)(zeroed + fit_words);
+  const Across across = {counts, counts + columns, counts + 2 * columns, trans_b ? 0 : N};
   __half* l_hi = w.take<__half>((size_t)l_rows * lp);
   __half* l_lo = w.take<__half>((size_t)l_rows * lp);
   __half* r_hi = w.take<__half>((size_t)rows * kp);
   __half* r_lo = w.take<__half>((size_t)rows * kp);
   float* l_down = w.take<float>((size_t)l_rows);
   float* r_down = w.take<float>((size_t)rows);
-  plan_kernel<<<1 + (experts + 63) / 64, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev,
-                                                              (uint32_t*)fit, (long long)experts * (sizeof(Fit) / 4));
+  const unsigned zero_ctas = (unsigned)((zeroed_n + 511) / 512 < 128 ? (zeroed_n + 511) / 512 : 128);
+  plan_kernel<<<1 + zero_ctas, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev, zeroed, (long long)zeroed_n);
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, nullptr, nullptr, 0,
-                          !trans_b, trans_b ? fit : nullptr)))
-    return rc;
-  if (trans_b) rc = split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, nullptr, begins, experts, false, fit);
-  else rc = split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, l_down, begins, experts);
+  rc = trans_b ? split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, fit, begins, experts, across, nullptr)
+               : split_rows<3>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, fit, begins, experts, across, nullptr);
+  if (rc) return rc;
+  rc = trans_b ? split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, fit, begins, experts, across, nullptr)
+               : split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, fit, begins, experts, across, l_down);
   if (rc) return rc;
   PairArgs a;
   a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = trans_b ? l_down : nullptr; a.r_down = r_down; a.bias = bias; a.plan = plan;
-  a.fit = trans_b ? fit : nullptr; a.begins = begins;
+  a.fit = fit; a.begins = begins;
   a.table = table; a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.l_mn = trans_b ? 0 : 1; a.experts = experts;
   a.weights = 0; a.act = act; a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;

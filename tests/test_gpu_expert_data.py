@@ -103,6 +103,34 @@ def test_sparse_columns_with_few_values_weights(stream, small):  # noqa: F811
     _hold("weights", sizes, X, dY, W)
 
 
+@pytest.mark.parametrize("route,sizes,n,k", SHAPES)
+@pytest.mark.parametrize("scale", [1e-6, 1e-8, 1e-10, 1e-13])
+@pytest.mark.parametrize("columns", [1, 10])
+def test_small_columns_of_the_matrices_input(stream, route, sizes, n, k, scale, columns):  # noqa: F811
+    """Columns of a matrix that are small in every row: all terms of a result are small."""
+    stream.set_option("gemm-auto-presplit", route)
+    rng, X, dY, W = _data(17, sizes, n, k)
+    W[:, :, rng.choice(k, columns, replace=False)] *= np.float32(scale)
+    _hold("input", sizes, X, dY, W)
+
+
+@pytest.mark.parametrize("route,sizes,n,k", SHAPES)
+@pytest.mark.parametrize("small", [-24, -34])
+@pytest.mark.parametrize("side", ["rows", "matrices"])
+def test_small_values_that_alone_meet_others_input(stream, route, sizes, n, k, small, side):  # noqa: F811
+    stream.set_option("gemm-auto-presplit", route)
+    rng, X, dY, W = _data(19, sizes, n, k)
+    at = rng.choice(n, max(1, n // 64), replace=False)
+    rest = np.setdiff1d(np.arange(n), at)
+    if side == "rows":
+        dY[0, at] *= np.float32(2.0 ** small)
+        W[0, rest, 5] = 0.0
+    else:
+        W[0, at, 5] *= np.float32(2.0 ** small)
+        dY[0, rest] = 0.0
+    _hold("input", sizes, X, dY, W)
+
+
 # ---- which way a call went: the fallback leaves the bits of a call that is certain to fall back ---------------------------
 
 def _fell_back(way, sizes, X, dY, W):
