@@ -36,7 +36,7 @@ static __device__ __noinline__ double act_transcendental(double v, int act) {
 }
 template <typename T> __device__ __forceinline__ T act_apply(T v, int act) {
   if (act == CB200_ACT_NONE) return v;
-  if (act == CB200_ACT_RELU) return v > (T)0 ? v : (T)0;
+  if (act == CB200_ACT_RELU) return groups::relu(v);
   return (T)act_transcendental((double)v, act);
 }
 

@@ -832,7 +832,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             v[j] = fmaf(v[j], p.alpha, b);
-            if (RELU) v[j] = v[j] > 0.f ? v[j] : 0.f;
+            if (RELU) v[j] = groups::relu(v[j]);
             *to = v[j];
             to += p.ldc;
           }
@@ -859,7 +859,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
             for (int j = 0; j < 8; ++j) {
               float v = fmaf(acc[j0 + j] * (l_scale * scales[j0 + j]), p.alpha, b);
               if (p.beta != 0.f) v += p.beta * old[j];
-              if (relu) v = v > 0.f ? v : 0.f;
+              if (relu) v = groups::relu(v);
               if (live && j0 + j < left) *to = v;
               to += p.ldc;
             }

@@ -98,7 +98,7 @@ __device__ __forceinline__ void store_columns(const RowsArgs& p, float* C, uint3
   }
   if (last && p.act == CB200_ACT_RELU) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(apply_act(__uint_as_float(r[j]), CB200_ACT_RELU));
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(groups::relu(__uint_as_float(r[j])));
   } else if (last && p.act != CB200_ACT_NONE) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(apply_act(__uint_as_float(r[j]), p.act));

@@ -186,3 +186,43 @@ def test_a_row_of_zeros_stays_on_halves_input(stream):  # noqa: F811
         dY2[4, 17] = bad
         got = _input(dY2, W, sizes)
         assert np.isnan(got[4]).all() and np.isfinite(np.delete(got[:sum(sizes)], 4, 0)).all()
+
+
+# ---- activations of what is no number ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("datatype", ["float", "double"])
+@pytest.mark.parametrize("act", ["relu", "tanh", "logistic"])
+# few rows, tiles that TMA cannot address, short reductions, long ones in a cluster's slices, halves and their fallback
+@pytest.mark.parametrize("route,sizes,n,k", [(0, [1, 2], 40, 64), (0, [1, 2], 39, 63), (1, [100, 33], 129, 63), (1, [100, 33], 128, 64),
+                                             (1, [30, 20], 128, 2048), (2, [100, 33], 128, 64), (2, [100, 33], 129, 63)])
+def test_a_nan_stays_a_nan_under_an_activation(stream, datatype, act, route, sizes, n, k):  # noqa: F811
+    stream.set_option("gemm-auto-presplit", route)
+    rng = np.random.default_rng(31)
+    X, W = rng.standard_normal((sum(sizes), k)), rng.standard_normal((2, n, k))
+    X[0, 3] = np.nan
+    W[1, 7, 2] = np.nan
+    np_type = np.float32 if datatype == "float" else np.float64
+    X, W = X.astype(np_type), W.astype(np_type)
+    Y = ct.new_tensor([len(X), n], datatype)
+    ct.expert_gemm(Y, True, 1.0, ct.to_tensor(X, datatype), ct.to_tensor(W, datatype), 0.0, ct.to_tensor(_offsets(sizes), "int"), act=act)
+    got = ct.to_array(Y).reshape(len(X), n)
+    want = np.zeros(got.shape, bool)
+    want[0] = True
+    want[sizes[0]:, 7] = True
+    assert np.array_equal(np.isnan(got), want)
+
+
+@pytest.mark.parametrize("route,sizes,n,k", [(0, [1, 2], 40, 64), (1, [100, 33], 128, 64), (1, [30, 20], 128, 2048), (2, [100, 33], 128, 64)])
+def test_an_infinity_under_relu_is_no_finite_number_above_zero(stream, route, sizes, n, k):  # noqa: F811
+    """Where 64 bits give +infinity the result is that or NaN (an infinity times a tail of zero), not a number."""
+    stream.set_option("gemm-auto-presplit", route)
+    rng = np.random.default_rng(37)
+    X, W = rng.standard_normal((sum(sizes), k)).astype(np.float32), rng.standard_normal((2, n, k)).astype(np.float32)
+    X[1, 3], W[0, :, 3] = np.inf, np.where(np.arange(n) % 2, 0.5, -0.5)      # exactly representable: no tail
+    if sizes[0] < 2:
+        X[0, 3] = np.inf
+    row = 0 if sizes[0] < 2 else 1
+    got = _forward(X, W, sizes, act="relu")
+    up = np.arange(n) % 2 == 1
+    assert not np.isfinite(got[row, up]).any()
+    assert not (np.isfinite(got[row, ~up]) & (got[row, ~up] != 0)).any()     # exactly: 0
