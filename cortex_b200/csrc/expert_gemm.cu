@@ -438,6 +438,10 @@ __device__ __forceinline__ void few_rows_mn(const Product<T>& p, const groups::T
 
 template <typename T, int V, bool MN>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 2) expert_few_rows_kernel(Product<T> p, int n_blocks, Slices s) {
+  if (groups::all_may_be_found(p.rows, p.experts, FEW) && blockIdx.x == gridDim.x - 1) {
+    groups::check_offsets(p.offsets, p.experts, p.rows, p.status);         // a CTA behind those of the tiles
+    return;
+  }
   const int unit = (int)blockIdx.x / s.count, slice = (int)blockIdx.x - unit * s.count, t = unit / n_blocks, block = unit - t * n_blocks;
   const int n0 = (block * FEW_WARPS + ((int)threadIdx.x >> 5)) * FEW_OUT;
   groups::Tile tile;
@@ -472,7 +476,7 @@ template <typename T> int run_few_rows(cb200_stream* s, const Product<T>& p) {
   constexpr int V = 16 / sizeof(T);
   const long long tiles = (p.rows + FEW - 1) / FEW + (p.experts < p.rows ? p.experts : p.rows) - 1;
   const long long per = p.trans_b ? FEW_WARPS * FEW_OUT : 32 * V, n_blocks = (p.N + per - 1) / per, ctas = tiles * n_blocks;
-  CB_REQUIRE(ctas <= 2147483647LL, "expert_gemm: too many tiles");
+  CB_REQUIRE(ctas < 2147483647LL, "expert_gemm: too many tiles");
   const bool wide = (((uintptr_t)p.A | (uintptr_t)p.B) & 15) == 0 && p.lda % V == 0 && p.ldb % V == 0 && p.b_stride % V == 0 && p.K % V == 0 &&
                     (p.trans_b || p.N % V == 0);
   const unsigned threads = FEW_WARPS * 32;
@@ -484,7 +488,7 @@ template <typename T> int run_few_rows(cb200_stream* s, const Product<T>& p) {
   Slices sl;
   const int rc = get_slices<T>(s, ctas, FEW * 32 * V, slices, sl);
   if (rc) return rc;
-  const unsigned grid = (unsigned)(ctas * slices);
+  const unsigned grid = (unsigned)(ctas * slices + (groups::all_may_be_found(p.rows, p.experts, FEW) ? 1 : 0));
   if (p.trans_b && wide) expert_few_rows_kernel<T, V, false><<<grid, threads, 0, s->stream>>>(p, (int)n_blocks, sl);
   else if (p.trans_b) expert_few_rows_kernel<T, 1, false><<<grid, threads, 0, s->stream>>>(p, (int)n_blocks, sl);
   else if (wide) expert_few_rows_kernel<T, V, true><<<grid, threads, 0, s->stream>>>(p, (int)n_blocks, sl);

@@ -922,6 +922,7 @@ int cb200_expert_rows_tc(cb200_stream* s, float* C, long long ldc, int trans_b, 
   const CUtensorMapSwizzle swz = bk == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tmW, tmX;
   int rc;
+  if (groups::all_may_be_found(rows, experts, BN)) ++units;
   CB_REQUIRE(units * slices <= 2147483647LL, "expert_gemm: too many tiles");
   if (meet && (rc = get_park(s, a, units, BN))) return rc;
   if ((rc = tmap_2d(&tmX, A, rows, K, lda, bk, BN < 64 ? BN : 64, swz))) return rc;

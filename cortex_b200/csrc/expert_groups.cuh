@@ -71,6 +71,21 @@ __device__ __forceinline__ bool find_tile(const int* offsets, int experts, int r
   return found;
 }
 
+// A search for a tile stops at the 32 groups around its own, and sees bad offsets no further.  One for a tile that there is not
+// sees all, and there is one unless as many tiles as there can be -- of `tile_rows` rows, a row each -- lie before the last groups.
+__host__ __device__ __forceinline__ bool all_may_be_found(int rows, int experts, int tile_rows) { return rows <= tile_rows && experts > 32; }
+
+// The whole CTA: looks over all offsets and reports bad ones.
+__device__ __forceinline__ void check_offsets(const int* offsets, int experts, int rows, int* status) {
+  bool bad = false;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+    const int lo = offsets[e], hi = offsets[e + 1];
+    bad = bad || lo < 0 || hi > rows || hi < lo;
+  }
+  if (__syncthreads_or(bad) && threadIdx.x == 0) report_bad(status);
+}
+
 // The whole warp: the rows of group `e`.
 __device__ __forceinline__ void group_rows(const int* offsets, int rows, int e, int* status, int& lo, int& hi) {
   const int lane = threadIdx.x & 31;
