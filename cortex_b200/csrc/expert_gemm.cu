@@ -795,6 +795,7 @@ int rows_tc(cb200_stream* s, Product<float> p) {
 }
 
 int weights_tc(cb200_stream* s, Product<float> p) {
+  if (p.rows == 0) return run_few_weights<float>(s, p);
   if (few_weights_ok(p) && s->opt_gemm_auto_presplit != 2 && s->opt_gemm_tile_n == 0) return run_few_weights<float>(s, p);
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
   const bool halves = cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts);

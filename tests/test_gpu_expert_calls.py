@@ -1,4 +1,4 @@
-"""Calls of the expert products that their documentation allows: bad offsets anywhere."""
+"""Calls of the expert products that their documentation allows: bad offsets anywhere, no rows under every option."""
 import numpy as np
 import pytest
 
@@ -35,3 +35,18 @@ def test_bad_offsets_of_groups_behind_the_last_row(b200_driver, datatype, tile_n
             want, size = plain.expert_gemm(np.zeros((rows, n)), trans_b, 1.0, X, W if trans_b else W.reshape(experts, k, n), 0.0, bad)
             _within(ct.to_array(out), want, size, _product_tol(datatype, k), trans_b)
     s.sync()
+
+
+@pytest.mark.parametrize("options", [{"gemm-tile-n": 64}, {"gemm-tile-n": 128, "gemm-k-slices": 4}, {"gemm-auto-presplit": 2}, {"gemm-auto-presplit": 1}])
+def test_no_rows_under_options(stream, options):  # noqa: F811
+    for name, value in options.items():
+        stream.set_option(name, value)
+    off = ct.to_tensor(np.zeros(4, np.int32), "int")
+    X, Y, D = (ct.new_tensor([0, c], "float") for c in (40, 80, 40))
+    W = ct.new_tensor([3, 80, 40], "float")
+    ct.expert_gemm(Y, True, 1.0, X, W, 0.0, off)
+    ct.expert_gemm(D, False, 1.0, Y, W, 0.0, off)
+    for beta in (0.5, 0.0):
+        dW, db = ct.to_tensor(np.ones((3, 80, 40)), "float"), ct.to_tensor(np.ones((3, 80)), "float")
+        ct.expert_gemm_weights(dW, 1.0, Y, X, beta, off, bias_gradient=db)
+        assert np.all(ct.to_array(dW) == beta) and np.all(ct.to_array(db) == beta)
