@@ -973,6 +973,17 @@ int check_apart(const char* what, const char* names, const void* a, int64_t lda,
   return CB200_OK;
 }
 
+// a vector of cols elements shares none with a matrix (which may have gaps between its rows)
+int check_vector_apart(const char* what, const char* matrix, const void* m, int64_t ld, int64_t rows, const char* vector, const void* v, int dtype,
+                       const cb200_block_desc* d) {
+  if (!m || !v || rows == 0) return CB200_OK;
+  const int64_t size = (int64_t)cb200_dtype_size(dtype), n = d->cols * size, pitch = ld * size;
+  const int64_t at = (int64_t)((intptr_t)v - (intptr_t)m);              // bytes from the matrix's first element
+  const int64_t r = at < n ? 0 : (at - n) / pitch + 1;                  // the first row that ends behind the vector's start
+  CB_REQUIRE(r >= rows || r * pitch >= at + n, "%s: %s overlaps %s", what, matrix, vector);
+  return CB200_OK;
+}
+
 template <typename T>
 int forward(cb200_stream* s, void* output, int64_t ld_output, void* total, int64_t ld_total, const void* block,
             int64_t ld_block, const void* residual, int64_t ld_residual, const void* gate, const void* after_scale,
@@ -1020,6 +1031,11 @@ int cb200_block_normalize(cb200_stream* s, int dtype, void* output, int64_t ld_o
       (rc = check_apart(what, "output and gate", output, ld_output, gate, d->cols, false, dtype, d->gate_rows, d)) ||
       (rc = check_apart(what, "total and gate", total, ld_total, gate, d->cols, false, dtype, d->gate_rows, d)))
     return rc;
+  struct { const char* name; const void* p; } vectors[4] = {{"a scale", after_scale}, {"a bias", after_bias}, {"a scale", before_scale}, {"a bias", before_bias}};
+  for (auto& v : vectors)
+    if ((rc = check_vector_apart(what, "output", output, ld_output, d->rows, v.name, v.p, dtype, d)) ||
+        (rc = check_vector_apart(what, "total", total, ld_total, d->rows, v.name, v.p, dtype, d)))
+      return rc;
   if (d->rows == 0) return CB200_OK;
   return dtype == CB200_FLOAT
              ? forward<float>(s, output, ld_output, total, ld_total, block, ld_block, residual, ld_residual, gate, after_scale,
@@ -1105,12 +1121,29 @@ int cb200_block_normalize_gradients(cb200_stream* s, int dtype, void* block_grad
       (rc = check_apart(what, "block_gradient and gate_gradient", block_gradient, ld_block_gradient, gate_gradient, d->cols, false, dtype, d->gate_rows, d)) ||
       (rc = check_apart(what, "residual_gradient and gate_gradient", residual_gradient, ld_residual_gradient, gate_gradient, d->cols, false, dtype, d->gate_rows, d)))
     return rc;
+  // the vectors, read and written
+  const void* read_vectors[3] = {after_scale, after_bias, before_scale};
+  const void* sums[4] = {after_scale_gradient, after_bias_gradient, before_scale_gradient, before_bias_gradient};
+  for (const void* v : read_vectors)
+    if ((rc = check_vector_apart(what, "block_gradient", block_gradient, ld_block_gradient, d->rows, "a scale or bias", v, dtype, d)) ||
+        (rc = check_vector_apart(what, "residual_gradient", residual_gradient, ld_residual_gradient, d->rows, "a scale or bias", v, dtype, d)) ||
+        (rc = check_vector_apart(what, "gate_gradient", gate_gradient, d->cols, d->gate_rows, "a scale or bias", v, dtype, d)))
+      return rc;
+  for (int i = 0; i < 4; ++i) {
+    const char* name = "the gradient of a scale or bias";
+    for (auto& m : in) if ((rc = check_vector_apart(what, m.name, m.p, m.ld, d->rows, name, sums[i], dtype, d))) return rc;
+    for (auto& m : out) if ((rc = check_vector_apart(what, m.name, m.p, m.ld, d->rows, name, sums[i], dtype, d))) return rc;
+    if ((rc = check_vector_apart(what, "gate", gate, d->cols, d->gate_rows, name, sums[i], dtype, d)) ||
+        (rc = check_vector_apart(what, "gate_gradient", gate_gradient, d->cols, d->gate_rows, name, sums[i], dtype, d)))
+      return rc;
+    for (const void* v : read_vectors) if ((rc = check_vector_apart(what, "a scale or bias", v, d->cols, 1, name, sums[i], dtype, d))) return rc;
+    for (int j = 0; j < i; ++j) if ((rc = check_vector_apart(what, name, sums[j], d->cols, 1, name, sums[i], dtype, d))) return rc;
+  }
   if (d->rows == 0) {
     // sums over no rows
     const size_t bytes = (size_t)d->cols * cb200_dtype_size(dtype);
     DeviceGuard guard(s->device);
-    void* sums[5] = {after_scale_gradient, after_bias_gradient, before_scale_gradient, before_bias_gradient, nullptr};
-    for (void* v : sums) if (v) CB_CUDA(cudaMemsetAsync(v, 0, bytes, s->stream));
+    for (const void* v : sums) if (v) CB_CUDA(cudaMemsetAsync(const_cast<void*>(v), 0, bytes, s->stream));
     if (gate_gradient) CB_CUDA(cudaMemsetAsync(gate_gradient, 0, bytes * d->gate_rows, s->stream));
     return CB200_OK;
   }

@@ -453,12 +453,12 @@ int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_str
  * Matrices are [rows, cols] with a pitch each; the scales and biases [cols], biases may be NULL; gate [gate_rows, cols]
  * dense or NULL (1), gate_rows divides rows and gate row g serves rows g * rows / gate_rows and on: 1 = one learned gate per
  * column, a row per sample, or one value per element.  total may be NULL without a block.  total or output may be written over
- * residual or block (the same matrix, same pitch), never over each other.
+ * residual or block (the same matrix, same pitch), never over each other, the gate, a scale or a bias.
  * The gradients take the forward call's total and block, output_gradient (with before_scale) and / or total_gradient (what
  * reaches the sum by the residual path), and overwrite (not accumulate): residual_gradient, block_gradient, gate_gradient
  * (summed over the rows that share a gate row), and the column sums of the scales and biases; NULL = not wanted, except
  * residual_gradient, and block_gradient where there is a block.  residual_gradient may be total_gradient itself; otherwise
- * gradients share no memory with operands.  float / double; statistics and sums in the element type, in a fixed order. */
+ * gradients share no memory with operands or one another.  float / double; statistics and sums in the element type, in a fixed order. */
 typedef struct cb200_block_desc {
   int32_t kind;
   double epsilon, residual_scale;

@@ -230,6 +230,44 @@ def test_c_abi_block_refusals():
         _refused(c[0], *c[1:], match=text)
 
 
+M12 = [P + i * 65536 for i in range(14)]
+
+
+def _block_call(out=M12[0], total=M12[1], block=M12[2], res=M12[3], gate=M12[4], aw=M12[5], ab=M12[6], bw=M12[7], bb=M12[8], ld=8, eps=1e-5,
+                dtype=4):
+    return ("cb200_block_normalize", dtype, out, ld, total, ld, block, ld, res, ld, gate, aw, ab, bw, bb,
+            C.byref(_lib.BlockDesc(0, eps, 1.0, 4, 8, 2)))
+
+
+def _block_gradient_call(bg=M12[0], rg=M12[1], gg=M12[2], gaw=M12[3], gab=M12[4], gbw=M12[5], gbb=M12[6], dy=M12[7], dt=M12[8], total=M12[9],
+                         block=M12[10], gate=M12[11], aw=M12[12], ab=M12[13], bw=M12[13] + 4096, ld=8, eps=1e-5, dtype=4):
+    return ("cb200_block_normalize_gradients", dtype, bg, ld, rg, ld, gg, gaw, gab, gbw, gbb, dy, ld, dt, ld, total, ld, block, ld, gate,
+            aw, ab, bw, C.byref(_lib.BlockDesc(0, eps, 1.0, 4, 8, 2)))
+
+
+def test_c_abi_block_results_over_scales_and_biases():
+    """No result is written over a scale, a bias or (of the gradients' vectors) anything else."""
+    for name in ("aw", "ab", "bw", "bb"):
+        for result, text in ((M12[0], "output overlaps"), (M12[1], "total overlaps")):
+            for at in (result, result + 3 * 32 + 28, result - 28, result + 40):
+                c = _block_call(**{name: at})
+                _refused(c[0], *c[1:], match=text)
+    for name in ("aw", "ab", "bw"):
+        for result, text in ((M12[0], "block_gradient overlaps"), (M12[1], "residual_gradient overlaps"), (M12[2], "gate_gradient overlaps")):
+            c = _block_gradient_call(**{name: result + 36})
+            _refused(c[0], *c[1:], match=text)
+    everything = [M12[0], M12[1], M12[2], M12[7], M12[8], M12[9], M12[10], M12[11], M12[12], M12[13], M12[13] + 4096]
+    for i, name in enumerate(("gaw", "gab", "gbw", "gbb")):
+        for other in everything + [M12[3 + j] for j in range(4) if j != i]:
+            c = _block_gradient_call(**{name: other + 20})
+            _refused(c[0], *c[1:], match="overlaps")
+    # a vector in the gap between a matrix's rows shares nothing with it: the next check refuses (a misfit of another kind)
+    c = _block_call(aw=M12[0] + 32, ld=16, out=M12[0], total=M12[0] + 4)
+    _refused(c[0], *c[1:], match="output and total")
+    c = _block_call(aw=M12[0] + 32, ab=M12[0] + 96, bw=M12[0] + 160, bb=M12[1] + 24, ld=16)
+    _refused(c[0], *c[1:], match="total overlaps a bias")
+
+
 def test_c_abi_clip_refusals():
     def lists(g, n, out):
         return (C.c_void_p * len(g))(*g), (C.c_int64 * len(n))(*n), (C.c_void_p * len(out))(*out)
