@@ -943,7 +943,8 @@ int check_desc(const char* what, int dtype, const cb200_block_desc* d) {
   CB_REQUIRE(dtype == CB200_FLOAT || dtype == CB200_DOUBLE, "%s: only float and double tensors", what);
   CB_REQUIRE(d, "%s: null descriptor", what);
   CB_REQUIRE(d->kind == KIND_RMS || d->kind == KIND_LAYER, "%s: unknown normalisation %d", what, d->kind);
-  CB_REQUIRE(d->epsilon > 0.0 && isfinite(d->epsilon), "%s: epsilon must be positive", what);
+  const double epsilon = dtype == CB200_FLOAT ? (double)(float)d->epsilon : d->epsilon;      // (as the kernels have it)
+  CB_REQUIRE(epsilon > 0.0 && isfinite(epsilon), "%s: epsilon must be positive in the element type", what);
   CB_REQUIRE(d->rows >= 0 && d->cols >= 1 && d->rows <= 2147483647LL && d->cols <= 2147483647LL, "%s: bad extents", what);
   CB_REQUIRE(d->gate_rows >= 1 && (d->rows == 0 || (d->gate_rows <= d->rows && d->rows % d->gate_rows == 0)),
              "%s: %lld gate rows do not divide %lld rows", what, (long long)d->gate_rows, (long long)d->rows);

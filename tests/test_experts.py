@@ -268,6 +268,17 @@ def test_c_abi_block_results_over_scales_and_biases():
     _refused(c[0], *c[1:], match="total overlaps a bias")
 
 
+@pytest.mark.parametrize("call", [_block_call, _block_gradient_call])
+def test_c_abi_block_epsilon_of_the_element_type(call):
+    """An epsilon that is 0 or infinite as a float: a row of zeros would become NaN."""
+    for eps, dtype in [(1e-46, 4), (1e39, 4), (float("inf"), 5), (0.0, 5)]:
+        c = call(eps=eps, dtype=dtype, ld=7)
+        _refused(c[0], *c[1:], match="epsilon")
+    for eps, dtype in [(1e-44, 4), (1e-300, 5)]:                       # these are fine: the next check refuses
+        c = call(eps=eps, dtype=dtype, ld=7)
+        _refused(c[0], *c[1:], match="pitch")
+
+
 def test_c_abi_clip_refusals():
     def lists(g, n, out):
         return (C.c_void_p * len(g))(*g), (C.c_int64 * len(n))(*n), (C.c_void_p * len(out))(*out)
