@@ -959,6 +959,14 @@ int check_matrix(const char* what, const char* name, const void* p, int64_t ld, 
   return CB200_OK;
 }
 
+// dense vectors and gates; null is fine
+int check_aligned(const char* what, std::initializer_list<const void*> ps, int dtype) {
+  uintptr_t bits = 0;
+  for (const void* p : ps) bits |= (uintptr_t)p;
+  CB_REQUIRE(bits % cb200_dtype_size(dtype) == 0, "%s: a gate, scale, bias or gradient of one is not aligned to its element type", what);
+  return CB200_OK;
+}
+
 // a result and another operand either are one and the same matrix (where `same_ok`) or share no memory
 int check_apart(const char* what, const char* names, const void* a, int64_t lda, const void* b, int64_t ldb, bool same_ok,
                 int dtype, int64_t b_rows, const cb200_block_desc* d, int64_t a_rows = -1) {
@@ -1021,7 +1029,8 @@ int cb200_block_normalize(cb200_stream* s, int dtype, void* output, int64_t ld_o
   CB_REQUIRE(block || (!gate && !after_scale), "block_normalize: gate and after-normalisation belong to a block");
   CB_REQUIRE((output != nullptr) == (before_scale != nullptr), "block_normalize: output and the normalisation before the next block go together");
   CB_REQUIRE((!after_bias || after_scale) && (!before_bias || before_scale), "block_normalize: a bias without a scale");
-  if ((rc = check_matrix(what, "output", output, ld_output, dtype, d)) || (rc = check_matrix(what, "total", total, ld_total, dtype, d)) ||
+  if ((rc = check_aligned(what, {gate, after_scale, after_bias, before_scale, before_bias}, dtype)) ||
+      (rc = check_matrix(what, "output", output, ld_output, dtype, d)) || (rc = check_matrix(what, "total", total, ld_total, dtype, d)) ||
       (rc = check_matrix(what, "block", block, ld_block, dtype, d)) ||
       (rc = check_matrix(what, "residual", residual, ld_residual, dtype, d)) ||
       (rc = check_apart(what, "output and total", output, ld_output, total, ld_total, false, dtype, d->rows, d)) ||
@@ -1103,6 +1112,9 @@ int cb200_block_normalize_gradients(cb200_stream* s, int dtype, void* block_grad
       {"total_gradient", total_gradient, ld_total_gradient}, {"total", total, ld_total}, {"block", block, ld_block}};
   struct { const char* name; const void* p; int64_t ld; } out[2] = {{"block_gradient", block_gradient, ld_block_gradient},
       {"residual_gradient", residual_gradient, ld_residual_gradient}};
+  if ((rc = check_aligned(what, {gate_gradient, after_scale_gradient, after_bias_gradient, before_scale_gradient, before_bias_gradient, gate, after_scale,
+                                 after_bias, before_scale}, dtype)))
+    return rc;
   for (auto& m : in) if ((rc = check_matrix(what, m.name, m.p, m.ld, dtype, d))) return rc;
   for (auto& m : out) if ((rc = check_matrix(what, m.name, m.p, m.ld, dtype, d))) return rc;
   for (int o = 0; o < 2; ++o)

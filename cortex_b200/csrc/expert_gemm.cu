@@ -834,7 +834,7 @@ int weights_tc(cb200_stream* s, Product<float> p) {
 // kernels step 32-bit indexes past the last row and column, by a tile or a warp's stride at most
 constexpr int64_t MAX_EXTENT = 2147483647LL - 65535;
 
-int check_common(const char* what, cb200_stream* s, int dtype, const void* C, const void* A, const void* B, int64_t rows,
+int check_common(const char* what, cb200_stream* s, int dtype, const void* C, const void* A, const void* B, const void* bias, int64_t rows,
                  int64_t experts, const int32_t* offsets) {
   CB_REQUIRE(s && C && A && B && offsets, "%s: null argument", what);
   CB_REQUIRE(dtype == CB200_FLOAT || dtype == CB200_DOUBLE, "%s: only defined for float and double tensors", what);
@@ -842,7 +842,7 @@ int check_common(const char* what, cb200_stream* s, int dtype, const void* C, co
   CB_REQUIRE(experts >= 1 && experts <= groups::MAX_EXPERTS, "%s: %lld experts outside [1, %d]", what, (long long)experts,
              (int)groups::MAX_EXPERTS);
   const uintptr_t size = cb200_dtype_size(dtype);
-  CB_REQUIRE((((uintptr_t)C | (uintptr_t)A | (uintptr_t)B) % size) == 0 && ((uintptr_t)offsets & 3) == 0,
+  CB_REQUIRE((((uintptr_t)C | (uintptr_t)A | (uintptr_t)B | (uintptr_t)bias) % size) == 0 && ((uintptr_t)offsets & 3) == 0,
              "%s: an operand is not aligned to its element type", what);
   return CB200_OK;
 }
@@ -870,7 +870,7 @@ extern "C" {
 int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int trans_b, double alpha, const void* A, int64_t rows,
                       int64_t a_cols, int64_t lda, const void* B, int64_t experts, int64_t b_cols, int64_t b_stride, int64_t ldb,
                       double beta, const int32_t* offsets, const void* bias, int act) {
-  int rc = check_common("expert_gemm", s, dtype, C, A, B, rows, experts, offsets);
+  int rc = check_common("expert_gemm", s, dtype, C, A, B, bias, rows, experts, offsets);
   if (rc) return rc;
   CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= MAX_EXTENT && b_cols <= MAX_EXTENT, "expert_gemm: bad extents");
   CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= (trans_b ? a_cols : b_cols), "expert_gemm: pitch smaller than the row");
@@ -887,7 +887,7 @@ int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int tran
 int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_stride, int64_t ldc, double alpha, const void* A,
                               int64_t rows, int64_t a_cols, int64_t lda, const void* B, int64_t b_cols, int64_t ldb,
                               int64_t experts, double beta, const int32_t* offsets, void* bias_gradient) {
-  int rc = check_common("expert_gemm_weights", s, dtype, C, A, B, rows, experts, offsets);
+  int rc = check_common("expert_gemm_weights", s, dtype, C, A, B, bias_gradient, rows, experts, offsets);
   if (rc) return rc;
   CB_REQUIRE(a_cols >= 1 && b_cols >= 1 && a_cols <= MAX_EXTENT && b_cols <= MAX_EXTENT, "expert_gemm_weights: bad extents");
   CB_REQUIRE(ldc >= b_cols && lda >= a_cols && ldb >= b_cols, "expert_gemm_weights: pitch smaller than the row");

@@ -279,6 +279,21 @@ def test_c_abi_block_epsilon_of_the_element_type(call):
         _refused(c[0], *c[1:], match="pitch")
 
 
+def test_c_abi_vectors_off_their_element_type():
+    """Gates, scales, biases and their gradients are loaded as elements: an address between two would fault on the device."""
+    for name in ("gate", "aw", "ab", "bw", "bb"):
+        for dtype, by in ((4, 2), (5, 4)):
+            c = _block_call(**{name: M12[4] + 1024 + by}, dtype=dtype)
+            _refused(c[0], *c[1:], match="aligned")
+    for name in ("gg", "gaw", "gab", "gbw", "gbb", "gate", "aw", "ab", "bw"):
+        for dtype, by in ((4, 2), (5, 4)):
+            c = _block_gradient_call(**{name: M12[2] + 1024 + by}, dtype=dtype)
+            _refused(c[0], *c[1:], match="aligned")
+    for dtype, by in ((4, 2), (5, 4)):
+        _refused("cb200_expert_gemm", dtype, P, 8, 1, 1.0, P + 4096, 4, 8, 8, P + 8192, 2, 8, 64, 8, 0.0, P + 16384, P + 32768 + by, 0, match="aligned")
+        _refused("cb200_expert_gemm_weights", dtype, P, 64, 8, 1.0, P + 4096, 4, 8, 8, P + 8192, 8, 8, 2, 0.0, P + 16384, P + 32768 + by, match="aligned")
+
+
 def test_c_abi_clip_refusals():
     def lists(g, n, out):
         return (C.c_void_p * len(g))(*g), (C.c_int64 * len(n))(*n), (C.c_void_p * len(out))(*out)
