@@ -6,8 +6,9 @@
 //
 // The buffers of one launch travel as a table in the kernel's parameters (no upload, nothing to keep alive, captured
 // into a graph as it is).  Each buffer is cut into chunks that start on a 16-byte boundary, CTAs take chunks in turn,
-// squares are summed in double (products of floats are exact there and cannot overflow), one partial sum per CTA goes
-// to a fixed slot, and the CTA that finishes last adds the slots in order: the result has the same bits on every run.
+// squares are summed in double (products of floats are exact there and cannot overflow; doubles whose squares could leave the
+// range are summed apart, scaled by a power of two), one partial sum per CTA goes to a fixed slot, and the CTA that finishes
+// last adds the slots in order: the result has the same bits on every run.
 #include "common.cuh"
 #include <math.h>
 #include <algorithm>
@@ -30,7 +31,57 @@ template <typename T, int MOST> struct Pieces {
 };
 
 // Where the norm and the scale of a call live between its kernels: words of the stream's partial-sum block.
-struct NormResult { double norm, scale; };
+// Gradients are multiplied by scale, then by tail (1, but where the product of the two is below the normal range).
+struct NormResult { double norm, scale, tail; };
+
+// Sums of squares.  Of doubles: those between 2^-480 and 2^480 as they are (2^43 of them stay in range), the others
+// times 2^-600 and 2^600, so that a norm is finite wherever it is a double, and no value is lost below it.
+template <typename T> struct Squares;
+template <> struct Squares<float> {
+  static constexpr int N = 1;
+  double s[1];
+  __device__ __forceinline__ void zero() { s[0] = 0.0; }
+  template <int M> __device__ __forceinline__ void add(const float (&x)[M]) {
+    double two[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < M; ++i) two[i & 1] += (double)x[i] * (double)x[i];
+    s[0] += two[0] + two[1];
+  }
+  __device__ __forceinline__ double norm() const { return sqrt(s[0]); }
+};
+template <> struct Squares<double> {
+  static constexpr int N = 3;
+  static constexpr double BIG = 0x1p480, SMALL = 0x1p-480, DOWN = 0x1p-600, UP = 0x1p600;
+  double s[3];                     // as they are, big, small
+  __device__ __forceinline__ void zero() { s[0] = s[1] = s[2] = 0.0; }
+  template <int M> __device__ __forceinline__ void add(const double (&x)[M]) {
+    double two[2] = {0.0, 0.0};
+    int least = 0x7fffffff, most = 0;                  // the words with the exponents
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int a = __double2hiint(x[i]) & 0x7fffffff;
+      least = min(least, a);
+      most = max(most, a);
+      two[i & 1] += x[i] * x[i];
+    }
+    if (least >= (1023 - 480) << 20 && most < (1023 + 480) << 20) {
+      s[0] += two[0] + two[1];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const double a = fabs(x[i]);
+      if (a > BIG) s[1] += a * DOWN * (a * DOWN);
+      else if (a < SMALL) s[2] += a * UP * (a * UP);
+      else s[0] += a * a;                              // (a NaN too)
+    }
+  }
+  __device__ __forceinline__ double norm() const {
+    if (s[1] != 0.0) return sqrt(s[1] + s[0] * DOWN * DOWN) * UP;
+    if (s[0] != 0.0) return sqrt(s[0] + s[2] * DOWN * DOWN);
+    return sqrt(s[2]) * DOWN;
+  }
+};
 
 template <typename T> struct Vec;
 template <> struct Vec<float> { struct alignas(16) type { float e[4]; }; static constexpr int N = 4; };
@@ -74,7 +125,8 @@ square_sum_kernel(const __grid_constant__ Pieces<T, MOST> t, double* partials, i
                   NormResult* result, T* norm_out, double max_norm) {
   typedef typename Vec<T>::type V;
   constexpr int N = Vec<T>::N, WHOLE = CHUNK / N / THREADS;           // 16-byte loads of a whole chunk per thread
-  double sum = 0.0;
+  Squares<T> sum;
+  sum.zero();
   const int chunks = t.first[t.n];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     int p;
@@ -86,37 +138,49 @@ square_sum_kernel(const __grid_constant__ Pieces<T, MOST> t, double* partials, i
       V x[WHOLE];
 #pragma unroll
       for (int i = 0; i < WHOLE; ++i) x[i] = v[threadIdx.x + i * THREADS];
-      double s[2] = {0.0, 0.0};
+      T all[WHOLE * N];
 #pragma unroll
       for (int i = 0; i < WHOLE; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[e & 1] += (double)x[i].e[e] * (double)x[i].e[e];
-      sum += s[0] + s[1];
+        for (int e = 0; e < N; ++e) all[i * N + e] = x[i].e[e];
+      sum.add(all);
     } else {
 #pragma unroll 4
       for (long long i = lo + threadIdx.x; i < hi; i += THREADS) {
-        const double v = (double)g[i];
-        sum += v * v;
+        const T one[1] = {g[i]};
+        sum.add(one);
       }
     }
   }
-  sum = block_sum(sum);
+#pragma unroll
+  for (int k = 0; k < Squares<T>::N; ++k) sum.s[k] = block_sum(sum.s[k]);
   __shared__ bool finish;
   if (threadIdx.x == 0) {
-    partials[slot0 + blockIdx.x] = sum;
+#pragma unroll
+    for (int k = 0; k < Squares<T>::N; ++k) partials[(slot0 + blockIdx.x) * Squares<T>::N + k] = sum.s[k];
     __threadfence();
     finish = last && atomicAdd(counter, 1) == (int)gridDim.x - 1;
   }
   __syncthreads();
   if (!finish) return;
   __threadfence();
-  double all = 0.0;
-  for (int i = threadIdx.x; i < slots; i += THREADS) all += __ldcg(partials + i);
-  all = block_sum(all);
+  sum.zero();
+  for (int i = threadIdx.x; i < slots; i += THREADS)
+#pragma unroll
+    for (int k = 0; k < Squares<T>::N; ++k) sum.s[k] += __ldcg(partials + (long long)i * Squares<T>::N + k);
+#pragma unroll
+  for (int k = 0; k < Squares<T>::N; ++k) sum.s[k] = block_sum(sum.s[k]);
   if (threadIdx.x == 0) {
-    const double norm = sqrt(all);
+    const double norm = sum.norm();
     result->norm = norm;
-    result->scale = (norm > max_norm && isfinite(norm)) ? max_norm / norm : 1.0;
+    result->scale = result->tail = 1.0;
+    if (norm > max_norm && isfinite(norm)) {
+      result->scale = max_norm / norm;
+      if (result->scale < 0x1p-900) {                  // (then norm is above 2^-173: times 2^-600 it keeps its bits)
+        result->scale = max_norm / (norm * 0x1p-600);
+        result->tail = 0x1p-600;
+      }
+    }
     if (norm_out) *norm_out = (T)norm;
     *counter = 0;                                    // left zero for the next launch
   }
@@ -128,7 +192,7 @@ template <typename T, int MOST>
 __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ Pieces<T, MOST> t, const NormResult* result) {
   typedef typename Vec<T>::type V;
   constexpr int N = Vec<T>::N, WHOLE = CHUNK / N / THREADS;
-  const T scale = (T)result->scale;
+  const T scale = (T)(result->scale * result->tail);
   const int chunks = t.first[t.n];
   const int c = chunks - 1 - (int)blockIdx.x;
   int p;
@@ -137,8 +201,8 @@ __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ 
   const T* g = t.g[p];
   T* o = t.out[p];
   if (scale == (T)1 && g == o) return;               // within the bound, in place: nothing changes
-  if (!(scale >= (T)1e-30)) {                      // a float scale down here would have lost its low bits
-    for (long long i = lo + threadIdx.x; i < hi; i += THREADS) o[i] = (T)((double)g[i] * result->scale);
+  if (!(scale >= (T)1e-30)) {                      // a scale down here would have lost its low bits
+    for (long long i = lo + threadIdx.x; i < hi; i += THREADS) o[i] = (T)((double)g[i] * result->scale * result->tail);
   } else if (hi - lo == CHUNK && ((uintptr_t)(o + lo) & 15) == 0) {
     const V* v = reinterpret_cast<const V*>(g + lo);
     V x[WHOLE];
@@ -183,7 +247,7 @@ int norm_and_clip_table(cb200_stream* s, int n, const void* const* g, const int6
   const int most = s->sm_count * 16;                  // CTAs of one launch
   void* block = nullptr;
   int* counter = nullptr;
-  int rc = cb200_partials(s, sizeof(NormResult) + (size_t)launches * most * sizeof(double), &block);
+  int rc = cb200_partials(s, sizeof(NormResult) + (size_t)launches * most * Squares<T>::N * sizeof(double), &block);
   if (rc) return rc;
   if ((rc = cb200_tile_flags(s, 1, &counter))) return rc;
   NormResult* result = (NormResult*)block;

@@ -481,7 +481,8 @@ int cb200_block_normalize_gradients(cb200_stream* s, int dtype, void* block_grad
  *   norm = sqrt(sum of all squares), written to the device element `norm` of the buffers' type;
  *   clip_gradients: clipped[i] = gradients[i] * max_norm / norm where norm > max_norm, otherwise (also when the norm is not
  *   finite) clipped[i] = gradients[i].  clipped[i] may be gradients[i] itself; norm may be NULL here.
- * Squares are summed in double and in a fixed order (same bits on every run).  The lists are read before the call returns. */
+ * Squares are summed in double (of doubles: so that no square leaves the range) and in a fixed order (same bits on every run).
+ * The norm is finite where it is a double: a norm that no float holds is written as an infinity, and scales all the same.  The lists are read before the call returns. */
 int cb200_global_norm(cb200_stream* s, int dtype, int n, const void* const* gradients, const int64_t* counts, void* norm);
 int cb200_clip_gradients(cb200_stream* s, int dtype, int n, const void* const* gradients, const int64_t* counts,
                          void* const* clipped, double max_norm, void* norm);
