@@ -436,7 +436,7 @@ int cb200_graph_destroy(cb200_graph* g);
  * way results of data of one magnitude are within about 1e-6 of the 64-bit ones (relative to their norm).  A row with an infinity or a
  * NaN gives no finite sum, but may give NaN where exact arithmetic gives an infinity; act then keeps a NaN (relu too) and turns
  * infinities into what it makes of them. Of the options below, gemm-auto-presplit
- * (1: never halves, 2: always), gemm-tile-n (32, 64, 128: rows or result rows per tile; larger values mean 128) and gemm-k-slices
+ * (1: never halves, 2: always), gemm-tile-n (64, 128: rows or result rows per tile; larger values mean 128) and gemm-k-slices
  * steer these calls too. */
 int cb200_expert_gemm(cb200_stream* s, int dtype, void* C, int64_t ldc, int trans_b, double alpha, const void* A,
                       int64_t rows, int64_t a_cols, int64_t lda, const void* B, int64_t experts, int64_t b_cols,

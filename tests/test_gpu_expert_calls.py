@@ -1,4 +1,5 @@
-"""Calls of the expert products that their documentation allows: bad offsets anywhere, no rows under every option."""
+"""Calls of the expert products that their documentation allows: bad offsets anywhere, no rows under every option, captured and
+replayed calls and calls of two streams at once on scaled halves, narrow tiles in slices."""
 import numpy as np
 import pytest
 
@@ -50,3 +51,100 @@ def test_no_rows_under_options(stream, options):  # noqa: F811
         dW, db = ct.to_tensor(np.ones((3, 80, 40)), "float"), ct.to_tensor(np.ones((3, 80)), "float")
         ct.expert_gemm_weights(dW, 1.0, Y, X, beta, off, bias_gradient=db)
         assert np.all(ct.to_array(dW) == beta) and np.all(ct.to_array(db) == beta)
+
+
+# sizes that take scaled halves by themselves, in every direction
+LARGE = ([700, 600, 0, 748], 2048, 1024)
+
+
+def _large(seed):
+    sizes, n, k = LARGE
+    rng = np.random.default_rng(seed)
+    rows = sum(sizes) + 3
+    return rng, [rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (rows, n), (len(sizes), n, k))]
+
+
+def _all_ways(X, dY, W, off, out):
+    y, dx, dw, db = out
+    ct.expert_gemm(y, True, 1.0, X, W, 0.0, off, act="relu")
+    ct.expert_gemm(dx, False, 1.0, dY, W, 0.0, off)
+    ct.expert_gemm_weights(dw, 1.0, dY, X, 1.0, off, bias_gradient=db)
+
+
+def _outputs(rows):
+    sizes, n, k = LARGE
+    return [ct.new_tensor(list(s), "float") for s in ((rows, n), (rows, k), (len(sizes), n, k), (len(sizes), n))]
+
+
+def test_scaled_halves_repeat_their_bits_and_replay(stream):  # noqa: F811
+    """A captured pass serves other routings and other data: such that fit halves, and such that fall back inside the replay."""
+    sizes, n, k = LARGE
+    rng, (X, dY, W) = _large(43)
+    rows = len(X)
+    off = ct.to_tensor(_offsets(sizes), "int")
+    Xt, dYt, Wt = (ct.to_tensor(a, "float") for a in (X, dY, W))
+    out, zero = _outputs(rows), lambda ts: [ct.assign(t, 0.0) for t in ts]
+    _all_ways(Xt, dYt, Wt, off, out)
+    first = [ct.to_array(t) for t in out]
+    zero(out)
+    _all_ways(Xt, dYt, Wt, off, out)
+    assert all(np.array_equal(a, ct.to_array(t)) for a, t in zip(first, out))
+    stream.begin_capture()
+    _all_ways(Xt, dYt, Wt, off, out)
+    graph = stream.end_capture()
+    wide = X.copy()
+    wide[5] *= np.exp2(-rng.integers(0, 60, k)).astype(np.float32)
+    wide[1000, 7] = 1e30
+    for sizes2, data in (([1, 0, 2000, 50], X), (sizes, wide), ([500, 500, 500, 551], X)):
+        ct.assign(off, ct.to_tensor(_offsets(sizes2), "int"))
+        ct.assign(Xt, ct.to_tensor(data, "float"))
+        zero(out)
+        graph.launch(stream)
+        replayed = [ct.to_array(t) for t in out]
+        zero(out)
+        _all_ways(Xt, dYt, Wt, off, out)
+        assert all(np.array_equal(a, ct.to_array(t)) for a, t in zip(replayed, out)), sizes2
+        want, size = plain.expert_gemm(np.zeros((rows, n)), True, 1.0, data, W, 0.0, _offsets(sizes2), act="relu")
+        _within(replayed[0], want, size, _product_tol("float", k), sizes2)
+    graph.release()
+
+
+def test_two_streams_at_once_on_scaled_halves(b200_driver):
+    device = b200_driver.default_device()
+    made = []
+    for seed in (47, 53):
+        s = device.create_stream()
+        with ct.with_stream(s):
+            _, arrays = _large(seed)
+            tensors = [ct.to_tensor(a, "float") for a in arrays] + [ct.to_tensor(_offsets(LARGE[0]), "int")]
+            alone = _outputs(len(arrays[0]))
+            _all_ways(*tensors, alone)
+            made.append((s, tensors, [ct.to_array(t) for t in alone], [_outputs(len(arrays[0])) for _ in range(4)]))
+    for s, _, _, _ in made:
+        s.sync()
+    for i in range(4):
+        for s, tensors, _, outs in made:
+            with ct.with_stream(s):
+                _all_ways(*tensors, outs[i])
+    for s, _, alone, outs in made:
+        with ct.with_stream(s):
+            assert all(np.array_equal(a, ct.to_array(t)) for out in outs for a, t in zip(alone, out))
+        s.sync()
+
+
+# even rows per expert up to 32, more than the kernels of few rows take: one slice, a cluster's slices, slices that meet in L2
+@pytest.mark.parametrize("trans_b", [True, False])
+@pytest.mark.parametrize("sizes,n,k", [([30, 20], 2048, 260), ([30, 20], 128, 2048), ([40, 0, 9], 300, 1100), ([30, 20], 128, 16000), ([33, 31], 64, 9000),
+                                       ([17], 100, 20000)])
+def test_narrow_tiles_in_slices(stream, trans_b, sizes, n, k):  # noqa: F811
+    rng = np.random.default_rng(59)
+    rows = sum(sizes) + 1
+    X, W, b = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (len(sizes),) + ((n, k) if trans_b else (k, n)), (len(sizes), n)))
+    C0 = rng.standard_normal((rows, n)).astype(np.float32)
+    for beta, act in ((0.0, None), (0.5, "relu")):
+        Y = ct.to_tensor(C0, "float")
+        ct.expert_gemm(Y, trans_b, 0.5, ct.to_tensor(X, "float"), ct.to_tensor(W, "float"), beta, ct.to_tensor(_offsets(sizes), "int"),
+                       bias=ct.to_tensor(b, "float"), act=act)
+        want, size = plain.expert_gemm(C0, trans_b, 0.5, X, W, beta, _offsets(sizes), b, act)
+        _within(ct.to_array(Y), want, size, _product_tol("float", k), (sizes, beta))
+        assert np.array_equal(ct.to_array(Y).reshape(rows, n)[-1], C0[-1])
