@@ -4,10 +4,13 @@
 //   x * s = h1 + h2,   h1 = half(x * s),  h2 = half(x * s - h1),   s = a power of two per operand row
 // carries 22 bits like hi + lo of 3xTF32 does, and the three products h1 h1, h1 h2, h2 h1 cost half of what they cost
 // there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-17 of
-// it keep their 22 bits, smaller ones an absolute error of 2^-39 of it.  Where that could show in an element of the result
-// (fits() has the condition and the proof: what is lost stays below 2^-18 of the sum of the element's |a||b|), where a
-// row's largest value is outside [2^-48, 2^60], and where there is an infinity or a NaN, a flag is raised in device memory;
-// the kernel here then does nothing and the 3xTF32 kernel launched behind it, which otherwise does nothing, does the work.
+// it keep their 22 bits, smaller ones an absolute error of 2^-25 (scaled).  Down to 2^-21 of the largest that is no more than
+// 2^-19 of the value, 2^-18 of the sum of |a||b| in every element of a result.  What the halves leave of values below that
+// (a few in a million of normal data) is written to a list, and the product's epilogue adds it, times what it meets, to the
+// elements that it belongs to: so every element is good, whatever it is made of.  Where a list overflows (data of a really wide
+// range, or a row of it), where a row's largest value is outside [2^-48, 2^60] or a value below 2^-100 when scaled, and where there is an
+// infinity or a NaN, a flag is raised in device memory; the kernel here then does nothing and the 3xTF32 kernel launched behind
+// it, which otherwise does nothing, does the work.
 //
 // Steps of a call: group bounds and the table of tiles (one warp); the operands' halves, K-contiguous, with their scales
 // (HBM-bound; operands whose reduction axis is not contiguous get a pass for the column maxima first); the product; the
@@ -44,8 +47,10 @@ constexpr int THREADS = (EPI_WARPS + 4) * 32;            // three warpgroups; th
 constexpr int L_TILE = BM * BK * 2, R_TILE = BN / 2 * BK * 2;       // 16 KiB each
 constexpr int R_BOX = 64;                                // rows of one box of the column operand
 constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
+constexpr int WHERE = 16384;                             // bits for where there are remainders (a few hundred are set for normal data)
+constexpr int WHERE_BYTES = WHERE / 8 + WHERE * 4;
 constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
-constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES;
+constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES + WHERE / 8;
 constexpr int TMEM_COLS = 2 * BN;
 constexpr int DRAIN = 256 / BK;                         // stages per accumulator filling
 
@@ -55,21 +60,26 @@ struct Plan {
   int tiles;                   // expert_gemm: row tiles in the table
   int padded;                  // expert_gemm_weights: padded positions in use
   int first_row, end_row;      // rows outside are in no group
-  int unused[3];
+  int later;                   // pieces in the list for add_rests_kernel
+  int unused[2];
 };
-// How an expert's vectors of halves (rows or columns of either operand, along the reduction) lie in the halves' range, vectors
-// of zeros apart.  All zero at the start of a call.
+// What an expert's operands have for the lists; all zero at the start of a call.
 struct alignas(16) Fit {
-  int bad;                     // a scaled row's (column's) largest value is outside the range of the scales
-  int deep;                    // a value is below DEEP, and not 0
-  int thin[2];                 // most values below BIG in a vector, zeros too: of the lanes' operand, of the columns'
-  int tiny[2];                 // most values below TINY in a vector, without the zeros
-  int zero_rows;               // a matrix scaled across the reduction: rows of zeros
-  int sparse;                  // and whether there is a row with too many values below BIG to count them by columns
+  int bad;                     // something does not fit scaled halves
+  int listed[2];               // remainders of the lanes' operand, of the columns'
+  int most;                    // no more of them than this in one lane or column
 };
-// of a scaled value (the largest of what was scaled together: 2^14 to 2^15)
-// (ACROSS: of matrices that are scaled across the reduction, where counting costs more)
-constexpr float BIG = 16.f, BIG_ACROSS = 4.f, TINY = 0.125f, DEEP = 1.f / 64;
+// What the two halves leave of a scaled value below SMALL: of lane or column `at` (of the expert's matrix; a row of the batch; a
+// column of a weight gradient's operand), at position k of the halves.
+struct alignas(16) Rest { int at, k; float rest; int unused; };
+constexpr float SMALL = 1.f / 64, LEAST = 0x1p-100f;
+constexpr int MOST_RESTS = 8;            // in a lane or column (they are added one after another; normal data: 4 in the largest calls)
+// An operand's lists, `cap` for every expert.  Both operands': by where remainders are, hashed, a bit -- a lane or a column without
+// it has none -- and (behind the bits) their number.
+struct Rests { Rest* list; uint32_t* where; int cap, side; };
+__device__ __forceinline__ int where_of(int side, int expert, int at) {
+  return (int)(((unsigned)at * 2u + (unsigned)side + (unsigned)expert * 0x9e3779b1u) * 0x85ebca6bu >> 18);
+}
 struct Entry { int expert, lo, hi, first; };   // expert_gemm: rows [lo, hi); expert_gemm_weights: rows and first padded position
 
 // bounds -> table.  WEIGHTS: entry e per expert (+ one behind the last, whose `first` ends the positions); otherwise an
@@ -106,10 +116,7 @@ __global__ void __launch_bounds__(128) plan_kernel(Plan* plan, Entry* table, int
     if (lane == 0) before = carry_max;
     lo = max(lo, before);
     hi = max(hi, lo);
-    if (e < experts && begins) {
-      begins[e] = lo;
-      if (e == experts - 1) begins[experts] = hi;
-    }
+    if (e < experts && begins) begins[e] = lo;
     if (e < experts && hi > lo) first_row = min(first_row, lo);
     const int mine = e < experts ? (weights ? (hi - lo + BK - 1) / BK * BK : (hi - lo + BN - 1) / BN) : 0;
     int sum = mine;
@@ -132,7 +139,7 @@ __global__ void __launch_bounds__(128) plan_kernel(Plan* plan, Entry* table, int
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) first_row = min(first_row, __shfl_xor_sync(0xffffffffu, first_row, d));
   if (lane == 0) {
-    plan->flag = 0;
+    plan->flag = plan->later = 0;
     plan->tiles = plan->padded = carry;
     plan->first_row = first_row;
     plan->end_row = carry_max;
@@ -159,50 +166,33 @@ __device__ __forceinline__ void split_half(float y, __half& h1, __half& h2) {
   h1 = __float2half_rn(y);
   h2 = __float2half_rn(y - __half2float(h1));
 }
-// Fewer than this in a vector count as this many, and are not written down.
-__host__ __device__ __forceinline__ int thin_floor(int K) { return K / 16; }
-__host__ __device__ __forceinline__ int tiny_floor(int K) { return K / 128; }
-// May the expert's product of reduction length K run on halves?  A scaled value y is off by 2^-22 |y|, or, below TINY, by
-// 2^-25.  Without values below DEEP that is 2^-19 of every value, and 2^-18 sum |a||b| in every element of the result.  With
-// them, at least K - thin - thin terms of a sum are products of two values of BIG or more, 2^8; and the values below TINY add
-// at most 2^-25 2^15 (tiny + tiny) to its error: 2^-18 of the former if their number is no larger (with BIG_ACROSS on one side:
-// products of 2^6, no more than a quarter of their number).
-__device__ __forceinline__ bool fits(const Fit& f, int K, bool across) {
-  const long long both = (long long)K - max(f.thin[0], thin_floor(K)) - max(f.thin[1], thin_floor(K));
-  const long long tiny = (long long)max(f.tiny[0], tiny_floor(K)) + max(f.tiny[1], tiny_floor(K));
-  return !f.bad && (!f.deep || (both >= 1 && both >= (across ? 4 : 1) * tiny));
-}
 union Half8 { __half h[8]; __half2 h2[4]; uint4 v; };
 
-// Eight values times `up` as halves.  split8_least: the smallest magnitude of them; split8: of the first n of them, how many are
-// below BIG and how many that are not 0 below TINY (added to what is there), and whether one is below DEEP.
-__device__ __forceinline__ float split8_least(const float (&w)[8], float up, Half8& a, Half8& b) {
-  __half2 least = __float2half2_rn(65504.f);
+// Eight values times `up` as halves; bit j: value j is below SMALL, and not 0.
+__device__ __forceinline__ uint32_t split8(const float (&w)[8], float up, Half8& a, Half8& b) {
+  __half2 least = __float2half2_rn(65504.f);               // two at a time
+  uint32_t small = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j]);
 #pragma unroll
   for (int j = 0; j < 4; ++j) least = __hmin2(least, __habs2(a.h2[j]));
-  return __half2float(__hmin(__low2half(least), __high2half(least)));
+  if (__half2float(__hmin(__low2half(least), __high2half(least))) < SMALL)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (w[j] != 0.f && fabsf(w[j] * up) < SMALL) small |= 1u << j;
+  return small;
 }
-__device__ __forceinline__ void split8(const float (&w)[8], float up, int n, Half8& a, Half8& b, int& thin, int& tiny, bool& deep) {
-  __half2 small = __float2half2_rn(0.f), least = __float2half2_rn(65504.f);        // two at a time
-#pragma unroll
-  for (int j = 0; j < 8; ++j) split_half(w[j] * up, a.h[j], b.h[j]);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const __half2 q = __habs2(a.h2[j]);
-    small = __hadd2(small, __hlt2(q, __float2half2_rn(BIG)));
-    least = __hmin2(least, q);
-  }
-  thin += (int)__half2float(__hadd(__low2half(small), __high2half(small)));
-  if (n < 8) thin -= 8 - n;                                // (the others are zeros)
-  if (__half2float(__hmin(__low2half(least), __high2half(least))) < TINY)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float y = fabsf(w[j] * up);
-      tiny += w[j] != 0.f && y < TINY;
-      deep = deep || (w[j] != 0.f && y < DEEP);
-    }
+__device__ __forceinline__ void keep_rest(Fit* fit, const Rests& rests, int expert, int at, int k, float y) {
+  Fit* f = fit + expert;
+  if (!(fabsf(y) >= LEAST)) f->bad = 1;
+  __half h1, h2;
+  split_half(y, h1, h2);
+  const float rest = (y - __half2float(h1)) - __half2float(h2);      // both differences are exact
+  if (rest == 0.f) return;
+  const int i = atomicAdd(&f->listed[rests.side], 1), h = where_of(rests.side, expert, at);
+  atomicOr(rests.where + (h >> 5), 1u << (h & 31));
+  atomicMax(&f->most, (int)atomicAdd(rests.where + WHERE / 32 + h, 1u) + 1);
+  if (i < rests.cap) rests.list[(long long)expert * rests.cap + i] = {at, k, rest, 0};
 }
 
 __device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
@@ -218,33 +208,19 @@ __device__ __forceinline__ void load8(const float* p, int left, bool vec, float 
 // One row of scaled halves: TPR threads per row, 8 values per thread and step, the first HOLD steps in registers between the
 // maximum and the split (longer rows are read again, from L2).  hi / lo: pitch kp (a multiple of 8).
 //   RAGGED = 0  the experts' matrices: row r at x + (r / rows_per) * stride + (r % rows_per) * ld
-//   RAGGED = 3  the same, of rows that run across the reduction: what lies low is counted by columns, in `across`; a row of
-//               zeros gets the inverse scale 0
+//   RAGGED = 3  the same, of rows that run across the reduction; a row of zeros gets the inverse scale 0
 //   RAGGED = 1  the ragged rows: rows in no group become zeros
 //   RAGGED = 2  the same, every value multiplied by 2^14 fold[expert of the row][column] first: the inverse scales of a matrix
 //               whose rows run across the reduction, which cannot be taken out of the sum behind it
-// `fit` is told what the rows look like.  Behind the CTAs of the rows (row_ctas) those of RAGGED = 2 turn the column counts of
-// the matrices before into their Fit.
-struct Across { int* zeros; int* small; int* tiny; int cols; };      // per expert and column: 0; else below BIG_ACROSS; below TINY
 template <int TPR, int RAGGED>
 __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* lo, float* down_out, const float* x, long long ld,
                                                          long long stride, int rows_per, long long rows, int cols, int kp,
-                                                         const Plan* plan, Fit* fit, const float* fold, const int* begins, int experts,
-                                                         Across across, unsigned row_ctas) {
+                                                         const Plan* plan, Fit* fit, Rests rests, const float* fold, const int* begins,
+                                                         int experts) {
   constexpr int HOLD = 4;
   constexpr bool MATRICES = RAGGED == 0 || RAGGED == 3;
   wait_for_previous_kernel();
-  if (RAGGED == 2 && blockIdx.x >= row_ctas) {
-    const long long i = (long long)(blockIdx.x - row_ctas) * 256 + threadIdx.x;
-    if (i >= (long long)experts * across.cols) return;
-    Fit* f = fit + i / across.cols;
-    const int zeros = across.zeros[i], thin = f->sparse ? cols : (zeros == cols - f->zero_rows ? 0 : zeros + across.small[i]), tiny = across.tiny[i];
-    if (thin > thin_floor(cols)) atomicMax(&f->thin[0], thin);
-    if (tiny > tiny_floor(cols)) atomicMax(&f->tiny[0], tiny);
-    return;
-  }
   __shared__ uint32_t part_max[8];
-  __shared__ int part_tiny[8], part_thin[8];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, warp = threadIdx.x >> 5;
   const long long r = (long long)blockIdx.x * (256 / TPR) + sub;
   const bool live = r < rows, grouped = MATRICES || (r >= plan->first_row && r < plan->end_row);
@@ -260,7 +236,6 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
     }
     return a;
   };
-  const int sparse = RAGGED == 3 && live ? __ldcg(&fit[r / rows_per].sparse) : 0;      // (set: the counts do not matter any more)
   const float* scales = nullptr;
   if (RAGGED == 2 && live && grouped) scales = fold + (long long)expert_of_row() * cols;
   auto fetch = [&](int c, float (&w)[8]) {
@@ -307,26 +282,17 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
   float up, down;
   const bool ok = scale_of(m, up, down);
   if (!ok) up = 0.f;
-  const long long by_expert = RAGGED == 3 && live ? r / rows_per * cols : 0;
-  const bool by_column = RAGGED == 3 && live && !sparse;
-  int tiny = 0, thin = 0;
-  bool deep = false;
   auto put = [&](int c, const float (&w)[8]) {
     Half8 a, b;
-    if (RAGGED != 3) {
-      split8(w, up, n - c, a, b, thin, tiny, deep);
-    } else if (split8_least(w, up, a, b) < BIG_ACROSS && m != 0 && ok) {     // (one step of eight warps in fifty)
-      for (int j = 0; j < min(8, n - c); ++j) {
-        const float x = src[c + j], y = fabsf(x * up);
-        if (y >= BIG_ACROSS) continue;
-        ++thin;
-        if (by_column) atomicAdd((x == 0.f ? across.zeros : across.small) + by_expert + c + j, 1);
-        if (by_column && x != 0.f && y < TINY) atomicAdd(across.tiny + by_expert + c + j, 1);
-        deep = deep || (x != 0.f && y < DEEP);
-      }
-    }
+    uint32_t small = split8(w, up, a, b);
     *reinterpret_cast<uint4*>(hi + r * kp + c) = a.v;      // pitch and position are multiples of 8 halves
     *reinterpret_cast<uint4*>(lo + r * kp + c) = b.v;
+    if (!ok) small = 0;
+    for (; small; small &= small - 1) {
+      const int at = c + __ffs(small) - 1, row = (int)(MATRICES ? r % rows_per : r);
+      const float y = (RAGGED == 2 ? src[at] * (16384.f * scales[at]) : src[at]) * up;
+      keep_rest(fit, rests, expert_of_row(), RAGGED == 3 ? at : row, RAGGED == 3 ? row : at, y);
+    }
   };
 #pragma unroll
   for (int it = 0; it < HOLD; ++it) {
@@ -338,33 +304,11 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
     fetch(c, w);
     put(c, w);
   }
-  tiny = (int)__reduce_add_sync(0xffffffffu, (unsigned)tiny);
-  thin = (int)__reduce_add_sync(0xffffffffu, (unsigned)thin);
-  deep = __any_sync(0xffffffffu, deep);
-  if (deep && ok && (threadIdx.x & 31) == 0) fit[expert_of_row()].deep = 1;
-  if (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) { part_tiny[warp] = tiny; part_thin[warp] = thin; }
-    __syncthreads();
-    tiny = thin = 0;
-#pragma unroll
-    for (int w = 0; w < TPR / 32; ++w) { tiny += part_tiny[sub * (TPR / 32) + w]; thin += part_thin[sub * (TPR / 32) + w]; }
-  }
   if (t == 0 && live) {
     // (a scale of 0 that is folded into the other operand takes what meets a row of zeros out of its row's maximum, but for
     // infinities and NaN)
     down_out[r] = RAGGED == 3 && m == 0 ? 0.f : down;
-    const bool many = thin > thin_floor(cols), many_tiny = tiny > tiny_floor(cols);
-    if (RAGGED == 3 && m == 0) {
-      atomicAdd(&fit[expert_of_row()].zero_rows, 1);
-    } else if (m != 0 && (!ok || many || (RAGGED != 3 && many_tiny))) {      // (ordinary rows: none of it)
-      Fit* f = fit + expert_of_row();
-      if (!ok) f->bad = 1;
-      else if (RAGGED == 3) f->sparse = 1;
-      else {
-        if (many) atomicMax(&f->thin[RAGGED ? 1 : 0], thin);
-        if (many_tiny) atomicMax(&f->tiny[RAGGED ? 1 : 0], tiny);
-      }
-    }
+    if (!ok) fit[expert_of_row()].bad = 1;
   }
 }
 
@@ -425,36 +369,19 @@ __global__ void __launch_bounds__(128) column_max_kernel(uint32_t* maxima, float
   }
 }
 
-// What split_columns_kernel counted in the columns of an operand, one word per group and column.
-struct ColumnCounts { const uint32_t* maxima; int* thin; int* tiny; int cols; };
-
-// The counts of both operands' columns into the groups' Fit: columns of r first, then those of l, 128 a CTA.  Beside, where `out`
-// is given,  out[g, c] = alpha * (the sums of the rows of group g in column c of r, block by block) + beta * out[g, c]
-__global__ void __launch_bounds__(128) column_fit_kernel(Fit* fit, ColumnCounts l, ColumnCounts r, const Entry* table, float* out, const float* sums,
-                                                         float alpha, float beta) {
+// bias_gradient[g, c] = alpha * (the sums of group g's rows, block by block) + beta * bias_gradient[g, c]
+__global__ void __launch_bounds__(128) column_sum_kernel(float* out, const float* sums, const Entry* table, int cols, float alpha, float beta) {
   wait_for_previous_kernel();
-  const int blocks_r = (r.cols + 127) / 128, g = blockIdx.y;
-  const bool is_r = (int)blockIdx.x < blocks_r;
-  const ColumnCounts& p = is_r ? r : l;
-  const int c = ((int)blockIdx.x - (is_r ? 0 : blocks_r)) * 128 + (int)threadIdx.x;
+  const int c = blockIdx.x * 128 + threadIdx.x, g = blockIdx.y;
+  if (c >= cols) return;
   const Entry e = table[g];
-  const int n = e.hi - e.lo;
-  const long long at = (long long)g * p.cols + c;
-  const bool counts = n > 0 && c < p.cols && p.maxima[at] != 0;
-  const unsigned thin = __reduce_max_sync(0xffffffffu, counts ? (unsigned)p.thin[at] : 0u);
-  const unsigned tiny = __reduce_max_sync(0xffffffffu, counts ? (unsigned)p.tiny[at] : 0u);
-  if ((threadIdx.x & 31) == 0) {
-    if ((int)thin > thin_floor(n)) atomicMax(&fit[g].thin[is_r ? 1 : 0], (int)thin);
-    if ((int)tiny > tiny_floor(n)) atomicMax(&fit[g].tiny[is_r ? 1 : 0], (int)tiny);
-  }
-  if (!out || !is_r || c >= p.cols) return;
   float s = 0.f;
-  if (n > 0) {
+  if (e.hi > e.lo) {
     const long long first = e.lo / 64, last = (e.hi - 1) / 64;
 #pragma unroll 8
-    for (long long b = first; b <= last; ++b) s += sums[(b + g) * p.cols + c];
+    for (long long b = first; b <= last; ++b) s += sums[(b + g) * cols + c];
   }
-  float* to = out + at;
+  float* to = out + (long long)g * cols + c;
   float v = alpha * s;
   if (beta != 0.f) v += beta * (*to);
   *to = v;
@@ -465,7 +392,7 @@ __global__ void __launch_bounds__(128) column_fit_kernel(Fit* fit, ColumnCounts 
 // blocks of 64 columns.
 __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* lo, float* down_out, const uint32_t* maxima, const float* x,
                                                             long long ld, const Entry* table, const int* owner, int cols, long long kp,
-                                                            const Plan* plan, Fit* fit, int* thin_out, int* tiny_out) {
+                                                            const Plan* plan, Fit* fit, Rests rests) {
   __shared__ float tile[2][32][65];
   wait_for_previous_kernel();
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
@@ -492,31 +419,26 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
     }
     __syncthreads();
     // a thread: 8 positions of one column of each block
-    const int valid = max(0, min(8, end - (r0 + p8)));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int c = blockIdx.x * 128 + h * 64 + col;
+      if (c >= cols) continue;
       float up, down, w[8];
       const bool ok = scale_of(m[h], up, down);
       Half8 a, z;
-      int thin = 0, tiny = 0;
-      bool deep = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = tile[h][p8 + j][col];
-      split8(w, up, valid, a, z, thin, tiny, deep);
-      if (c < cols) {
-        *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;           // kp is a multiple of 64
-        *reinterpret_cast<uint4*>(lo + c * kp + pos + p8) = z.v;
-        if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
-        if (!ok) fit[g].bad = 1;
-        else if (deep) fit[g].deep = 1;
+      uint32_t small = split8(w, up, a, z);
+      *reinterpret_cast<uint4*>(hi + c * kp + pos + p8) = a.v;             // kp is a multiple of 64
+      *reinterpret_cast<uint4*>(lo + c * kp + pos + p8) = z.v;
+      if (p8 == 0 && begins) down_out[(long long)g * cols + c] = down;
+      if (!ok) {
+        fit[g].bad = 1;
+        small = 0;
       }
-      int both = thin | tiny << 8;                         // at most 32 each in the column's four threads
-      both += __shfl_xor_sync(0xffffffffu, both, 1);
-      both += __shfl_xor_sync(0xffffffffu, both, 2);
-      if (p8 == 0 && c < cols && ok && m[h] != 0) {
-        if (both & 255) atomicAdd(thin_out + (long long)g * cols + c, both & 255);
-        if (both >> 8) atomicAdd(tiny_out + (long long)g * cols + c, both >> 8);
+      for (; small; small &= small - 1) {
+        const int j = __ffs(small) - 1;
+        keep_rest(fit, rests, g, c, (int)pos + p8 + j, tile[h][p8 + j][col] * up);
       }
     }
   }
@@ -530,7 +452,12 @@ struct PairArgs {
   const float* bias;
   Plan* plan;
   const Fit* fit;               // per expert
-  const int* begins;            // expert_gemm: the groups' first rows, and the last one's end
+  Rests l_rests, r_rests;
+  int4* later;                  // pieces that wait for their remainders: expert, first lane, first column, columns
+  // the halves: the lane operand's element (expert, lane, k) at expert * l_expert + lane * l_lane + k * l_k, the column operand's
+  // (row, k) at row * r_pitch + k
+  const __half* l_hi; const __half* l_lo; const __half* r_hi; const __half* r_lo;
+  long long l_expert, l_lane, l_k, r_pitch;
   const Entry* table;
   int* status;
   int lanes, cols;              // extents: lanes of one expert's matrix; WEIGHTS: columns of one result
@@ -589,6 +516,113 @@ __host__ __device__ __forceinline__ uint32_t make_idesc_f16(int m, int n, int a_
   return (1u << 4) | ((uint32_t)(a_mn_major & 1) << 15) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// The next of n remainders in the order of (at, k) -- whatever order they were written in -- with at in [first, end), by the
+// whole warp; returns how many there are from it on.  `key` starts as 0.
+__device__ __forceinline__ int next_rest(const Rest* list, int n, int first, int end, unsigned long long& key, int& at, int& k, float& rest) {
+  const int lane = threadIdx.x & 31;
+  unsigned long long best = ~0ull;
+  int count = 0;
+  rest = 0.f;
+#pragma unroll 2
+  for (int i = lane; i < n; i += 32) {
+    const int4 v = __ldg(reinterpret_cast<const int4*>(list) + i);
+    const unsigned long long own = ((unsigned long long)(unsigned)v.x << 32 | (unsigned)v.y) + 1;
+    if (v.x >= first && v.x < end && own > key) {
+      ++count;
+      if (own < best) { best = own; rest = __int_as_float(v.z); }
+    }
+  }
+  count = (int)__reduce_add_sync(0xffffffffu, (unsigned)count);
+  if (count == 0) return 0;
+  const unsigned high = __reduce_min_sync(0xffffffffu, (unsigned)(best >> 32));
+  const unsigned low = __reduce_min_sync(0xffffffffu, (unsigned)(best >> 32) == high ? (unsigned)best : 0xffffffffu);
+  const unsigned owner = __ballot_sync(0xffffffffu, best == ((unsigned long long)high << 32 | low));
+  rest = __shfl_sync(0xffffffffu, rest, __ffs(owner) - 1);
+  key = (unsigned long long)high << 32 | low;
+  at = (int)((key - 1) >> 32);
+  k = (int)(key - 1);
+  return count;
+}
+
+// The pieces (32 lanes, up to 128 columns) that the product has left for later: what the halves leave out of the operands' small
+// values -- remainders of the lanes times the columns' values (these with their own remainders), those of the columns times the
+// lanes' halves -- and the activation.  A CTA a piece, a warp 16 columns of it.  (Most calls have a piece or none: loops are kept
+// short, since fetching their code is what takes the time.)
+__global__ void __launch_bounds__(256) add_rests_kernel(const __grid_constant__ PairArgs p) {
+  constexpr int OWN = BN / 2 / 8;
+  __shared__ float sums[8][OWN][32];
+  wait_for_previous_kernel();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = p.plan->later;
+#pragma unroll 1
+  for (int i = blockIdx.x; i < pieces; i += gridDim.x) {
+    const int4 piece = p.later[i];
+    const int expert = piece.x, l = piece.y + lane, r_first = piece.z + warp * OWN, cols = min(OWN, piece.w - warp * OWN);
+    if (cols <= 0) continue;
+    const Fit f = p.fit[expert];
+    float (&sum)[OWN][32] = sums[warp];
+#pragma unroll 1
+    for (int j = 0; j < cols; ++j) sum[j][lane] = 0.f;
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+      const Rest* list = (side ? p.r_rests.list : p.l_rests.list) + (long long)expert * (side ? p.r_rests.cap : p.l_rests.cap);
+      const int first = side ? r_first : piece.y, end = side ? r_first + cols : piece.y + 32;
+      unsigned long long key = 0;
+      int at, k;
+      float rest;
+#pragma unroll 1
+      while (next_rest(list, f.listed[side], first, end, key, at, k, rest)) {
+        const long long r_at = (long long)(side ? at : r_first + lane) * p.r_pitch + k, l_at = expert * p.l_expert + l * p.l_lane + k * p.l_k;
+        const bool there = side ? l < p.lanes : lane < cols;
+        float x = there ? __half2float((side ? p.l_hi : p.r_hi)[side ? l_at : r_at]) + __half2float((side ? p.l_lo : p.r_lo)[side ? l_at : r_at]) : 0.f;
+        if (side) {
+          sum[at - r_first][lane] = fmaf(rest, x, sum[at - r_first][lane]);
+          continue;
+        }
+        const Rest* of_r = p.r_rests.list + (long long)expert * p.r_rests.cap;
+#pragma unroll 1
+        for (int b = 0; b < f.listed[1]; b += 32) {
+          const int4 v = b + lane < f.listed[1] ? __ldg(reinterpret_cast<const int4*>(of_r) + b + lane) : make_int4(-1, -1, 0, 0);
+#pragma unroll 1
+          for (unsigned hit = __ballot_sync(0xffffffffu, v.y == k && v.x >= r_first && v.x < r_first + cols); hit; hit &= hit - 1) {
+            const int c = __shfl_sync(0xffffffffu, v.x, __ffs(hit) - 1) - r_first;
+            const float its = __int_as_float(__shfl_sync(0xffffffffu, v.z, __ffs(hit) - 1));
+            if (c == lane) x += its;
+          }
+        }
+        __syncwarp();
+        if (lane < cols) sum[lane][at - piece.y] = fmaf(rest, x, sum[lane][at - piece.y]);
+        __syncwarp();
+      }
+    }
+    const float r_scale = lane < cols ? p.r_down[(p.weights ? (long long)expert * p.cols : 0) + r_first + lane] : 0.f;
+    float l_scale = 0.f, old[OWN];
+    float* c = p.C + (p.weights ? expert * p.c_stride : 0) + (long long)r_first * p.ldc + l;
+    if (l < p.lanes) {
+      l_scale = p.l_down ? p.l_down[(long long)expert * p.lanes + l] : 1.f / 16384.f;
+#pragma unroll
+      for (int j = 0; j < OWN; ++j) old[j] = j < cols ? c[(long long)j * p.ldc] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < OWN; ++j) {
+      const float scale = l_scale * __shfl_sync(0xffffffffu, r_scale, j);
+      if (j < cols) old[j] = fmaf(sum[j][lane] * scale, p.alpha, old[j]);
+    }
+    if (l < p.lanes) {
+#pragma unroll
+      for (int j = 0; j < OWN; ++j)
+        if (j < cols) sum[j][lane] = old[j];
+#pragma unroll 1
+      for (int j = 0; j < cols; ++j) {
+        float v = sum[j][lane];
+        if (p.act == CB200_ACT_RELU) v = groups::relu(v);
+        else if (p.act != CB200_ACT_NONE) v = apply_act_transcendental(v, p.act);
+        c[(long long)j * p.ldc] = v;
+      }
+    }
+    __syncwarp();
+  }
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmLlo, const __grid_constant__ CUtensorMap tmR,
                    const __grid_constant__ CUtensorMap tmRlo, const __grid_constant__ PairArgs p) {
@@ -606,19 +640,18 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   const int n_clusters = (int)gridDim.x >> 1, cluster_id = (int)blockIdx.x >> 1;
 
   wait_for_previous_kernel();
-  int no_fit = 0;
+  uint32_t* where = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE + 256 + SCALES);
+  int* most_rests = reinterpret_cast<int*>(smem + STAGES * STAGE + 248);
+  if (threadIdx.x < WHERE / 128) reinterpret_cast<uint4*>(where)[threadIdx.x] = reinterpret_cast<const uint4*>(p.l_rests.where)[threadIdx.x];
+  int no_fit = 0, most = 0;
   for (int e = threadIdx.x; e < p.experts; e += THREADS) {
     const Fit f = p.fit[e];
-    int n, K = p.K;                                        // the group's rows, the length of its reduction
-    if (p.weights) {
-      const Entry t = p.table[e];
-      n = K = t.hi - t.lo;
-    } else {
-      const int first = p.begins[e];
-      n = p.begins[e + 1] - first;
-    }
-    no_fit |= f.bad | (n > 0 && !fits(f, K, p.l_mn));
+    no_fit |= f.bad | (f.listed[0] > p.l_rests.cap) | (f.listed[1] > p.r_rests.cap) | (f.most > MOST_RESTS);
+    most = max(most, f.most);
   }
+  if (threadIdx.x == 0) *most_rests = 0;
+  __syncthreads();
+  if (most > 0) atomicMax(most_rests, most);
   if (__syncthreads_or(no_fit)) {         // every CTA comes to the same: nothing has been set up yet
     if (threadIdx.x == 0) p.plan->flag = 1;
     return;
@@ -812,9 +845,41 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
         if (lane == 0) mbar_arrive_cluster(leader_drained + 8 * (fill & 1));
       }
       if (!ok) break;
+      // What the halves have left out, in the lanes and columns with remainders: one is at most 2^-25 and meets at most 2^15, so
+      // where a sum itself is 2^8 times their number, all of them together are below 2^-18 of it (normal data: hardly anywhere
+      // not).  Other pieces are left to add_rests_kernel, with the activation.
+      bool later = false;
+      if (!none && left > 0) {
+        const int r_first = u.r0 + half * (BN / 2);
+        int h = where_of(0, u.expert, l);
+        const bool of_lane = (where[h >> 5] >> (h & 31) & 1) && l < p.lanes;
+        unsigned of_columns[BN / 64];
+#pragma unroll
+        for (int i = 0; i < BN / 64; ++i) {
+          h = where_of(1, u.expert, r_first + i * 32 + lane);
+          of_columns[i] = __ballot_sync(0xffffffffu, i * 32 + lane < left && (where[h >> 5] >> (h & 31) & 1));
+        }
+        const bool any_lane = __any_sync(0xffffffffu, of_lane);
+        // (an element has those of its lane and those of its column)
+        const float bound = (any_lane && (of_columns[0] | of_columns[1] | of_columns[2] | of_columns[3]) ? 512.f : 256.f) * (float)*most_rests;
+        if (any_lane) {
+          float least = INFINITY;
+#pragma unroll
+          for (int j = 0; j < BN / 2; ++j) least = fminf(least, j < left ? fabsf(acc[j]) : INFINITY);
+          later = of_lane && least < bound;
+        }
+#pragma unroll
+        for (int i = 0; i < BN / 64; ++i)
+          if (of_columns[i]) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) later = later || ((of_columns[i] >> j & 1) && fabsf(acc[i * 32 + j]) < bound && l < p.lanes);
+          }
+        later = __any_sync(0xffffffffu, later);
+        if (later && lane == 0) p.later[atomicAdd(&p.plan->later, 1)] = make_int4(u.expert, l, r_first, min(left, BN / 2));
+      }
       // out of registers, while the tensor cores work on the pair's next tile
       float* c = p.C + (p.weights ? u.expert * p.c_stride : 0) + (long long)(u.r0 + half * (BN / 2)) * p.ldc + l;
-      const bool live = l < p.lanes, relu = p.act == CB200_ACT_RELU;
+      const bool live = l < p.lanes, relu = p.act == CB200_ACT_RELU && !later;
       // whole warps of whole tiles without a beta: about 9 instructions per value (24 with predicates, shuffles and the
       // three factors apart, which held the epilogue to 9 us per tile where the product takes 3)
       const bool whole = left >= BN / 2 && __all_sync(0xffffffffu, live) && p.beta == 0.f;
@@ -867,7 +932,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
         }
       }
       __syncwarp();                                        // the list is rewritten for the next tile
-      if (p.act > CB200_ACT_RELU && live) {
+      if (p.act > CB200_ACT_RELU && live && !later) {
         // tanh / logistic over what was just stored: a call among 128 live accumulators would spill them
         const int n = min(left, BN / 2);
 #pragma unroll 1
@@ -948,26 +1013,25 @@ int launch_next(cb200_stream* s, void (*kernel)(P...), dim3 grid, int threads, s
 
 template <int RAGGED>
 int split_rows(cb200_stream* s, __half* hi, __half* lo, float* down, const float* x, long long ld, long long stride, int rows_per,
-               long long rows, int cols, int kp, const Plan* plan, Fit* fit, const int* begins, int experts, Across across, const float* fold) {
-  const long long more = RAGGED == 2 ? ((long long)experts * across.cols + 255) / 256 : 0;
+               long long rows, int cols, int kp, const Plan* plan, Fit* fit, const Rests& rests, const int* begins, int experts,
+               const float* fold) {
   const int rows_a_cta = cols <= 1024 ? 8 : (cols <= 4096 ? 2 : 1);
-  const unsigned ctas = (unsigned)((rows + rows_a_cta - 1) / rows_a_cta);
   auto* kernel = cols <= 1024 ? split_rows_kernel<32, RAGGED> : (cols <= 4096 ? split_rows_kernel<128, RAGGED> : split_rows_kernel<256, RAGGED>);
-  return launch_next(s, kernel, dim3((unsigned)(ctas + more)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows, cols, kp, plan, fit, fold,
-                     begins, experts, across, ctas);
+  return launch_next(s, kernel, dim3((unsigned)((rows + rows_a_cta - 1) / rows_a_cta)), 256, 0, 1, hi, lo, down, x, ld, stride, rows_per, rows,
+                     cols, kp, plan, fit, rests, fold, begins, experts);
 }
 
 // `sums` (may be null): workspace for the column sums of 64-row blocks, ((rows + 63) / 64 + groups_n) x cols
 int split_columns(cb200_stream* s, __half* hi, __half* lo, float* down, uint32_t* maxima, float* sums, const float* x, long long ld,
-                  const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, const Plan* plan, Fit* fit, int* thin,
-                  int* tiny) {
+                  const Entry* table, const int* owner, int groups_n, int rows, int cols, long long kp, const Plan* plan, Fit* fit,
+                  const Rests& rests) {
   const long long chunks = (rows + 63) / 64, blocks = kp / POS;
   const dim3 grid_max((unsigned)((cols + 127) / 128), (unsigned)(chunks < 65535 ? chunks : 65535));
   const bool vec = ((uintptr_t)x & 15) == 0 && ld % 4 == 0 && cols % 4 == 0;
   int rc = launch_next(s, vec ? column_max_kernel<4> : column_max_kernel<1>, grid_max, 128, 0, 1, maxima, sums, x, ld, table, groups_n, rows, cols);
   if (rc) return rc;
   return launch_next(s, split_columns_kernel, dim3((unsigned)((cols + 127) / 128), (unsigned)(blocks < 65535 ? blocks : 65535)), 256, 0, 1, hi,
-                     lo, down, maxima, x, ld, table, owner, cols, kp, plan, fit, thin, tiny);
+                     lo, down, maxima, x, ld, table, owner, cols, kp, plan, fit, rests);
 }
 
 int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long long l_rows, long long l_cols, long long l_pitch,
@@ -985,8 +1049,12 @@ int launch_pair(cb200_stream* s, const __half* l_hi, const __half* l_lo, long lo
       (rc = half_map(&tmR, r_hi, r_rows, r_cols, r_pitch, 64, R_BOX)) || (rc = half_map(&tmRlo, r_lo, r_rows, r_cols, r_pitch, 64, R_BOX)))
     return rc;
   const long long clusters = units < s->sm_count / 2 ? units : s->sm_count / 2;
-  return launch_next(s, expert_pair_kernel, dim3((unsigned)(2 * clusters)), THREADS, SMEM, 2, tmL, tmLlo, tmR, tmRlo, a);
+  if ((rc = launch_next(s, expert_pair_kernel, dim3((unsigned)(2 * clusters)), THREADS, SMEM, 2, tmL, tmLlo, tmR, tmRlo, a))) return rc;
+  return launch_next(s, add_rests_kernel, dim3((unsigned)(2 * s->sm_count)), 256, 0, 1, a);
 }
+
+// pieces of 32 lanes x 128 columns that `units` of the product consist of, which may all have to wait for their remainders
+constexpr int PIECES = 2 * BM / 32 * 2;
 
 inline long long up8(long long v) { return (v + 7) / 8 * 8; }
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -1002,6 +1070,9 @@ struct Carve {
   }
 };
 
+// Room in an expert's list of remainders for `values` of an operand: six times what normal data bring (2.4 in a million)
+long long rests_room(double values) { return 64 + (long long)(values / 65536 < 4032 ? values / 65536 : 4032); }
+
 constexpr size_t MOST_WORKSPACE = (size_t)2 << 30;
 
 }  // namespace
@@ -1013,7 +1084,7 @@ constexpr size_t MOST_WORKSPACE = (size_t)2 << 30;
 bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
   const double l = (double)experts * N * K, r = (double)rows * K;
-  if ((l + r + 3.0 * experts * N) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
+  if ((l + r) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * N > 2000000000LL || experts * K > 2000000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * K;
   // (halves that do not stay in L2 between the split and the product are read from memory)
@@ -1026,8 +1097,8 @@ bool cb200_expert_f16_ok(cb200_stream* s, long long rows, long long K, long long
 }
 bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, long long N, long long experts) {
   if (s->opt_gemm_auto_presplit == 1) return false;
-  const double operands = (double)(rows + BK * experts) * (M + N), counts = 3.0 * experts * (M + N);
-  if ((operands + counts) * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
+  const double operands = (double)(rows + BK * experts) * (M + N);
+  if (operands * 4 > (double)MOST_WORKSPACE - (64 << 20) || experts * (M + N) > 500000000LL) return false;
   if (s->opt_gemm_auto_presplit == 2) return true;
   const double flops = 2.0 * rows * N * M, results = (double)experts * N * M;
   const double here = 28.0 + operands * 1.85e-6 + results * 0.67e-6 + flops / 300e6, there = 12.0 + results * 1e-6 + flops / 125e6;
@@ -1042,10 +1113,12 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   // the matrices' rows as they are stored: [N, K] reduces along them, [K, N] (the gradient of the input) across them
   const int l_per = trans_b ? N : K, l_cols = trans_b ? K : N;
   const long long kp = up8(K), lp = up8(l_cols), l_rows = (long long)experts * l_per;
-  // zero at the start of the call: the experts' Fit, and the counts by columns of matrices that are scaled across the reduction
-  const size_t fit_words = (size_t)experts * (sizeof(Fit) / 4), columns = trans_b ? 0 : (size_t)experts * N, zeroed_n = fit_words + 3 * columns;
+  // (groups up to 16 times the average have room enough)
+  Rests l_rests = {nullptr, nullptr, (int)rests_room((double)N * K), 0}, r_rests = {nullptr, nullptr, (int)rests_room(16.0 * rows * K / experts), 1};
   const size_t tiles = (size_t)((rows + BN - 1) / BN + (experts < rows ? experts : rows));
-  const size_t bytes = up256(sizeof(Plan)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)(experts + 1) * 4) + up256(zeroed_n * 4) +
+  const long long units = (long long)tiles * ((N + 2 * BM - 1) / (2 * BM));
+  const size_t bytes = up256(sizeof(Plan)) + up256((size_t)units * PIECES * sizeof(int4)) + up256((tiles + 1) * sizeof(Entry)) + up256((size_t)experts * 4) + up256((size_t)experts * sizeof(Fit) + WHERE_BYTES) +
+                       up256((size_t)experts * l_rests.cap * sizeof(Rest)) + up256((size_t)experts * r_rests.cap * sizeof(Rest)) +
                        2 * up256((size_t)l_rows * lp * 2) + 2 * up256((size_t)rows * kp * 2) + up256((size_t)l_rows * 4) +
                        up256((size_t)rows * 4);
   void* ws = nullptr;
@@ -1054,33 +1127,36 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
   Entry* table = w.take<Entry>(tiles + 1);
-  int* begins = w.take<int>((size_t)experts + 1);
-  uint32_t* zeroed = w.take<uint32_t>(zeroed_n);
+  int* begins = w.take<int>((size_t)experts);
+  char* zeroed = w.take<char>((size_t)experts * sizeof(Fit) + WHERE_BYTES);
   Fit* fit = (Fit*)zeroed;
-  int* counts = (int*)(zeroed + fit_words);
-  const Across across = {counts, counts + columns, counts + 2 * columns, trans_b ? 0 : N};
+  l_rests.where = r_rests.where = (uint32_t*)(fit + experts);
+  l_rests.list = w.take<Rest>((size_t)experts * l_rests.cap);
+  r_rests.list = w.take<Rest>((size_t)experts * r_rests.cap);
   __half* l_hi = w.take<__half>((size_t)l_rows * lp);
   __half* l_lo = w.take<__half>((size_t)l_rows * lp);
   __half* r_hi = w.take<__half>((size_t)rows * kp);
   __half* r_lo = w.take<__half>((size_t)rows * kp);
   float* l_down = w.take<float>((size_t)l_rows);
   float* r_down = w.take<float>((size_t)rows);
-  const unsigned zero_ctas = (unsigned)((zeroed_n + 511) / 512 < 128 ? (zeroed_n + 511) / 512 : 128);
-  plan_kernel<<<1 + zero_ctas, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev, zeroed, (long long)zeroed_n);
+  plan_kernel<<<65, 128, 0, s->stream>>>(plan, table, nullptr, begins, offsets, experts, rows, 0, s->status_dev, (uint32_t*)zeroed,
+                                                       (long long)experts * (sizeof(Fit) / 4) + WHERE_BYTES / 4);
   CB_LAUNCH_CHECK(s);
-  rc = trans_b ? split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, fit, begins, experts, across, nullptr)
-               : split_rows<3>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, fit, begins, experts, across, nullptr);
+  rc = trans_b ? split_rows<0>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, fit, l_rests, begins, experts, nullptr)
+               : split_rows<3>(s, l_hi, l_lo, l_down, B, ldb, b_stride, l_per, l_rows, l_cols, (int)lp, plan, fit, l_rests, begins, experts, nullptr);
   if (rc) return rc;
-  rc = trans_b ? split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, fit, begins, experts, across, nullptr)
-               : split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, fit, begins, experts, across, l_down);
+  rc = trans_b ? split_rows<1>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, fit, r_rests, begins, experts, nullptr)
+               : split_rows<2>(s, r_hi, r_lo, r_down, A, lda, 0, rows, rows, K, (int)kp, plan, fit, r_rests, begins, experts, l_down);
   if (rc) return rc;
   PairArgs a;
+  a.later = w.take<int4>((size_t)units * PIECES);
   a.C = C; a.ldc = ldc; a.c_stride = 0; a.l_down = trans_b ? l_down : nullptr; a.r_down = r_down; a.bias = bias; a.plan = plan;
-  a.fit = fit; a.begins = begins;
+  a.fit = fit; a.l_rests = l_rests; a.r_rests = r_rests; a.l_hi = l_hi; a.l_lo = l_lo; a.r_hi = r_hi; a.r_lo = r_lo;
+  a.l_expert = l_per * lp; a.l_lane = trans_b ? lp : 1; a.l_k = trans_b ? 1 : lp; a.r_pitch = kp;
   a.table = table; a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.l_mn = trans_b ? 0 : 1; a.experts = experts;
   a.weights = 0; a.act = act; a.alpha = alpha; a.beta = beta;
   *guard_out = &plan->flag;
-  return launch_pair(s, l_hi, l_lo, l_rows, l_cols, lp, r_hi, r_lo, rows, K, kp, a, (long long)tiles * ((N + 2 * BM - 1) / (2 * BM)));
+  return launch_pair(s, l_hi, l_lo, l_rows, l_cols, lp, r_hi, r_lo, rows, K, kp, a, units);
 }
 
 int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long long ldc, float alpha, const float* A, int rows, int M,
@@ -1089,10 +1165,13 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   DeviceGuard guard(s->device);
   // C_e[m, n] = sum A[r, m] B[r, n]: n in the lanes, m in the columns
   const long long kp = ((long long)rows + (BK - 1LL) * (experts < rows ? experts : rows) + BK - 1) / BK * BK;
+  Rests l_rests = {nullptr, nullptr, (int)rests_room(16.0 * rows * N / experts), 0}, r_rests = {nullptr, nullptr, (int)rests_room(16.0 * rows * M / experts), 1};
   const size_t sums_n = bias_gradient ? ((size_t)(rows + 63) / 64 + experts) * M : 0;
-  const size_t bytes = up256(sizeof(Plan)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
+  const long long units = (long long)experts * ((M + BN - 1) / BN) * ((N + 2 * BM - 1) / (2 * BM));
+  const size_t bytes = up256(sizeof(Plan)) + up256((size_t)units * PIECES * sizeof(int4)) + up256(((size_t)experts + 1) * sizeof(Entry)) + 2 * up256((size_t)N * kp * 2) +
                        2 * up256((size_t)M * kp * 2) + up256((size_t)(kp / POS) * 4) + up256((size_t)experts * N * 4) + up256((size_t)experts * M * 4) +
-                       up256(((size_t)experts * (M + N) * 3 + (size_t)experts * (sizeof(Fit) / 4)) * 4) + up256(sums_n * 4);
+                       up256(((size_t)experts * (M + N) + (size_t)experts * (sizeof(Fit) / 4)) * 4 + WHERE_BYTES) +
+                       up256((size_t)experts * l_rests.cap * sizeof(Rest)) + up256((size_t)experts * r_rests.cap * sizeof(Rest)) + up256(sums_n * 4);
   void* ws = nullptr;
   int rc = cb200_scratch(s, bytes, &ws);
   if (rc) return rc;
@@ -1107,30 +1186,31 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   float* l_down = w.take<float>((size_t)experts * N);
   float* r_down = w.take<float>((size_t)experts * M);
   // (one block, so that it is zeroed in one go)
-  const size_t l_n = (size_t)experts * N, r_n = (size_t)experts * M, fit_words = (size_t)experts * (sizeof(Fit) / 4);
-  uint32_t* zeroed = w.take<uint32_t>((l_n + r_n) * 3 + fit_words);
+  const size_t l_n = (size_t)experts * N, r_n = (size_t)experts * M, fit_words = (size_t)experts * (sizeof(Fit) / 4) + WHERE_BYTES / 4;
+  uint32_t* zeroed = w.take<uint32_t>(l_n + r_n + fit_words);
   Fit* fit = (Fit*)zeroed;
+  l_rests.where = r_rests.where = zeroed + (size_t)experts * (sizeof(Fit) / 4);
   uint32_t* l_max = zeroed + fit_words;
   uint32_t* r_max = l_max + l_n;
-  int* l_thin = (int*)(r_max + r_n);
-  int* r_thin = l_thin + l_n;
-  int* l_tiny = r_thin + r_n;
-  int* r_tiny = l_tiny + l_n;
+  l_rests.list = w.take<Rest>((size_t)experts * l_rests.cap);
+  r_rests.list = w.take<Rest>((size_t)experts * r_rests.cap);
   float* sums = bias_gradient ? w.take<float>(sums_n) : nullptr;
   plan_kernel<<<129, 128, 0, s->stream>>>(plan, table, owner, nullptr, offsets, experts, rows, 1, s->status_dev, zeroed,
-                                          (long long)((l_n + r_n) * 3 + fit_words));
+                                          (long long)(l_n + r_n + fit_words));
   CB_LAUNCH_CHECK(s);
-  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, nullptr, B, ldb, table, owner, experts, rows, N, kp, plan, fit, l_thin, l_tiny))) return rc;
-  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, sums, A, lda, table, owner, experts, rows, M, kp, plan, fit, r_thin, r_tiny))) return rc;
-  const ColumnCounts l_counts = {l_max, l_thin, l_tiny, N}, r_counts = {r_max, r_thin, r_tiny, M};
-  if ((rc = launch_next(s, column_fit_kernel, dim3((unsigned)((M + 127) / 128 + (N + 127) / 128), (unsigned)experts), 128, 0, 1, fit, l_counts, r_counts,
-                        table, bias_gradient, sums, alpha, beta)))
+  if ((rc = split_columns(s, l_hi, l_lo, l_down, l_max, nullptr, B, ldb, table, owner, experts, rows, N, kp, plan, fit, l_rests))) return rc;
+  if ((rc = split_columns(s, r_hi, r_lo, r_down, r_max, sums, A, lda, table, owner, experts, rows, M, kp, plan, fit, r_rests))) return rc;
+  if (bias_gradient && (rc = launch_next(s, column_sum_kernel, dim3((unsigned)((M + 127) / 128), (unsigned)experts), 128, 0, 1, bias_gradient,
+                                         sums, table, M, alpha, beta)))
     return rc;
   PairArgs a;
-  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.fit = fit; a.begins = nullptr; a.table = table;
+  a.later = w.take<int4>((size_t)units * PIECES);
+  a.C = C; a.ldc = ldc; a.c_stride = c_stride; a.l_down = l_down; a.r_down = r_down; a.bias = nullptr; a.plan = plan; a.fit = fit; a.table = table;
   a.status = s->status_dev; a.lanes = N; a.cols = M; a.K = 0; a.l_mn = 0; a.experts = experts; a.weights = 1; a.act = CB200_ACT_NONE;
   a.alpha = alpha; a.beta = beta;
+  a.l_rests = l_rests; a.r_rests = r_rests; a.l_hi = l_hi; a.l_lo = l_lo; a.r_hi = r_hi; a.r_lo = r_lo;
+  a.l_expert = 0; a.l_lane = kp; a.l_k = 1; a.r_pitch = kp;
   *guard_out = &plan->flag;
   return launch_pair(s, l_hi, l_lo, N, kp, kp, r_hi, r_lo, M, kp, kp, a,
-                     (long long)experts * ((M + BN - 1) / BN) * ((N + 2 * BM - 1) / (2 * BM)));
+                     units);
 }

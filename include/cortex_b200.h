@@ -431,9 +431,11 @@ int cb200_graph_destroy(cb200_graph* g);
  * Offsets that decrease or leave [0, rows] are clamped on the device (nothing outside the operands is touched, rows are
  * never computed twice) and the call is reported as CB200_ERR_CUDA by the next cb200_stream_sync.
  * fp32 arithmetic, by the sizes: plain FMAs (few rows per expert), the split arithmetic of gemm!, or (large products) operands as
- * two fp16 halves of values scaled by a power of two per row or column, where the data allow it: a value's place below its row's
- * largest is checked on the device, and a call whose data do not fit falls back to the former inside its own launches.  Either
- * way results of data of one magnitude are within about 1e-6 of the 64-bit ones (relative to their norm).  A row with an infinity or a
+ * two fp16 halves of values scaled by a power of two per row or column, where the data allow it: what the halves leave out of
+ * values far below the largest of their row or column is added apart, and a call with too many of those (or with values outside
+ * 2^-48 .. 2^60, or an infinity or a NaN) falls back to the former inside its own launches.  Either way each element of
+ * a reduction over K values is within (2 K + 128) 2^-24 of the sum of its |alpha a b|, and results of data of one magnitude are
+ * within about 1e-6 of the 64-bit ones (relative to their norm). A row with an infinity or a
  * NaN gives no finite sum, but may give NaN where exact arithmetic gives an infinity; act then keeps a NaN (relu too) and turns
  * infinities into what it makes of them. Of the options below, gemm-auto-presplit
  * (1: never halves, 2: always), gemm-tile-n (64, 128: rows or result rows per tile; larger values mean 128) and gemm-k-slices

@@ -131,6 +131,69 @@ def test_small_values_that_alone_meet_others_input(stream, route, sizes, n, k, s
     _hold("input", sizes, X, dY, W)
 
 
+@pytest.mark.parametrize("way", ["forward", "input", "weights"])
+@pytest.mark.parametrize("act", [None, "relu", "tanh"])
+def test_remainders_of_small_values(stream, way, act):  # noqa: F811
+    """Some values far below the largest of their rows and columns, in both operands and at the same places, met by zeros but for
+    them; results, signs and an accumulation into what is there; the same bits every time."""
+    stream.set_option("gemm-auto-presplit", 2)
+    sizes, n, k = [300, 1, 257, 0, 3], 260, 392
+    rng, X, dY, W = _data(61, sizes, n, k)
+    rows, e = len(X), len(sizes)
+    for _ in range(40):
+        lo, hi = [(0, 300), (301, 558)][rng.integers(2)]
+        g = 0 if lo == 0 else 2
+        r, i, j, small = rng.integers(lo, hi), rng.integers(n), rng.integers(k), np.float32(2.0 ** -rng.integers(22, 60))
+        X[r, j] *= small
+        dY[r, i] *= small
+        W[g, i, j] *= small
+        if way == "forward" and rng.random() < 0.5:
+            keep = X[r, j]
+            X[r] = 0.0                                  # the row meets the matrix there only
+            X[r, j], X[r, (j + 7) % k] = keep, 0.0
+            W[g, i, (j + 1) % k] = 0.0
+    if way == "forward":
+        for r, i, j in ((5, 9, 100), (400, 250, 391)):     # small times small, and nothing else
+            g = 0 if r < 300 else 2
+            W[g, i], W[g, i, j], W[g, i, (j + 5) % k] = 0.0, 2.0 ** -30, 1.0
+            X[r, j], X[r, (j + 5) % k] = 2.0 ** -28, 0.0
+    elif way == "input":
+        for r, i, j in ((5, 9, 100), (400, 250, 391)):
+            g = 0 if r < 300 else 2
+            W[g, :, j], W[g, i, j], W[g, (i + 5) % n, j] = 0.0, 2.0 ** -30, 1.0
+            dY[r, i], dY[r, (i + 5) % n] = 2.0 ** -28, 0.0
+    else:
+        for r, i, j in ((5, 9, 100), (400, 250, 391)):
+            lo, hi = (0, 300) if r < 300 else (301, 558)
+            X[lo:hi, j], X[r, j], X[r + 1, j] = 0.0, 2.0 ** -30, 1.0
+            dY[r, i], dY[r + 1, i] = 2.0 ** -28, 0.0
+    off, bias = ct.to_tensor(_offsets(sizes), "int"), rng.standard_normal((e, n)).astype(np.float32) * np.float32(1e-3)
+    Xt, dYt, Wt = (ct.to_tensor(a, "float") for a in (X, dY, W))
+    for alpha, beta in ((1.0, 0.0), (-2.0, 0.5)):
+        if way == "weights":
+            C0 = rng.standard_normal(W.shape).astype(np.float32) * np.float32(1e-6)
+            run = lambda C: ct.expert_gemm_weights(C, alpha, dYt, Xt, beta, off)
+            want, size = plain.expert_gemm_weights(C0, alpha, dY, X, beta, _offsets(sizes))[:2]
+            length = max(sizes)
+        else:
+            C0 = rng.standard_normal((rows, n if way == "forward" else k)).astype(np.float32) * np.float32(1e-6)
+            if way == "forward":
+                run = lambda C: ct.expert_gemm(C, True, alpha, Xt, Wt, beta, off, bias=ct.to_tensor(bias, "float") if act else None, act=act)
+                want, size = plain.expert_gemm(C0, True, alpha, X, W, beta, _offsets(sizes), bias if act else None, act)
+            else:
+                run = lambda C: ct.expert_gemm(C, False, alpha, dYt, Wt, beta, off, act=act)
+                want, size = plain.expert_gemm(C0, False, alpha, dY, W, beta, _offsets(sizes), None, act)
+            length = k if way == "forward" else n
+        bits = []
+        for _ in range(3):
+            C = ct.to_tensor(C0, "float")
+            run(C)
+            bits.append(ct.to_array(C))
+        assert all(np.array_equal(bits[0], b) for b in bits[1:])
+        _within(bits[0], want, size + (np.abs(want) * 8 * 2.0 ** -24 / _product_tol("float", length) if act == "tanh" else 0.0),
+                _product_tol("float", length), (way, alpha))
+
+
 # ---- which way a call went: the fallback leaves the bits of a call that is certain to fall back ---------------------------
 
 def _fell_back(way, sizes, X, dY, W):
@@ -162,6 +225,10 @@ def test_ordinary_data_stays_on_halves(stream, way):  # noqa: F811
     else:
         assert not _fell_back(way, sizes, _relu(X), dY, W)
         assert not _fell_back(way, sizes, X, dY * (rng.random(dY.shape) < 0.5), W)
+        rare = _relu(X)
+        rare[:, ::10] *= rng.random(rare[:, ::10].shape) < 0.02            # features that hardly any row has
+        assert not _fell_back(way, sizes, rare, dY * (rng.random(dY.shape) < 0.5), W)
+    assert not _fell_back(way, sizes, X, dY, W * (rng.random(W.shape) < 0.1))      # most weights pruned
     large = np.float32(1e25)
     assert _fell_back(way, sizes, X * (large if way == "forward" else 1), dY * (large if way != "forward" else 1), W)
 
