@@ -60,7 +60,7 @@ def global_norm(gradients, norm=None):
     (`norm`, or a new one).  Squares are summed in double, in a fixed order."""
     datatype, addresses, counts = _gradient_list(gradients, "global-norm")
     norm = _norm_tensor(norm, datatype, gradients[0].device)
-    ct.check_stream().global_norm(datatype, addresses, counts, norm.buffer)
+    ct._stream_on(gradients[0].device).global_norm(datatype, addresses, counts, norm.buffer)
     return norm
 
 
@@ -78,7 +78,7 @@ def clip_gradients(gradients, max_norm, clipped=None, norm=None):
         c_type, destinations, c_counts = _gradient_list(clipped, "clip-gradients")
         if c_type != datatype or c_counts != counts or clipped[0].device is not gradients[0].device:
             raise ct.TensorError("Destinations must match the gradients in number, size, datatype and device")
-    ct.check_stream().clip_gradients(datatype, gradient_addresses, counts, destinations, max_norm, norm.buffer)
+    ct._stream_on(gradients[0].device).clip_gradients(datatype, gradient_addresses, counts, destinations, max_norm, norm.buffer)
     return norm
 
 

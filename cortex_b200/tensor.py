@@ -685,6 +685,14 @@ def _ensure_float_operands(name, *tensors):
     return datatype
 
 
+def _stream_on(device):
+    """The bound stream, which must be on the arguments' device: its kernels cannot reach another one's memory."""
+    stream = check_stream()
+    if stream.device is not device:
+        raise TensorError("The stream is on another device than the arguments: %r %r" % (stream.device, device))
+    return stream
+
+
 def _ensure_offsets(name, offsets, experts, device):
     if offsets.buffer.dtype != "int" or offsets.device is not device:
         raise TensorError("%s: offsets must be an integer tensor on the arguments' device: %r" % (name, offsets))
@@ -711,8 +719,8 @@ def expert_gemm(C, trans_b, alpha, A, B, beta, offsets, bias=None, act=None):
     if bias is not None:
         _ensure_dense_vector(bias, [experts, n], "bias")
     _ensure_apart(C, "C", A, B, bias, offsets)
-    check_stream().expert_gemm(C.buffer, ldc, trans_b, alpha, A.buffer, rows, k, lda, B.buffer, experts, n, b_stride, ldb, beta,
-                               offsets.buffer, bias.buffer if bias is not None else None, act)
+    _stream_on(C.device).expert_gemm(C.buffer, ldc, trans_b, alpha, A.buffer, rows, k, lda, B.buffer, experts, n, b_stride, ldb, beta,
+                                     offsets.buffer, bias.buffer if bias is not None else None, act)
     return C
 
 
@@ -731,8 +739,8 @@ def expert_gemm_weights(C, alpha, A, B, beta, offsets, bias_gradient=None):
     if bias_gradient is not None:
         _ensure_dense_vector(bias_gradient, [experts, n], "bias_gradient")
         _ensure_apart(bias_gradient, "bias_gradient", A, B, offsets)
-    check_stream().expert_gemm_weights(C.buffer, c_stride, ldc, alpha, A.buffer, rows, n, lda, B.buffer, k, ldb, experts, beta,
-                                       offsets.buffer, bias_gradient.buffer if bias_gradient is not None else None)
+    _stream_on(C.device).expert_gemm_weights(C.buffer, c_stride, ldc, alpha, A.buffer, rows, n, lda, B.buffer, k, ldb, experts, beta,
+                                            offsets.buffer, bias_gradient.buffer if bias_gradient is not None else None)
     return C
 
 
@@ -815,7 +823,7 @@ def block_normalize(output, total, block, residual, gate, residual_scale, after,
     datatype = _ensure_float_operands("block-normalize", residual, output, total, block, gate, a_scale, a_bias, b_scale, b_bias)
     rows, cols, pitch = _matrix(residual, "residual")
     shape = (rows, cols)
-    check_stream().block_normalize(
+    _stream_on(residual.device).block_normalize(
         datatype, _block_matrices(shape, output, total, block) + [residual.buffer.ptr, pitch],
         [_address(gate)] + _block_vectors(cols, a_scale, a_bias, b_scale, b_bias),
         _block_desc(shape, gate, None, residual_scale, epsilon, kind))
@@ -869,7 +877,7 @@ def block_normalize_gradients(block_gradient, residual_gradient, gate_gradient, 
                 if hi > a and b > lo:
                     raise TensorError("The gradient of a scale or bias overlaps another argument: %r" % (t,))
             spans.append(span)
-    check_stream().block_normalize_gradients(
+    _stream_on(residual_gradient.device).block_normalize_gradients(
         datatype, _block_matrices(shape, block_gradient) + [residual_gradient.buffer.ptr, pitch],
         [_address(gate_gradient)] + sum_addresses,
         _block_matrices(shape, output_gradient, total_gradient, total, block), [_address(gate)] + vectors, desc)

@@ -460,7 +460,9 @@ int cb200_expert_gemm_weights(cb200_stream* s, int dtype, void* C, int64_t c_str
  * reaches the sum by the residual path), and overwrite (not accumulate): residual_gradient, block_gradient, gate_gradient
  * (summed over the rows that share a gate row), and the column sums of the scales and biases; NULL = not wanted, except
  * residual_gradient, and block_gradient where there is a block.  residual_gradient may be total_gradient itself; otherwise
- * gradients share no memory with operands or one another.  float / double; statistics and sums in the element type, in a fixed order. */
+ * gradients share no memory with operands or one another.  float / double; statistics and sums in the element type, in a fixed
+ * order: a row whose squares add up to more than the type holds (floats above 1e19) comes out as before_bias, or as NaN where its
+ * values do too; other rows do not notice. */
 typedef struct cb200_block_desc {
   int32_t kind;
   double epsilon, residual_scale;

@@ -154,6 +154,26 @@ def test_clip_refusals(bound):
         optimize.global_norm([_t([3], "int")])
 
 
+def test_streams_of_another_device_are_refused(oracle_driver):
+    """A stream's kernels cannot reach the memory of another device: the call is refused before it is launched."""
+    from oracle.cpu_backend import OracleDriver
+    other = OracleDriver().default_device().create_stream()
+    with ct.with_stream(oracle_driver.default_device().create_stream()), ct.with_datatype("double"):
+        x, w, y, off, v = _t([6, 4]), _t([3, 5, 4]), _t([6, 5]), _t([4], "int"), _t([4])
+        a, b, c, d, norm = _t([6, 4]), _t([6, 4]), _t([6, 4]), _t([6, 4]), _t([1])
+    calls = [lambda: ct.expert_gemm(y, True, 1.0, x, w, 0.0, off), lambda: ct.expert_gemm_weights(w, 1.0, y, x, 0.0, off),
+             lambda: ct.block_normalize(a, b, c, x, None, 1.0, None, (v, None), 1e-5),
+             lambda: ct.block_normalize_gradients(a, b, None, None, None, c, None, x, d, None, 1.0, None, (v, None), 1e-5),
+             lambda: optimize.global_norm([x], norm=norm), lambda: optimize.clip_gradients([x], 1.0, norm=norm)]
+    with ct.with_stream(oracle_driver.default_device().create_stream()), ct.with_datatype("double"):
+        for call in calls:
+            call()
+    with ct.with_stream(other), ct.with_datatype("double"):
+        for call in calls:
+            with pytest.raises(ct.TensorError, match="another device"):
+                call()
+
+
 # ---- the C ABI refuses before it touches a device: a block of zeros stands in for the stream, and made-up addresses that
 # ---- nothing reads for the buffers
 
