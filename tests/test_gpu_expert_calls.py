@@ -148,3 +148,25 @@ def test_narrow_tiles_in_slices(stream, trans_b, sizes, n, k):  # noqa: F811
         want, size = plain.expert_gemm(C0, trans_b, 0.5, X, W, beta, _offsets(sizes), b, act)
         _within(ct.to_array(Y), want, size, _product_tol("float", k), (sizes, beta))
         assert np.array_equal(ct.to_array(Y).reshape(rows, n)[-1], C0[-1])
+
+
+@pytest.mark.parametrize("route", [1, 2])
+@pytest.mark.parametrize("sizes,n,k", [([1], 1, 1), ([3, 0, 2], 2, 1), ([1, 1], 1, 9), ([5, 300], 7, 8), ([65, 64, 63], 31, 65), ([0, 1, 2] * 300, 24, 16),
+                                       ([256, 257, 255], 257, 127), ([4], 8200, 3), ([2, 1], 3, 8200)])
+def test_smallest_and_oddest_sizes_on_either_route(stream, route, sizes, n, k):  # noqa: F811
+    stream.set_option("gemm-auto-presplit", route)
+    rng = np.random.default_rng(67)
+    rows, e = sum(sizes) + 1, len(sizes)
+    X, dY, W = (rng.standard_normal(s).astype(np.float32) for s in ((rows, k), (rows, n), (e, n, k)))
+    off = ct.to_tensor(_offsets(sizes), "int")
+    Xt, dYt, Wt = (ct.to_tensor(a, "float") for a in (X, dY, W))
+    Y, dX, dW, db = (ct.new_tensor(list(s), "float") for s in ((rows, n), (rows, k), (e, n, k), (e, n)))
+    ct.expert_gemm(Y, True, 1.0, Xt, Wt, 0.0, off)
+    ct.expert_gemm(dX, False, 1.0, dYt, Wt, 0.0, off)
+    ct.expert_gemm_weights(dW, 1.0, dYt, Xt, 0.0, off, bias_gradient=db)
+    o = _offsets(sizes)
+    _within(ct.to_array(Y), *plain.expert_gemm(np.zeros((rows, n)), True, 1.0, X, W, 0.0, o), _product_tol("float", k), "forward")
+    _within(ct.to_array(dX), *plain.expert_gemm(np.zeros((rows, k)), False, 1.0, dY, W, 0.0, o), _product_tol("float", n), "input")
+    w, ws, b, bs = plain.expert_gemm_weights(np.zeros((e, n, k)), 1.0, dY, X, 0.0, o, np.zeros((e, n)))
+    _within(ct.to_array(dW), w, ws, _product_tol("float", max(sizes)), "weights")
+    _within(ct.to_array(db), b, bs, (max(sizes) + 8) * 2.0 ** -24, "bias")
