@@ -77,6 +77,13 @@ template <int BN, int BK> struct RowsCfg {
   static_assert(BM * BN * 4 <= STAGES * STAGE, "a parked tile must fit the pipeline stages");
 };
 
+// A guarded launch is set up while its predecessors end, and waits for them here.
+__device__ __forceinline__ bool nothing_to_do(const int* only_if) {
+  if (!only_if) return false;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  return *only_if == 0;
+}
+
 // 32 accumulator columns (rows first .. first + 31 of C) of one output feature per lane.  No branch between the values: one
 // per value (the activation's) keeps a warp from having more than one in flight (42 cycles a store; a weight gradient of 8
 // experts of 1024 x 4096 with 32 rows each 121 us, 68 without).
@@ -128,7 +135,7 @@ expert_tf32x3_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   int* where = (int*)(tmem_slot + 2);                        // {found, expert, lo, hi, index}, then a word for arrivals
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.only_if && *p.only_if == 0) return;
+  if (nothing_to_do(p.only_if)) return;
   const int tiles_n = (p.N + BM - 1) / BM;
   const int first_unit = (int)blockIdx.x / p.slices, slice = (int)blockIdx.x - first_unit * p.slices;
   const uint32_t smem_base = smem_u32(smem);
@@ -496,7 +503,7 @@ expert_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_const
   Entry* ring = (Entry*)(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.only_if && *p.only_if == 0) return;
+  if (nothing_to_do(p.only_if)) return;
   const int tiles_n = (p.N + BM - 1) / BM;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bar_full = smem_u32(bars), bar_conv = smem_u32(bars + STAGES), bar_empty = smem_u32(bars + 2 * STAGES),
@@ -825,13 +832,18 @@ int launch(cb200_stream* s, int smem, const CUtensorMap& tmA, const CUtensorMap&
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  if (a.only_if) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
   cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, tmA, tmB, a);
   if (e != cudaSuccess) return cb200_cuda_fail(e, "cudaLaunchKernelEx(expert kernel)", __FILE__, __LINE__);
   CB_LAUNCH_CHECK(s);
