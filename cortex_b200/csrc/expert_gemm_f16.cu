@@ -4,17 +4,22 @@
 //   x * s = h1 + h2,   h1 = half(x * s),  h2 = half(x * s - h1),   s = a power of two per operand row
 // carries 22 bits like hi + lo of 3xTF32 does, and the three products h1 h1, h1 h2, h2 h1 cost half of what they cost
 // there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-17 of
-// it keep their 22 bits, smaller ones an absolute error of 2^-25 (scaled).  Down to 2^-21 of the largest that is no more than
+// it keep their 22 bits, smaller ones an absolute error of 2^-25 (scaled).  Down to 2^-20 of the largest that is at most
 // 2^-19 of the value, 2^-18 of the sum of |a||b| in every element of a result.  What the halves leave of values below that
-// (a few in a million of normal data) is written to a list, and the product's epilogue adds it, times what it meets, to the
-// elements that it belongs to: so every element is good, whatever it is made of.  Where a list overflows (data of a really wide
-// range, or a row of it), where a row's largest value is outside [2^-48, 2^60] or a value below 2^-100 when scaled, and where there is an
-// infinity or a NaN, a flag is raised in device memory; the kernel here then does nothing and the 3xTF32 kernel launched behind
-// it, which otherwise does nothing, does the work.
+// (2.3 in a million of normal data) is written to lists, and elements of the result in which it could show -- whose sum is not
+// far above what can be missing: next to none of dense data -- get it, times what it meets, in a small launch behind the
+// product.  So every element is good, whatever it is made of.  Where there are too many such values (in all or in one row),
+// where a row's largest value is outside [2^-48, 2^60] or a scaled value below 2^-100, and where there is an infinity or a NaN,
+// a flag is raised in device memory; the kernels here then do nothing more and the 3xTF32 kernel launched behind them, which
+// otherwise does nothing, does the work.
+// (Measured against a check that let 1 in 64 values of a row lie low and bounded no element, us: 8000 rows over 32 experts of
+// 2048 x 1024 204 -> 209 forward, 224 -> 226 input gradient, 211 -> 210 weight gradient; a piece that needs remainders costs
+// the call about 6 more.  A proof from counts of low values per row and column instead of the lists: 211, 230 and 214, but 490
+// for ReLU'd or rarely used features and 2000 for pruned matrices, which it had to send to 3xTF32.)
 //
 // Steps of a call: group bounds and the table of tiles (one warp); the operands' halves, K-contiguous, with their scales
-// (HBM-bound; operands whose reduction axis is not contiguous get a pass for the column maxima first); the product; the
-// guarded 3xTF32 kernel.
+// and lists (HBM-bound; operands whose reduction axis is not contiguous get a pass for the column maxima first); the product;
+// remainders; the guarded 3xTF32 kernel.
 //
 // The product runs on CTA pairs (tcgen05.mma.cta_group::2, 256 lanes x up to 256 columns per pair), persistent, three
 // pipeline stages of 64 KB (128-byte rows), as the pre-split layer GEMM: every TMA load is a plain one into the issuing CTA, completing on
@@ -859,10 +864,8 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
           h = where_of(1, u.expert, r_first + i * 32 + lane);
           of_columns[i] = __ballot_sync(0xffffffffu, i * 32 + lane < left && (where[h >> 5] >> (h & 31) & 1));
         }
-        const bool any_lane = __any_sync(0xffffffffu, of_lane);
-        // (an element has those of its lane and those of its column)
-        const float bound = (any_lane && (of_columns[0] | of_columns[1] | of_columns[2] | of_columns[3]) ? 512.f : 256.f) * (float)*most_rests;
-        if (any_lane) {
+        const float bound = 512.f * (float)*most_rests;      // (an element has those of its lane and those of its column)
+        if (__any_sync(0xffffffffu, of_lane)) {
           float least = INFINITY;
 #pragma unroll
           for (int j = 0; j < BN / 2; ++j) least = fminf(least, j < left ? fabsf(acc[j]) : INFINITY);

@@ -14,7 +14,7 @@ enum { MAX_EXPERTS = 4096, STATUS_BAD_OFFSETS = 600 };
 struct Tile { int expert, lo, hi, index; };   // rows [lo, hi) of the group; index: which row tile of the group this is
 
 // max(v, 0) that keeps a NaN
-template <typename T> __device__ __forceinline__ T relu(T v) { return v < (T)0 ? (T)0 : v; }
+template <typename T> __device__ __forceinline__ T relu(T v) { return v <= (T)0 ? (T)0 : v; }
 
 __device__ __forceinline__ void report_bad(int* status) {
   if (atomicCAS(status, 0, 1 /* CB200_ERR_INVALID */) == 0) status[1] = STATUS_BAD_OFFSETS;
