@@ -13,7 +13,7 @@
 // a flag is raised in device memory; the kernels here then do nothing more and the 3xTF32 kernel launched behind them, which
 // otherwise does nothing, does the work.
 // (Measured against a check that let 1 in 64 values of a row lie low and bounded no element, us: 8000 rows over 32 experts of
-// 2048 x 1024 204 -> 209 forward, 224 -> 226 input gradient, 211 -> 210 weight gradient; a piece that needs remainders costs
+// 2048 x 1024 206 -> 212 forward, 225 -> 226 input gradient, 211 -> 209 weight gradient; a piece that needs remainders costs
 // the call about 6 more.  A proof from counts of low values per row and column instead of the lists: 211, 230 and 214, but 490
 // for ReLU'd or rarely used features and 2000 for pruned matrices, which it had to send to 3xTF32.)
 //
@@ -827,6 +827,15 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
         else if (!none) l_scale = 1.f / 16384.f;           // (2^14 of the folded scales)
         if (p.bias) b = p.bias[(long long)u.expert * p.lanes + l];
       }
+      const int r_first = u.r0 + half * (BN / 2);
+      auto rests_at = [&](int side, int at) {
+        const int h = where_of(side, u.expert, at);
+        return (where[h >> 5] >> (h & 31) & 1) != 0;
+      };
+      bool with_rests = rests_at(0, l) && l < p.lanes;       // (before the wait)
+#pragma unroll
+      for (int i = 0; i < BN / 64; ++i) with_rests = with_rests || (i * 32 + lane < left && rests_at(1, r_first + i * 32 + lane));
+      with_rests = __any_sync(0xffffffffu, with_rests && !none);
 #pragma unroll
       for (int j = 0; j < BN / 2; ++j) acc[j] = 0.f;
 #pragma unroll 1
@@ -854,16 +863,11 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       // where a sum itself is 2^8 times their number, all of them together are below 2^-18 of it (normal data: hardly anywhere
       // not).  Other pieces are left to add_rests_kernel, with the activation.
       bool later = false;
-      if (!none && left > 0) {
-        const int r_first = u.r0 + half * (BN / 2);
-        int h = where_of(0, u.expert, l);
-        const bool of_lane = (where[h >> 5] >> (h & 31) & 1) && l < p.lanes;
+      if (with_rests) {
+        const bool of_lane = rests_at(0, l) && l < p.lanes;
         unsigned of_columns[BN / 64];
 #pragma unroll
-        for (int i = 0; i < BN / 64; ++i) {
-          h = where_of(1, u.expert, r_first + i * 32 + lane);
-          of_columns[i] = __ballot_sync(0xffffffffu, i * 32 + lane < left && (where[h >> 5] >> (h & 31) & 1));
-        }
+        for (int i = 0; i < BN / 64; ++i) of_columns[i] = __ballot_sync(0xffffffffu, i * 32 + lane < left && rests_at(1, r_first + i * 32 + lane));
         const float bound = 512.f * (float)*most_rests;      // (an element has those of its lane and those of its column)
         if (__any_sync(0xffffffffu, of_lane)) {
           float least = INFINITY;
