@@ -760,19 +760,32 @@ int pack(cb200_stream* s, float* dst, const float* src, long long ld, long long 
   return CB200_OK;
 }
 
+// No memory left for the halves (up to 2 GB)?  The call goes on without them.
+bool no_room(int rc, const int* only_if) {
+  if (rc != CB200_ERR_NOMEM || only_if) return false;
+  cudaGetLastError();                                            // (or the next launch would report it)
+  return true;
+}
+
 int rows_tc(cb200_stream* s, Product<float> p) {
   if (few_rows_ok(p) && s->opt_gemm_auto_presplit != 2 && s->opt_gemm_tile_n == 0) return run_few_rows<float>(s, p);
   const long long b_rows = p.trans_b ? p.N : p.K;
   const int b_cols = p.trans_b ? p.K : p.N;
   if (p.experts == 1) p.b_stride = b_rows * p.ldb;
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, p.b_stride);
-  if (cb200_expert_f16_ok(s, p.rows, p.K, p.N, p.experts)) {
+  bool halves = cb200_expert_f16_ok(s, p.rows, p.K, p.N, p.experts);
+  if (halves) {
     // products at twice the rate; what follows runs only where the data do not fit scaled halves
-    int rc = cb200_expert_rows_f16(s, p.C, p.ldc, p.trans_b, p.alpha, p.A, p.rows, p.K, p.lda, p.B, p.experts, p.N, p.b_stride, p.ldb,
+    const int rc = cb200_expert_rows_f16(s, p.C, p.ldc, p.trans_b, p.alpha, p.A, p.rows, p.K, p.lda, p.B, p.experts, p.N, p.b_stride, p.ldb,
                                    p.beta, p.offsets, p.bias, p.act, &p.only_if);
-    if (rc) return rc;
-    if (pack_a || pack_b) return run_rows<float>(s, p);         // (the workspace holds the halves)
-  } else if (pack_a || pack_b) {
+    if (!no_room(rc, p.only_if)) {
+      if (rc) return rc;
+      if (pack_a || pack_b) return run_rows<float>(s, p);       // (the workspace holds the halves)
+    } else {
+      halves = false;
+    }
+  }
+  if (!halves && (pack_a || pack_b)) {
     DeviceGuard guard(s->device);
     const long long lda = (p.K + 3) / 4 * 4, ldb = (b_cols + 3) / 4 * 4;
     const size_t a_n = pack_a ? (size_t)p.rows * lda : 0, b_n = pack_b ? (size_t)p.experts * b_rows * ldb : 0;
@@ -798,19 +811,24 @@ int weights_tc(cb200_stream* s, Product<float> p) {
   if (p.rows == 0) return run_few_weights<float>(s, p);
   if (few_weights_ok(p) && s->opt_gemm_auto_presplit != 2 && s->opt_gemm_tile_n == 0) return run_few_weights<float>(s, p);
   const bool pack_a = !cb200_expert_tc_ok(p.A, p.lda, p.A, 4, 4), pack_b = !cb200_expert_tc_ok(p.B, p.ldb, p.B, 4, 4);
-  const bool halves = cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts);
+  bool halves = cb200_expert_weights_f16_ok(s, p.rows, p.M, p.N, p.experts);
+  if (halves) {
+    const int rc = cb200_expert_weights_f16(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta,
+                                      p.offsets, p.bias_g, &p.only_if);
+    if (!no_room(rc, p.only_if)) {
+      if (rc) return rc;
+      p.bias_g = nullptr;                                        // done with the column pass
+      if (pack_a || pack_b) return run_weights<float>(s, p);
+    } else {
+      halves = false;
+    }
+  }
   if (!halves && p.bias_g) {
     DeviceGuard guard(s->device);
     int rc = run_bias_gradient<float>(s, p);
     if (rc) return rc;
   }
-  if (halves) {
-    int rc = cb200_expert_weights_f16(s, p.C, p.c_stride, p.ldc, p.alpha, p.A, p.rows, p.M, p.lda, p.B, p.N, p.ldb, p.experts, p.beta,
-                                      p.offsets, p.bias_g, &p.only_if);
-    if (rc) return rc;
-    p.bias_g = nullptr;                                          // done with the column pass
-    if (pack_a || pack_b) return run_weights<float>(s, p);
-  } else if (pack_a || pack_b) {
+  if (!halves && (pack_a || pack_b)) {
     DeviceGuard guard(s->device);
     const long long lda = (p.M + 3) / 4 * 4, ldb = (p.N + 3) / 4 * 4;
     const size_t a_n = pack_a ? (size_t)p.rows * lda : 0, b_n = pack_b ? (size_t)p.rows * ldb : 0;

@@ -1112,7 +1112,8 @@ bool cb200_expert_weights_f16_ok(cb200_stream* s, long long rows, long long M, l
   return rows >= 96 * experts && here < there;
 }
 
-// The flag that the guarded 3xTF32 launch reads is returned through `guard`.
+// The flag that the guarded 3xTF32 launch reads is returned through `guard_out`, which is left alone where there is no room for
+// the workspace (CB200_ERR_NOMEM; nothing has been launched then).
 int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b, float alpha, const float* A, int rows, int K,
                           long long lda, const float* B, int experts, int N, long long b_stride, long long ldb, float beta,
                           const int* offsets, const float* bias, int act, const int** guard_out) {
@@ -1133,6 +1134,7 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   if (rc) return rc;
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
+  *guard_out = &plan->flag;
   Entry* table = w.take<Entry>(tiles + 1);
   int* begins = w.take<int>((size_t)experts);
   char* zeroed = w.take<char>((size_t)experts * sizeof(Fit) + WHERE_BYTES);
@@ -1162,7 +1164,6 @@ int cb200_expert_rows_f16(cb200_stream* s, float* C, long long ldc, int trans_b,
   a.l_expert = l_per * lp; a.l_lane = trans_b ? lp : 1; a.l_k = trans_b ? 1 : lp; a.r_pitch = kp;
   a.table = table; a.status = s->status_dev; a.lanes = N; a.cols = 0; a.K = K; a.l_mn = trans_b ? 0 : 1; a.experts = experts;
   a.weights = 0; a.act = act; a.alpha = alpha; a.beta = beta;
-  *guard_out = &plan->flag;
   return launch_pair(s, l_hi, l_lo, l_rows, l_cols, lp, r_hi, r_lo, rows, K, kp, a, units);
 }
 
@@ -1184,6 +1185,7 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   if (rc) return rc;
   Carve w = {(char*)ws, 0};
   Plan* plan = w.take<Plan>(1);
+  *guard_out = &plan->flag;
   Entry* table = w.take<Entry>((size_t)experts + 1);
   int* owner = w.take<int>((size_t)(kp / POS));
   __half* l_hi = w.take<__half>((size_t)N * kp);
@@ -1217,7 +1219,6 @@ int cb200_expert_weights_f16(cb200_stream* s, float* C, long long c_stride, long
   a.alpha = alpha; a.beta = beta;
   a.l_rests = l_rests; a.r_rests = r_rests; a.l_hi = l_hi; a.l_lo = l_lo; a.r_hi = r_hi; a.r_lo = r_lo;
   a.l_expert = 0; a.l_lane = kp; a.l_k = 1; a.r_pitch = kp;
-  *guard_out = &plan->flag;
   return launch_pair(s, l_hi, l_lo, N, kp, kp, r_hi, r_lo, M, kp, kp, a,
                      units);
 }

@@ -170,3 +170,34 @@ def test_smallest_and_oddest_sizes_on_either_route(stream, route, sizes, n, k): 
     w, ws, b, bs = plain.expert_gemm_weights(np.zeros((e, n, k)), 1.0, dY, X, 0.0, o, np.zeros((e, n)))
     _within(ct.to_array(dW), w, ws, _product_tol("float", max(sizes)), "weights")
     _within(ct.to_array(db), b, bs, (max(sizes) + 8) * 2.0 ** -24, "bias")
+
+
+def test_no_memory_left_for_the_halves(b200_driver):
+    """The halves' workspace does not fit beside what a program holds: the call runs without them."""
+    device = b200_driver.default_device()
+    s = device.create_stream()
+    s.set_option("gemm-auto-presplit", 2)
+    sizes, n, k = [130, 0, 126, 256], 4096, 4096                 # halves of 268 MB
+    rows = sum(sizes)
+    rng = np.random.default_rng(73)
+    X, W, dY = rng.standard_normal((rows, k)).astype(np.float32), rng.standard_normal((4, n, k)).astype(np.float32), None
+    dY = rng.standard_normal((rows, n)).astype(np.float32)
+    with ct.with_stream(s):
+        off, Xt, Wt, dYt = ct.to_tensor(_offsets(sizes), "int"), ct.to_tensor(X, "float"), ct.to_tensor(W, "float"), ct.to_tensor(dY, "float")
+        Y, dX = ct.new_tensor([rows, n], "float"), ct.new_tensor([rows, k], "float")
+        s.sync()
+        held, room = [], device.memory_info()["free"] - (96 << 20)
+        while room > (8 << 20):
+            size = min(room, 8 << 30)
+            held.append(device.allocate_device_buffer(size // 8, "double"))
+            room = min(room - size, device.memory_info()["free"] - (96 << 20))
+        ct.expert_gemm(Y, True, 1.0, Xt, Wt, 0.0, off)
+        ct.expert_gemm(dX, False, 1.0, dYt, Wt, 0.0, off)
+        s.sync()
+        for b in held:
+            b.release()
+        lo, hi = 120, 140                                        # rows of two experts
+        w, ws = plain.expert_gemm(np.zeros((20, n)), True, 1.0, X[lo:hi], W[[0, 2]], 0.0, [0, 10, 20])
+        _within(ct.to_array(Y).reshape(rows, n)[lo:hi], w, ws, _product_tol("float", k), "forward")
+        w, ws = plain.expert_gemm(np.zeros((20, k)), False, 1.0, dY[lo:hi], W[[0, 2]], 0.0, [0, 10, 20])
+        _within(ct.to_array(dX).reshape(rows, k)[lo:hi], w, ws, _product_tol("float", n), "input")
