@@ -6,7 +6,7 @@
 // there.  What tf32 has and fp16 lacks is range: s puts a row's largest value into [2^14, 2^15), values down to 2^-17 of
 // it keep their 22 bits, smaller ones an absolute error of 2^-25 (scaled).  Down to 2^-20 of the largest that is at most
 // 2^-19 of the value, 2^-18 of the sum of |a||b| in every element of a result.  What the halves leave of values below that
-// (2.3 in a million of normal data) is written to lists, and elements of the result in which it could show -- whose sum is not
+// (2.3 in a million of normal data; of values below TINY all) is written to lists, and elements of the result in which it could show -- whose sum is not
 // far above what can be missing: next to none of dense data -- get it, times what it meets, in a small launch behind the
 // product.  So every element is good, whatever it is made of.  Where there are too many such values (in all or in one row),
 // where a row's largest value is outside [2^-48, 2^60] or a scaled value below 2^-100, and where there is an infinity or a NaN,
@@ -52,10 +52,10 @@ constexpr int THREADS = (EPI_WARPS + 4) * 32;            // three warpgroups; th
 constexpr int L_TILE = BM * BK * 2, R_TILE = BN / 2 * BK * 2;       // 16 KiB each
 constexpr int R_BOX = 64;                                // rows of one box of the column operand
 constexpr int RAW = L_TILE + R_TILE, STAGE = 2 * RAW, STAGES = 196608 / STAGE;
-constexpr int WHERE = 16384;                             // bits for where there are remainders (a few hundred are set for normal data)
-constexpr int WHERE_BYTES = WHERE / 8 + WHERE * 4;
+constexpr int WHERE = 16384;                             // places for remainders (normal data: a few hundred are taken), two bits each
+constexpr int WHERE_BYTES = WHERE / 4 + WHERE * 4;
 constexpr int SCALES = EPI_WARPS * (BN / 2) * 4;           // a column-scale list per epilogue warp
-constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES + WHERE / 8;
+constexpr int SMEM = STAGES * STAGE + 1024 + 256 + SCALES + WHERE / 4;
 constexpr int TMEM_COLS = 2 * BN;
 constexpr int DRAIN = 256 / BK;                         // stages per accumulator filling
 
@@ -77,10 +77,12 @@ struct alignas(16) Fit {
 // What the two halves leave of a scaled value below SMALL: of lane or column `at` (of the expert's matrix; a row of the batch; a
 // column of a weight gradient's operand), at position k of the halves.
 struct alignas(16) Rest { int at, k; float rest; int unused; };
-constexpr float SMALL = 1.f / 64, LEAST = 0x1p-100f;
+// A value below TINY is left to the list as a whole: the tensor core adds products of halves whose first half is not normal with as
+// many bits less as that has leading zeros (three of either operand at TINY: 18 left; 10 at 2^-24).
+constexpr float SMALL = 1.f / 64, TINY = 0x1p-17f, LEAST = 0x1p-100f;
 constexpr int MOST_RESTS = 8;            // in a lane or column (they are added one after another; normal data: 4 in the largest calls)
-// An operand's lists, `cap` for every expert.  Both operands': by where remainders are, hashed, a bit -- a lane or a column without
-// it has none -- and (behind the bits) their number.
+// An operand's lists, `cap` for every expert.  Both operands': by where remainders are, hashed, two bits -- a lane or a column without
+// the lower has none, one with the higher has values below TINY -- and (behind the bits) the number of remainders.
 struct Rests { Rest* list; uint32_t* where; int cap, side; };
 __device__ __forceinline__ int where_of(int side, int expert, int at) {
   return (int)(((unsigned)at * 2u + (unsigned)side + (unsigned)expert * 0x9e3779b1u) * 0x85ebca6bu >> 18);
@@ -184,7 +186,10 @@ __device__ __forceinline__ uint32_t split8(const float (&w)[8], float up, Half8&
   if (__half2float(__hmin(__low2half(least), __high2half(least))) < SMALL)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (w[j] != 0.f && fabsf(w[j] * up) < SMALL) small |= 1u << j;
+      if (w[j] != 0.f && fabsf(w[j] * up) < SMALL) {
+        small |= 1u << j;
+        if (fabsf(w[j] * up) < TINY) a.h[j] = b.h[j] = __float2half_rn(0.f);
+      }
   return small;
 }
 __device__ __forceinline__ void keep_rest(Fit* fit, const Rests& rests, int expert, int at, int k, float y) {
@@ -192,11 +197,12 @@ __device__ __forceinline__ void keep_rest(Fit* fit, const Rests& rests, int expe
   if (!(fabsf(y) >= LEAST)) f->bad = 1;
   __half h1, h2;
   split_half(y, h1, h2);
-  const float rest = (y - __half2float(h1)) - __half2float(h2);      // both differences are exact
+  const bool tiny = fabsf(y) < TINY;
+  const float rest = tiny ? y : (y - __half2float(h1)) - __half2float(h2);      // both differences are exact
   if (rest == 0.f) return;
   const int i = atomicAdd(&f->listed[rests.side], 1), h = where_of(rests.side, expert, at);
-  atomicOr(rests.where + (h >> 5), 1u << (h & 31));
-  atomicMax(&f->most, (int)atomicAdd(rests.where + WHERE / 32 + h, 1u) + 1);
+  atomicOr(rests.where + (h >> 4), (tiny ? 3u : 1u) << 2 * (h & 15));
+  atomicMax(&f->most, (int)atomicAdd(rests.where + WHERE / 16 + h, 1u) + 1);
   if (i < rests.cap) rests.list[(long long)expert * rests.cap + i] = {at, k, rest, 0};
 }
 
@@ -647,7 +653,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   wait_for_previous_kernel();
   uint32_t* where = reinterpret_cast<uint32_t*>(smem + STAGES * STAGE + 256 + SCALES);
   int* most_rests = reinterpret_cast<int*>(smem + STAGES * STAGE + 248);
-  if (threadIdx.x < WHERE / 128) reinterpret_cast<uint4*>(where)[threadIdx.x] = reinterpret_cast<const uint4*>(p.l_rests.where)[threadIdx.x];
+  if (threadIdx.x < WHERE / 64) reinterpret_cast<uint4*>(where)[threadIdx.x] = reinterpret_cast<const uint4*>(p.l_rests.where)[threadIdx.x];
   int no_fit = 0, most = 0;
   for (int e = threadIdx.x; e < p.experts; e += THREADS) {
     const Fit f = p.fit[e];
@@ -830,12 +836,13 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       const int r_first = u.r0 + half * (BN / 2);
       auto rests_at = [&](int side, int at) {
         const int h = where_of(side, u.expert, at);
-        return (where[h >> 5] >> (h & 31) & 1) != 0;
+        return where[h >> 4] >> 2 * (h & 15) & 3;            // 0: none
       };
-      bool with_rests = rests_at(0, l) && l < p.lanes;       // (before the wait)
+      unsigned with_rests = l < p.lanes ? rests_at(0, l) : 0u;       // (before the wait)
 #pragma unroll
-      for (int i = 0; i < BN / 64; ++i) with_rests = with_rests || (i * 32 + lane < left && rests_at(1, r_first + i * 32 + lane));
-      with_rests = __any_sync(0xffffffffu, with_rests && !none);
+      for (int i = 0; i < BN / 64; ++i)
+        if (i * 32 + lane < left) with_rests |= rests_at(1, r_first + i * 32 + lane);
+      with_rests = __reduce_or_sync(0xffffffffu, none ? 0u : with_rests);
 #pragma unroll
       for (int j = 0; j < BN / 2; ++j) acc[j] = 0.f;
 #pragma unroll 1
@@ -861,19 +868,19 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
       if (!ok) break;
       // What the halves have left out, in the lanes and columns with remainders: one is at most 2^-25 and meets at most 2^15, so
       // where a sum itself is 2^8 times their number, all of them together are below 2^-18 of it (normal data: hardly anywhere
-      // not).  Other pieces are left to add_rests_kernel, with the activation.
-      bool later = false;
+      // not).  Other pieces, and those with values below TINY, are left to add_rests_kernel, with the activation.
+      bool later = (with_rests & 2) != 0;
       if (with_rests) {
-        const bool of_lane = rests_at(0, l) && l < p.lanes;
+        const bool of_lane = rests_at(0, l) != 0 && l < p.lanes;
         unsigned of_columns[BN / 64];
 #pragma unroll
-        for (int i = 0; i < BN / 64; ++i) of_columns[i] = __ballot_sync(0xffffffffu, i * 32 + lane < left && rests_at(1, r_first + i * 32 + lane));
+        for (int i = 0; i < BN / 64; ++i) of_columns[i] = __ballot_sync(0xffffffffu, i * 32 + lane < left && rests_at(1, r_first + i * 32 + lane) != 0);
         const float bound = 512.f * (float)*most_rests;      // (an element has those of its lane and those of its column)
         if (__any_sync(0xffffffffu, of_lane)) {
           float least = INFINITY;
 #pragma unroll
           for (int j = 0; j < BN / 2; ++j) least = fminf(least, j < left ? fabsf(acc[j]) : INFINITY);
-          later = of_lane && least < bound;
+          later = later || (of_lane && least < bound);
         }
 #pragma unroll
         for (int i = 0; i < BN / 64; ++i)

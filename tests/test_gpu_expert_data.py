@@ -194,6 +194,54 @@ def test_remainders_of_small_values(stream, way, act):  # noqa: F811
                 _product_tol("float", length), (way, alpha))
 
 
+def _any_data(rng, shape):
+    """Normal values, spread in every way over up to 60 powers of two, with outliers, with zeros in every way."""
+    x = rng.standard_normal(shape)
+    kind, a = rng.integers(8), rng.choice([0, 2, 5, 9, 14, 22, 30])
+    rows, columns = shape[:-1] + (1,), (1,) * (len(shape) - 1) + shape[-1:]
+    if kind in (1, 2, 3):
+        where = (shape, rows, columns)[kind - 1]
+        x = x * np.exp2(rng.uniform(-a, a, where))
+    if kind == 4:
+        x = _relu(x)
+    if kind == 5:
+        x = x * np.where(rng.random(shape) < rng.choice([1e-4, 1e-3, 1e-2]), np.exp2(-rng.uniform(18, 45, shape)), 1.0)
+    if kind == 6:
+        x = x * np.where(rng.random(shape) < 1e-4, np.exp2(rng.uniform(10, 40, shape)), 1.0)
+    if rng.random() < 0.5:
+        x = x * (rng.random(shape) < rng.choice([0.5, 0.1, 0.01]))
+    for where in (rows, columns):
+        if rng.random() < 0.3:
+            x = x * (rng.random(where) < 0.9)
+    return x.astype(np.float32)
+
+
+@pytest.mark.parametrize("route", [1, 2])
+@pytest.mark.parametrize("first", [900, 1000, 1250, 0, 100, 200, 300, 400])
+def test_any_data_within_the_bound_of_its_own_terms(stream, route, first):  # noqa: F811
+    """Every element of every direction, whatever it is made of."""
+    stream.set_option("gemm-auto-presplit", route)
+    for seed in range(first, first + 60):
+        rng = np.random.default_rng(seed)
+        sizes = [int(v) for v in rng.choice([0, 1, 2, 3, 7, 31, 64, 100, 256, 257, 300], rng.integers(1, 7))]
+        n, k = int(rng.choice([1, 3, 8, 33, 64, 129, 200, 256, 300])), int(rng.choice([1, 2, 5, 16, 40, 64, 100, 130, 257, 520]))
+        rows, e, o = sum(sizes) + 1, len(sizes), _offsets(sizes)
+        X, W, dY = _any_data(rng, (rows, k)), _any_data(rng, (e, n, k)), _any_data(rng, (rows, n))
+        off, Xt, Wt, dYt = ct.to_tensor(o, "int"), ct.to_tensor(X, "float"), ct.to_tensor(W, "float"), ct.to_tensor(dY, "float")
+        alpha, beta = [(1.0, 0.0), (-0.5, 1.0)][rng.integers(2)]
+        Y0, act = (rng.standard_normal((rows, n)) * 1e-3).astype(np.float32), [None, "relu"][rng.integers(2)]
+        Y, dX, dW = ct.to_tensor(Y0, "float"), ct.new_tensor([rows, k], "float"), ct.new_tensor([e, n, k], "float")
+        ct.expert_gemm(Y, True, alpha, Xt, Wt, beta, off, act=act)
+        ct.expert_gemm(dX, False, 1.0, dYt, Wt, 0.0, off)
+        ct.expert_gemm_weights(dW, 1.0, dYt, Xt, 0.0, off)
+        least = 2.0 ** -120                                      # below the normal range nothing is promised
+        for name, got, (want, size), length in (
+                ("forward", Y, plain.expert_gemm(Y0, True, alpha, X, W, beta, o, None, act), k),
+                ("input", dX, plain.expert_gemm(np.zeros((rows, k)), False, 1.0, dY, W, 0.0, o), n),
+                ("weights", dW, plain.expert_gemm_weights(np.zeros((e, n, k)), 1.0, dY, X, 0.0, o)[:2], max(sizes + [1]))):
+            _within(ct.to_array(got), want, size + least / _product_tol("float", length), _product_tol("float", length), (seed, name))
+
+
 # ---- which way a call went: the fallback leaves the bits of a call that is certain to fall back ---------------------------
 
 def _fell_back(way, sizes, X, dY, W):
