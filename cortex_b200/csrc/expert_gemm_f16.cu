@@ -68,9 +68,9 @@ struct Plan {
   int later;                   // pieces in the list for add_rests_kernel
   int unused[2];
 };
-// What an expert's operands have for the lists; all zero at the start of a call.
-struct alignas(16) Fit {
-  int bad;                     // something does not fit scaled halves
+// What an expert's operands have for the lists; all zero at the start of a call.  (A line each: the counts are atomics.)
+struct alignas(128) Fit {
+  int bad;                     // something does not fit scaled halves, or its list
   int listed[2];               // remainders of the lanes' operand, of the columns'
   int most;                    // no more of them than this in one lane or column
 };
@@ -192,6 +192,14 @@ __device__ __forceinline__ uint32_t split8(const float (&w)[8], float up, Half8&
       }
   return small;
 }
+// Are there so many that lists are no use?  (Data of a wide range would queue up at the counts: 2048 x 1024 values over 60 powers
+// of two for each of 32 experts 100 ms.)
+__device__ __forceinline__ bool too_many(Fit* fit, int expert, uint32_t small) {
+  const unsigned lanes = __activemask();
+  const bool many = __popc(__ballot_sync(lanes, small != 0)) > MOST_RESTS || __popc(small) > 2;
+  if (many) fit[expert].bad = 1;
+  return many || __ldcg(&fit[expert].bad) != 0;
+}
 __device__ __forceinline__ void keep_rest(Fit* fit, const Rests& rests, int expert, int at, int k, float y) {
   Fit* f = fit + expert;
   if (!(fabsf(y) >= LEAST)) f->bad = 1;
@@ -202,8 +210,10 @@ __device__ __forceinline__ void keep_rest(Fit* fit, const Rests& rests, int expe
   if (rest == 0.f) return;
   const int i = atomicAdd(&f->listed[rests.side], 1), h = where_of(rests.side, expert, at);
   atomicOr(rests.where + (h >> 4), (tiny ? 3u : 1u) << 2 * (h & 15));
-  atomicMax(&f->most, (int)atomicAdd(rests.where + WHERE / 16 + h, 1u) + 1);
-  if (i < rests.cap) rests.list[(long long)expert * rests.cap + i] = {at, k, rest, 0};
+  const int here = (int)atomicAdd(rests.where + WHERE / 16 + h, 1u) + 1;
+  atomicMax(&f->most, here);
+  if (i >= rests.cap || here > MOST_RESTS) f->bad = 1;
+  else rests.list[(long long)expert * rests.cap + i] = {at, k, rest, 0};
 }
 
 __device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
@@ -298,7 +308,7 @@ __global__ void __launch_bounds__(256, 4) split_rows_kernel(__half* hi, __half* 
     uint32_t small = split8(w, up, a, b);
     *reinterpret_cast<uint4*>(hi + r * kp + c) = a.v;      // pitch and position are multiples of 8 halves
     *reinterpret_cast<uint4*>(lo + r * kp + c) = b.v;
-    if (!ok) small = 0;
+    if (!ok || (small && too_many(fit, expert_of_row(), small))) small = 0;
     for (; small; small &= small - 1) {
       const int at = c + __ffs(small) - 1, row = (int)(MATRICES ? r % rows_per : r);
       const float y = (RAGGED == 2 ? src[at] * (16384.f * scales[at]) : src[at]) * up;
@@ -447,6 +457,7 @@ __global__ void __launch_bounds__(256) split_columns_kernel(__half* hi, __half* 
         fit[g].bad = 1;
         small = 0;
       }
+      if (small && too_many(fit, g, small)) small = 0;
       for (; small; small &= small - 1) {
         const int j = __ffs(small) - 1;
         keep_rest(fit, rests, g, c, (int)pos + p8 + j, tile[h][p8 + j][col] * up);
@@ -657,7 +668,7 @@ expert_pair_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constan
   int no_fit = 0, most = 0;
   for (int e = threadIdx.x; e < p.experts; e += THREADS) {
     const Fit f = p.fit[e];
-    no_fit |= f.bad | (f.listed[0] > p.l_rests.cap) | (f.listed[1] > p.r_rests.cap) | (f.most > MOST_RESTS);
+    no_fit |= f.bad;
     most = max(most, f.most);
   }
   if (threadIdx.x == 0) *most_rests = 0;

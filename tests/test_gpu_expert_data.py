@@ -277,6 +277,8 @@ def test_ordinary_data_stays_on_halves(stream, way):  # noqa: F811
         rare[:, ::10] *= rng.random(rare[:, ::10].shape) < 0.02            # features that hardly any row has
         assert not _fell_back(way, sizes, rare, dY * (rng.random(dY.shape) < 0.5), W)
     assert not _fell_back(way, sizes, X, dY, W * (rng.random(W.shape) < 0.1))      # most weights pruned
+    spread = lambda a: a * np.exp2(rng.uniform(-30, 30, a.shape)).astype(np.float32)
+    assert _fell_back(way, sizes, spread(X), spread(dY), spread(W))                 # far too many small values
     large = np.float32(1e25)
     assert _fell_back(way, sizes, X * (large if way == "forward" else 1), dY * (large if way != "forward" else 1), W)
 
